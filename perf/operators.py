@@ -155,9 +155,10 @@ def _quantize_plain(x, tiles):
     padded = torch.nn.functional.pad(x.float(), (0, _blocks(k) * BLOCK - k, 0, -rows % high))
     cells = padded.view(*lead, padded.shape[-2] // high, high, _blocks(k), BLOCK)
     amax = cells.abs().amax(dim=(-3, -1)).clamp(min=AMAX_FLOOR)
-    q = (cells * (E4M3_MAX / amax)[..., :, None, :, None]).clamp(-E4M3_MAX, E4M3_MAX)
+    most = torch.full_like(amax, E4M3_MAX)  # a tensor: a quotient with a number is a product with its inverse
+    q = (cells * (most / amax)[..., :, None, :, None]).clamp(-E4M3_MAX, E4M3_MAX)
     q = q.view(padded.shape)[..., :rows, :k].to(torch.float8_e4m3fn).contiguous()
-    return q, amax / E4M3_MAX
+    return q, amax / most
 
 
 def _dequantize(q, s, tiles, kind=torch.float32):
