@@ -17,7 +17,7 @@ from heliostune_b200.errors import KernelError
 PACKAGE_DIR = Path(__file__).resolve().parent
 LIBRARY_PATH = PACKAGE_DIR / "libheliostune_b200.so"
 HEADER_PATH = PACKAGE_DIR.parent / "include" / "heliostune_b200.h"
-SOURCES = (PACKAGE_DIR / "csrc" / "capi.cu",)
+SOURCES = (PACKAGE_DIR / "csrc" / "capi.cu", PACKAGE_DIR / "csrc" / "grouped_api.cu")
 NVCC_FLAGS = (
     "-gencode",
     "arch=compute_100a,code=sm_100a",
@@ -27,6 +27,8 @@ NVCC_FLAGS = (
     "-Xcompiler",
     "-fPIC",
     "-shared",
+    "-t",
+    "0",
 )
 
 HST_OK = 0
@@ -44,6 +46,14 @@ FAMILY_PERSISTENT = 1
 FAMILY_SPLIT_K = 2
 FAMILY_STREAM = 3
 FAMILY_PAIR = 4
+
+HST_F16 = 0
+HST_BF16 = 1
+HST_WEIGHT_KN = 0
+HST_WEIGHT_NK = 1
+GROUPED_FORWARD = 0
+GROUPED_WEIGHT_GRAD = 1
+GROUPED_SCALED = 2
 
 #: Every symbol include/heliostune_b200.h declares.
 EXPORTED_SYMBOLS = (
@@ -71,6 +81,11 @@ EXPORTED_SYMBOLS = (
     "hst_ipc_close",
     "hst_pair_stream_k_tiles",
     "hst_rmsnorm_matmul_stream",
+    "hst_grouped_workspace_size",
+    "hst_grouped_matmul",
+    "hst_grouped_weight_grad",
+    "hst_matmul_blockscaled",
+    "hst_quantize_e4m3",
 )
 
 
@@ -179,6 +194,27 @@ def _declare(lib: ctypes.CDLL) -> None:
         ),
         "hst_peer_barrier": (
             [ctypes.POINTER(ctypes.c_void_p), _i32, _i32, _i32, ctypes.c_uint64, ctypes.c_uint64, _ptr],
+            ctypes.c_int,
+        ),
+        "hst_grouped_workspace_size": (
+            [_i32, _i64, _i32, _i64, _i64, ctypes.c_int, ctypes.POINTER(_size)],
+            ctypes.c_int,
+        ),
+        "hst_grouped_matmul": (
+            [_i32, _ptr, _i64, _ptr, _i64, _i64, _i32, _ptr, _i32, _ptr, _i64, _i64, _i64, _ptr, _size, _ptr],
+            ctypes.c_int,
+        ),
+        "hst_grouped_weight_grad": (
+            [_i32, _ptr, _i64, _ptr, _i64, _ptr, _i32, _ptr, _i64, _i64, _i64, _ptr, _size, _ptr],
+            ctypes.c_int,
+        ),
+        "hst_matmul_blockscaled": (
+            [_i32, _ptr, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _i32, _ptr,
+             _i64, _i64, _i64, _ptr, _size, _ptr],
+            ctypes.c_int,
+        ),
+        "hst_quantize_e4m3": (
+            [_i32, _i32, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _ptr],
             ctypes.c_int,
         ),
         "hst_matmul_split_k_noalloc": (

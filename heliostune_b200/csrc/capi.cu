@@ -20,16 +20,18 @@
 #include "gemm_stream.cuh"
 #include "gemm_stream_cluster.cuh"
 #include "gemm_tile.cuh"
+#include "host.h"
 #include "rmsnorm.cuh"
 
 namespace hst {
-namespace {
 
 // ------------------------------------------------------------------------------------------
 // Errors
 // ------------------------------------------------------------------------------------------
 
+namespace {
 thread_local std::string t_error;
+}
 
 int fail(int code, const char* fmt, ...) {
   char buf[512];
@@ -41,37 +43,16 @@ int fail(int code, const char* fmt, ...) {
   return code;
 }
 
-#define HST_CUDA(call)                                                                   \
-  do {                                                                                   \
-    cudaError_t err_ = (call);                                                           \
-    if (err_ != cudaSuccess)                                                             \
-      return fail(HST_ERR_CUDA, "%s failed: %s", #call, cudaGetErrorString(err_));       \
-  } while (0)
-
-#define HST_TRY(call)          \
-  do {                                \
-    int rc_ = (call);                 \
-    if (rc_ != HST_OK) return rc_;    \
-  } while (0)
-
 // ------------------------------------------------------------------------------------------
 // Per-device state
 // ------------------------------------------------------------------------------------------
 
+namespace {
 __device__ int g_status_word;  // OR of StatusBits raised by kernels on this device
 
-constexpr int kMaxDevices = 64;
-constexpr int kMaxDynamicSmem = 232448;  // 227 KB per CTA on sm_100
-constexpr int kSmemPerSm = 233472;       // 228 KB per SM
-constexpr int kSmemReservedPerCta = 1024;
-
-struct DeviceState {
-  std::atomic<bool> ready{false};
-  int sm_count = 0;
-  int* status = nullptr;
-};
 DeviceState g_devices[kMaxDevices];
 std::mutex g_device_mutex;
+}  // namespace
 
 int device_state(DeviceState** out) {
   int dev = 0;
@@ -90,19 +71,7 @@ int device_state(DeviceState** out) {
   return HST_OK;
 }
 
-// Raises the dynamic shared-memory limit of a kernel once per device.
-template <typename Kernel>
-int allow_smem(Kernel kernel, std::atomic<uint64_t>& done_mask) {
-  int dev = 0;
-  HST_CUDA(cudaGetDevice(&dev));
-  const uint64_t bit = 1ull << dev;
-  if (!(done_mask.load(std::memory_order_acquire) & bit)) {
-    HST_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  kMaxDynamicSmem));
-    done_mask.fetch_or(bit, std::memory_order_release);
-  }
-  return HST_OK;
-}
+namespace {
 
 // Dynamic shared memory to request so that co-resident CTAs never ask for more than the SM's
 // 512 TMEM columns in total (tcgen05.alloc would otherwise stall a CTA until another exits).
@@ -121,9 +90,10 @@ PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 std::once_flag g_encode_once;
 cudaError_t g_encode_error = cudaSuccess;
 
-int encode_tiled_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
-                    uint64_t row_stride_elems, uint32_t box_inner, uint32_t box_outer,
-                    CUtensorMapDataType type = CU_TENSOR_MAP_DATA_TYPE_FLOAT16) {
+}  // namespace
+
+int encode_tiled(CUtensorMap* map, CUtensorMapDataType type, uint32_t rank, const void* base,
+                 const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box) {
   std::call_once(g_encode_once, [] {
     cudaDriverEntryPointQueryResult q;
     g_encode_error = cudaGetDriverEntryPointByVersion(
@@ -137,30 +107,45 @@ int encode_tiled_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t
     return fail(HST_ERR_CUDA, "cuTensorMapEncodeTiled unavailable: %s",
                 cudaGetErrorString(g_encode_error));
   }
-  const cuuint64_t dims[2] = {inner, outer};
-  const cuuint64_t strides[1] = {row_stride_elems * 2};
-  const cuuint32_t box[2] = {box_inner, box_outer};
-  const cuuint32_t elem_strides[2] = {1, 1};
-  const CUresult r = g_encode(map, type, 2, const_cast<void*>(base),
-                              dims, strides, box, elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const cuuint32_t elem_strides[3] = {1, 1, 1};
+  auto encode = [&] {
+    return g_encode(map, type, rank, const_cast<void*>(base), dims, strides_bytes, box,
+                    elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    // A thread (autograd's) that has not used the runtime yet: cudaSetDevice makes the current
+    // device's primary context its own.
+    int dev = 0;
+    HST_CUDA(cudaGetDevice(&dev));
+    HST_CUDA(cudaSetDevice(dev));
+    r = encode();
+  }
   if (r != CUDA_SUCCESS) {
     return fail(HST_ERR_CUDA,
-                "cuTensorMapEncodeTiled failed (%d): dims %llu x %llu, row stride %llu, box %u x %u",
-                static_cast<int>(r), static_cast<unsigned long long>(inner),
-                static_cast<unsigned long long>(outer),
-                static_cast<unsigned long long>(row_stride_elems), box_inner, box_outer);
+                "cuTensorMapEncodeTiled failed (%d): dims %llu x %llu, row stride %llu bytes, box %u x %u",
+                static_cast<int>(r), static_cast<unsigned long long>(dims[0]),
+                static_cast<unsigned long long>(dims[1]),
+                static_cast<unsigned long long>(strides_bytes[0]), box[0], box[1]);
   }
   return HST_OK;
+}
+
+namespace {
+
+int encode_tiled_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
+                    uint64_t row_stride_elems, uint32_t box_inner, uint32_t box_outer,
+                    CUtensorMapDataType type = CU_TENSOR_MAP_DATA_TYPE_FLOAT16) {
+  const uint64_t dims[2] = {inner, outer};
+  const uint64_t strides[1] = {row_stride_elems * 2};
+  const uint32_t box[2] = {box_inner, box_outer};
+  return encode_tiled(map, type, 2, base, dims, strides, box);
 }
 
 // ------------------------------------------------------------------------------------------
 // Operand layouts
 // ------------------------------------------------------------------------------------------
-
-int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
-int64_t round_up(int64_t a, int64_t b) { return cdiv(a, b) * b; }
 
 // A row-major view [rows, cols] with element strides (s0, s1).
 struct View {

@@ -1,0 +1,358 @@
+// C ABI of the grouped and block-scaled products and of the quantisers: argument checks, tensor
+// maps, workspace sizes and the choice of kernel. See include/heliostune_b200.h.
+#include <algorithm>
+
+#include "gemm_grouped.cuh"
+#include "host.h"
+#include "quantize.cuh"
+
+namespace hst {
+namespace {
+
+constexpr int64_t kMaxExtent = INT32_MAX / 2;
+
+// What the host knows of one grouped product.
+struct GroupedProblem {
+  int64_t rows;      // T
+  int groups;
+  int64_t cols;      // output columns
+  int64_t lrows;     // kWeightGrad: rows of one output
+  int64_t k_blocks;  // forward, scaled
+  int width_cap;
+};
+
+// Rows on the R side of a kScaledStream tile: the epilogue keeps that many FP32 sums a thread.
+constexpr int kStreamWidth = 64;
+
+int check_groups(const char* what, int64_t rows, int32_t groups, const void* ends) {
+  if (groups < 1 || groups > kMaxGroups)
+    return fail(HST_ERR_INVALID, "%s serves 1 to %d groups, got %d", what, kMaxGroups, groups);
+  if (ends == nullptr && groups != 1) return fail(HST_ERR_INVALID, "group ends are null");
+  if (rows < 0 || rows > kMaxExtent) return fail(HST_ERR_INVALID, "%s: bad row count %lld", what, (long long)rows);
+  return HST_OK;
+}
+
+int check_extents(const char* what, int64_t a, int64_t b) {
+  if (a < 0 || b < 0 || a > kMaxExtent || b > kMaxExtent)
+    return fail(HST_ERR_INVALID, "%s: bad extents %lld, %lld", what, (long long)a, (long long)b);
+  return HST_OK;
+}
+
+// A row-major operand TMA can read: 16-byte aligned base and strides, rows no shorter than `cols`.
+int check_operand(const char* what, const void* p, int64_t ld, int64_t cols, int64_t elem) {
+  if (p == nullptr) return fail(HST_ERR_INVALID, "%s is null", what);
+  if ((reinterpret_cast<uintptr_t>(p) & 15) != 0 || ld * elem % 16 != 0 || ld < cols)
+    return fail(HST_ERR_INVALID, "%s must be row-major with 16-byte aligned rows of at least %lld values", what,
+                (long long)cols);
+  return HST_OK;
+}
+
+template <GroupMode MODE>
+int64_t max_iterations(const GroupedProblem& p) {
+  const int64_t cols = cdiv(p.cols, 256);
+  if (MODE == GroupMode::kWeightGrad) return cols * cdiv(p.lrows, 256) * (p.rows / 64 + p.groups);
+  const int64_t tiles = group_rows_on_r(MODE) ? p.rows / p.width_cap + p.groups : p.rows / 256 + p.groups;
+  return cols * std::min(tiles, p.rows) * p.k_blocks;
+}
+
+// Iterations a share has at least: below it, joining a tile's pieces costs more than another pair
+// saves.
+constexpr int kMinBlocks = 4;
+
+template <GroupMode MODE>
+int plan_pairs(const GroupedProblem& p, int sms) {
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms / 2, max_iterations<MODE>(p) / kMinBlocks)));
+}
+
+template <GroupMode MODE>
+int piece_floats(const GroupedProblem& p) {
+  return 128 * (group_rows_on_r(MODE) ? p.width_cap : 256);
+}
+
+template <GroupMode MODE>
+size_t workspace_bytes(const GroupedProblem& p, int sms) {
+  return static_cast<size_t>(plan_pairs<MODE>(p, sms)) * 4 * piece_floats<MODE>(p) * sizeof(float);
+}
+
+int width_cap(int64_t rows, int most) { return static_cast<int>(std::min<int64_t>(most, round_up(std::max<int64_t>(rows, 1), 32))); }
+
+// The two launches of one product. `maps` and the operand fields of `args` are set by the caller.
+template <GroupMode MODE, bool L_MN, typename T>
+int launch_grouped(const GroupedProblem& p, const GroupedMaps& maps, GroupedArgs args, int r_bytes, void* workspace,
+                   size_t workspace_size, cudaStream_t stream) {
+  using S = GroupedShape<MODE>;
+  DeviceState* dev = nullptr;
+  HST_TRY(device_state(&dev));
+  if (max_iterations<MODE>(p) > INT32_MAX) return fail(HST_ERR_UNSUPPORTED, "the grouped product has too many tiles");
+  const size_t need = workspace_bytes<MODE>(p, dev->sm_count);
+  if (workspace_size < need || workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)
+    return fail(HST_ERR_WORKSPACE, "workspace of %zu bytes, 16-byte aligned, needed; got %zu", need, workspace_size);
+  args.groups = p.groups;
+  args.rows = static_cast<int>(p.rows);
+  args.cols = static_cast<int>(p.cols);
+  args.lrows = static_cast<int>(p.lrows);
+  args.k_blocks = static_cast<int>(p.k_blocks);
+  args.width_cap = p.width_cap;
+  args.r_bytes = r_bytes;
+  args.pairs = plan_pairs<MODE>(p, dev->sm_count);
+  args.min_blocks = kMinBlocks;
+  args.vec = (p.cols % 16 == 0) && (reinterpret_cast<uintptr_t>(args.out) % 32 == 0);
+  args.status = dev->status;
+  args.partials = static_cast<float*>(workspace);
+  args.piece_floats = piece_floats<MODE>(p);
+  int stages = kMaxStages;
+  while (stages > 2 && S::smem_bytes(stages, r_bytes, p.groups) > kMaxDynamicSmem) --stages;
+  args.stages = stages;
+  if (p.rows > 0) {
+    static std::atomic<uint64_t> smem_done{0};
+    HST_TRY(allow_smem(grouped_gemm_kernel<MODE, L_MN, T>, smem_done));
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3(static_cast<unsigned>(2 * args.pairs));
+    lc.blockDim = dim3(group_threads(MODE));
+    lc.dynamicSmemBytes = S::smem_bytes(stages, r_bytes, p.groups);
+    lc.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    lc.attrs = attr;
+    lc.numAttrs = 1;
+    HST_CUDA(cudaLaunchKernelEx(&lc, grouped_gemm_kernel<MODE, L_MN, T>, maps, args));
+  }
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3(static_cast<unsigned>(std::max(1, args.pairs - 1)), 2, kFinishChunks);
+  lc.blockDim = dim3(kFinishThreads);
+  lc.dynamicSmemBytes = static_cast<size_t>(p.groups + 1) * 8;
+  lc.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  lc.attrs = attr;
+  lc.numAttrs = p.rows > 0 ? 1 : 0;
+  HST_CUDA(cudaLaunchKernelEx(&lc, grouped_finish_kernel<MODE, T>, args));
+  return HST_OK;
+}
+
+// A row matrix [rows, cols] of `elem`-byte values in boxes of 128 bytes x `box_rows`.
+int encode_rows(CUtensorMap* map, CUtensorMapDataType type, int64_t elem, const void* base, int64_t rows, int64_t cols,
+                int64_t ld, int box_rows) {
+  const uint64_t dims[2] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(rows)};
+  const uint64_t strides[1] = {static_cast<uint64_t>(ld * elem)};
+  const uint32_t box[2] = {static_cast<uint32_t>(128 / elem), static_cast<uint32_t>(box_rows)};
+  return encode_tiled(map, type, 2, base, dims, strides, box);
+}
+
+// Weights [groups, outer, inner].
+int encode_weights(CUtensorMap* map, CUtensorMapDataType type, int64_t elem, const void* base, int64_t groups,
+                   int64_t outer, int64_t inner, int64_t stride, int64_t ld, int box_rows) {
+  const uint64_t dims[3] = {static_cast<uint64_t>(inner), static_cast<uint64_t>(outer), static_cast<uint64_t>(groups)};
+  if (groups == 1) stride = outer * ld;  // not used; the map wants one
+  const uint64_t strides[2] = {static_cast<uint64_t>(ld * elem), static_cast<uint64_t>(stride * elem)};
+  const uint32_t box[3] = {static_cast<uint32_t>(128 / elem), static_cast<uint32_t>(box_rows), 1};
+  return encode_tiled(map, type, 3, base, dims, strides, box);
+}
+
+CUtensorMapDataType map_type(int32_t dtype) {
+  return dtype == HST_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+}
+
+int box_rows_of(int index) { return 128 >> index; }
+
+int zero_output(void* out, int64_t values, cudaStream_t stream) {
+  if (values > 0) HST_CUDA(cudaMemsetAsync(out, 0, static_cast<size_t>(values) * 2, stream));
+  return HST_OK;
+}
+
+GroupedProblem forward_problem(int64_t rows, int groups, int64_t n, int64_t k) {
+  return GroupedProblem{rows, groups, n, 0, cdiv(k, 64), width_cap(rows, 256)};
+}
+GroupedProblem grad_problem(int64_t rows, int groups, int64_t lcols, int64_t rcols) {
+  return GroupedProblem{rows, groups, rcols, lcols, 0, 256};
+}
+// Few rows a group: the weights stream past on the L side. From 64 rows a group on average the wide
+// form's cheaper promotion pays for the part of its 256-row tiles that stays empty.
+bool scaled_streams(int64_t rows, int groups) { return rows <= static_cast<int64_t>(kStreamWidth) * groups; }
+GroupedProblem scaled_problem(int64_t rows, int groups, int64_t n, int64_t k) {
+  return GroupedProblem{rows, groups, n, 0, cdiv(k, 128), width_cap(rows, kStreamWidth)};
+}
+
+}  // namespace
+}  // namespace hst
+
+using namespace hst;
+
+extern "C" {
+
+int hst_grouped_workspace_size(int32_t op, int64_t rows, int32_t groups, int64_t n, int64_t k, int device,
+                               size_t* bytes) {
+  if (bytes == nullptr) return fail(HST_ERR_INVALID, "bytes is null");
+  if (groups < 1 || groups > kMaxGroups || rows < 0 || n < 0 || k < 0 || rows > kMaxExtent || n > kMaxExtent || k > kMaxExtent)
+    return fail(HST_ERR_INVALID, "bad grouped product");
+  int sms = 0;
+  HST_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+  switch (op) {
+    case HST_GROUPED_FORWARD:
+      *bytes = workspace_bytes<GroupMode::kForward>(forward_problem(rows, groups, n, k), sms);
+      return HST_OK;
+    case HST_GROUPED_WEIGHT_GRAD:
+      *bytes = workspace_bytes<GroupMode::kWeightGrad>(grad_problem(rows, groups, k, n), sms);
+      return HST_OK;
+    case HST_GROUPED_SCALED: {
+      const GroupedProblem p = scaled_problem(rows, groups, n, k);
+      *bytes = scaled_streams(rows, groups) ? workspace_bytes<GroupMode::kScaledStream>(p, sms)
+                                            : workspace_bytes<GroupMode::kScaledWide>(p, sms);
+      return HST_OK;
+    }
+    default:
+      return fail(HST_ERR_INVALID, "unknown grouped product %d", op);
+  }
+}
+
+int hst_grouped_matmul(int32_t dtype, const void* x, int64_t ldx, const void* w, int64_t w_group, int64_t ldw,
+                       int32_t w_layout, const int32_t* ends, int32_t groups, void* y, int64_t rows, int64_t n,
+                       int64_t k, void* workspace, size_t workspace_bytes, void* stream) {
+  if (dtype != HST_F16 && dtype != HST_BF16) return fail(HST_ERR_INVALID, "unknown data type %d", dtype);
+  if (w_layout != HST_WEIGHT_KN && w_layout != HST_WEIGHT_NK) return fail(HST_ERR_INVALID, "unknown weight layout %d", w_layout);
+  HST_TRY(check_groups("the grouped matmul", rows, groups, ends));
+  HST_TRY(check_extents("the grouped matmul", n, k));
+  if (rows == 0 || n == 0) return HST_OK;
+  if (y == nullptr) return fail(HST_ERR_INVALID, "y is null");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (k == 0) return zero_output(y, rows * n, s);
+  const bool kn = w_layout == HST_WEIGHT_KN;
+  const int64_t outer = kn ? k : n, inner = kn ? n : k;
+  HST_TRY(check_operand("x", x, ldx, k, 2));
+  HST_TRY(check_operand("w", w, ldw, inner, 2));
+  if (groups > 1 && (w_group % 8 != 0 || w_group < 8)) return fail(HST_ERR_INVALID, "w's group stride must be a positive multiple of 8");
+  const GroupedProblem p = forward_problem(rows, groups, n, k);
+  GroupedMaps maps = {};
+  HST_TRY(encode_weights(&maps.l, map_type(dtype), 2, w, groups, outer, inner, w_group, ldw, kn ? 64 : 128));
+  for (int i = 0; i < 4; ++i) HST_TRY(encode_rows(&maps.r[i], map_type(dtype), 2, x, rows, k, ldx, box_rows_of(i)));
+  GroupedArgs args = {};
+  args.ends = ends;
+  args.out = y;
+  const int r_bytes = box_rows_of(group_box(p.width_cap / 2)) * 128;
+#define HST_GROUPED_CASE(KN_, DT_, T_) \
+  if (kn == KN_ && dtype == DT_)       \
+    return launch_grouped<GroupMode::kForward, KN_, T_>(p, maps, args, r_bytes, workspace, workspace_bytes, s);
+  HST_GROUPED_CASE(true, HST_F16, __half)
+  HST_GROUPED_CASE(false, HST_F16, __half)
+  HST_GROUPED_CASE(true, HST_BF16, __nv_bfloat16)
+  HST_GROUPED_CASE(false, HST_BF16, __nv_bfloat16)
+#undef HST_GROUPED_CASE
+  return HST_ERR_UNSUPPORTED;
+}
+
+int hst_grouped_weight_grad(int32_t dtype, const void* left, int64_t ldl, const void* right, int64_t ldr,
+                            const int32_t* ends, int32_t groups, void* out, int64_t rows, int64_t lcols,
+                            int64_t rcols, void* workspace, size_t workspace_bytes, void* stream) {
+  if (dtype != HST_F16 && dtype != HST_BF16) return fail(HST_ERR_INVALID, "unknown data type %d", dtype);
+  HST_TRY(check_groups("the grouped weight gradient", rows, groups, ends));
+  HST_TRY(check_extents("the grouped weight gradient", lcols, rcols));
+  if (lcols == 0 || rcols == 0) return HST_OK;
+  if (out == nullptr) return fail(HST_ERR_INVALID, "out is null");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (rows == 0) return zero_output(out, lcols * rcols * groups, s);
+  HST_TRY(check_operand("left", left, ldl, lcols, 2));
+  HST_TRY(check_operand("right", right, ldr, rcols, 2));
+  const GroupedProblem p = grad_problem(rows, groups, lcols, rcols);
+  GroupedMaps maps = {};
+  HST_TRY(encode_rows(&maps.l, map_type(dtype), 2, left, rows, lcols, ldl, 64));
+  HST_TRY(encode_rows(&maps.r[0], map_type(dtype), 2, right, rows, rcols, ldr, 64));
+  GroupedArgs args = {};
+  args.ends = ends;
+  args.out = out;
+  if (dtype == HST_F16)
+    return launch_grouped<GroupMode::kWeightGrad, true, __half>(p, maps, args, 16384, workspace, workspace_bytes, s);
+  return launch_grouped<GroupMode::kWeightGrad, true, __nv_bfloat16>(p, maps, args, 16384, workspace, workspace_bytes, s);
+}
+
+int hst_matmul_blockscaled(int32_t out_dtype, const void* a, int64_t lda, const float* a_scales, int64_t sa_row,
+                           int64_t sa_block, const void* b, int64_t b_group, int64_t ldb, const float* b_scales,
+                           int64_t sb_group, int64_t sb_row, int64_t sb_block, const int32_t* ends, int32_t groups,
+                           void* y, int64_t rows, int64_t n, int64_t k, void* workspace, size_t workspace_bytes,
+                           void* stream) {
+  if (out_dtype != HST_F16 && out_dtype != HST_BF16) return fail(HST_ERR_INVALID, "unknown data type %d", out_dtype);
+  HST_TRY(check_groups("the block-scaled matmul", rows, groups, ends));
+  HST_TRY(check_extents("the block-scaled matmul", n, k));
+  if (rows == 0 || n == 0) return HST_OK;
+  if (y == nullptr) return fail(HST_ERR_INVALID, "y is null");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (k == 0) return zero_output(y, rows * n, s);
+  HST_TRY(check_operand("a", a, lda, k, 1));
+  HST_TRY(check_operand("b", b, ldb, k, 1));
+  if (a_scales == nullptr || b_scales == nullptr) return fail(HST_ERR_INVALID, "scales are null");
+  if (groups > 1 && (b_group % 16 != 0 || b_group < 16)) return fail(HST_ERR_INVALID, "b's group stride must be a positive multiple of 16");
+  const bool streams = scaled_streams(rows, groups);
+  const GroupedProblem p = scaled_problem(rows, groups, n, k);
+  const CUtensorMapDataType type = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  GroupedMaps maps = {};
+  if (streams) {
+    HST_TRY(encode_weights(&maps.l, type, 1, b, groups, n, k, b_group, ldb, 128));
+    for (int i = 0; i < 4; ++i) HST_TRY(encode_rows(&maps.r[i], type, 1, a, rows, k, lda, box_rows_of(i)));
+  } else {
+    HST_TRY(encode_rows(&maps.l, type, 1, a, rows, k, lda, 128));
+    for (int i = 0; i < 4; ++i) HST_TRY(encode_weights(&maps.r[i], type, 1, b, groups, n, k, b_group, ldb, box_rows_of(i)));
+  }
+  GroupedArgs args = {};
+  args.ends = ends;
+  args.out = y;
+  args.row_scales = a_scales;
+  args.rs_row = sa_row;
+  args.rs_k = sa_block;
+  args.tile_scales = b_scales;
+  args.ts_group = sb_group;
+  args.ts_n = sb_row;
+  args.ts_k = sb_block;
+  const int r_bytes = streams ? box_rows_of(group_box(p.width_cap / 2)) * 128 : 16384;
+#define HST_SCALED_CASE(DT_, T_)                                                                                       \
+  if (out_dtype == DT_) {                                                                                              \
+    if (streams)                                                                                                       \
+      return launch_grouped<GroupMode::kScaledStream, false, T_>(p, maps, args, r_bytes, workspace, workspace_bytes, s); \
+    return launch_grouped<GroupMode::kScaledWide, false, T_>(p, maps, args, r_bytes, workspace, workspace_bytes, s);   \
+  }
+  HST_SCALED_CASE(HST_F16, __half)
+  HST_SCALED_CASE(HST_BF16, __nv_bfloat16)
+#undef HST_SCALED_CASE
+  return HST_ERR_UNSUPPORTED;
+}
+
+int hst_quantize_e4m3(int32_t dtype, int32_t tiles, const void* x, int64_t x_batch, int64_t x_row, int64_t x_col,
+                      void* q, int64_t q_batch, int64_t q_row, float* scales, int64_t s_batch, int64_t s_row,
+                      int64_t s_col, int64_t batch, int64_t rows, int64_t cols, void* stream) {
+  if (dtype != HST_F16 && dtype != HST_BF16) return fail(HST_ERR_INVALID, "unknown data type %d", dtype);
+  HST_TRY(check_extents("the quantiser", rows, cols));
+  if (batch < 0 || batch > 65535) return fail(HST_ERR_INVALID, "the quantiser serves at most 65535 matrices");
+  if (!tiles && batch > 1) return fail(HST_ERR_INVALID, "row scales are for one matrix");
+  if (rows == 0 || cols == 0 || batch == 0) return HST_OK;
+  if (x == nullptr || q == nullptr || scales == nullptr) return fail(HST_ERR_INVALID, "null pointer");
+  if (q_row < cols) return fail(HST_ERR_INVALID, "q's rows are shorter than its columns");
+  const int64_t col_blocks = cdiv(cols, 128), row_blocks = cdiv(rows, 128);
+  if (rows * col_blocks > INT32_MAX || (tiles && row_blocks > 65535))
+    return fail(HST_ERR_UNSUPPORTED, "the quantiser's matrix is too large");
+  QuantizeArgs a = {x, x_batch, x_row, x_col, static_cast<uint8_t*>(q), q_batch, q_row, scales, s_batch, s_row, s_col,
+                    static_cast<int>(rows), static_cast<int>(cols), static_cast<int>(col_blocks)};
+  const bool vec = (x_col == 1 || cols == 1) && cols % 8 == 0 && x_row % 8 == 0 && x_batch % 8 == 0 && q_row % 8 == 0 &&
+                   q_batch % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (reinterpret_cast<uintptr_t>(q) & 7) == 0;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (tiles) {
+    const dim3 grid(static_cast<unsigned>(col_blocks), static_cast<unsigned>(row_blocks), static_cast<unsigned>(batch));
+    if (vec && dtype == HST_F16) quantize_tiles_kernel<__half><<<grid, kQuantThreads, 0, st>>>(a);
+    else if (vec) quantize_tiles_kernel<__nv_bfloat16><<<grid, kQuantThreads, 0, st>>>(a);
+    else if (dtype == HST_F16) quantize_tiles_any_kernel<__half><<<grid, kQuantThreads, 0, st>>>(a);
+    else quantize_tiles_any_kernel<__nv_bfloat16><<<grid, kQuantThreads, 0, st>>>(a);
+  } else {
+    const int64_t units = rows * col_blocks;
+    const unsigned vec_grid = static_cast<unsigned>(cdiv(units, kQuantThreads / 16 * kQuantUnroll));
+    const unsigned any_grid = static_cast<unsigned>(cdiv(units, kQuantThreads / 32));
+    if (vec && dtype == HST_F16) quantize_rows_kernel<__half><<<vec_grid, kQuantThreads, 0, st>>>(a);
+    else if (vec) quantize_rows_kernel<__nv_bfloat16><<<vec_grid, kQuantThreads, 0, st>>>(a);
+    else if (dtype == HST_F16) quantize_rows_any_kernel<__half><<<any_grid, kQuantThreads, 0, st>>>(a);
+    else quantize_rows_any_kernel<__nv_bfloat16><<<any_grid, kQuantThreads, 0, st>>>(a);
+  }
+  HST_CUDA(cudaGetLastError());
+  return HST_OK;
+}
+
+}  // extern "C"

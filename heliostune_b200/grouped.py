@@ -1,0 +1,192 @@
+"""Matrix products over rows grouped by expert, with their gradients (mixture-of-experts layers).
+
+The rows of ``x [T, K]`` are sorted by expert; ``group_ends [E]`` (int32, on the GPU) holds each
+expert's end, so expert ``e`` owns rows ``group_ends[e - 1]`` to ``group_ends[e]``::
+
+    y = grouped_matmul(x, weight, group_ends)      # y[t] = x[t] @ weight[e(t)], weight [E, K, N]
+
+``weight`` may also be the transposed view of ``[E, N, K]`` storage (``nn.Linear``'s): both are read
+in place. The result is differentiable in ``x`` and ``weight``: ``dx[t] = dy[t] @ weight[e(t)].T`` is
+the same kernel on the transposed view, ``dweight[e] = x[e].T @ dy[e]`` its own
+(:func:`grouped_weight_grad`).
+
+Nothing is read back from the GPU: the sizes stay there, and a call can be captured into a CUDA
+graph and replayed with other ends. Rows past the last end belong to no expert: their outputs and
+input gradients are zero, and they enter no weight gradient. An expert without rows gets a zero
+weight gradient. Each end is taken clamped to ``[previous end, T]``.
+
+The heliostune reference has no counterpart (its products have one weight).
+"""
+
+from __future__ import annotations
+
+import ctypes
+import functools
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from heliostune_b200 import _native
+from heliostune_b200.kernel import _device_guard, _stream
+
+#: Most experts one call serves.
+MAX_GROUPS = 1024
+
+_DTYPES = {torch.float16: _native.HST_F16, torch.bfloat16: _native.HST_BF16}
+
+
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(op: int, rows: int, groups: int, n: int, k: int, device: int) -> int:
+    size = ctypes.c_size_t(0)
+    _native.check(_native.library().hst_grouped_workspace_size(op, rows, groups, n, k, device, ctypes.byref(size)))
+    return size.value
+
+
+def _workspace(op: int, rows: int, groups: int, n: int, k: int, device: torch.device) -> torch.Tensor:
+    """The FP32 pieces of tiles shared between CTA pairs; a tensor of this call alone."""
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    return torch.empty(_workspace_bytes(op, rows, groups, n, k, index), device=device, dtype=torch.uint8)
+
+
+def _aligned_rows(t: torch.Tensor) -> bool:
+    """Whether a tensor map can describe ``t`` (2-D, or 3-D with one matrix per group): unit stride
+    in the last dimension, the others multiples of 16 bytes that do not overlap, and the base too."""
+    unit = 16 // t.element_size()
+    if t.data_ptr() % 16 != 0 or (t.shape[-1] > 1 and t.stride(-1) != 1):
+        return False
+    if t.shape[-2] > 1 and (t.stride(-2) % unit != 0 or t.stride(-2) < t.shape[-1]):
+        return False
+    if t.ndim == 3 and t.shape[0] > 1:
+        return t.stride(0) % unit == 0 and t.stride(0) >= _row_stride(t) * t.shape[1]
+    return True
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    unit = 16 // t.element_size()
+    return t.stride(-2) if t.shape[-2] > 1 else -(-t.shape[-1] // unit) * unit
+
+
+def _readable(t: torch.Tensor) -> torch.Tensor:
+    """``t``, or a copy with 16-byte aligned rows where a tensor map cannot describe it."""
+    if _aligned_rows(t):
+        return t
+    unit = 16 // t.element_size()
+    width = -(-t.shape[-1] // unit) * unit
+    padded = torch.empty((*t.shape[:-1], width), device=t.device, dtype=t.dtype)[..., : t.shape[-1]]
+    return padded.copy_(t)
+
+
+def _check_ends(group_ends: torch.Tensor, groups: int, device: torch.device) -> None:
+    if group_ends.ndim != 1 or group_ends.shape[0] != groups:
+        raise ValueError(f"group_ends must have one entry for each of {groups} weights, got {tuple(group_ends.shape)}")
+    if group_ends.dtype != torch.int32:
+        raise ValueError("group_ends must have dtype torch.int32")
+    if group_ends.device != device:
+        raise ValueError("group_ends must be on the device of the operands")
+    if not group_ends.is_contiguous():
+        raise ValueError("group_ends must be contiguous")
+
+
+def _check_operands(what: str, x: torch.Tensor, other: torch.Tensor, names: tuple[str, str]) -> None:
+    if x.device.type != "cuda" or other.device != x.device:
+        raise ValueError(f"{names[0]} and {names[1]} must be on the same CUDA device")
+    if x.dtype not in _DTYPES or other.dtype != x.dtype:
+        raise ValueError(f"{what} serves torch.float16 or torch.bfloat16, the same for {names[0]} and {names[1]}")
+
+
+def _forward(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tensor) -> torch.Tensor:
+    groups, k, n = (int(v) for v in weight.shape)
+    rows = int(x.shape[0])
+    y = torch.empty((rows, n), device=x.device, dtype=x.dtype)
+    x = _readable(x)
+    # The layout whose last dimension is contiguous; a weight with neither is copied.
+    transposed = weight.transpose(1, 2)
+    if not _aligned_rows(weight) and _aligned_rows(transposed):
+        layout, stored = _native.HST_WEIGHT_NK, transposed
+    elif weight.stride(1) == 1 and weight.stride(2) != 1:
+        layout, stored = _native.HST_WEIGHT_NK, _readable(transposed)
+    else:
+        layout, stored = _native.HST_WEIGHT_KN, _readable(weight)
+    workspace = _workspace(_native.GROUPED_FORWARD, rows, groups, n, k, x.device)
+    with _device_guard(x.device):
+        _native.check(
+            _native.library().hst_grouped_matmul(
+                _DTYPES[x.dtype], x.data_ptr(), _row_stride(x), stored.data_ptr(), stored.stride(0),
+                _row_stride(stored), layout, group_ends.data_ptr(), groups, y.data_ptr(), rows, n, k,
+                workspace.data_ptr(), workspace.numel(), _stream(x.device),
+            )
+        )  # fmt: skip
+    return y
+
+
+def _weight_grad(left: torch.Tensor, right: torch.Tensor, group_ends: torch.Tensor) -> torch.Tensor:
+    groups, rows = int(group_ends.shape[0]), int(left.shape[0])
+    lcols, rcols = int(left.shape[1]), int(right.shape[1])
+    out = torch.empty((groups, lcols, rcols), device=left.device, dtype=left.dtype)
+    left, right = _readable(left), _readable(right)
+    workspace = _workspace(_native.GROUPED_WEIGHT_GRAD, rows, groups, rcols, lcols, left.device)
+    with _device_guard(left.device):
+        _native.check(
+            _native.library().hst_grouped_weight_grad(
+                _DTYPES[left.dtype], left.data_ptr(), _row_stride(left), right.data_ptr(), _row_stride(right),
+                group_ends.data_ptr(), groups, out.data_ptr(), rows, lcols, rcols, workspace.data_ptr(),
+                workspace.numel(), _stream(left.device),
+            )
+        )  # fmt: skip
+    return out
+
+
+def grouped_weight_grad(x: torch.Tensor, dy: torch.Tensor, group_ends: torch.Tensor) -> torch.Tensor:
+    """``out[e] = x[rows of e].T @ dy[rows of e]``, ``[E, K, N]``: the weight gradient of
+    :func:`grouped_matmul`, with FP32 sums over the rows and one rounding. ``x [T, K]`` and ``dy [T, N]``
+    are FP16 or BF16 with any strides (copied once where their rows are not 16-byte aligned)."""
+    if x.ndim != 2 or dy.ndim != 2 or x.shape[0] != dy.shape[0]:
+        raise ValueError(f"grouped_weight_grad expects x [T, K] and dy [T, N], got {tuple(x.shape)} and {tuple(dy.shape)}")
+    _check_operands("grouped_weight_grad", x, dy, ("x", "dy"))
+    groups = int(group_ends.shape[0]) if group_ends.ndim == 1 else 0
+    if not 1 <= groups <= MAX_GROUPS:
+        raise ValueError(f"grouped_weight_grad serves 1 to {MAX_GROUPS} experts, got {groups}")
+    _check_ends(group_ends, groups, x.device)
+    if torch.is_grad_enabled() and (x.requires_grad or dy.requires_grad):
+        raise ValueError("grouped_weight_grad has no gradient; detach its inputs")
+    return _weight_grad(x, dy, group_ends)
+
+
+class _GroupedMatmul(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, group_ends):  # type: ignore[no-untyped-def]
+        ctx.save_for_backward(x, weight, group_ends)
+        return _forward(x, weight, group_ends)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):  # type: ignore[no-untyped-def]
+        x, weight, group_ends = ctx.saved_tensors
+        dx = dweight = None
+        if ctx.needs_input_grad[0]:
+            dx = _forward(dy, weight.transpose(1, 2), group_ends)
+        if ctx.needs_input_grad[1]:
+            if weight.stride(1) == 1 and weight.stride(2) != 1:
+                # [E, N, K] storage: the gradient in the same layout, so that it adds up in place.
+                dweight = _weight_grad(dy, x, group_ends).transpose(1, 2)
+            else:
+                dweight = _weight_grad(x, dy, group_ends)
+        return dx, dweight, None
+
+
+def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tensor) -> torch.Tensor:
+    """``y[t] = x[t] @ weight[e(t)]`` with FP32 accumulation: ``x [T, K]``, ``weight [E, K, N]`` (either of
+    its last two dimensions contiguous), both FP16 or both BF16, ``y [T, N]`` of their type; 1 to
+    :data:`MAX_GROUPS` experts. Any strides are served; operands whose rows are not 16-byte aligned
+    are copied once. Differentiable in ``x`` and ``weight`` (once)."""
+    if x.ndim != 2 or weight.ndim != 3:
+        raise ValueError("grouped_matmul expects x [T, K] and weight [E, K, N]")
+    if x.shape[1] != weight.shape[1]:
+        raise ValueError(f"incompatible shapes: x {tuple(x.shape)} and weight {tuple(weight.shape)}")
+    _check_operands("grouped_matmul", x, weight, ("x", "weight"))
+    if not 1 <= weight.shape[0] <= MAX_GROUPS:
+        raise ValueError(f"grouped_matmul serves 1 to {MAX_GROUPS} experts, got {weight.shape[0]}")
+    _check_ends(group_ends, int(weight.shape[0]), x.device)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        return _GroupedMatmul.apply(x, weight, group_ends)
+    return _forward(x, weight, group_ends)

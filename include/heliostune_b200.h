@@ -178,6 +178,67 @@ int hst_gated_mlp_stream(int32_t block_m, int32_t block_k, int32_t num_stages, i
                          const void* w_up, int64_t ld_up, void* out, int64_t ldo, int64_t m,
                          int64_t n, int64_t k, void* stream);
 
+/* Data types of the grouped products and the quantisers. */
+#define HST_F16 0
+#define HST_BF16 1
+
+/* Layout of one group's weight: [k, n] or [n, k], its last dimension contiguous. */
+#define HST_WEIGHT_KN 0
+#define HST_WEIGHT_NK 1
+
+/* Products over rows grouped by expert (no reference counterpart). Group g owns rows
+ * [ends[g - 1], ends[g]) (ends[-1] = 0) of a row matrix; `ends` is int32 on the GPU and read there,
+ * so nothing is known of the sizes on the host. Each end is taken clamped to [previous end, rows]:
+ * no value leads out of the matrices. 1 to 1024 groups; a null `ends` with one group is all rows.
+ * Operands: 16-byte aligned bases and strides. Outputs are contiguous and written whole: rows past
+ * the last group, and the weight gradients of groups without rows, are zero. FP32 accumulation, one
+ * rounding, bitwise reproducible. The caller gives a 16-byte aligned workspace of
+ * hst_grouped_workspace_size bytes (no initialisation needed); calls that share one must not overlap
+ * on the GPU. Each product is two launches on the stream and can be captured. */
+#define HST_GROUPED_FORWARD 0      /* hst_grouped_matmul: n, k */
+#define HST_GROUPED_WEIGHT_GRAD 1  /* hst_grouped_weight_grad: n = rcols, k = lcols */
+#define HST_GROUPED_SCALED 2       /* hst_matmul_blockscaled: n, k */
+int hst_grouped_workspace_size(int32_t op, int64_t rows, int32_t groups, int64_t n, int64_t k,
+                               int device, size_t* bytes);
+
+/* y[t, :] = x[t, :] W[g(t)]: x [rows, k] (row stride ldx), w [groups, k, n] or [groups, n, k]
+ * (w_layout; group stride w_group, row stride ldw), y [rows, n], all of `dtype`. The input
+ * gradient is the same call with dy for x and the other layout. */
+int hst_grouped_matmul(int32_t dtype, const void* x, int64_t ldx, const void* w, int64_t w_group,
+                       int64_t ldw, int32_t w_layout, const int32_t* ends, int32_t groups, void* y,
+                       int64_t rows, int64_t n, int64_t k, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/* out[g] = left[rows of g]^T right[rows of g]: left [rows, lcols], right [rows, rcols], out
+ * [groups, lcols, rcols], all of `dtype`. The weight gradient of hst_grouped_matmul. */
+int hst_grouped_weight_grad(int32_t dtype, const void* left, int64_t ldl, const void* right,
+                            int64_t ldr, const int32_t* ends, int32_t groups, void* out, int64_t rows,
+                            int64_t lcols, int64_t rcols, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* y[t, j] = sum over blocks c of 128 values of k: a_scales[t, c] * b_scales[g, j / 128, c] *
+ * sum over the block of a[t, i] * b[g, j, i]. a [rows, k] and b [groups, n, k] E4M3, FP32 scales
+ * with the strides given (elements), y [rows, n] of out_dtype. The block sums and their scaled sum
+ * are FP32. For a plain product pass one group and a null `ends`. */
+int hst_matmul_blockscaled(int32_t out_dtype, const void* a, int64_t lda, const float* a_scales,
+                           int64_t sa_row, int64_t sa_block, const void* b, int64_t b_group,
+                           int64_t ldb, const float* b_scales, int64_t sb_group, int64_t sb_row,
+                           int64_t sb_block, const int32_t* ends, int32_t groups, void* y,
+                           int64_t rows, int64_t n, int64_t k, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* E4M3 with FP32 scales: for every block amax = max(max |x|, 2^-100), scale = amax / 448 and
+ * q = e4m3(x * (448 / amax)), the quotients and the product rounded to FP32, q to nearest even.
+ * A block is 128 consecutive values of a row (tiles = 0, one matrix) or 128 x 128 values of a
+ * matrix (tiles = 1, `batch` matrices); blocks at the edges are shorter. x [batch, rows, cols] of
+ * `dtype` with any strides, q with unit column stride, scales [batch, rows or rows / 128,
+ * cols / 128] (rounded up) with any strides. Infinity or NaN in a block makes its scale infinite or
+ * NaN. */
+int hst_quantize_e4m3(int32_t dtype, int32_t tiles, const void* x, int64_t x_batch, int64_t x_row,
+                      int64_t x_col, void* q, int64_t q_batch, int64_t q_row, float* scales,
+                      int64_t s_batch, int64_t s_row, int64_t s_col, int64_t batch, int64_t rows,
+                      int64_t cols, void* stream);
+
 /* Peer writes of hst_matmul_pair_fanout: coalesced 16-byte stores from the epilogue warps, or
  * one TMA tensor store per peer of each staged sub-tile. */
 #define HST_PEER_STORES 0

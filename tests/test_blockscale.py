@@ -1,0 +1,391 @@
+"""The E4M3 quantisers and the block-scaled products (``blockscale``) against their formulas.
+
+Quantisers: bit for bit against the same FP32 formula on the CPU. Products: against 64-bit sums of the
+same 8-bit operands. A product of two E4M3 values has 8 significant bits, exact in FP32; a block's sum of 128
+of them and the scaled sum over the blocks are off by at most one unit (2^-23) of the sum of magnitudes at
+each step, the scale's own product by half of one: ``(128 + blocks + 2) * 2^-23 * sum |a||b| sa sb``, and the
+output by ``eps / 2``.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from heliostune_b200 import _native, blockscale, grouped
+from tests.test_grouped import _bounds, _ends
+
+gpu = pytest.mark.gpu
+DTYPES = (torch.float16, torch.bfloat16)
+
+
+@pytest.fixture(autouse=True)
+def _status(request: pytest.FixtureRequest):  # type: ignore[no-untyped-def]
+    yield
+    if request.node.get_closest_marker("gpu") and torch.cuda.is_available():
+        assert _native.status(torch.cuda.current_device()) == 0
+
+
+def _quantize_cpu(x: torch.Tensor, tiles: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """The formula on the CPU, block by block."""
+    x = x.detach().cpu().float()
+    rows, cols = x.shape
+    high = 128 if tiles else 1
+    q = torch.empty((rows, cols), dtype=torch.float8_e4m3fn)
+    scales = torch.empty((-(-rows // high), -(-cols // 128)))
+    for i in range(scales.shape[0]):
+        for j in range(scales.shape[1]):
+            at = (slice(i * high, (i + 1) * high), slice(j * 128, (j + 1) * 128))
+            amax = x[at].abs().max().clamp(min=2.0**-100)
+            most = torch.tensor(448.0)  # a tensor: torch takes 448.0 / amax as 448.0 * (1 / amax)
+            scales[i, j] = amax / most
+            q[at] = (x[at] * (most / amax)).clamp(-448.0, 448.0).to(torch.float8_e4m3fn)
+    return q, scales
+
+
+def _same_bits(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Equal values, NaN where the other has NaN."""
+    a, b = a.detach().float().cpu(), b.detach().float().cpu()
+    return a.shape == b.shape and bool(((a == b) | (a.isnan() & b.isnan())).all())
+
+
+def _dequantize(q: torch.Tensor, s: torch.Tensor, tiles: bool) -> torch.Tensor:
+    s = s.double().repeat_interleave(128, -1)[..., : q.shape[-1]]
+    if tiles:
+        s = s.repeat_interleave(128, -2)[..., : q.shape[-2], :]
+    return q.double() * s
+
+
+def _assert_product(y: torch.Tensor, a: torch.Tensor, b: torch.Tensor) -> None:
+    """``y`` against ``a @ b.T`` for the dequantised operands in 64 bits."""
+    exact, magnitude = a @ b.T, a.abs() @ b.abs().T
+    half_step = torch.finfo(y.dtype).eps / 2
+    slack = (128 + -(-a.shape[1] // 128) + 2) * 2.0**-23 * magnitude
+    bound = half_step * exact.abs() + (1 + half_step) * slack + 2.0**-25
+    error = (y.double() - exact).abs()
+    assert y.shape == exact.shape
+    assert bool((error <= bound).all()), ((error - bound).max().item(), error.max().item())
+
+
+def _operands(rows: int, n: int, k: int, seed: int, groups: int = 0):  # type: ignore[no-untyped-def]
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn((rows, k), generator=g, device="cuda") * torch.exp(torch.randn((rows, 1), generator=g, device="cuda"))
+    shape = (groups, n, k) if groups else (n, k)
+    w = torch.randn(shape, generator=g, device="cuda") / k**0.5
+    a, sa = blockscale.quantize_rows(x.bfloat16())
+    b, sb = blockscale.quantize_tiles(w.bfloat16())
+    return a, sa, b, sb
+
+
+# ------------------------------------------------------------------------------------------
+# Refusals, before any CUDA work
+# ------------------------------------------------------------------------------------------
+
+
+def test_inputs_are_checked_before_any_cuda_work() -> None:
+    a = torch.zeros((4, 128), dtype=torch.float8_e4m3fn)
+    s = torch.zeros((4, 1))
+    with pytest.raises(ValueError, match=r"a \[T, K\]"):
+        blockscale.matmul_blockscaled(a[0], s, a, s[:1])
+    with pytest.raises(ValueError, match=r"a \[T, K\]"):
+        blockscale.matmul_blockscaled(a, s, a, s[:1], torch.zeros(1, dtype=torch.int32))
+    with pytest.raises(ValueError, match="incompatible shapes"):
+        blockscale.matmul_blockscaled(a, s, a[:, :64], s[:1])
+    with pytest.raises(ValueError, match="same CUDA device"):
+        blockscale.matmul_blockscaled(a, s, a, s[:1])
+    with pytest.raises(ValueError, match=r"x \[T, K\]"):
+        blockscale.quantize_rows(s[0])
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        blockscale.quantize_rows(s)
+    with pytest.raises(ValueError, match=r"weight \[N, K\]"):
+        blockscale.quantize_tiles(s[0])
+
+
+def test_the_library_refuses_bad_calls_before_any_cuda_work() -> None:
+    _native.build_library()
+    lib = _native.library()
+
+    def scaled(out=0, a=16, lda=128, sa=16, b=16, stride=1024, ldb=128, sb=16, ends=16, groups=2, y=16, rows=4, n=8, k=128):  # type: ignore[no-untyped-def]
+        return lib.hst_matmul_blockscaled(
+            out, a, lda, sa, 1, 1, b, stride, ldb, sb, 1, 1, 1, ends, groups, y, rows, n, k, None, 0, None
+        )
+
+    for kwargs, message in (
+        ({"out": 3}, b"data type"),
+        ({"groups": 0}, b"1 to 1024"),
+        ({"ends": None}, b"ends are null"),
+        ({"k": -1}, b"extents"),
+        ({"a": 17}, b"a must be"),
+        ({"lda": 120}, b"a must be"),
+        ({"ldb": 64}, b"b must be"),
+        ({"sa": None}, b"scales"),
+        ({"stride": 8}, b"group stride"),
+        ({"y": None}, b"y is null"),
+    ):
+        assert scaled(**kwargs) == _native.HST_ERR_INVALID, kwargs
+        assert message in lib.hst_last_error(), kwargs
+
+    def quantize(dtype=0, tiles=0, x=16, q=16, q_row=128, s=16, batch=1, rows=4, cols=128):  # type: ignore[no-untyped-def]
+        return lib.hst_quantize_e4m3(dtype, tiles, x, 0, 128, 1, q, 0, q_row, s, 0, 1, 1, batch, rows, cols, None)
+
+    for kwargs, message in (
+        ({"dtype": 2}, b"data type"),
+        ({"rows": -1}, b"extents"),
+        ({"batch": 2}, b"one matrix"),
+        ({"tiles": 1, "batch": 65536}, b"65535"),
+        ({"x": None}, b"null"),
+        ({"q_row": 127}, b"shorter"),
+    ):
+        assert quantize(**kwargs) == _native.HST_ERR_INVALID, kwargs
+        assert message in lib.hst_last_error(), kwargs
+    assert quantize(rows=0) == _native.HST_OK
+
+
+# ------------------------------------------------------------------------------------------
+# Quantisers
+# ------------------------------------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tiles", (False, True))
+@pytest.mark.parametrize("rows,cols", ((1, 1), (1, 128), (3, 129), (128, 128), (130, 264), (257, 1000), (5, 4096), (129, 77)))
+def test_quantisers_match_the_formula(dtype: torch.dtype, tiles: bool, rows: int, cols: int) -> None:
+    g = torch.Generator(device="cuda").manual_seed(rows * cols)
+    x = (torch.randn((rows, cols), generator=g, device="cuda") * torch.exp(2 * torch.randn((rows, 1), generator=g, device="cuda"))).to(dtype)
+    q, s = (blockscale.quantize_tiles if tiles else blockscale.quantize_rows)(x)
+    expected_q, expected_s = _quantize_cpu(x, tiles)
+    assert q.dtype == torch.float8_e4m3fn and s.dtype == torch.float32
+    assert _same_bits(s, expected_s) and _same_bits(q, expected_q)
+    # And what they stand for: half a step of E4M3 (2^-4 of the value, or half of the least step, 2^-10, of the scale).
+    exact = x.double()
+    off = (_dequantize(q, s, tiles) - exact).abs()
+    scale = _dequantize(torch.ones_like(exact), s, tiles)
+    assert bool((off <= exact.abs() * 2.0**-4 * (1 + 1e-6) + scale * 2.0**-10 * (1 + 1e-6)).all())
+
+
+@gpu
+@pytest.mark.parametrize("tiles", (False, True))
+@pytest.mark.parametrize("cols", (256, 250))  # vector and general loads
+def test_quantisers_at_the_ends_of_the_range(tiles: bool, cols: int) -> None:
+    quantize = blockscale.quantize_tiles if tiles else blockscale.quantize_rows
+    for dtype in DTYPES:
+        least = torch.finfo(dtype).smallest_normal
+        for values in (
+            [0.0], [-0.0], [least], [least / 4, 0.0], [torch.finfo(dtype).max], [1.0, -3.0, 448.0], [17.0, 0.0, 448.0, 18.0],
+            [float("inf"), 1.0], [float("-inf"), float("nan")], [float("nan")], [1e-6, 5.0],
+        ):  # fmt: skip
+            x = torch.zeros((2, cols), device="cuda", dtype=dtype)
+            x[0, : len(values)] = torch.tensor(values, dtype=dtype)
+            x[1, 130 : 130 + len(values)] = torch.tensor(values, dtype=dtype)
+            q, s = quantize(x)
+            expected_q, expected_s = _quantize_cpu(x, tiles)
+            # A maximum over a block with NaN is NaN in both.
+            assert _same_bits(s, expected_s), (dtype, values)
+            assert _same_bits(q, expected_q), (dtype, values)
+
+
+@gpu
+def test_quantisers_take_any_strides_and_stacks() -> None:
+    g = torch.Generator(device="cuda").manual_seed(1)
+    base = torch.randn((3, 200, 320), generator=g, device="cuda").half()
+    for x in (base[0].T, base[1, ::2], base[1, :, ::3], base[0, :, 1:130], base[2, 5:6].expand(9, 320), base[:, 7, :]):
+        for tiles, quantize in ((False, blockscale.quantize_rows), (True, blockscale.quantize_tiles)):
+            q, s = quantize(x)
+            expected_q, expected_s = _quantize_cpu(x, tiles)
+            assert _same_bits(s, expected_s) and _same_bits(q, expected_q)
+    for stack in (base, base.transpose(1, 2), base[:, ::2], base[:, :, 3:141]):
+        q, s = blockscale.quantize_tiles(stack)
+        for i in range(3):
+            expected_q, expected_s = _quantize_cpu(stack[i], True)
+            assert _same_bits(s[i], expected_s) and _same_bits(q[i], expected_q)
+    for empty in (base[0, :0], base[0, :, :0]):
+        for quantize in (blockscale.quantize_rows, blockscale.quantize_tiles):
+            q, s = quantize(empty)
+            assert q.shape == empty.shape and s.numel() == 0
+
+
+# ------------------------------------------------------------------------------------------
+# Products
+# ------------------------------------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("out_dtype", DTYPES)
+@pytest.mark.parametrize("rows", (1, 2, 31, 33, 64, 65, 127, 128, 200, 256, 257, 600))
+@pytest.mark.parametrize("n,k", ((128, 128), (136, 264), (520, 1040), (72, 4096), (1000, 16)))
+def test_dense(out_dtype: torch.dtype, rows: int, n: int, k: int) -> None:
+    a, sa, b, sb = _operands(rows, n, k, seed=rows + n + k)
+    y = blockscale.matmul_blockscaled(a, sa, b, sb, out_dtype=out_dtype)
+    assert y.dtype == out_dtype
+    _assert_product(y, _dequantize(a, sa, False), _dequantize(b, sb, True))
+
+
+@gpu
+@pytest.mark.parametrize("rows", (1, 40, 300))
+@pytest.mark.parametrize("n,k", ((1, 1), (17, 13), (129, 129), (130, 1001)))
+def test_extents_and_strides_that_tma_cannot_read(rows: int, n: int, k: int) -> None:
+    a, sa, b, sb = _operands(rows, n, k, seed=rows + n + k)
+    expected = _dequantize(a, sa, False), _dequantize(b, sb, True)
+    forms = [(a, sa, b, sb), (a.contiguous(), sa.contiguous(), b.contiguous(), sb.T.contiguous().T)]
+    wide = torch.zeros((rows, k + 7), device="cuda", dtype=torch.uint8)
+    wide[:, 3 : 3 + k] = a.view(torch.uint8) if a.is_contiguous() else a.contiguous().view(torch.uint8)
+    forms.append((wide.view(torch.float8_e4m3fn)[:, 3 : 3 + k], sa, b.T.contiguous().T, sb))
+    spread = torch.zeros((rows * 2, sa.shape[1] * 3), device="cuda")
+    spread[::2, ::3] = sa
+    forms.append((a, spread[::2, ::3], b, sb))
+    for form in forms:
+        _assert_product(blockscale.matmul_blockscaled(*form), *expected)
+
+
+@gpu
+@pytest.mark.parametrize(
+    "rows,ends",
+    ((1, [0, 1]), (9, [3, 3, 8]), (96, [40, 41, 96]), (300, [0, 255, 255, 300]), (700, [256, 513, 700]), (40, [0, 0, 0]), (1111, [600, 600, 1100])),
+)
+@pytest.mark.parametrize("n,k", ((136, 264), (520, 1040)))
+def test_grouped(rows: int, ends: list[int], n: int, k: int) -> None:
+    a, sa, b, sb = _operands(rows, n, k, seed=rows + n, groups=len(ends))
+    y = blockscale.matmul_blockscaled(a, sa, b, sb, _ends(ends), out_dtype=torch.float16)
+    last = 0
+    da, db = _dequantize(a, sa, False), _dequantize(b, sb, True)
+    for e, (start, end) in enumerate(_bounds(ends, rows)):
+        _assert_product(y[start:end], da[start:end], db[e])
+        last = end
+    assert bool((y[last:] == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("rows", (40, 400))
+def test_nan_and_infinity_stay_in_their_rows_and_columns(rows: int) -> None:
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.randn((rows, 300), generator=g, device="cuda").bfloat16()
+    w = (torch.randn((200, 300), generator=g, device="cuda") / 17).bfloat16()
+    x[3, 140] = float("inf")
+    x[rows - 1, 299] = float("nan")
+    w[150, 7] = float("nan")
+    a, sa = blockscale.quantize_rows(x)
+    b, sb = blockscale.quantize_tiles(w)
+    y = blockscale.matmul_blockscaled(a, sa, b, sb)
+    bad = torch.zeros((rows, 200), dtype=torch.bool, device="cuda")
+    bad[3] = bad[rows - 1] = True
+    bad[:, 128:] = True  # the scale of the tile that holds the NaN
+    assert torch.equal(~torch.isfinite(y), bad)
+
+
+@gpu
+def test_groups_keep_to_their_rows_next_to_nan() -> None:
+    ends = [37, 120, 250]
+    a, sa, b, sb = _operands(260, 136, 264, seed=3, groups=3)
+    clean = blockscale.matmul_blockscaled(a, sa, b, sb, _ends(ends))
+    sa = sa.clone()
+    sa[37:120] = float("nan")
+    sa[250:] = float("nan")
+    y = blockscale.matmul_blockscaled(a, sa, b, sb, _ends(ends))
+    assert bool(torch.isnan(y[37:120]).all())
+    y[37:120] = clean[37:120]
+    assert torch.equal(y, clean)
+
+
+@gpu
+def test_empty_extents_and_refusals() -> None:
+    a, sa, b, sb = _operands(8, 136, 256, seed=4)
+    assert blockscale.matmul_blockscaled(a[:0], sa[:0], b, sb).shape == (0, 136)
+    assert blockscale.matmul_blockscaled(a, sa, b[:0], sb[:0]).shape == (8, 0)
+    assert bool((blockscale.matmul_blockscaled(a[:, :0], sa[:, :0], b[:, :0], sb[:, :0]) == 0).all())
+    for args, message in (
+        ((a.float(), sa, b, sb), "float8_e4m3fn"),
+        ((a, sa[:, :1], b, sb), "a_scales must have shape"),
+        ((a, sa, b, sb[:1]), "b_scales must have shape"),
+        ((a, sa.double(), b, sb), "float32"),
+        ((a, sa.cpu(), b, sb), "on the device"),
+        ((a, sa.clone().requires_grad_(), b, sb), "no gradient"),
+    ):
+        with pytest.raises(ValueError, match=message):
+            blockscale.matmul_blockscaled(*args)
+    with pytest.raises(ValueError, match="out_dtype"):
+        blockscale.matmul_blockscaled(a, sa, b, sb, out_dtype=torch.float32)
+    with pytest.raises(ValueError, match="no gradient"):
+        blockscale.quantize_rows(torch.zeros((2, 128), device="cuda", dtype=torch.float16, requires_grad=True))
+    with pytest.raises(ValueError, match="float16 or torch.bfloat16"):
+        blockscale.quantize_tiles(torch.zeros((2, 128), device="cuda"))
+
+
+@gpu
+@pytest.mark.parametrize("rows", (3, 700))
+def test_captured_and_concurrent_calls(rows: int) -> None:
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn((rows, 1040), generator=g, device="cuda").bfloat16()
+    w = (torch.randn((520, 1040), generator=g, device="cuda") / 32).bfloat16()
+    b, sb = blockscale.quantize_tiles(w)
+
+    def step() -> torch.Tensor:
+        return blockscale.matmul_blockscaled(*blockscale.quantize_rows(x), b, sb)
+
+    expected = step()
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    results = []
+    for i in range(8):
+        with torch.cuda.stream(streams[i % 2]):
+            results.append(step())
+    torch.cuda.synchronize()
+    assert all(torch.equal(expected, y) for y in results)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = step()
+    for _ in range(3):
+        x.mul_(-1.5)
+        graph.replay()
+        assert torch.equal(y, step())
+
+
+# ------------------------------------------------------------------------------------------
+# Together
+# ------------------------------------------------------------------------------------------
+
+
+@gpu
+def test_an_expert_layer_trained_in_16_bits_and_served_in_8() -> None:
+    """Tokens routed to two of four experts: the layer in 16 bits with its gradients, then the same weights
+    quantised. Against the 64-bit layer; the 8-bit one against the 64-bit layer of its own operands."""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    tokens, experts, hidden, inner = 70, 4, 264, 392
+    x = torch.randn((tokens, hidden), generator=g, device="cuda").bfloat16().requires_grad_()
+    up = (torch.randn((experts, inner, hidden), generator=g, device="cuda") / hidden**0.5).bfloat16().requires_grad_()
+    down = (torch.randn((experts, hidden, inner), generator=g, device="cuda") / inner**0.5).bfloat16().requires_grad_()
+    choice = torch.randn((tokens, experts), generator=g, device="cuda").topk(2).indices.reshape(-1)
+    order = torch.argsort(choice, stable=True)
+    ends = torch.cumsum(torch.bincount(choice, minlength=experts), 0).to(torch.int32)
+    source = order // 2
+    bounds = _bounds(ends.tolist(), 2 * tokens)
+
+    def layer(rows, first, second, product):  # type: ignore[no-untyped-def]
+        h = torch.relu(product(rows, first))
+        return torch.zeros((tokens, hidden), device="cuda", dtype=h.dtype).index_add(0, source, product(h, second))
+
+    y = layer(x[source], up, down, lambda a, w: grouped.grouped_matmul(a, w.transpose(1, 2), ends))
+    y.sum().backward()
+    leaves = [t.detach().double().requires_grad_() for t in (x, up, down)]
+    exact = layer(leaves[0][source], leaves[1], leaves[2], lambda a, w: torch.cat([a[s:e] @ w[i].T for i, (s, e) in enumerate(bounds)]))
+    exact.sum().backward()
+    # Norms: each of the layer's BF16 roundings is off by at most 2^-8 of its value; a value passes at most
+    # three of them forward (h, product, sum) and five on the way back, and where a rounding moves h across zero, relu's
+    # share follows continuously.
+    for got, want, steps in ((y, exact, 3), *((a.grad, b.grad, 8) for a, b in zip((x, up, down), leaves, strict=True))):
+        assert (got.double() - want).norm() <= steps * 2.0**-8 * want.norm()
+
+    w8 = [blockscale.quantize_tiles(w.detach()) for w in (up, down)]
+    with torch.no_grad():
+        rows = x.detach()[source]
+        a, sa = blockscale.quantize_rows(rows)
+        h = blockscale.matmul_blockscaled(a, sa, *w8[0], ends)
+        for i, (s, e) in enumerate(bounds):
+            _assert_product(h[s:e], _dequantize(a, sa, False)[s:e], _dequantize(*w8[0], True)[i])
+        a, sa = blockscale.quantize_rows(torch.relu(h))
+        out = blockscale.matmul_blockscaled(a, sa, *w8[1], ends)
+        for i, (s, e) in enumerate(bounds):
+            _assert_product(out[s:e], _dequantize(a, sa, False)[s:e], _dequantize(*w8[1], True)[i])
+        served = torch.zeros((tokens, hidden), device="cuda").index_add(0, source, out.float())
+    # Four operands rounded to E4M3 (2^-4 of the value each at most, independent signs).
+    assert (served.double() - exact).norm() <= 4 * 2.0**-4 * exact.norm()

@@ -1,0 +1,410 @@
+"""The products over rows grouped by expert (``grouped.grouped_matmul``, ``grouped_weight_grad``) against
+the same sums in 64 bits.
+
+Tolerance: one rounding to the output type, at most ``eps / 2`` of the value, and the FP32 sum of ``K``
+exact products, each step of which is off by at most one unit in the last place (2^-23) of the sum of
+magnitudes so far: ``K * 2^-23 * sum |a||b|``. FP16 results below 2^-14 are off by up to half a
+subnormal step, 2^-25.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from heliostune_b200 import _native, grouped
+
+gpu = pytest.mark.gpu
+DTYPES = (torch.float16, torch.bfloat16)
+
+
+@pytest.fixture(autouse=True)
+def _status(request: pytest.FixtureRequest):  # type: ignore[no-untyped-def]
+    yield
+    if request.node.get_closest_marker("gpu") and torch.cuda.is_available():
+        assert _native.status(torch.cuda.current_device()) == 0
+
+
+def _bounds(ends: list[int], rows: int) -> list[tuple[int, int]]:
+    """The rows of each group as the operators take them: every end clamped to [previous end, rows]."""
+    out, start = [], 0
+    for end in ends:
+        end = max(start, min(max(end, 0), rows))
+        out.append((start, end))
+        start = end
+    return out
+
+
+def _assert_close(out: torch.Tensor, exact: torch.Tensor, magnitude: torch.Tensor, terms: int) -> None:
+    assert out.shape == exact.shape
+    half_step = torch.finfo(out.dtype).eps / 2
+    slack = (terms + 1) * 2.0**-23 * magnitude
+    bound = half_step * exact.abs() + (1 + half_step) * slack + 2.0**-25
+    error = (out.double() - exact).abs()
+    assert bool((error <= bound).all()), ((error - bound).max().item(), error.max().item())
+
+
+def _check_forward(y: torch.Tensor, x: torch.Tensor, w: torch.Tensor, ends: list[int]) -> None:
+    covered = 0
+    for e, (start, end) in enumerate(_bounds(ends, x.shape[0])):
+        a, b = x[start:end].double(), w[e].double()
+        _assert_close(y[start:end], a @ b, a.abs() @ b.abs(), x.shape[1])
+        covered = end
+    assert bool((y[covered:] == 0).all())
+
+
+def _check_weight_grad(dw: torch.Tensor, x: torch.Tensor, dy: torch.Tensor, ends: list[int]) -> None:
+    for e, (start, end) in enumerate(_bounds(ends, x.shape[0])):
+        a, b = x[start:end].double().T, dy[start:end].double()
+        _assert_close(dw[e], a @ b, a.abs() @ b.abs(), end - start)
+        if start == end:
+            assert bool((dw[e] == 0).all())
+
+
+def _operands(rows: int, groups: int, k: int, n: int, dtype: torch.dtype, layout: str, seed: int):  # type: ignore[no-untyped-def]
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn((rows, k), generator=g, device="cuda").to(dtype)
+    shape = (groups, k, n) if layout == "kn" else (groups, n, k)
+    w = (torch.randn(shape, generator=g, device="cuda") / max(k, 1) ** 0.5).to(dtype)
+    dy = torch.randn((rows, n), generator=g, device="cuda").to(dtype)
+    return x, w if layout == "kn" else w.transpose(1, 2), dy
+
+
+def _ends(values: list[int]) -> torch.Tensor:
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+# ------------------------------------------------------------------------------------------
+# Refusals, before any CUDA work
+# ------------------------------------------------------------------------------------------
+
+
+def test_inputs_are_checked_before_any_cuda_work() -> None:
+    x = torch.zeros((4, 16), dtype=torch.float16)
+    w = torch.zeros((2, 16, 8), dtype=torch.float16)
+    ends = torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match=r"x \[T, K\]"):
+        grouped.grouped_matmul(x[0], w, ends)
+    with pytest.raises(ValueError, match="incompatible shapes"):
+        grouped.grouped_matmul(x[:, :8], w, ends)
+    with pytest.raises(ValueError, match="same CUDA device"):
+        grouped.grouped_matmul(x, w, ends)
+    with pytest.raises(ValueError, match=r"x \[T, K\] and dy"):
+        grouped.grouped_weight_grad(x, x[:3], ends)
+    with pytest.raises(ValueError, match="same CUDA device"):
+        grouped.grouped_weight_grad(x, x, ends)
+
+
+def test_the_library_refuses_bad_calls_before_any_cuda_work() -> None:
+    _native.build_library()
+    lib = _native.library()
+
+    def matmul(dtype=0, layout=0, groups=2, rows=4, n=8, k=16, x=16, ldx=16, w=16, stride=128, ldw=8, ends=16, y=16):  # type: ignore[no-untyped-def]
+        return lib.hst_grouped_matmul(dtype, x, ldx, w, stride, ldw, layout, ends, groups, y, rows, n, k, None, 0, None)
+
+    for kwargs, message in (
+        ({"dtype": 7}, b"data type"),
+        ({"layout": 2}, b"layout"),
+        ({"groups": 0}, b"1 to 1024"),
+        ({"groups": 1025}, b"1 to 1024"),
+        ({"ends": None}, b"ends are null"),
+        ({"rows": -1}, b"row count"),
+        ({"n": -1}, b"extents"),
+        ({"y": None}, b"y is null"),
+        ({"x": 8}, b"x must be"),
+        ({"ldx": 12}, b"x must be"),
+        ({"ldx": 8}, b"x must be"),
+        ({"w": None}, b"w is null"),
+        ({"ldw": 4}, b"w must be"),
+        ({"stride": 0}, b"group stride"),
+        ({"stride": 12}, b"group stride"),
+    ):
+        assert matmul(**kwargs) == _native.HST_ERR_INVALID, kwargs
+        assert message in lib.hst_last_error(), kwargs
+    assert matmul(rows=0) == _native.HST_OK
+    assert lib.hst_grouped_weight_grad(0, 16, 12, 16, 8, 16, 2, 16, 4, 16, 8, None, 0, None) == _native.HST_ERR_INVALID
+    assert b"left must be" in lib.hst_last_error()
+
+
+# ------------------------------------------------------------------------------------------
+# Values
+# ------------------------------------------------------------------------------------------
+
+#: (rows, ends): one row; tile edges of 32, 256 and their neighbours; empty groups first, last and between;
+#: rows past the last end; all groups empty.
+ROWS = (
+    (1, [1]),
+    (1, [0, 1, 1]),
+    (7, [3, 3, 7]),
+    (96, [32, 63, 96]),
+    (300, [0, 255, 255, 300]),
+    (700, [256, 513, 700]),
+    (530, [1, 2, 259, 500]),
+    (40, [0, 0, 0]),
+    (1111, [600, 600, 1100]),
+)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ("kn", "nk"))
+@pytest.mark.parametrize("rows,ends", ROWS)
+@pytest.mark.parametrize("k,n", ((64, 256), (200, 264), (1000, 72)))
+def test_forward_and_gradients(dtype: torch.dtype, layout: str, rows: int, ends: list[int], k: int, n: int) -> None:
+    x, w, dy = _operands(rows, len(ends), k, n, dtype, layout, seed=rows + k)
+    x.requires_grad_()
+    w = w.detach().requires_grad_()
+    y = grouped.grouped_matmul(x, w, _ends(ends))
+    assert y.dtype == dtype
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    x, w = x.detach(), w.detach()
+    _check_forward(y.detach(), x, w, ends)
+    _check_forward(dx, dy, w.transpose(1, 2), ends)
+    _check_weight_grad(dw, x, dy, ends)
+    assert dw.stride() == w.stride()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ("kn", "nk"))
+@pytest.mark.parametrize("k,n", ((1, 1), (13, 17), (65, 7), (8, 1001)))
+def test_extents_that_tma_cannot_read(dtype: torch.dtype, layout: str, k: int, n: int) -> None:
+    ends = [5, 5, 40, 70]
+    x, w, dy = _operands(75, 4, k, n, dtype, layout, seed=k * n)
+    _check_forward(grouped.grouped_matmul(x, w, _ends(ends)), x, w, ends)
+    _check_forward(grouped.grouped_matmul(dy, w.transpose(1, 2), _ends(ends)), dy, w.transpose(1, 2), ends)
+    _check_weight_grad(grouped.grouped_weight_grad(x, dy, _ends(ends)), x, dy, ends)
+
+
+@gpu
+def test_long_sums_and_many_tiles_are_joined_across_pairs() -> None:
+    ends = [40, 41, 300]
+    x, w, dy = _operands(300, 3, 4104, 520, torch.bfloat16, "kn", seed=3)
+    _check_forward(grouped.grouped_matmul(x, w, _ends(ends)), x, w, ends)
+    ends = [5000, 5003, 9000]
+    x, w, dy = _operands(9001, 3, 136, 520, torch.float16, "nk", seed=4)
+    _check_weight_grad(grouped.grouped_weight_grad(x, dy, _ends(ends)), x, dy, ends)
+    _check_forward(grouped.grouped_matmul(x, w, _ends(ends)), x, w, ends)
+
+
+@gpu
+def test_many_groups() -> None:
+    groups = grouped.MAX_GROUPS
+    counts = torch.randint(0, 4, (groups,), generator=torch.Generator().manual_seed(1))
+    ends = torch.cumsum(counts, 0).tolist()
+    x, w, dy = _operands(ends[-1] + 2, groups, 64, 40, torch.float16, "kn", seed=5)
+    _check_forward(grouped.grouped_matmul(x, w, _ends(ends)), x, w, ends)
+    _check_weight_grad(grouped.grouped_weight_grad(x, dy, _ends(ends)), x, dy, ends)
+
+
+@gpu
+@pytest.mark.parametrize("ends", ([50, 20, 90], [-5, 30, 1000], [2**31 - 1, 0, 10], [-1, -2, -3], [20, -(2**31), 60]))
+def test_ends_out_of_order_or_range_are_clamped(ends: list[int]) -> None:
+    x, w, dy = _operands(80, 3, 72, 48, torch.float16, "kn", seed=6)
+    _check_forward(grouped.grouped_matmul(x, w, _ends(ends)), x, w, ends)
+    _check_weight_grad(grouped.grouped_weight_grad(x, dy, _ends(ends)), x, dy, ends)
+
+
+@gpu
+@pytest.mark.parametrize("poison", (float("nan"), float("inf")))
+def test_what_stands_in_other_rows_stays_out(poison: float) -> None:
+    """Groups end inside 16-row steps and 64-row blocks; the rows of group 1 and past the last group hold
+    NaN or infinity in both operands."""
+    ends = [37, 37 + 75, 37 + 75 + 130]
+    rows = ends[-1] + 9
+    x, w, dy = _operands(rows, 3, 264, 136, torch.bfloat16, "kn", seed=7)
+    bad = slice(ends[0], ends[1])
+    clean = x.clone(), dy.clone()
+    for t in (x, dy):
+        t[bad] = poison
+        t[ends[2] :] = poison
+    y = grouped.grouped_matmul(x, w, _ends(ends))
+    dw = grouped.grouped_weight_grad(x, dy, _ends(ends))
+    assert not bool(torch.isfinite(y[bad]).any()) and not bool(torch.isfinite(dw[1]).any())
+    y[bad] = 0
+    assert bool(torch.isfinite(y).all()) and bool((y[ends[2] :] == 0).all())
+    expected = grouped.grouped_weight_grad(*clean, _ends(ends))
+    assert torch.equal(dw[0], expected[0]) and torch.equal(dw[2], expected[2])
+
+
+@gpu
+def test_strides_views_and_broadcasts() -> None:
+    ends = [33, 70, 100]
+    g = torch.Generator(device="cuda").manual_seed(8)
+    wide = torch.randn((100, 3 * 80), generator=g, device="cuda").half()
+    w = (torch.randn((3, 64, 80), generator=g, device="cuda") / 8).half()
+    for x in (wide[:, 80:144], wide[:, 3:67], wide.T.contiguous().T[:, 8:72], wide[:, ::3][:, :64], wide[0, :64].expand(100, 64)):
+        _check_forward(grouped.grouped_matmul(x, w, _ends(ends)), x, w, ends)
+        _check_weight_grad(grouped.grouped_weight_grad(x, wide[:, :24], _ends(ends)), x, wide[:, :24], ends)
+    x = wide[:, :64]
+    for v in (w[1].expand(3, 64, 80), w[:, :, ::2], w.flip(0)[:, :, 8:40], w[:, :, 1:9], w.permute(1, 0, 2).contiguous().permute(1, 0, 2)):
+        _check_forward(grouped.grouped_matmul(x, v, _ends(ends)), x, v, ends)
+    # One weight broadcast to every expert and a loss that sums: both gradients are sums of shared entries.
+    one = w[:1].detach().requires_grad_()
+    leaf = x.detach().clone().requires_grad_()
+    grouped.grouped_matmul(leaf, one.expand(3, 64, 80), _ends(ends)).sum().backward()
+    exact = x.double().sum(0)[:, None].expand(64, 80)
+    # Three rounded gradients of the experts, then their rounded sum: at most four half steps of the magnitudes.
+    bound = 4 * 2.0**-11 * x.double().abs().sum(0)[:, None]
+    assert bool(((one.grad[0].double() - exact).abs() <= bound).all())
+    exact = w[0].double().sum(1)
+    _assert_close(leaf.grad, exact.expand(100, 64), w[0].double().abs().sum(1).expand(100, 64), 80)
+
+
+@gpu
+def test_empty_extents() -> None:
+    ends = _ends([2, 4])
+    x, w, dy = _operands(4, 2, 16, 24, torch.float16, "kn", seed=9)
+    assert grouped.grouped_matmul(x[:0], w, ends).shape == (0, 24)
+    assert grouped.grouped_matmul(x, w[:, :, :0], ends).shape == (4, 0)
+    assert bool((grouped.grouped_matmul(x[:, :0], w[:, :0], ends) == 0).all())
+    assert bool((grouped.grouped_weight_grad(x[:0], dy[:0], ends) == 0).all())
+    assert grouped.grouped_weight_grad(x[:, :0], dy, ends).shape == (2, 0, 24)
+
+
+@gpu
+def test_gradients_match_differences() -> None:
+    """y is linear in x and in w, so (Y(x + d) - Y(x - d)) / 2 is the derivative along d exactly; Y in 64 bits."""
+    ends = [19, 19, 83]
+    x, w, dy = _operands(90, 3, 96, 56, torch.float16, "nk", seed=10)
+    x.requires_grad_()
+    w = w.detach().requires_grad_()
+    dx, dw = torch.autograd.grad(grouped.grouped_matmul(x, w, _ends(ends)), (x, w), dy)
+
+    def loss(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
+        parts = [(a[s:e] @ b[i] * dy[s:e].double()).sum() for i, (s, e) in enumerate(_bounds(ends, 90))]
+        return torch.stack(parts).sum()
+
+    xd, wd = x.detach().double(), w.detach().double()
+    g = torch.Generator(device="cuda").manual_seed(11)
+    for grad, size, along in (
+        (dx, xd, lambda d: (loss(xd + d, wd) - loss(xd - d, wd)) / 2),
+        (dw, wd, lambda d: (loss(xd, wd + d) - loss(xd, wd - d)) / 2),
+    ):
+        d = torch.randn(size.shape, generator=g, device="cuda", dtype=torch.float64)
+        # Every entry of the gradient is off by its rounding, 2^-11, and FP32 sums well below that.
+        slack = (2.0**-10 * grad.double().abs() * d.abs()).sum() + 1e-3
+        assert abs((grad.double() * d).sum() - along(d)) <= slack
+
+
+@gpu
+def test_only_the_gradients_asked_for_and_no_second_derivative() -> None:
+    ends = _ends([4, 9])
+    x, w, dy = _operands(9, 2, 32, 16, torch.float16, "kn", seed=12)
+    leaf = x.clone().requires_grad_()
+    (dx,) = torch.autograd.grad(grouped.grouped_matmul(leaf, w, ends), (leaf,), dy)
+    _check_forward(dx, dy, w.transpose(1, 2), [4, 9])
+    leaf = w.clone().requires_grad_()
+    grouped.grouped_matmul(x, leaf, ends).backward(dy)
+    _check_weight_grad(leaf.grad, x, dy, [4, 9])
+    leaf = x.clone().requires_grad_()
+    (dx,) = torch.autograd.grad(grouped.grouped_matmul(leaf, w, ends), (leaf,), dy, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
+    with pytest.raises(ValueError, match="no gradient"):
+        grouped.grouped_weight_grad(leaf, dy, ends)
+
+
+@gpu
+def test_bad_arguments_are_rejected() -> None:
+    x, w, dy = _operands(9, 2, 32, 16, torch.float16, "kn", seed=13)
+    ends = _ends([4, 9])
+    for args, message in (
+        ((x.float(), w.float(), ends), "float16 or torch.bfloat16"),
+        ((x, w.bfloat16(), ends), "float16 or torch.bfloat16"),
+        ((x, w, ends[:1]), "one entry"),
+        ((x, w, ends.long()), "int32"),
+        ((x, w, ends.cpu()), "on the device"),
+        ((x, w, _ends([4, 0, 9, 0])[::2]), "contiguous"),
+        ((x, w[:0], ends[:0]), "1 to 1024"),
+    ):
+        with pytest.raises(ValueError, match=message):
+            grouped.grouped_matmul(*args)
+    with pytest.raises(ValueError, match="1 to 1024"):
+        grouped.grouped_weight_grad(x, dy, ends[:0])
+
+
+# ------------------------------------------------------------------------------------------
+# Streams, graphs, repeats
+# ------------------------------------------------------------------------------------------
+
+
+@gpu
+def test_repeats_are_bitwise_identical() -> None:
+    ends = _ends([130, 130, 391, 900])
+    x, w, dy = _operands(900, 4, 520, 392, torch.bfloat16, "kn", seed=14)
+    y, dw = grouped.grouped_matmul(x, w, ends), grouped.grouped_weight_grad(x, dy, ends)
+    for _ in range(3):
+        assert torch.equal(y, grouped.grouped_matmul(x, w, ends))
+        assert torch.equal(dw, grouped.grouped_weight_grad(x, dy, ends))
+
+
+@gpu
+def test_two_streams_at_once() -> None:
+    ends = [100, 300, 640]
+    x, w, dy = _operands(640, 3, 1032, 520, torch.float16, "kn", seed=15)
+    e = _ends(ends)
+    expected = grouped.grouped_matmul(x, w, e), grouped.grouped_weight_grad(x, dy, e)
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    results = []
+    for i in range(8):
+        with torch.cuda.stream(streams[i % 2]):
+            results.append((grouped.grouped_matmul(x, w, e), grouped.grouped_weight_grad(x, dy, e)))
+    torch.cuda.synchronize()
+    for y, dw in results:
+        assert torch.equal(y, expected[0]) and torch.equal(dw, expected[1])
+
+
+@gpu
+def test_captured_steps_follow_new_ends_and_inputs() -> None:
+    """Two graphs of a training step, replayed in turn with other ends and inputs than they were captured with."""
+    x, w, dy = _operands(300, 3, 264, 200, torch.float16, "kn", seed=16)
+    ends = _ends([100, 200, 300])
+    x.requires_grad_()
+    w.requires_grad_()
+
+    def step():  # type: ignore[no-untyped-def]
+        y = grouped.grouped_matmul(x, w, ends)
+        return (y.detach(), *torch.autograd.grad(y, (x, w), dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outputs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outputs.append(step())
+        graphs.append(graph)
+    for i, values in enumerate(([0, 300, 300], [17, 18, 290], [300, 300, 300], [5, 5, 5])):
+        with torch.no_grad():
+            ends.copy_(_ends(values))
+            x.mul_(-1)
+        graphs[i % 2].replay()
+        y, dx, dw = outputs[i % 2]
+        _check_forward(y, x.detach(), w.detach(), values)
+        _check_forward(dx, dy, w.detach().transpose(1, 2), values)
+        _check_weight_grad(dw, x.detach(), dy, values)
+
+
+@gpu
+def test_the_workspace_is_checked_and_its_contents_do_not_matter() -> None:
+    x, w, dy = _operands(120, 2, 520, 264, torch.float16, "kn", seed=17)
+    ends = _ends([50, 120])
+    lib = _native.library()
+    size = grouped._workspace_bytes(_native.GROUPED_FORWARD, 120, 2, 264, 520, 0)
+    y = torch.empty((120, 264), device="cuda", dtype=torch.float16)
+
+    def call(workspace: torch.Tensor) -> int:
+        return lib.hst_grouped_matmul(
+            0, x.data_ptr(), 520, w.data_ptr(), 520 * 264, 264, 0, ends.data_ptr(), 2, y.data_ptr(), 120, 264, 520,
+            workspace.data_ptr(), workspace.numel(), torch.cuda.current_stream().cuda_stream,
+        )  # fmt: skip
+
+    assert call(torch.empty(size - 1, device="cuda", dtype=torch.uint8)) == _native.HST_ERR_WORKSPACE
+    for fill in (0, 255):
+        assert call(torch.full((size,), fill, device="cuda", dtype=torch.uint8)) == _native.HST_OK
+        _check_forward(y, x, w, [50, 120])
