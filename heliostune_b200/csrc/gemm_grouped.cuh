@@ -28,8 +28,8 @@
 // block's UMMAs fill another buffer.
 //
 // Schedule: all (tile, K block) iterations of all groups in one line, cut into one equal share per
-// pair (contiguous, so neighbours in a share use the same weights out of L2). A tile cut by a
-// share's end leaves FP32 pieces in the workspace, which a second small kernel
+// pair (GroupTable). A tile cut by a share's end leaves FP32 pieces in the workspace, which a second
+// small kernel
 // (grouped_finish_kernel, a programmatic dependent) adds in K order. No CTA ever waits for another
 // pair, no atomics: results are bitwise reproducible, and the two kernels can be captured and
 // replayed. The second kernel also writes the zeros of rows past the last group and of the weight
@@ -77,7 +77,7 @@ struct GroupedArgs {
   int r_bytes;          // bytes of the R operand's part of a stage
   int pairs;            // CTA pairs launched
   int min_blocks;       // iterations a share has at least
-  int vec;              // output rows allow 32-byte stores
+  int vec;              // bytes of a store the output rows' alignment allows: 32, 16, 8, 4 or 2
   int* status;
   void* out;            // [rows, cols], or [groups, lrows, cols], contiguous
   float* partials;      // [pairs][2 pieces][2 CTAs][piece_floats]
@@ -112,18 +112,52 @@ __host__ __device__ inline int group_blocks(const GroupedArgs& a, int rows) {
   return MODE == GroupMode::kWeightGrad ? ceil_div(rows, 64) : a.k_blocks;
 }
 
-template <GroupMode MODE>
-__host__ __device__ inline int group_iterations(const GroupedArgs& a, int rows) {
-  return group_row_tiles<MODE>(a, rows) * ceil_div(a.cols, 256) * group_blocks<MODE>(a, rows);
-}
+// The tiles of all groups, numbered group by group, and how the pairs share them.
+//
+// The tiles are dealt to `shares` columns like cards (tile t * shares + c is number t of column c; the
+// last, part-filled row is spread evenly over the columns), the columns are put end to end into one
+// line of (tile, K block) iterations, and the line is cut into equal shares. Share c then runs along
+// column c, give or take a part of a tile, so at any moment the pairs work on neighbouring tiles: with
+// contiguous runs of the group-by-group order instead, the 74 weight panels in use passed L2's size
+// (8194 x 14336 x 4096 over 8 groups: 1007 us, 577 ns a block, against 0.28 for the UMMAs alone).
+struct GroupTable {
+  const int* start;      // [groups + 1] first row of each group
+  const int* tile_base;  // [groups + 1] first tile of each group
+  const int* col_base;   // [pairs + 1] first iteration of each column
+  int groups;
+  int tiles, shares, total;
+  int per_column, extra;  // tiles / shares and tiles % shares
 
-// start[e]: first row of group e; base[e]: first iteration of group e; both with an entry past the
-// last group. Ends are taken as they would be if clamped to [previous end, rows], so no value of
-// `ends` leads out of the matrices. One warp.
+  __device__ int column_first(int c) const { return c * per_column + c * extra / shares; }
+  __device__ int tile_of(int c, int t) const {
+    return t < per_column ? t * shares + c : per_column * shares + c * extra / shares;
+  }
+  __device__ int share_begin(int p) const { return p * (total / shares) + min(p, total % shares); }
+  __device__ int group_of(int tile) const {
+    int e = 0, top = groups - 1;  // last group whose first tile is <= tile; groups without tiles come before it
+    while (e < top) {
+      const int mid = (e + top + 1) >> 1;
+      if (tile_base[mid] <= tile) {
+        e = mid;
+      } else {
+        top = mid - 1;
+      }
+    }
+    return e;
+  }
+};
+
+constexpr __host__ __device__ int group_table_ints(int groups, int pairs) { return 2 * (groups + 1) + pairs + 1 + 4; }
+
+// Builds the table in shared memory. Ends are taken as they would be if clamped to
+// [previous end, rows], so no value of `ends` leads out of the matrices. All threads of the block
+// (128 or more); the caller synchronises before and after, and reads it with group_table.
 template <GroupMode MODE>
-__device__ inline void build_group_table(const GroupedArgs& a, int* start, int* base) {
+__device__ inline void build_group_rows(const GroupedArgs& a, int* mem) {
+  int* start = mem;
+  int* tile_base = start + a.groups + 1;
   const int lane = static_cast<int>(lane_id());
-  int row = 0, it = 0;
+  int row = 0, tiles = 0, total = 0;
   for (int g0 = 0; g0 < a.groups; g0 += 32) {
     const int g = g0 + lane;
     int end = 0;
@@ -136,32 +170,87 @@ __device__ inline void build_group_table(const GroupedArgs& a, int* start, int* 
     end = max(end, row);
     int begin = __shfl_up_sync(0xffffffffu, end, 1);
     if (lane == 0) begin = row;
-    const int its = g < a.groups ? group_iterations<MODE>(a, end - begin) : 0;
-    int sum = its;
+    const int mine = g < a.groups ? group_row_tiles<MODE>(a, end - begin) * ceil_div(a.cols, 256) : 0;
+    int sum = mine;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
       const int o = __shfl_up_sync(0xffffffffu, sum, d);
       if (lane >= d) sum += o;
     }
+    total += __reduce_add_sync(0xffffffffu, mine * group_blocks<MODE>(a, end - begin));
     if (g < a.groups) {
       start[g] = begin;
-      base[g] = it + sum - its;
+      tile_base[g] = tiles + sum - mine;
     }
     row = __shfl_sync(0xffffffffu, end, 31);
-    it += __shfl_sync(0xffffffffu, sum, 31);
+    tiles += __shfl_sync(0xffffffffu, sum, 31);
   }
   if (lane == 0) {
     start[a.groups] = row;
-    base[a.groups] = it;
+    tile_base[a.groups] = tiles;
+    int* head = mem + 2 * (a.groups + 1) + a.pairs + 1;
+    head[0] = tiles;
+    head[1] = max(1, min(a.pairs, total / a.min_blocks));
+    head[2] = total;
   }
 }
 
-// Pairs that get a share, and the first iteration of share p.
-__device__ inline int group_shares(const GroupedArgs& a, int total) {
-  return max(1, min(a.pairs, total / a.min_blocks));
+__device__ inline GroupTable group_table(const GroupedArgs& a, const int* mem) {
+  GroupTable t;
+  t.start = mem;
+  t.tile_base = mem + a.groups + 1;
+  t.col_base = t.tile_base + a.groups + 1;
+  t.groups = a.groups;
+  const int* head = t.col_base + a.pairs + 1;
+  t.tiles = head[0];
+  t.shares = head[1];
+  t.total = head[2];
+  t.per_column = t.tiles / t.shares;
+  t.extra = t.tiles % t.shares;
+  return t;
 }
-__device__ inline int share_begin(int total, int shares, int p) {
-  return static_cast<int>(int64_t(total) * p / shares);
+
+// Second step, after a barrier: the columns' first iterations.
+template <GroupMode MODE>
+__device__ inline void build_group_columns(const GroupedArgs& a, int* mem) {
+  const GroupTable t = group_table(a, mem);
+  int* col_base = mem + 2 * (a.groups + 1);
+  if constexpr (MODE != GroupMode::kWeightGrad) {
+    for (int c = static_cast<int>(threadIdx.x); c <= t.shares; c += static_cast<int>(blockDim.x)) {
+      col_base[c] = t.column_first(c) * a.k_blocks;
+    }
+  } else {
+    // K blocks differ by group: the first warp sums each column and scans the sums.
+    if (threadIdx.x >= 32) return;
+    const int lane = static_cast<int>(lane_id());
+    int before = 0;
+    for (int c0 = 0; c0 <= t.shares; c0 += 32) {
+      const int c = c0 + lane;
+      int sum = 0;
+      if (c < t.shares) {
+        const int whole = t.per_column * t.shares;  // tiles of the full rows
+        for (int e = 0; e < a.groups; ++e) {
+          const int lo = min(t.tile_base[e], whole), hi = min(t.tile_base[e + 1], whole);
+          if (hi <= lo) continue;
+          // Tiles of column c below x: those t * shares + c < x.
+          const int count = (hi - c + t.shares - 1) / t.shares - (lo - c + t.shares - 1) / t.shares;
+          sum += count * group_blocks<MODE>(a, t.start[e + 1] - t.start[e]);
+        }
+        if (t.column_first(c + 1) - t.column_first(c) > t.per_column) {
+          const int e = t.group_of(t.tile_of(c, t.per_column));
+          sum += group_blocks<MODE>(a, t.start[e + 1] - t.start[e]);
+        }
+      }
+      int scan = sum;
+#pragma unroll
+      for (int d = 1; d < 32; d *= 2) {
+        const int o = __shfl_up_sync(0xffffffffu, scan, d);
+        if (lane >= d) scan += o;
+      }
+      if (c <= t.shares) col_base[c] = before + scan - sum;
+      before += __shfl_sync(0xffffffffu, scan, 31);
+    }
+  }
 }
 
 // One run of K blocks of one tile.
@@ -174,16 +263,16 @@ struct GroupSegment {
   bool first;         // the share's first segment
 };
 
-// Tile `q` of group `e`: where it lies.
+// Tile `tile` of group `e`: where it lies.
 template <GroupMode MODE>
-__device__ inline void group_tile(const GroupedArgs& a, const int* start, int e, int q, GroupSegment& s) {
+__device__ inline void group_tile(const GroupedArgs& a, const GroupTable& t, int e, int tile, GroupSegment& s) {
   s.group = e;
-  s.row0 = start[e];
-  s.row_end = start[e + 1];
+  s.row0 = t.start[e];
+  s.row_end = t.start[e + 1];
   const int rows = s.row_end - s.row0;
-  const int row_tiles = group_row_tiles<MODE>(a, rows);
+  s.blocks = group_blocks<MODE>(a, rows);
   int pr, pc;
-  grouped_tile(q, row_tiles, ceil_div(a.cols, 256), kGroupRaster, pr, pc);
+  grouped_tile(tile - t.tile_base[e], group_row_tiles<MODE>(a, rows), ceil_div(a.cols, 256), kGroupRaster, pr, pc);
   if (group_rows_on_r(MODE)) {
     s.width = group_width(rows, a.width_cap);
     s.r0 = s.row0 + pr * s.width;
@@ -195,35 +284,63 @@ __device__ inline void group_tile(const GroupedArgs& a, const int* start, int e,
   }
 }
 
+// A place in the line: the tile that iteration `it` belongs to.
 template <GroupMode MODE>
-struct GroupWalk {
-  int it, lo, hi, e;
-  __device__ GroupWalk(const GroupedArgs& a, const int* base, int pair) {
-    const int total = base[a.groups];
-    const int shares = group_shares(a, total);
-    lo = pair < shares ? share_begin(total, shares, pair) : total;
-    hi = pair < shares ? share_begin(total, shares, pair + 1) : total;
-    it = lo;
-    e = 0;
-    int top = a.groups - 1;  // last group whose base is <= lo
-    while (e < top) {
-      const int mid = (e + top + 1) >> 1;
-      if (base[mid] <= lo) {
-        e = mid;
-      } else {
-        top = mid - 1;
-      }
+struct GroupPlace {
+  int c, n;    // column, and number of the tile in it
+  int tile, e;
+  int begin;   // the tile's first iteration
+  int blocks;
+
+  __device__ void set_tile(const GroupedArgs& a, const GroupTable& t) {
+    tile = t.tile_of(c, n);
+    e = t.group_of(tile);
+    blocks = group_blocks<MODE>(a, t.start[e + 1] - t.start[e]);
+  }
+  // `guess`: a column near the place. it < total.
+  __device__ void find(const GroupedArgs& a, const GroupTable& t, int it, int guess) {
+    c = guess;
+    while (t.col_base[c] > it) --c;
+    while (t.col_base[c + 1] <= it) ++c;
+    if constexpr (MODE != GroupMode::kWeightGrad) {
+      n = (it - t.col_base[c]) / a.k_blocks;
+      begin = t.col_base[c] + n * a.k_blocks;
+      set_tile(a, t);
+    } else {
+      n = 0;
+      begin = t.col_base[c];
+      set_tile(a, t);
+      while (begin + blocks <= it) step(a, t);
     }
   }
-  __device__ bool next(const GroupedArgs& a, const int* start, const int* base, GroupSegment& s) {
+  __device__ void step(const GroupedArgs& a, const GroupTable& t) {
+    begin += blocks;
+    ++n;
+    while (begin >= t.col_base[c + 1]) {  // the next column that has tiles
+      ++c;
+      n = 0;
+    }
+    set_tile(a, t);
+  }
+};
+
+// The segments of one share in order.
+template <GroupMode MODE>
+struct GroupWalk {
+  int it, lo, hi;
+  GroupPlace<MODE> place;
+  __device__ GroupWalk(const GroupedArgs& a, const GroupTable& t, int pair) {
+    lo = pair < t.shares ? t.share_begin(pair) : t.total;
+    hi = pair < t.shares ? t.share_begin(pair + 1) : t.total;
+    it = lo;
+    if (lo < hi) place.find(a, t, lo, pair);
+  }
+  __device__ bool next(const GroupedArgs& a, const GroupTable& t, GroupSegment& s) {
     if (it >= hi) return false;
-    while (it >= base[e + 1]) ++e;  // past groups without rows
-    const int blocks = group_blocks<MODE>(a, start[e + 1] - start[e]);
-    const int q = (it - base[e]) / blocks;
-    group_tile<MODE>(a, start, e, q, s);
-    s.blocks = blocks;
-    s.kb0 = it - base[e] - q * blocks;
-    s.kb1 = min(blocks, s.kb0 + hi - it);
+    if (it >= place.begin + place.blocks) place.step(a, t);
+    group_tile<MODE>(a, t, place.e, place.tile, s);
+    s.kb0 = it - place.begin;
+    s.kb1 = min(place.blocks, s.kb0 + hi - it);
     s.first = it == lo;
     it += s.kb1 - s.kb0;
     return true;
@@ -298,20 +415,85 @@ __device__ __forceinline__ void store_rows_across(T* out, int64_t ldo, const flo
   }
 }
 
-// One lane's 16 consecutive output columns of its own row (32 bytes).
+// One lane's 16 consecutive output columns of its own row, in stores of 32, 16, 8 or 4 bytes (what
+// the rows' alignment allows); the ragged end value by value.
 template <typename T>
-__device__ __forceinline__ void store_cols_16(T* p, const float (&v)[16], int left, bool vec) {
-  if (vec && left >= 16) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p),
-                 "r"(pack_f32<T>(v[0], v[1])), "r"(pack_f32<T>(v[2], v[3])), "r"(pack_f32<T>(v[4], v[5])),
-                 "r"(pack_f32<T>(v[6], v[7])), "r"(pack_f32<T>(v[8], v[9])), "r"(pack_f32<T>(v[10], v[11])),
-                 "r"(pack_f32<T>(v[12], v[13])), "r"(pack_f32<T>(v[14], v[15]))
+__device__ __forceinline__ void store_cols_16(T* p, const float (&v)[16], int left, int vec) {
+  uint32_t w[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) w[j] = pack_f32<T>(v[2 * j], v[2 * j + 1]);
+  if (left >= 16 && vec == 32) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                  : "memory");
+  } else if (vec >= 16) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {  // rows are a multiple of 8 values: no part of a store is ragged
+      if (8 * j < left) reinterpret_cast<uint4*>(p)[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+    }
+  } else if (vec == 8) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (4 * j < left) reinterpret_cast<uint2*>(p)[j] = make_uint2(w[2 * j], w[2 * j + 1]);
+    }
   } else {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      if (j < left) p[j] = from_f32<T>(v[j]);
+    for (int j = 0; j < 8; ++j) {
+      if (2 * j < left) reinterpret_cast<uint32_t*>(p)[j] = w[j];
     }
+  }
+}
+
+// Transposes the warp's 32 x 32 matrix: v[i] of lane j becomes v[j] of lane i.
+__device__ __forceinline__ void warp_transpose(float (&v)[32]) {
+  const uint32_t lane = lane_id();
+#pragma unroll
+  for (int d = 16; d >= 1; d /= 2) {
+    const bool upper = (lane & d) != 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      if ((i & d) == 0) {
+        const float give = upper ? v[i] : v[i + d];
+        const float got = __shfl_xor_sync(0xffffffffu, give, d);
+        if (upper) {
+          v[i] = got;
+        } else {
+          v[i + d] = got;
+        }
+      }
+    }
+  }
+}
+
+// The warp's 32 rows x 32 columns, one row a lane, `cols` an odd number: two-byte stores along the
+// rows, after a transpose, instead of 32 rows at a time (256 x 256 tiles: 32 sectors a store).
+template <typename T>
+__device__ __forceinline__ void store_cols_odd(T* row0, int64_t ldo, float (&v)[32], int rows, int left) {
+  warp_transpose(v);
+  const int lane = static_cast<int>(lane_id());
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    if (i < rows && lane < left) row0[static_cast<int64_t>(i) * ldo + lane] = from_f32<T>(v[i]);
+  }
+}
+
+// 32 columns of the warp's 32 rows from column `col` on, one row a lane: `first` is the warp's first
+// row in the output, `rows` how many of the 32 exist.
+template <typename T>
+__device__ __forceinline__ void store_cols_32(T* out, int64_t first, int rows, int col, const GroupedArgs& a, float (&v)[32]) {
+  const int left = a.cols - col;
+  if (a.vec == 2) {
+    store_cols_odd(out + first * a.cols + col, a.cols, v, rows, left);
+    return;
+  }
+  if (static_cast<int>(lane_id()) >= rows) return;
+  T* p = out + (first + lane_id()) * a.cols + col;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float f[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) f[j] = v[16 * h + j];
+    store_cols_16(p + 16 * h, f, left - 16 * h, a.vec);
   }
 }
 
@@ -320,8 +502,8 @@ struct GroupedShape {
   static constexpr int kBarriers = 3 * kMaxStages + 2 * 8 + 1;
   static constexpr int kBarrierBytes = kBarriers * 8 + 16;
   __host__ __device__ static constexpr int stage_bytes(int r_bytes) { return kGroupLBytes + r_bytes; }
-  __host__ __device__ static constexpr int smem_bytes(int stages, int r_bytes, int groups) {
-    return 1024 + stages * stage_bytes(r_bytes) + kBarrierBytes + (groups + 1) * 8;
+  __host__ __device__ static constexpr int smem_bytes(int stages, int r_bytes, int groups, int pairs) {
+    return 1024 + stages * stage_bytes(r_bytes) + kBarrierBytes + group_table_ints(groups, pairs) * 4;
   }
 };
 
@@ -355,8 +537,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
   uint64_t* mma_done = tmem_empty + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* start = reinterpret_cast<int*>(tmem_slot + 4);
-  int* base = start + args.groups + 1;
+  int* table_mem = reinterpret_cast<int*>(tmem_slot + 4);
 
   const int warp = threadIdx.x >> 5;
   const uint32_t lane = lane_id();
@@ -384,11 +565,14 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
     tmem_alloc_pair(tmem_slot, 512);
     tmem_relinquish_pair();
   }
-  if (warp == 2) build_group_table<MODE>(args, start, base);
+  if (warp == 2) build_group_rows<MODE>(args, table_mem);
+  __syncthreads();
+  build_group_columns<MODE>(args, table_mem);
   tc_fence_before_sync();
   cluster_sync();  // both CTAs' barriers exist before either signals the other
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
+  const GroupTable table = group_table(args, table_mem);
 
   if (warp == 0 && lane == 0) {
     // ---------------- TMA producer (both CTAs) ----------------
@@ -398,9 +582,9 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
     uint32_t armed_mask = 0, armed_parity = 0;  // stages this thread has armed (leader)
     uint32_t tail_mask = 0, tail_parity = 0;    // tail barriers used; parity of their next use
     bool ok = true;
-    GroupWalk<MODE> walk(args, base, pair);
+    GroupWalk<MODE> walk(args, table, pair);
     GroupSegment s;
-    while (ok && walk.next(args, start, base, s)) {
+    while (ok && walk.next(args, table, s)) {
       const int half = s.width / 2;
       const int box = kGrad ? 0 : group_box(half);
       const uint32_t r_bytes = kGrad ? static_cast<uint32_t>(half) * 128u : (128u >> box) * 128u;
@@ -486,9 +670,9 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
     const uint64_t l_desc0 = smem_desc(smem_addr(ring), L_MN ? 8192 : 16, 1024);
     const uint64_t r_desc0 = smem_desc(smem_addr(ring) + kGroupLBytes, kGrad ? 8192 : 16, 1024);
     constexpr uint32_t kLStep = (L_MN ? 2048 : 32) >> 4, kRStep = (kGrad ? 2048 : 32) >> 4;
-    GroupWalk<MODE> walk(args, base, pair);
+    GroupWalk<MODE> walk(args, table, pair);
     GroupSegment s;
-    while (ok && walk.next(args, start, base, s)) {
+    while (ok && walk.next(args, table, s)) {
       const uint32_t idesc = kIdescBase | (static_cast<uint32_t>(s.width >> 3) << 17);
       const int tail = kGrad ? (s.row_end - s.row0) - (s.blocks - 1) * 64 : 0;
       for (int kb = s.kb0; kb < s.kb1; ++kb) {
@@ -541,10 +725,10 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
     // ---------------- masking warp (both CTAs): rows past the group in its last block ----------
     int stage = 0;
     uint32_t parity = 0;  // bit s: parity of the next use of tail_full[s]
-    GroupWalk<MODE> walk(args, base, pair);
+    GroupWalk<MODE> walk(args, table, pair);
     GroupSegment s;
     bool ok = true;
-    while (ok && walk.next(args, start, base, s)) {
+    while (ok && walk.next(args, table, s)) {
       const int blocks = s.kb1 - s.kb0;
       const int tail = (s.row_end - s.row0) - (s.blocks - 1) * 64;
       if (s.kb1 == s.blocks && (tail & 15) != 0) {
@@ -602,10 +786,10 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
       return args.partials +
              (static_cast<size_t>(pair * 2 + (s.first ? 0 : 1)) * 2 + rank) * static_cast<size_t>(args.piece_floats);
     };
-    GroupWalk<MODE> walk(args, base, pair);
+    GroupWalk<MODE> walk(args, table, pair);
     GroupSegment s;
     if constexpr (!kScaled) {
-      while (walk.next(args, start, base, s)) {
+      while (walk.next(args, table, s)) {
         if (!wait_buf()) break;
         const uint32_t taddr = lane_base + static_cast<uint32_t>(buf * kBufCols);
         const int l = s.l0 + static_cast<int>(rank) * 128 + row;
@@ -622,16 +806,11 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
               st_global_v4(dst + static_cast<size_t>(j) * 512, v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
             }
           } else if constexpr (kGrad) {
-            if (l < args.lrows) {
-              T* p = out + (static_cast<int64_t>(s.group) * args.lrows + l) * args.cols + s.r0 + c;
+            float f[32];
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                float f[16];
-#pragma unroll
-                for (int j = 0; j < 16; ++j) f[j] = __uint_as_float(v[16 * h + j]);
-                store_cols_16(p + 16 * h, f, args.cols - (s.r0 + c + 16 * h), args.vec != 0);
-              }
-            }
+            for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
+            const int l32 = l - static_cast<int>(lane);
+            store_cols_32(out, static_cast<int64_t>(s.group) * args.lrows + l32, args.lrows - l32, s.r0 + c, args, f);
           } else {
             float f[32];
 #pragma unroll
@@ -643,7 +822,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
       }
     } else if constexpr (MODE == GroupMode::kScaledWide) {
       const int half = (warp - 2) / 4;  // 128 of the tile's 256 columns
-      while (walk.next(args, start, base, s)) {
+      while (walk.next(args, table, s)) {
         const int t = s.l0 + static_cast<int>(rank) * 128 + row;
         const bool live = half * 128 < s.width && s.r0 + half * 128 < args.cols;
         const float* sa = args.row_scales + static_cast<int64_t>(min(t, args.rows - 1)) * args.rs_row;
@@ -680,18 +859,16 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
         if (!ready) break;
         if (!live) continue;
         if (s.kb0 == 0 && s.kb1 == s.blocks) {
-          if (t < s.row_end) {
-            T* p = out + static_cast<int64_t>(t) * args.cols + s.r0 + half * 128;
+          const int t32 = t - static_cast<int>(lane);
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              float f[16];
+          for (int c = 0; c < 4; ++c) {
+            float f[32];
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                f[2 * j] = __uint_as_float(static_cast<uint32_t>(acc[8 * c + j]));
-                f[2 * j + 1] = __uint_as_float(static_cast<uint32_t>(acc[8 * c + j] >> 32));
-              }
-              store_cols_16(p + 16 * c, f, args.cols - (s.r0 + half * 128 + 16 * c), args.vec != 0);
+            for (int j = 0; j < 16; ++j) {
+              f[2 * j] = __uint_as_float(static_cast<uint32_t>(acc[16 * c + j]));
+              f[2 * j + 1] = __uint_as_float(static_cast<uint32_t>(acc[16 * c + j] >> 32));
             }
+            store_cols_32(out, t32, s.row_end - t32, s.r0 + half * 128 + 32 * c, args, f);
           }
         } else {
           float* dst = piece_of(s) + (static_cast<size_t>(half * 32) * 128 + row) * 4;
@@ -704,7 +881,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
         }
       }
     } else {
-      while (walk.next(args, start, base, s)) {
+      while (walk.next(args, table, s)) {
         const int l = s.l0 + static_cast<int>(rank) * 128 + row;
         const int valid = min(s.row_end - s.r0, s.width);  // rows of the tile
         // This CTA's 128 output columns share one weight scale per block.
@@ -771,63 +948,58 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
 }
 
 constexpr int kFinishThreads = 128;
-constexpr int kFinishChunks = 4;  // blocks along a piece's columns
+constexpr int kFinishCols = 32;  // columns of a piece one block joins
 
-// Joins the tiles that shares cut: block (p, CTA half, chunk) takes the tile in which share p + 1
-// begins, if that is the first share to begin inside it, and adds its FP32 pieces in K order. Then
-// all blocks write the zeros nobody else writes.
+// Joins the tiles that shares cut: block (p, CTA half, chunk of columns) takes the tile in which share
+// p + 1 begins, if that is the first share to begin inside it, and adds its FP32 pieces in K order.
+// Then all blocks write the zeros nobody else writes.
 template <GroupMode MODE, typename T>
 __global__ void __launch_bounds__(kFinishThreads) grouped_finish_kernel(const __grid_constant__ GroupedArgs args) {
   extern __shared__ int finish_table[];
-  int* start = finish_table;
-  int* base = start + args.groups + 1;
-  if (threadIdx.x < 32) build_group_table<MODE>(args, start, base);
+  if (threadIdx.x < 32) build_group_rows<MODE>(args, finish_table);
   __syncthreads();
+  build_group_columns<MODE>(args, finish_table);
+  __syncthreads();
+  const GroupTable table = group_table(args, finish_table);
   wait_for_primary();
   T* out = static_cast<T*>(args.out);
-  const int total = base[args.groups];
-  const int shares = group_shares(args, total);
   const int p = static_cast<int>(blockIdx.x) + 1;
   const int rank = static_cast<int>(blockIdx.y);
-  if (p < shares) {
-    const int cut = share_begin(total, shares, p);
-    int e = 0;
-    while (cut >= base[e + 1]) ++e;
-    const int blocks = group_blocks<MODE>(args, start[e + 1] - start[e]);
-    const int q = (cut - base[e]) / blocks;
-    const int tile_begin = base[e] + q * blocks;
-    const int tile_end = tile_begin + blocks;
-    const int before = share_begin(total, shares, p - 1);
-    if (cut > tile_begin && before <= tile_begin) {
-      GroupSegment s;
-      group_tile<MODE>(args, start, e, q, s);
+  if (p < table.shares) {
+    const int cut = table.share_begin(p);
+    GroupPlace<MODE> place;
+    place.find(args, table, cut, p);
+    const int end = place.begin + place.blocks;
+    GroupSegment s;
+    group_tile<MODE>(args, table, place.e, place.tile, s);
+    const int c = static_cast<int>(blockIdx.z) * kFinishCols;
+    if (cut > place.begin && table.share_begin(p - 1) <= place.begin && c < s.width) {
       const int row = static_cast<int>(threadIdx.x);
-      for (int c = static_cast<int>(blockIdx.z) * 4; c < s.width; c += kFinishChunks * 4) {
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int o = p - 1; o < shares && share_begin(total, shares, o) < tile_end; ++o) {
-          const int piece = share_begin(total, shares, o) >= tile_begin ? 0 : 1;
-          const float* src = args.partials +
-                             (static_cast<size_t>(o * 2 + piece) * 2 + rank) * static_cast<size_t>(args.piece_floats) +
-                             (static_cast<size_t>(c / 4) * 128 + row) * 4;
-          const float4 v = *reinterpret_cast<const float4*>(src);
-          sum.x += v.x;
-          sum.y += v.y;
-          sum.z += v.z;
-          sum.w += v.w;
+      float v[kFinishCols];
+#pragma unroll
+      for (int j = 0; j < kFinishCols; ++j) v[j] = 0.f;
+      for (int o = p - 1; o < table.shares && table.share_begin(o) < end; ++o) {
+        const int piece = table.share_begin(o) >= place.begin ? 0 : 1;
+        const float* src = args.partials +
+                           (static_cast<size_t>(o * 2 + piece) * 2 + rank) * static_cast<size_t>(args.piece_floats) +
+                           (static_cast<size_t>(c / 4) * 128 + row) * 4;
+#pragma unroll
+        for (int j = 0; j < kFinishCols / 4; ++j) {
+          const float4 f = *reinterpret_cast<const float4*>(src + j * 512);
+          v[4 * j] += f.x;
+          v[4 * j + 1] += f.y;
+          v[4 * j + 2] += f.z;
+          v[4 * j + 3] += f.w;
         }
-        const float v[4] = {sum.x, sum.y, sum.z, sum.w};
-        const int l = s.l0 + rank * 128 + row;
-        if constexpr (group_rows_on_r(MODE)) {
-          store_rows_across(out, args.cols, v, s.r0 + c, min(s.row_end, s.r0 + s.width), l, args.cols);
-        } else {
-          const bool inside = MODE == GroupMode::kWeightGrad ? l < args.lrows : l < s.row_end;
-          const int64_t line = MODE == GroupMode::kWeightGrad ? static_cast<int64_t>(e) * args.lrows + l : l;
-          if (inside) {
-            for (int j = 0; j < 4; ++j) {
-              if (s.r0 + c + j < args.cols) out[line * args.cols + s.r0 + c + j] = from_f32<T>(v[j]);
-            }
-          }
-        }
+      }
+      const int l = s.l0 + rank * 128 + row;
+      if constexpr (group_rows_on_r(MODE)) {
+        store_rows_across(out, args.cols, v, s.r0 + c, min(s.row_end, s.r0 + s.width), l, args.cols);
+      } else {
+        const int l32 = l - static_cast<int>(lane_id());
+        const bool grad = MODE == GroupMode::kWeightGrad;
+        store_cols_32(out, grad ? static_cast<int64_t>(place.e) * args.lrows + l32 : l32,
+                      (grad ? args.lrows : s.row_end) - l32, s.r0 + c, args, v);
       }
     }
   }
@@ -845,10 +1017,10 @@ __global__ void __launch_bounds__(kFinishThreads) grouped_finish_kernel(const __
   if constexpr (MODE == GroupMode::kWeightGrad) {
     const int64_t size = static_cast<int64_t>(args.lrows) * args.cols;
     for (int g = 0; g < args.groups; ++g) {
-      if (start[g + 1] == start[g]) zero(out + g * size, size);
+      if (table.start[g + 1] == table.start[g]) zero(out + g * size, size);
     }
   } else {
-    const int64_t from = start[args.groups];
+    const int64_t from = table.start[args.groups];
     if (from < args.rows) zero(out + from * args.cols, (args.rows - from) * args.cols);
   }
 }

@@ -96,12 +96,13 @@ int launch_grouped(const GroupedProblem& p, const GroupedMaps& maps, GroupedArgs
   args.r_bytes = r_bytes;
   args.pairs = plan_pairs<MODE>(p, dev->sm_count);
   args.min_blocks = kMinBlocks;
-  args.vec = (p.cols % 16 == 0) && (reinterpret_cast<uintptr_t>(args.out) % 32 == 0);
+  args.vec = 32;
+  while (args.vec > 2 && (p.cols * 2 % args.vec != 0 || reinterpret_cast<uintptr_t>(args.out) % args.vec != 0)) args.vec /= 2;
   args.status = dev->status;
   args.partials = static_cast<float*>(workspace);
   args.piece_floats = piece_floats<MODE>(p);
   int stages = kMaxStages;
-  while (stages > 2 && S::smem_bytes(stages, r_bytes, p.groups) > kMaxDynamicSmem) --stages;
+  while (stages > 2 && S::smem_bytes(stages, r_bytes, p.groups, args.pairs) > kMaxDynamicSmem) --stages;
   args.stages = stages;
   if (p.rows > 0) {
     static std::atomic<uint64_t> smem_done{0};
@@ -109,7 +110,7 @@ int launch_grouped(const GroupedProblem& p, const GroupedMaps& maps, GroupedArgs
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3(static_cast<unsigned>(2 * args.pairs));
     lc.blockDim = dim3(group_threads(MODE));
-    lc.dynamicSmemBytes = S::smem_bytes(stages, r_bytes, p.groups);
+    lc.dynamicSmemBytes = S::smem_bytes(stages, r_bytes, p.groups, args.pairs);
     lc.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -121,9 +122,10 @@ int launch_grouped(const GroupedProblem& p, const GroupedMaps& maps, GroupedArgs
     HST_CUDA(cudaLaunchKernelEx(&lc, grouped_gemm_kernel<MODE, L_MN, T>, maps, args));
   }
   cudaLaunchConfig_t lc = {};
-  lc.gridDim = dim3(static_cast<unsigned>(std::max(1, args.pairs - 1)), 2, kFinishChunks);
+  lc.gridDim = dim3(static_cast<unsigned>(std::max(1, args.pairs - 1)), 2,
+                    static_cast<unsigned>(args.piece_floats / 128 / kFinishCols));
   lc.blockDim = dim3(kFinishThreads);
-  lc.dynamicSmemBytes = static_cast<size_t>(p.groups + 1) * 8;
+  lc.dynamicSmemBytes = static_cast<size_t>(group_table_ints(p.groups, args.pairs)) * 4;
   lc.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
