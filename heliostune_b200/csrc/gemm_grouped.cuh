@@ -1,38 +1,37 @@
 // Matrix products over rows grouped by expert, on CTA pairs (tcgen05.mma.cta_group::2).
 //
 // Group e owns rows [ends[e - 1], ends[e]) of a row matrix; `ends` lives on the GPU, so nothing
-// about the sizes is known on the host. Four products share this kernel:
-//   kForward       y[t, :] = x[t, :] W[e(t)]          16-bit x [T, K], W [E, K, N] (either of its
-//                                                     two inner dimensions contiguous)
-//   kWeightGrad    D[e] = L[rows of e]^T R[rows of e]  16-bit L [T, Lc], R [T, Rc]
-//   kScaledWide    y[t, n] = sum_b sa[t, b] sb[e, n/128, b] sum_{k in block b} a[t, k] b[e, n, k]
-//   kScaledStream  the same                            E4M3 a [T, K], b [E, N, K], FP32 scales of
-//                                                     128 (a) and 128 x 128 (b) values
+// about the sizes is known on the host. Three products share this kernel:
+//   kForward     y[t, :] = x[t, :] W[e(t)]           16-bit x [T, K], W [E, K, N] (either of its two
+//                                                    inner dimensions contiguous)
+//   kWeightGrad  D[e] = L[rows of e]^T R[rows of e]   16-bit L [T, Lc], R [T, Rc]
+//   kScaled      y[t, n] = sum_b sa[t, b] sb[e, n/128, b] sum_{k in block b} a[t, k] b[e, n, k]
+//                                                    E4M3 a [T, K], b [E, N, K], FP32 scales of 128
+//                                                    (a) and 128 x 128 (b) values
 //
 // One pair of CTAs computes a 256 x width tile: CTA r owns 128 rows of the L operand and half of
-// the R operand's `width` columns. Which side the rows are on decides what raggedness costs:
-//   * kForward and kScaledStream put the weights on the L side (M = 256 output columns) and the
-//     rows on the R side, whose width is a run-time field of the UMMA descriptor (32..256). A
-//     group's rows are cut into equal widths, so a group of r rows costs round_up(r / tiles, 32)
-//     columns of tensor-core time per tile instead of the next multiple of 256, and each weight is
-//     read once for up to 256 rows;
-//   * kScaledWide keeps the rows on the L side, where one row is one TMEM lane: its scale is one
-//     register, and the promotion below costs one FMA per element;
+// the R operand's `width` columns. Each weight is read once for up to 256 rows, so few rows a group
+// are bound by HBM, many by the tensor cores.
+//   * kForward puts the weights on the L side (M = 256 output columns) and the rows on the R side,
+//     whose width is a run-time field of the UMMA descriptor (32..256): a group's rows are cut into
+//     equal widths, and raggedness costs round_up(rows / tiles, 32) columns of tensor-core time
+//     instead of the next multiple of 256.
 //   * kWeightGrad reduces over the rows, 64 at a time. Rows past the group's end in its last block
-//     belong to other groups: a fourth kind of warp zeroes those of the last 16-row UMMA step in
-//     shared memory (both operands, so that NaN or infinity there stays out), and the UMMA steps
-//     past them are not issued.
-//
-// The scaled products accumulate each 128-deep block in a TMEM buffer of its own; the epilogue
-// warps read it, multiply by the block's scales and add it to FP32 registers, while the next
-// block's UMMAs fill another buffer.
+//     belong to other groups: one more warp zeroes those of the last 16-row UMMA step in shared
+//     memory (both operands, so that NaN or infinity there stays out), and the steps past them are
+//     not issued.
+//   * kScaled accumulates each 128-deep block in a TMEM buffer of its own; the epilogue warps read
+//     it, multiply by the block's scales and add it to FP32 registers, while the next block's UMMAs
+//     fill the other buffer. The rows are on the L side, where a row is a TMEM lane and its scale
+//     one register: with the rows on the R side the scales were 128 a thread and block, and their
+//     broadcast loads from shared memory, beside the UMMAs' operands, took three times the UMMAs'
+//     time (1.5 us a block of 256 rows against 0.5).
 //
 // Schedule: all (tile, K block) iterations of all groups in one line, cut into one equal share per
 // pair (GroupTable). A tile cut by a share's end leaves FP32 pieces in the workspace, which a second
-// small kernel
-// (grouped_finish_kernel, a programmatic dependent) adds in K order. No CTA ever waits for another
-// pair, no atomics: results are bitwise reproducible, and the two kernels can be captured and
-// replayed. The second kernel also writes the zeros of rows past the last group and of the weight
+// small kernel (grouped_finish_kernel, a programmatic dependent) adds in K order. No CTA ever waits
+// for another pair, no atomics: results are bitwise reproducible, and the two kernels can be captured
+// and replayed. The second kernel also writes the zeros of rows past the last group and of the weight
 // gradients of empty groups.
 #pragma once
 
@@ -45,24 +44,26 @@
 
 namespace hst {
 
-enum class GroupMode { kForward, kWeightGrad, kScaledWide, kScaledStream };
+enum class GroupMode { kForward, kWeightGrad, kScaled };
 
 constexpr int kMaxGroups = 1024;
 constexpr int kGroupLBytes = 16384;  // 128 L rows x 128 bytes of K (or 2 boxes of 64 x 64)
 constexpr int kGroupRaster = 8;      // row tiles before the next column tile
 
-__host__ __device__ constexpr bool group_scaled(GroupMode m) { return m == GroupMode::kScaledWide || m == GroupMode::kScaledStream; }
-// Rows of the row matrix on the R side (their count is the tile's width).
-__host__ __device__ constexpr bool group_rows_on_r(GroupMode m) { return m == GroupMode::kForward || m == GroupMode::kScaledStream; }
-__host__ __device__ constexpr int group_epilogue_warps(GroupMode m) { return m == GroupMode::kScaledWide ? 8 : 4; }
+// Warps: 0 loads, 1 issues the UMMAs; then the epilogue, and for kWeightGrad the masking warp. kScaled
+// holds 128 x 256 FP32 sums in the registers of 8 epilogue warps, which therefore form warpgroups
+// of their own (2 and 3 idle).
+__host__ __device__ constexpr int group_first_epilogue_warp(GroupMode m) { return m == GroupMode::kScaled ? 4 : 2; }
+__host__ __device__ constexpr int group_epilogue_warps(GroupMode m) { return m == GroupMode::kScaled ? 8 : 4; }
 __host__ __device__ constexpr int group_threads(GroupMode m) {
-  return 64 + 32 * group_epilogue_warps(m) + (m == GroupMode::kWeightGrad ? 32 : 0);
+  return 32 * (group_first_epilogue_warp(m) + group_epilogue_warps(m) + (m == GroupMode::kWeightGrad ? 1 : 0));
 }
-__host__ __device__ constexpr int group_tmem_bufs(GroupMode m) { return m == GroupMode::kScaledStream ? 8 : 2; }
 
+// Boxes of 128, 64, 32 and 16 rows on the side that needs them (kForward: R, kScaled: L), else one
+// (kScaled's R: 128 and 64; kWeightGrad: 64 x 64).
 struct GroupedMaps {
-  CUtensorMap l;
-  CUtensorMap r[4];  // R boxes of 128, 64, 32 and 16 rows (kWeightGrad: r[0], 64 x 64)
+  CUtensorMap l[4];
+  CUtensorMap r[4];
 };
 
 struct GroupedArgs {
@@ -72,7 +73,7 @@ struct GroupedArgs {
   int cols;             // columns of the output
   int lrows;            // kWeightGrad: rows of one group's output
   int k_blocks;         // K blocks of a tile (kWeightGrad: by group)
-  int width_cap;        // rows on the R side: most of them in a tile (a multiple of 32)
+  int width_cap;        // kForward: most rows in a tile (a multiple of 32)
   int stages;
   int r_bytes;          // bytes of the R operand's part of a stage
   int pairs;            // CTA pairs launched
@@ -84,6 +85,7 @@ struct GroupedArgs {
   int piece_floats;
   const float* row_scales;  // sa: strides below, in elements
   int64_t rs_row, rs_k;
+  int rs_vec;               // sa is stored by rows, four values at a time
   const float* tile_scales;  // sb
   int64_t ts_group, ts_n, ts_k;
 };
@@ -97,13 +99,13 @@ __host__ __device__ inline int group_width(int rows, int cap) {
   return ceil_div(ceil_div(rows, tiles), 32) * 32;
 }
 
-// Index among the R boxes (128, 64, 32, 16 rows) of the smallest that holds half a tile's width.
-__host__ __device__ inline int group_box(int half) { return half > 64 ? 0 : (half > 32 ? 1 : (half > 16 ? 2 : 3)); }
+// Index among the boxes (128, 64, 32, 16 rows) of the smallest that holds `rows`.
+__host__ __device__ inline int group_box(int rows) { return rows > 64 ? 0 : (rows > 32 ? 1 : (rows > 16 ? 2 : 3)); }
 
 template <GroupMode MODE>
 __host__ __device__ inline int group_row_tiles(const GroupedArgs& a, int rows) {
   if (rows <= 0) return 0;
-  if (group_rows_on_r(MODE)) return ceil_div(rows, group_width(rows, a.width_cap));
+  if (MODE == GroupMode::kForward) return ceil_div(rows, group_width(rows, a.width_cap));
   return ceil_div(MODE == GroupMode::kWeightGrad ? a.lrows : rows, 256);
 }
 
@@ -129,6 +131,8 @@ struct GroupTable {
   int per_column, extra;  // tiles / shares and tiles % shares
 
   __device__ int column_first(int c) const { return c * per_column + c * extra / shares; }
+  // The column of the line's tile v: the last c with column_first(c) = floor(c * tiles / shares) <= v.
+  __device__ int column_of(int v) const { return ((v + 1) * shares - 1) / tiles; }
   __device__ int tile_of(int c, int t) const {
     return t < per_column ? t * shares + c : per_column * shares + c * extra / shares;
   }
@@ -210,7 +214,7 @@ __device__ inline GroupTable group_table(const GroupedArgs& a, const int* mem) {
   return t;
 }
 
-// Second step, after a barrier: the columns' first iterations.
+// Second step, after a barrier; all threads, and a barrier before the table is used.
 template <GroupMode MODE>
 __device__ inline void build_group_columns(const GroupedArgs& a, int* mem) {
   const GroupTable t = group_table(a, mem);
@@ -220,27 +224,31 @@ __device__ inline void build_group_columns(const GroupedArgs& a, int* mem) {
       col_base[c] = t.column_first(c) * a.k_blocks;
     }
   } else {
-    // K blocks differ by group: the first warp sums each column and scans the sums.
-    if (threadIdx.x >= 32) return;
+    // K blocks differ by group: one warp sums a column, its lanes over the groups; then a scan.
     const int lane = static_cast<int>(lane_id());
+    const int whole = t.per_column * t.shares;  // tiles of the full rows
+    for (int c = static_cast<int>(threadIdx.x >> 5); c < t.shares; c += static_cast<int>(blockDim.x >> 5)) {
+      int sum = 0;
+      for (int e = lane; e < a.groups; e += 32) {
+        const int lo = min(t.tile_base[e], whole), hi = min(t.tile_base[e + 1], whole);
+        if (hi <= lo) continue;
+        // Tiles of column c below x: those with number * shares + c < x.
+        const int count = (hi - c + t.shares - 1) / t.shares - (lo - c + t.shares - 1) / t.shares;
+        sum += count * group_blocks<MODE>(a, t.start[e + 1] - t.start[e]);
+      }
+      sum = __reduce_add_sync(0xffffffffu, sum);
+      if (t.column_first(c + 1) - t.column_first(c) > t.per_column) {
+        const int e = t.group_of(t.tile_of(c, t.per_column));
+        sum += group_blocks<MODE>(a, t.start[e + 1] - t.start[e]);
+      }
+      if (lane == 0) col_base[c] = sum;
+    }
+    __syncthreads();
+    if (threadIdx.x >= 32) return;
     int before = 0;
     for (int c0 = 0; c0 <= t.shares; c0 += 32) {
       const int c = c0 + lane;
-      int sum = 0;
-      if (c < t.shares) {
-        const int whole = t.per_column * t.shares;  // tiles of the full rows
-        for (int e = 0; e < a.groups; ++e) {
-          const int lo = min(t.tile_base[e], whole), hi = min(t.tile_base[e + 1], whole);
-          if (hi <= lo) continue;
-          // Tiles of column c below x: those t * shares + c < x.
-          const int count = (hi - c + t.shares - 1) / t.shares - (lo - c + t.shares - 1) / t.shares;
-          sum += count * group_blocks<MODE>(a, t.start[e + 1] - t.start[e]);
-        }
-        if (t.column_first(c + 1) - t.column_first(c) > t.per_column) {
-          const int e = t.group_of(t.tile_of(c, t.per_column));
-          sum += group_blocks<MODE>(a, t.start[e + 1] - t.start[e]);
-        }
-      }
+      const int sum = c < t.shares ? col_base[c] : 0;
       int scan = sum;
 #pragma unroll
       for (int d = 1; d < 32; d *= 2) {
@@ -273,7 +281,7 @@ __device__ inline void group_tile(const GroupedArgs& a, const GroupTable& t, int
   s.blocks = group_blocks<MODE>(a, rows);
   int pr, pc;
   grouped_tile(tile - t.tile_base[e], group_row_tiles<MODE>(a, rows), ceil_div(a.cols, 256), kGroupRaster, pr, pc);
-  if (group_rows_on_r(MODE)) {
+  if (MODE == GroupMode::kForward) {
     s.width = group_width(rows, a.width_cap);
     s.r0 = s.row0 + pr * s.width;
     s.l0 = pc * 256;
@@ -284,65 +292,90 @@ __device__ inline void group_tile(const GroupedArgs& a, const GroupTable& t, int
   }
 }
 
-// A place in the line: the tile that iteration `it` belongs to.
-template <GroupMode MODE>
-struct GroupPlace {
-  int c, n;    // column, and number of the tile in it
-  int tile, e;
-  int begin;   // the tile's first iteration
-  int blocks;
-
-  __device__ void set_tile(const GroupedArgs& a, const GroupTable& t) {
-    tile = t.tile_of(c, n);
-    e = t.group_of(tile);
-    blocks = group_blocks<MODE>(a, t.start[e + 1] - t.start[e]);
-  }
-  // `guess`: a column near the place. it < total.
-  __device__ void find(const GroupedArgs& a, const GroupTable& t, int it, int guess) {
-    c = guess;
-    while (t.col_base[c] > it) --c;
-    while (t.col_base[c + 1] <= it) ++c;
-    if constexpr (MODE != GroupMode::kWeightGrad) {
-      n = (it - t.col_base[c]) / a.k_blocks;
-      begin = t.col_base[c] + n * a.k_blocks;
-      set_tile(a, t);
-    } else {
-      n = 0;
-      begin = t.col_base[c];
-      set_tile(a, t);
-      while (begin + blocks <= it) step(a, t);
-    }
-  }
-  __device__ void step(const GroupedArgs& a, const GroupTable& t) {
-    begin += blocks;
-    ++n;
-    while (begin >= t.col_base[c + 1]) {  // the next column that has tiles
-      ++c;
-      n = 0;
-    }
-    set_tile(a, t);
-  }
-};
-
-// The segments of one share in order.
+// The tiles of one stretch [lo, hi) of the line in order, by a whole warp: each lane works out one
+// tile of a batch of 32, since a tile's place takes about a dozen divisions (one at a time, they cost
+// the UMMA issuer half a microsecond a tile).
 template <GroupMode MODE>
 struct GroupWalk {
-  int it, lo, hi;
-  GroupPlace<MODE> place;
-  __device__ GroupWalk(const GroupedArgs& a, const GroupTable& t, int pair) {
-    lo = pair < t.shares ? t.share_begin(pair) : t.total;
-    hi = pair < t.shares ? t.share_begin(pair + 1) : t.total;
-    it = lo;
-    if (lo < hi) place.find(a, t, lo, pair);
+  int lo, hi;
+  int v;           // first tile of the next batch, counted along the line
+  int line;        // its first iteration
+  int cur, count;  // the batch's next lane, and the end of its live lanes
+  int begin;       // this lane's tile: its first iteration,
+  int tile;        // its number
+  GroupSegment mine;
+
+  // `guess`: a column near lo.
+  __device__ GroupWalk(const GroupedArgs& a, const GroupTable& t, int lo_, int hi_, int guess)
+      : lo(lo_), hi(hi_), cur(0), count(0) {
+    v = 0;
+    line = hi;
+    if (lo >= hi) return;
+    int c = guess;
+    while (t.col_base[c] > lo) --c;
+    while (t.col_base[c + 1] <= lo) ++c;
+    v = t.column_first(c);
+    line = t.col_base[c];
+    if constexpr (MODE != GroupMode::kWeightGrad) {
+      const int n = (lo - line) / a.k_blocks;
+      v += n;
+      line += n * a.k_blocks;
+    }
   }
+  // The share of `pair`.
+  __device__ GroupWalk(const GroupedArgs& a, const GroupTable& t, int pair)
+      : GroupWalk(a, t, pair < t.shares ? t.share_begin(pair) : 0, pair < t.shares ? t.share_begin(pair + 1) : 0,
+                  min(pair, t.shares - 1)) {}
+
+  __device__ void refill(const GroupedArgs& a, const GroupTable& t) {
+    const int lane = static_cast<int>(lane_id());
+    uint32_t live = 0;
+    while (live == 0 && line < hi) {  // kWeightGrad: batches before lo are passed over
+      int blocks = 0, e = 0;
+      if (v + lane < t.tiles) {
+        const int c = t.column_of(v + lane);
+        tile = t.tile_of(c, v + lane - t.column_first(c));
+        e = t.group_of(tile);
+        blocks = group_blocks<MODE>(a, t.start[e + 1] - t.start[e]);
+      }
+      int scan = blocks;
+#pragma unroll
+      for (int d = 1; d < 32; d *= 2) {
+        const int o = __shfl_up_sync(0xffffffffu, scan, d);
+        if (lane >= d) scan += o;
+      }
+      begin = line + scan - blocks;
+      const bool mine_live = blocks > 0 && begin < hi && begin + blocks > lo;
+      live = __ballot_sync(0xffffffffu, mine_live);
+      if (mine_live) {
+        group_tile<MODE>(a, t, e, tile, mine);
+        mine.kb0 = max(lo - begin, 0);
+        mine.kb1 = min(blocks, hi - begin);
+        mine.first = begin <= lo;
+      }
+      line += __shfl_sync(0xffffffffu, scan, 31);
+      v += 32;
+    }
+    cur = live != 0 ? __ffs(static_cast<int>(live)) - 1 : 0;
+    count = 32 - __clz(static_cast<int>(live));
+  }
+
   __device__ bool next(const GroupedArgs& a, const GroupTable& t, GroupSegment& s) {
-    if (it >= hi) return false;
-    if (it >= place.begin + place.blocks) place.step(a, t);
-    group_tile<MODE>(a, t, place.e, place.tile, s);
-    s.kb0 = it - place.begin;
-    s.kb1 = min(place.blocks, s.kb0 + hi - it);
-    s.first = it == lo;
-    it += s.kb1 - s.kb0;
+    if (cur >= count) {
+      refill(a, t);
+      if (cur >= count) return false;
+    }
+    const int from = cur++;
+    s.group = __shfl_sync(0xffffffffu, mine.group, from);
+    s.row0 = __shfl_sync(0xffffffffu, mine.row0, from);
+    s.row_end = __shfl_sync(0xffffffffu, mine.row_end, from);
+    s.l0 = __shfl_sync(0xffffffffu, mine.l0, from);
+    s.r0 = __shfl_sync(0xffffffffu, mine.r0, from);
+    s.width = __shfl_sync(0xffffffffu, mine.width, from);
+    s.kb0 = __shfl_sync(0xffffffffu, mine.kb0, from);
+    s.kb1 = __shfl_sync(0xffffffffu, mine.kb1, from);
+    s.blocks = __shfl_sync(0xffffffffu, mine.blocks, from);
+    s.first = __shfl_sync(0xffffffffu, static_cast<int>(mine.first), from) != 0;
     return true;
   }
 };
@@ -356,14 +389,43 @@ __device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* m
       : "memory");
 }
 
-// D (TMEM of both CTAs) (+)= A * B, E4M3 inputs, FP32 accumulator. Issued by one thread of the leader.
-__device__ __forceinline__ void umma_f8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                             uint32_t accumulate) {
+// The `steps` (1..4) UMMAs of one K block: D (TMEM of both CTAs) (+)= A * B, operands advancing by
+// LSTEP and RSTEP in descriptor units. A whole, converged warp calls it and one elected lane
+// issues: with the operands' arithmetic in code all lanes share, it stays in uniform registers,
+// which the instruction takes (issued from a branch of one lane, each UMMA cost 66 cycles).
+template <bool F8, int LSTEP, int RSTEP>
+__device__ __forceinline__ void umma_block_pair(uint32_t d, uint64_t l, uint64_t r, uint32_t idesc, uint32_t accumulate,
+                                                int steps) {
+#define HST_UMMA_BLOCK(KIND)                                                                             \
+  asm volatile(                                                                                          \
+      "{\n\t.reg .pred e, p, q;\n\t.reg .b64 l, r;\n\t"                                                  \
+      "elect.sync _|e, 0xffffffff;\n\t"                                                                  \
+      "setp.ne.b32 p, %4, 0;\n\t"                                                                        \
+      "@e tcgen05.mma.cta_group::2.kind::" KIND " [%0], %1, %2, %3, p;\n\t"                              \
+      "setp.gt.and.s32 q, %5, 1, e;\n\tadd.s64 l, %1, %6;\n\tadd.s64 r, %2, %7;\n\tsetp.eq.b32 p, 0, 0;\n\t" \
+      "@q tcgen05.mma.cta_group::2.kind::" KIND " [%0], l, r, %3, p;\n\t"                                \
+      "setp.gt.and.s32 q, %5, 2, e;\n\tadd.s64 l, l, %6;\n\tadd.s64 r, r, %7;\n\t"                       \
+      "@q tcgen05.mma.cta_group::2.kind::" KIND " [%0], l, r, %3, p;\n\t"                                \
+      "setp.gt.and.s32 q, %5, 3, e;\n\tadd.s64 l, l, %6;\n\tadd.s64 r, r, %7;\n\t"                       \
+      "@q tcgen05.mma.cta_group::2.kind::" KIND " [%0], l, r, %3, p;\n\t}\n" ::"r"(d),                   \
+      "l"(l), "l"(r), "r"(idesc), "r"(accumulate), "r"(steps), "n"(LSTEP), "n"(RSTEP)                    \
+      : "memory")
+  if constexpr (F8) {
+    HST_UMMA_BLOCK("f8f6f4");
+  } else {
+    HST_UMMA_BLOCK("f16");
+  }
+#undef HST_UMMA_BLOCK
+}
+
+// umma_commit_pair_multicast by the lane that umma_block_pair elects.
+__device__ __forceinline__ void umma_commit_elected(uint32_t bar) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred e;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}\n" ::"r"(
+          bar),
+      "h"(static_cast<uint16_t>(3))
       : "memory");
 }
 
@@ -402,16 +464,29 @@ __device__ __forceinline__ uint32_t pack_f32<__nv_bfloat16>(float lo, float hi) 
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
-// One warp's lanes are 32 consecutive output columns, v[j] the value of row `row + j`: 2-byte
-// stores, 64 consecutive bytes per row and warp.
+// One warp's lanes are 32 consecutive output columns from `col` on, v[j] the value of row `row + j`. With
+// rows of an even length neighbouring lanes trade every second row's value, so that each stores two
+// columns of one row (64 consecutive bytes per row and warp, half the stores). The whole warp.
 template <typename T, int N>
-__device__ __forceinline__ void store_rows_across(T* out, int64_t ldo, const float (&v)[N], int row, int row_end,
-                                                  int col, int cols) {
-  if (col >= cols) return;
-  T* p = out + static_cast<int64_t>(row) * ldo + col;
+__device__ __forceinline__ void store_rows_across(T* out, const GroupedArgs& a, const float (&v)[N], int row,
+                                                  int row_end, int col) {
+  const int lane = static_cast<int>(lane_id());
+  if (a.vec >= 4) {
+    const bool odd = (lane & 1) != 0;
+    uint32_t* p = reinterpret_cast<uint32_t*>(out + static_cast<int64_t>(row + (odd ? 1 : 0)) * a.cols + col + (lane & ~1));
+    const bool inside = col + (lane & ~1) < a.cols;
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    if (row + j < row_end) p[static_cast<int64_t>(j) * ldo] = from_f32<T>(v[j]);
+    for (int j = 0; j < N; j += 2) {
+      const float got = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[j + 1], 1);
+      const uint32_t w = odd ? pack_f32<T>(got, v[j + 1]) : pack_f32<T>(v[j], got);
+      if (inside && row + j + (odd ? 1 : 0) < row_end) p[static_cast<int64_t>(j) * (a.cols / 2)] = w;
+    }
+  } else if (col + lane < a.cols) {
+    T* p = out + static_cast<int64_t>(row) * a.cols + col + lane;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (row + j < row_end) p[static_cast<int64_t>(j) * a.cols] = from_f32<T>(v[j]);
+    }
   }
 }
 
@@ -497,9 +572,21 @@ __device__ __forceinline__ void store_cols_32(T* out, int64_t first, int rows, i
   }
 }
 
+// Takes `regs` registers a thread from, or gives them to, the calling warpgroup. The kernel is
+// launched with 384 x 168; 128 x 56 + 256 x 224 is the same number.
+template <int REGS>
+__device__ __forceinline__ void registers_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+template <int REGS>
+__device__ __forceinline__ void registers_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+
+// Shared memory: the ring, the barriers and the table.
 template <GroupMode MODE>
 struct GroupedShape {
-  static constexpr int kBarriers = 3 * kMaxStages + 2 * 8 + 1;
+  static constexpr int kBarriers = 3 * kMaxStages + 2 * 2 + 1;
   static constexpr int kBarrierBytes = kBarriers * 8 + 16;
   __host__ __device__ static constexpr int stage_bytes(int r_bytes) { return kGroupLBytes + r_bytes; }
   __host__ __device__ static constexpr int smem_bytes(int stages, int r_bytes, int groups, int pairs) {
@@ -513,14 +600,13 @@ template <GroupMode MODE, bool L_MN, typename T>
 __global__ void __launch_bounds__(group_threads(MODE), 1)
     grouped_gemm_kernel(const __grid_constant__ GroupedMaps maps, const __grid_constant__ GroupedArgs args) {
   using S = GroupedShape<MODE>;
-  constexpr bool kScaled = group_scaled(MODE);
+  constexpr bool kScaled = MODE == GroupMode::kScaled;
   constexpr bool kGrad = MODE == GroupMode::kWeightGrad;
+  constexpr int kFirstEpilogue = group_first_epilogue_warp(MODE);
   constexpr int kEpilogueWarps = group_epilogue_warps(MODE);
-  constexpr int kBufs = group_tmem_bufs(MODE);
-  constexpr int kBufCols = 512 / kBufs;
-  constexpr int kSteps = 4;                       // UMMA K steps of a block: 128 bytes of K
-  constexpr int kBlockK = kScaled ? 128 : 64;     // K values of a block
-  constexpr bool kBf16 = sizeof(T) == 2 && !kScaled && std::is_same<T, __nv_bfloat16>::value;
+  constexpr int kSteps = 4;                    // UMMA K steps of a block: 128 bytes of K
+  constexpr int kBlockK = kScaled ? 128 : 64;  // K values of a block
+  constexpr bool kBf16 = !kScaled && std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t kIdescBase = (1u << 4) | (kBf16 ? (1u << 7) | (1u << 10) : 0u) | (L_MN ? 1u << 15 : 0u) |
                                   (kGrad ? 1u << 16 : 0u) | ((256u >> 4) << 24);
 
@@ -533,8 +619,8 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
   uint64_t* empty = full + kMaxStages;
   uint64_t* tail_full = empty + kMaxStages;  // kWeightGrad: this CTA's own part of a block to be masked
   uint64_t* tmem_full = tail_full + kMaxStages;
-  uint64_t* tmem_empty = tmem_full + 8;
-  uint64_t* mma_done = tmem_empty + 8;
+  uint64_t* tmem_empty = tmem_full + 2;
+  uint64_t* mma_done = tmem_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* table_mem = reinterpret_cast<int*>(tmem_slot + 4);
@@ -551,15 +637,15 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
       mbar_init(&empty[s], 1);
       mbar_init(&tail_full[s], 1);
     }
-    for (int b = 0; b < kBufs; ++b) {
+    for (int b = 0; b < 2; ++b) {
       mbar_init(&tmem_full[b], 1);
       mbar_init(&tmem_empty[b], 2 * kEpilogueWarps);  // the epilogue warps of both CTAs (leader's copy)
     }
     mbar_init(mma_done, 1);
     *abort_flag = 0;
     fence_mbarrier_init();
-    tma_prefetch_map(&maps.l);
-    for (int i = 0; i < (kGrad ? 1 : 4); ++i) tma_prefetch_map(&maps.r[i]);
+    tma_prefetch_map(&maps.l[0]);
+    tma_prefetch_map(&maps.r[0]);
   }
   if (warp == 1) {
     tmem_alloc_pair(tmem_slot, 512);
@@ -573,9 +659,12 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
   const GroupTable table = group_table(args, table_mem);
+  if constexpr (kScaled) {
+    if (warp < kFirstEpilogue) registers_down<56>();
+  }
 
-  if (warp == 0 && lane == 0) {
-    // ---------------- TMA producer (both CTAs) ----------------
+  if (warp == 0) {
+    // ---------------- TMA producer (both CTAs): the warp walks, lane 0 issues ----------------
     const uint64_t policy = l2_policy_evict_normal();
     int stage = 0;
     uint32_t phase = 0;
@@ -586,70 +675,81 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
     GroupSegment s;
     while (ok && walk.next(args, table, s)) {
       const int half = s.width / 2;
-      const int box = kGrad ? 0 : group_box(half);
-      const uint32_t r_bytes = kGrad ? static_cast<uint32_t>(half) * 128u : (128u >> box) * 128u;
       const int tail = kGrad ? (s.row_end - s.row0) - (s.blocks - 1) * 64 : 0;
       const int l0 = s.l0 + static_cast<int>(rank) * 128;
       const int r0 = s.r0 + static_cast<int>(rank) * half;
+      const int box = group_box(half);
+      // kScaled: rows the tile has in this CTA, and in both; what a box of them leaves of the stage
+      // holds what it held (those lanes are not stored).
+      const int left = s.row_end - s.l0;
+      const int mine = min(128, left - static_cast<int>(rank) * 128);
+      auto box_bytes = [](int rows) { return rows <= 0 ? 0u : (128u >> group_box(rows)) * 128u; };
+      const uint32_t r_bytes = kGrad ? static_cast<uint32_t>(half) * 128u : (128u >> box) * 128u;
+      const uint32_t both_bytes = 2 * r_bytes + (kScaled ? box_bytes(left) + box_bytes(left - 128) : 2 * kGroupLBytes);
       for (int kb = s.kb0; kb < s.kb1; ++kb) {
-        if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag)) {
-          raise_abort(args.status, abort_flag, kStatusProducerTimeout);
-          ok = false;
-          break;
-        }
-        uint8_t* l_dst = ring + stage * stage_bytes;
-        uint8_t* r_dst = l_dst + kGroupLBytes;
-        const uint32_t leader_full = map_to_rank(smem_addr(&full[stage]), 0);
-        if (kGrad && kb == s.blocks - 1 && (tail & 15) != 0) {
-          // The group's last rows: into this CTA's own barrier, for the masking warp.
-          mbar_arrive_expect_tx(&tail_full[stage], kGroupLBytes + r_bytes);
-          tail_mask |= 1u << stage;
-          tail_parity ^= 1u << stage;
-          armed_mask &= ~(1u << stage);
-          const int y = s.row0 + kb * 64;
-          for (int i = 0; i < 2; ++i) tma_load_2d(l_dst + i * 8192, &maps.l, &tail_full[stage], l0 + 64 * i, y, policy);
-          for (int i = 0; i < half / 64; ++i) {
-            tma_load_2d(r_dst + i * 8192, &maps.r[0], &tail_full[stage], r0 + 64 * i, y, policy);
-          }
-        } else {
-          if (rank == 0) {
-            mbar_arrive_expect_tx(&full[stage], 2 * (kGroupLBytes + r_bytes));
-            armed_mask |= 1u << stage;
-            armed_parity = (armed_parity & ~(1u << stage)) | (phase << stage);
-          } else if (kGrad) {
-            mbar_arrive_cluster(leader_full);
-          }
-          if constexpr (kGrad) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1u, abort_flag));
+        if (!ok) break;
+        if (lane == 0) {
+          uint8_t* l_dst = ring + stage * stage_bytes;
+          uint8_t* r_dst = l_dst + kGroupLBytes;
+          const uint32_t leader_full = map_to_rank(smem_addr(&full[stage]), 0);
+          if (kGrad && kb == s.blocks - 1 && (tail & 15) != 0) {
+            // The group's last rows: into this CTA's own barrier, for the masking warp.
+            mbar_arrive_expect_tx(&tail_full[stage], kGroupLBytes + r_bytes);
+            tail_mask |= 1u << stage;
+            tail_parity ^= 1u << stage;
+            armed_mask &= ~(1u << stage);
             const int y = s.row0 + kb * 64;
-            for (int i = 0; i < 2; ++i) tma_load_2d_pair(l_dst + i * 8192, &maps.l, leader_full, l0 + 64 * i, y, policy);
+            for (int i = 0; i < 2; ++i) {
+              tma_load_2d(l_dst + i * 8192, &maps.l[0], &tail_full[stage], l0 + 64 * i, y, policy);
+            }
             for (int i = 0; i < half / 64; ++i) {
-              tma_load_2d_pair(r_dst + i * 8192, &maps.r[0], leader_full, r0 + 64 * i, y, policy);
+              tma_load_2d(r_dst + i * 8192, &maps.r[0], &tail_full[stage], r0 + 64 * i, y, policy);
             }
           } else {
-            const int k0 = kb * kBlockK;
-            if constexpr (MODE == GroupMode::kScaledWide) {
-              tma_load_2d_pair(l_dst, &maps.l, leader_full, k0, l0, policy);
-              tma_load_3d_pair(r_dst, &maps.r[box], leader_full, k0, r0, s.group, policy);
-            } else {
-              if constexpr (L_MN) {
-                for (int i = 0; i < 2; ++i) {
-                  tma_load_3d_pair(l_dst + i * 8192, &maps.l, leader_full, l0 + 64 * i, k0, s.group, policy);
-                }
-              } else {
-                tma_load_3d_pair(l_dst, &maps.l, leader_full, k0, l0, s.group, policy);
+            if (rank == 0) {
+              mbar_arrive_expect_tx(&full[stage], both_bytes);
+              armed_mask |= 1u << stage;
+              armed_parity = (armed_parity & ~(1u << stage)) | (phase << stage);
+            } else if (kGrad) {
+              mbar_arrive_cluster_relaxed(leader_full);
+            }
+            if constexpr (kGrad) {
+              const int y = s.row0 + kb * 64;
+              for (int i = 0; i < 2; ++i) {
+                tma_load_2d_pair(l_dst + i * 8192, &maps.l[0], leader_full, l0 + 64 * i, y, policy);
               }
-              tma_load_2d_pair(r_dst, &maps.r[box], leader_full, k0, r0, policy);
+              for (int i = 0; i < half / 64; ++i) {
+                tma_load_2d_pair(r_dst + i * 8192, &maps.r[0], leader_full, r0 + 64 * i, y, policy);
+              }
+            } else {
+              const int k0 = kb * kBlockK;
+              if constexpr (kScaled) {
+                if (mine > 0) tma_load_2d_pair(l_dst, &maps.l[group_box(mine)], leader_full, k0, l0, policy);
+                tma_load_3d_pair(r_dst, &maps.r[box], leader_full, k0, r0, s.group, policy);
+              } else {
+                if constexpr (L_MN) {
+                  for (int i = 0; i < 2; ++i) {
+                    tma_load_3d_pair(l_dst + i * 8192, &maps.l[0], leader_full, l0 + 64 * i, k0, s.group, policy);
+                  }
+                } else {
+                  tma_load_3d_pair(l_dst, &maps.l[0], leader_full, k0, l0, s.group, policy);
+                }
+                tma_load_2d_pair(r_dst, &maps.r[box], leader_full, k0, r0, policy);
+              }
             }
           }
         }
+        __syncwarp();
         if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
         }
       }
     }
-    if (!ok) {  // drain the copies in flight before the pair can exit
-      for (int st = 0; st < stages; ++st) {
+    if (!ok && lane == 0) {
+      raise_abort(args.status, abort_flag, kStatusProducerTimeout);
+      for (int st = 0; st < stages; ++st) {  // drain the copies in flight before the pair can exit
         if (rank == 0 && (armed_mask & (1u << st)) &&
             !mbar_wait(&full[st], (armed_parity >> st) & 1u, nullptr, 200000000ull)) {
           atomicOr(args.status, kStatusDrainTimeout);
@@ -660,8 +760,8 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
         }
       }
     }
-  } else if (warp == 1 && lane == 0 && rank == 0) {
-    // ---------------- UMMA issuer (leader only) ----------------
+  } else if (warp == 1 && rank == 0) {
+    // ---------------- UMMA issuer (leader only): the warp walks, lane 0 issues ----------------
     int stage = 0;
     uint32_t phase = 0;
     int buf = 0;
@@ -669,7 +769,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
     bool ok = true;
     const uint64_t l_desc0 = smem_desc(smem_addr(ring), L_MN ? 8192 : 16, 1024);
     const uint64_t r_desc0 = smem_desc(smem_addr(ring) + kGroupLBytes, kGrad ? 8192 : 16, 1024);
-    constexpr uint32_t kLStep = (L_MN ? 2048 : 32) >> 4, kRStep = (kGrad ? 2048 : 32) >> 4;
+    constexpr int kLStep = (L_MN ? 2048 : 32) >> 4, kRStep = (kGrad ? 2048 : 32) >> 4;
     GroupWalk<MODE> walk(args, table, pair);
     GroupSegment s;
     while (ok && walk.next(args, table, s)) {
@@ -677,75 +777,60 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
       const int tail = kGrad ? (s.row_end - s.row0) - (s.blocks - 1) * 64 : 0;
       for (int kb = s.kb0; kb < s.kb1; ++kb) {
         if (kScaled || kb == s.kb0) {
-          if (!mbar_wait(&tmem_empty[buf], buf_phase ^ 1u, abort_flag)) {
-            raise_abort(args.status, abort_flag, kStatusMmaTimeout);
-            ok = false;
-            break;
-          }
+          ok = __all_sync(0xffffffffu, mbar_wait(&tmem_empty[buf], buf_phase ^ 1u, abort_flag));
+          if (!ok) break;
           tc_fence_after_sync();
         }
-        // kWeightGrad: the peer's masking warp wrote its shared memory (cluster-scope acquire).
-        if (!(kGrad ? mbar_wait_cluster(&full[stage], phase, abort_flag) : mbar_wait(&full[stage], phase, abort_flag))) {
-          raise_abort(args.status, abort_flag, kStatusMmaTimeout);
-          ok = false;
-          break;
-        }
+        // A masked block: the peer's masking warp wrote its shared memory, which takes an acquire at
+        // cluster scope (1.0 us a block when every wait was one, against 0.5).
+        const bool masked = kGrad && kb == s.blocks - 1 && (tail & 15) != 0;
+        ok = __all_sync(0xffffffffu, masked ? mbar_wait_cluster(&full[stage], phase, abort_flag)
+                                            : mbar_wait(&full[stage], phase, abort_flag));
+        if (!ok) break;
         tc_fence_after_sync();
         const uint64_t off = static_cast<uint64_t>(stage * (stage_bytes >> 4));
         const int steps = kGrad && kb == s.blocks - 1 ? (tail + 15) / 16 : kSteps;
-        const uint32_t d = tmem_base + static_cast<uint32_t>(buf * kBufCols);
-#pragma unroll
-        for (int kk = 0; kk < kSteps; ++kk) {
-          if (kk < steps) {
-            const uint32_t accumulate = kScaled ? (kk != 0) : (kb != s.kb0 || kk != 0);
-            if constexpr (kScaled) {
-              umma_f8_pair(d, l_desc0 + off + kk * kLStep, r_desc0 + off + kk * kRStep, idesc, accumulate);
-            } else {
-              umma_f16_pair(d, l_desc0 + off + kk * kLStep, r_desc0 + off + kk * kRStep, idesc, accumulate);
-            }
-          }
-        }
-        umma_commit_pair_multicast(smem_addr(&empty[stage]), 3);
+        umma_block_pair<kScaled, kLStep, kRStep>(tmem_base + static_cast<uint32_t>(buf * 256), l_desc0 + off, r_desc0 + off,
+                                                 idesc, !kScaled && kb != s.kb0, steps);
+        umma_commit_elected(smem_addr(&empty[stage]));
         if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
         }
         if (kScaled || kb + 1 == s.kb1) {
-          umma_commit_pair_multicast(smem_addr(&tmem_full[buf]), 3);
-          if (++buf == kBufs) {
-            buf = 0;
-            buf_phase ^= 1u;
-          }
+          umma_commit_elected(smem_addr(&tmem_full[buf]));
+          buf ^= 1;
+          if (buf == 0) buf_phase ^= 1u;
         }
       }
     }
-    umma_commit_pair(smem_addr(mma_done));
-    if (!mbar_wait(mma_done, 0, nullptr, 200000000ull)) atomicOr(args.status, kStatusDrainTimeout);
-  } else if (kGrad && warp == 6) {
+    if (!ok && lane == 0) raise_abort(args.status, abort_flag, kStatusMmaTimeout);
+    umma_commit_elected(smem_addr(mma_done));
+    if (!mbar_wait(mma_done, 0, nullptr, 200000000ull) && lane == 0) atomicOr(args.status, kStatusDrainTimeout);
+  } else if (kGrad && warp == kFirstEpilogue + kEpilogueWarps) {
     // ---------------- masking warp (both CTAs): rows past the group in its last block ----------
     int stage = 0;
     uint32_t parity = 0;  // bit s: parity of the next use of tail_full[s]
     GroupWalk<MODE> walk(args, table, pair);
     GroupSegment s;
-    bool ok = true;
-    while (ok && walk.next(args, table, s)) {
+    while (walk.next(args, table, s)) {
       const int blocks = s.kb1 - s.kb0;
       const int tail = (s.row_end - s.row0) - (s.blocks - 1) * 64;
       if (s.kb1 == s.blocks && (tail & 15) != 0) {
         const int st = (stage + blocks - 1) % stages;
-        ok = __all_sync(0xffffffffu, mbar_wait(&tail_full[st], (parity >> st) & 1u, abort_flag));
-        if (!ok) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&tail_full[st], (parity >> st) & 1u, abort_flag))) {
           if (lane == 0) raise_abort(args.status, abort_flag, kStatusEpilogueTimeout);
           break;
         }
         parity ^= 1u << st;
-        // A box is 64 rows of 128 bytes; the swizzle moves 16-byte chunks within a row only.
-        const int from = tail, count = ((tail + 15) & ~15) - tail;
-        const int boxes = 2 + s.width / 128;
-        const uint32_t st_addr = smem_addr(ring + st * stage_bytes);
-        for (int i = static_cast<int>(lane); i < boxes * count * 8; i += 32) {
-          const int chunk = i & 7, r = (i >> 3) % count, b = (i >> 3) / count;
-          st_shared_v4(st_addr + b * 8192 + (from + r) * 128 + chunk * 16, 0, 0, 0, 0);
+        // A box is 64 rows of 128 bytes; the swizzle moves 16-byte chunks within a row only. One
+        // 512-byte store of the warp clears four rows.
+        const int end = (tail + 15) & ~15;
+        const uint32_t st_addr = smem_addr(ring + st * stage_bytes) + (lane & 7u) * 16;
+        for (int b = 0; b < 2 + s.width / 128; ++b) {
+          for (int r = tail + static_cast<int>(lane >> 3); r < end; r += 4) {
+            st_shared_v4(st_addr + b * 8192 + r * 128, 0, 0, 0, 0);
+          }
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -753,8 +838,9 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
       }
       stage = (stage + blocks) % stages;
     }
-  } else if (warp >= 2 && warp < 2 + kEpilogueWarps) {
+  } else if (warp >= kFirstEpilogue && warp < kFirstEpilogue + kEpilogueWarps) {
     // ---------------- epilogue (both CTAs, own 128 TMEM lanes) ----------------
+    if constexpr (kScaled) registers_up<224>();
     const int quarter = warp & 3;
     const int row = quarter * 32 + static_cast<int>(lane);  // TMEM lane
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
@@ -777,10 +863,8 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
           mbar_arrive_cluster_relaxed(map_to_rank(smem_addr(&tmem_empty[buf]), 0));
         }
       }
-      if (++buf == kBufs) {
-        buf = 0;
-        buf_phase ^= 1u;
-      }
+      buf ^= 1;
+      if (buf == 0) buf_phase ^= 1u;
     };
     auto piece_of = [&](const GroupSegment& s) {
       return args.partials +
@@ -791,146 +875,129 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
     if constexpr (!kScaled) {
       while (walk.next(args, table, s)) {
         if (!wait_buf()) break;
-        const uint32_t taddr = lane_base + static_cast<uint32_t>(buf * kBufCols);
-        const int l = s.l0 + static_cast<int>(rank) * 128 + row;
+        const uint32_t taddr = lane_base + static_cast<uint32_t>(buf * 256);
+        const int l32 = s.l0 + static_cast<int>(rank) * 128 + quarter * 32;  // the warp's first L row
         const bool whole = s.kb0 == 0 && s.kb1 == s.blocks;
-#pragma unroll 1
-        for (int c = 0; c < s.width; c += 32) {
-          uint32_t v[32];
-          tmem_ld_32x32b_x32(taddr + c, v);
-          tmem_ld_wait();
+        // 32 columns at a time, the next ones in flight while these are stored.
+        uint32_t v[2][32];
+        tmem_ld_32x32b_x32(taddr, v[0]);
+        tmem_ld_wait();
+        tmem_ld_fence_regs(v[0]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int c = 32 * i;
+          if (c >= s.width) break;
+          uint32_t(&now)[32] = v[i & 1];
+          if (c + 32 < s.width) {
+            tmem_ld_32x32b_x32(taddr + c + 32, v[(i & 1) ^ 1]);
+          }
           if (!whole) {
             float* dst = piece_of(s) + (static_cast<size_t>(c / 4) * 128 + row) * 4;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              st_global_v4(dst + static_cast<size_t>(j) * 512, v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+              st_global_v4(dst + static_cast<size_t>(j) * 512, now[4 * j], now[4 * j + 1], now[4 * j + 2], now[4 * j + 3]);
             }
-          } else if constexpr (kGrad) {
-            float f[32];
-#pragma unroll
-            for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
-            const int l32 = l - static_cast<int>(lane);
-            store_cols_32(out, static_cast<int64_t>(s.group) * args.lrows + l32, args.lrows - l32, s.r0 + c, args, f);
           } else {
             float f[32];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[j]);
-            store_rows_across(out, args.cols, f, s.r0 + c, min(s.row_end, s.r0 + s.width), l, args.cols);
+            for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(now[j]);
+            if constexpr (kGrad) {
+              store_cols_32(out, static_cast<int64_t>(s.group) * args.lrows + l32, args.lrows - l32, s.r0 + c, args, f);
+            } else {
+              store_rows_across(out, args, f, s.r0 + c, min(s.row_end, s.r0 + s.width), l32);
+            }
           }
+          tmem_ld_wait();
+          tmem_ld_fence_regs(v[(i & 1) ^ 1]);
         }
         release_buf();
       }
-    } else if constexpr (MODE == GroupMode::kScaledWide) {
-      const int half = (warp - 2) / 4;  // 128 of the tile's 256 columns
+    } else {
+      // Two warps share a TMEM quarter, each with 128 of the tile's 256 columns: one weight scale a
+      // block. The scales of four blocks are fetched while the four before are in use.
+      const int side = (warp - kFirstEpilogue) / 4;
       while (walk.next(args, table, s)) {
-        const int t = s.l0 + static_cast<int>(rank) * 128 + row;
-        const bool live = half * 128 < s.width && s.r0 + half * 128 < args.cols;
-        const float* sa = args.row_scales + static_cast<int64_t>(min(t, args.rows - 1)) * args.rs_row;
-        const float* sb = args.tile_scales + s.group * args.ts_group + ((s.r0 >> 7) + (live ? half : 0)) * args.ts_n;
+        const int l32 = s.l0 + static_cast<int>(rank) * 128 + quarter * 32;
+        const int col = s.r0 + side * 128;
+        const bool live = l32 < s.row_end && col < args.cols;  // warp-uniform
+        const float* sa = args.row_scales + static_cast<int64_t>(min(l32 + static_cast<int>(lane), args.rows - 1)) * args.rs_row;
+        const float* sb = args.tile_scales + s.group * args.ts_group + (min(col, args.cols - 1) >> 7) * args.ts_n;
+        float scale[4], next_a[4], next_b[4];
+        auto fetch = [&](int kb4) {  // the scales of blocks kb4 to kb4 + 3
+          if (args.rs_vec && kb4 + 4 <= s.blocks) {
+            const float4 f = *reinterpret_cast<const float4*>(sa + kb4);
+            next_a[0] = f.x; next_a[1] = f.y; next_a[2] = f.z; next_a[3] = f.w;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) next_a[i] = sa[min(kb4 + i, s.blocks - 1) * args.rs_k];
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) next_b[i] = sb[min(kb4 + i, s.blocks - 1) * args.ts_k];
+        };
+        if (live) fetch(s.kb0 & ~3);
         uint64_t acc[64];
 #pragma unroll
         for (int j = 0; j < 64; ++j) acc[j] = 0;
-        float scale = sa[s.kb0 * args.rs_k] * sb[s.kb0 * args.ts_k];
         bool ready = true;
         for (int kb = s.kb0; kb < s.kb1; ++kb) {
-          const int ahead = min(kb + 1, s.kb1 - 1);
-          const float next_a = sa[ahead * args.rs_k], next_b = sb[ahead * args.ts_k];
+          if (live && (kb == s.kb0 || (kb & 3) == 0)) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) scale[i] = next_a[i] * next_b[i];
+            for (int i = kb & 3; i > 0; --i) {  // a segment that begins inside four blocks
+              scale[0] = scale[1];
+              scale[1] = scale[2];
+              scale[2] = scale[3];
+            }
+            if ((kb | 3) + 1 < s.kb1) fetch((kb | 3) + 1);
+          }
           ready = wait_buf();
           if (!ready) break;
           if (live) {
-            const uint64_t scale2 = pack_b32x2(__float_as_uint(scale), __float_as_uint(scale));
-            const uint32_t taddr = lane_base + static_cast<uint32_t>(buf * kBufCols + half * 128);
-            uint32_t v[2][16];
-            tmem_ld_32x32b_x16(taddr, v[0]);
+            const uint64_t scale2 = pack_b32x2(__float_as_uint(scale[0]), __float_as_uint(scale[0]));
+            scale[0] = scale[1];
+            scale[1] = scale[2];
+            scale[2] = scale[3];
+            const uint32_t taddr = lane_base + static_cast<uint32_t>(buf * 256 + side * 128);
+            uint32_t v[2][32];
+            tmem_ld_32x32b_x32(taddr, v[0]);
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
+            for (int i = 0; i < 4; ++i) {
               tmem_ld_wait();
-              tmem_ld_fence_regs(v[c & 1]);
-              if (c < 7) tmem_ld_32x32b_x16(taddr + (c + 1) * 16, v[(c + 1) & 1]);
+              tmem_ld_fence_regs(v[i & 1]);
+              if (i < 3) {
+                tmem_ld_32x32b_x32(taddr + 32 * (i + 1), v[(i + 1) & 1]);
+              } else {
+                release_buf();
+              }
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                fma_f32x2(acc[8 * c + j], pack_b32x2(v[c & 1][2 * j], v[c & 1][2 * j + 1]), scale2);
+              for (int j = 0; j < 16; ++j) {
+                fma_f32x2(acc[16 * i + j], pack_b32x2(v[i & 1][2 * j], v[i & 1][2 * j + 1]), scale2);
               }
             }
+          } else {
+            release_buf();
           }
-          release_buf();
-          scale = next_a * next_b;
         }
         if (!ready) break;
         if (!live) continue;
-        if (s.kb0 == 0 && s.kb1 == s.blocks) {
-          const int t32 = t - static_cast<int>(lane);
+        const bool whole = s.kb0 == 0 && s.kb1 == s.blocks;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
+        for (int i = 0; i < 4; ++i) {
+          if (whole) {
             float f[32];
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-              f[2 * j] = __uint_as_float(static_cast<uint32_t>(acc[16 * c + j]));
-              f[2 * j + 1] = __uint_as_float(static_cast<uint32_t>(acc[16 * c + j] >> 32));
+              f[2 * j] = __uint_as_float(static_cast<uint32_t>(acc[16 * i + j]));
+              f[2 * j + 1] = __uint_as_float(static_cast<uint32_t>(acc[16 * i + j] >> 32));
             }
-            store_cols_32(out, t32, s.row_end - t32, s.r0 + half * 128 + 32 * c, args, f);
-          }
-        } else {
-          float* dst = piece_of(s) + (static_cast<size_t>(half * 32) * 128 + row) * 4;
+            store_cols_32(out, l32, s.row_end - l32, col + 32 * i, args, f);
+          } else {
+            float* dst = piece_of(s) + (static_cast<size_t>((side * 128 + 32 * i) / 4) * 128 + row) * 4;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            st_global_v4(dst + static_cast<size_t>(j) * 512, static_cast<uint32_t>(acc[2 * j]),
-                         static_cast<uint32_t>(acc[2 * j] >> 32), static_cast<uint32_t>(acc[2 * j + 1]),
-                         static_cast<uint32_t>(acc[2 * j + 1] >> 32));
-          }
-        }
-      }
-    } else {
-      while (walk.next(args, table, s)) {
-        const int l = s.l0 + static_cast<int>(rank) * 128 + row;
-        const int valid = min(s.row_end - s.r0, s.width);  // rows of the tile
-        // This CTA's 128 output columns share one weight scale per block.
-        const int nb = min((s.l0 >> 7) + static_cast<int>(rank), (args.cols - 1) >> 7);
-        const float* sb = args.tile_scales + s.group * args.ts_group + nb * args.ts_n;
-        // Lane j holds the scales of rows j and j + 32.
-        const float* sa0 = args.row_scales + static_cast<int64_t>(min(s.r0 + static_cast<int>(lane), args.rows - 1)) * args.rs_row;
-        const float* sa1 =
-            args.row_scales + static_cast<int64_t>(min(s.r0 + 32 + static_cast<int>(lane), args.rows - 1)) * args.rs_row;
-        float acc[64];
-#pragma unroll
-        for (int j = 0; j < 64; ++j) acc[j] = 0.f;
-        float a0 = sa0[s.kb0 * args.rs_k], a1 = sa1[s.kb0 * args.rs_k], b = sb[s.kb0 * args.ts_k];
-        bool ready = true;
-        for (int kb = s.kb0; kb < s.kb1; ++kb) {
-          const int ahead = min(kb + 1, s.kb1 - 1);
-          const float next_a0 = sa0[ahead * args.rs_k], next_a1 = sa1[ahead * args.rs_k], next_b = sb[ahead * args.ts_k];
-          ready = wait_buf();
-          if (!ready) break;
-          const uint32_t taddr = lane_base + static_cast<uint32_t>(buf * kBufCols);
-          const float s0 = a0 * b, s1 = a1 * b;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            if (c * 16 < valid) {  // warp-uniform
-              uint32_t v[16];
-              tmem_ld_32x32b_x16(taddr + c * 16, v);
-              tmem_ld_wait();
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                const float sc = __shfl_sync(0xffffffffu, c < 2 ? s0 : s1, (c & 1) * 16 + j);
-                acc[16 * c + j] = fmaf(__uint_as_float(v[j]), sc, acc[16 * c + j]);
-              }
-            }
-          }
-          release_buf();
-          a0 = next_a0;
-          a1 = next_a1;
-          b = next_b;
-        }
-        if (!ready) break;
-        if (s.kb0 == 0 && s.kb1 == s.blocks) {
-          store_rows_across(out, args.cols, acc, s.r0, s.r0 + valid, l, args.cols);
-        } else {
-          float* dst = piece_of(s) + static_cast<size_t>(row) * 4;
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            if (4 * j < s.width) {
-              st_global_v4(dst + static_cast<size_t>(j) * 512, __float_as_uint(acc[4 * j]), __float_as_uint(acc[4 * j + 1]),
-                           __float_as_uint(acc[4 * j + 2]), __float_as_uint(acc[4 * j + 3]));
+            for (int j = 0; j < 8; ++j) {
+              st_global_v4(dst + static_cast<size_t>(j) * 512, static_cast<uint32_t>(acc[16 * i + 2 * j]),
+                           static_cast<uint32_t>(acc[16 * i + 2 * j] >> 32), static_cast<uint32_t>(acc[16 * i + 2 * j + 1]),
+                           static_cast<uint32_t>(acc[16 * i + 2 * j + 1] >> 32));
             }
           }
         }
@@ -967,19 +1034,18 @@ __global__ void __launch_bounds__(kFinishThreads) grouped_finish_kernel(const __
   const int rank = static_cast<int>(blockIdx.y);
   if (p < table.shares) {
     const int cut = table.share_begin(p);
-    GroupPlace<MODE> place;
-    place.find(args, table, cut, p);
-    const int end = place.begin + place.blocks;
+    GroupWalk<MODE> walk(args, table, cut, cut + 1, p);
     GroupSegment s;
-    group_tile<MODE>(args, table, place.e, place.tile, s);
+    walk.next(args, table, s);
+    const int begin = cut - s.kb0, end = begin + s.blocks;
     const int c = static_cast<int>(blockIdx.z) * kFinishCols;
-    if (cut > place.begin && table.share_begin(p - 1) <= place.begin && c < s.width) {
+    if (cut > begin && table.share_begin(p - 1) <= begin && c < s.width) {
       const int row = static_cast<int>(threadIdx.x);
       float v[kFinishCols];
 #pragma unroll
       for (int j = 0; j < kFinishCols; ++j) v[j] = 0.f;
       for (int o = p - 1; o < table.shares && table.share_begin(o) < end; ++o) {
-        const int piece = table.share_begin(o) >= place.begin ? 0 : 1;
+        const int piece = table.share_begin(o) >= begin ? 0 : 1;
         const float* src = args.partials +
                            (static_cast<size_t>(o * 2 + piece) * 2 + rank) * static_cast<size_t>(args.piece_floats) +
                            (static_cast<size_t>(c / 4) * 128 + row) * 4;
@@ -992,13 +1058,12 @@ __global__ void __launch_bounds__(kFinishThreads) grouped_finish_kernel(const __
           v[4 * j + 3] += f.w;
         }
       }
-      const int l = s.l0 + rank * 128 + row;
-      if constexpr (group_rows_on_r(MODE)) {
-        store_rows_across(out, args.cols, v, s.r0 + c, min(s.row_end, s.r0 + s.width), l, args.cols);
+      const int l32 = s.l0 + rank * 128 + (row & ~31);
+      if constexpr (MODE == GroupMode::kForward) {
+        store_rows_across(out, args, v, s.r0 + c, min(s.row_end, s.r0 + s.width), l32);
       } else {
-        const int l32 = l - static_cast<int>(lane_id());
         const bool grad = MODE == GroupMode::kWeightGrad;
-        store_cols_32(out, grad ? static_cast<int64_t>(place.e) * args.lrows + l32 : l32,
+        store_cols_32(out, grad ? static_cast<int64_t>(s.group) * args.lrows + l32 : l32,
                       (grad ? args.lrows : s.row_end) - l32, s.r0 + c, args, v);
       }
     }

@@ -18,11 +18,8 @@ struct GroupedProblem {
   int64_t cols;      // output columns
   int64_t lrows;     // kWeightGrad: rows of one output
   int64_t k_blocks;  // forward, scaled
-  int width_cap;
+  int width_cap;     // columns of a piece; kForward: most rows in a tile
 };
-
-// Rows on the R side of a kScaledStream tile: the epilogue keeps that many FP32 sums a thread.
-constexpr int kStreamWidth = 64;
 
 int check_groups(const char* what, int64_t rows, int32_t groups, const void* ends) {
   if (groups < 1 || groups > kMaxGroups)
@@ -51,8 +48,7 @@ template <GroupMode MODE>
 int64_t max_iterations(const GroupedProblem& p) {
   const int64_t cols = cdiv(p.cols, 256);
   if (MODE == GroupMode::kWeightGrad) return cols * cdiv(p.lrows, 256) * (p.rows / 64 + p.groups);
-  const int64_t tiles = group_rows_on_r(MODE) ? p.rows / p.width_cap + p.groups : p.rows / 256 + p.groups;
-  return cols * std::min(tiles, p.rows) * p.k_blocks;
+  return cols * std::min(p.rows / (MODE == GroupMode::kForward ? p.width_cap : 256) + p.groups, p.rows) * p.k_blocks;
 }
 
 // Iterations a share has at least: below it, joining a tile's pieces costs more than another pair
@@ -65,13 +61,8 @@ int plan_pairs(const GroupedProblem& p, int sms) {
 }
 
 template <GroupMode MODE>
-int piece_floats(const GroupedProblem& p) {
-  return 128 * (group_rows_on_r(MODE) ? p.width_cap : 256);
-}
-
-template <GroupMode MODE>
 size_t workspace_bytes(const GroupedProblem& p, int sms) {
-  return static_cast<size_t>(plan_pairs<MODE>(p, sms)) * 4 * piece_floats<MODE>(p) * sizeof(float);
+  return static_cast<size_t>(plan_pairs<MODE>(p, sms)) * 4 * 128 * p.width_cap * sizeof(float);
 }
 
 int width_cap(int64_t rows, int most) { return static_cast<int>(std::min<int64_t>(most, round_up(std::max<int64_t>(rows, 1), 32))); }
@@ -100,7 +91,7 @@ int launch_grouped(const GroupedProblem& p, const GroupedMaps& maps, GroupedArgs
   while (args.vec > 2 && (p.cols * 2 % args.vec != 0 || reinterpret_cast<uintptr_t>(args.out) % args.vec != 0)) args.vec /= 2;
   args.status = dev->status;
   args.partials = static_cast<float*>(workspace);
-  args.piece_floats = piece_floats<MODE>(p);
+  args.piece_floats = 128 * p.width_cap;
   int stages = kMaxStages;
   while (stages > 2 && S::smem_bytes(stages, r_bytes, p.groups, args.pairs) > kMaxDynamicSmem) --stages;
   args.stages = stages;
@@ -172,11 +163,8 @@ GroupedProblem forward_problem(int64_t rows, int groups, int64_t n, int64_t k) {
 GroupedProblem grad_problem(int64_t rows, int groups, int64_t lcols, int64_t rcols) {
   return GroupedProblem{rows, groups, rcols, lcols, 0, 256};
 }
-// Few rows a group: the weights stream past on the L side. From 64 rows a group on average the wide
-// form's cheaper promotion pays for the part of its 256-row tiles that stays empty.
-bool scaled_streams(int64_t rows, int groups) { return rows <= static_cast<int64_t>(kStreamWidth) * groups; }
 GroupedProblem scaled_problem(int64_t rows, int groups, int64_t n, int64_t k) {
-  return GroupedProblem{rows, groups, n, 0, cdiv(k, 128), width_cap(rows, kStreamWidth)};
+  return GroupedProblem{rows, groups, n, 0, cdiv(k, 128), 256};
 }
 
 }  // namespace
@@ -200,12 +188,9 @@ int hst_grouped_workspace_size(int32_t op, int64_t rows, int32_t groups, int64_t
     case HST_GROUPED_WEIGHT_GRAD:
       *bytes = workspace_bytes<GroupMode::kWeightGrad>(grad_problem(rows, groups, k, n), sms);
       return HST_OK;
-    case HST_GROUPED_SCALED: {
-      const GroupedProblem p = scaled_problem(rows, groups, n, k);
-      *bytes = scaled_streams(rows, groups) ? workspace_bytes<GroupMode::kScaledStream>(p, sms)
-                                            : workspace_bytes<GroupMode::kScaledWide>(p, sms);
+    case HST_GROUPED_SCALED:
+      *bytes = workspace_bytes<GroupMode::kScaled>(scaled_problem(rows, groups, n, k), sms);
       return HST_OK;
-    }
     default:
       return fail(HST_ERR_INVALID, "unknown grouped product %d", op);
   }
@@ -229,7 +214,7 @@ int hst_grouped_matmul(int32_t dtype, const void* x, int64_t ldx, const void* w,
   if (groups > 1 && (w_group % 8 != 0 || w_group < 8)) return fail(HST_ERR_INVALID, "w's group stride must be a positive multiple of 8");
   const GroupedProblem p = forward_problem(rows, groups, n, k);
   GroupedMaps maps = {};
-  HST_TRY(encode_weights(&maps.l, map_type(dtype), 2, w, groups, outer, inner, w_group, ldw, kn ? 64 : 128));
+  HST_TRY(encode_weights(&maps.l[0], map_type(dtype), 2, w, groups, outer, inner, w_group, ldw, kn ? 64 : 128));
   for (int i = 0; i < 4; ++i) HST_TRY(encode_rows(&maps.r[i], map_type(dtype), 2, x, rows, k, ldx, box_rows_of(i)));
   GroupedArgs args = {};
   args.ends = ends;
@@ -260,7 +245,7 @@ int hst_grouped_weight_grad(int32_t dtype, const void* left, int64_t ldl, const 
   HST_TRY(check_operand("right", right, ldr, rcols, 2));
   const GroupedProblem p = grad_problem(rows, groups, lcols, rcols);
   GroupedMaps maps = {};
-  HST_TRY(encode_rows(&maps.l, map_type(dtype), 2, left, rows, lcols, ldl, 64));
+  HST_TRY(encode_rows(&maps.l[0], map_type(dtype), 2, left, rows, lcols, ldl, 64));
   HST_TRY(encode_rows(&maps.r[0], map_type(dtype), 2, right, rows, rcols, ldr, 64));
   GroupedArgs args = {};
   args.ends = ends;
@@ -286,38 +271,25 @@ int hst_matmul_blockscaled(int32_t out_dtype, const void* a, int64_t lda, const 
   HST_TRY(check_operand("b", b, ldb, k, 1));
   if (a_scales == nullptr || b_scales == nullptr) return fail(HST_ERR_INVALID, "scales are null");
   if (groups > 1 && (b_group % 16 != 0 || b_group < 16)) return fail(HST_ERR_INVALID, "b's group stride must be a positive multiple of 16");
-  const bool streams = scaled_streams(rows, groups);
   const GroupedProblem p = scaled_problem(rows, groups, n, k);
   const CUtensorMapDataType type = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   GroupedMaps maps = {};
-  if (streams) {
-    HST_TRY(encode_weights(&maps.l, type, 1, b, groups, n, k, b_group, ldb, 128));
-    for (int i = 0; i < 4; ++i) HST_TRY(encode_rows(&maps.r[i], type, 1, a, rows, k, lda, box_rows_of(i)));
-  } else {
-    HST_TRY(encode_rows(&maps.l, type, 1, a, rows, k, lda, 128));
-    for (int i = 0; i < 4; ++i) HST_TRY(encode_weights(&maps.r[i], type, 1, b, groups, n, k, b_group, ldb, box_rows_of(i)));
-  }
+  for (int i = 0; i < 4; ++i) HST_TRY(encode_rows(&maps.l[i], type, 1, a, rows, k, lda, box_rows_of(i)));
+  for (int i = 0; i < 2; ++i) HST_TRY(encode_weights(&maps.r[i], type, 1, b, groups, n, k, b_group, ldb, box_rows_of(i)));
   GroupedArgs args = {};
   args.ends = ends;
   args.out = y;
   args.row_scales = a_scales;
   args.rs_row = sa_row;
   args.rs_k = sa_block;
+  args.rs_vec = sa_block == 1 && sa_row % 4 == 0 && (reinterpret_cast<uintptr_t>(a_scales) & 15) == 0;
   args.tile_scales = b_scales;
   args.ts_group = sb_group;
   args.ts_n = sb_row;
   args.ts_k = sb_block;
-  const int r_bytes = streams ? box_rows_of(group_box(p.width_cap / 2)) * 128 : 16384;
-#define HST_SCALED_CASE(DT_, T_)                                                                                       \
-  if (out_dtype == DT_) {                                                                                              \
-    if (streams)                                                                                                       \
-      return launch_grouped<GroupMode::kScaledStream, false, T_>(p, maps, args, r_bytes, workspace, workspace_bytes, s); \
-    return launch_grouped<GroupMode::kScaledWide, false, T_>(p, maps, args, r_bytes, workspace, workspace_bytes, s);   \
-  }
-  HST_SCALED_CASE(HST_F16, __half)
-  HST_SCALED_CASE(HST_BF16, __nv_bfloat16)
-#undef HST_SCALED_CASE
-  return HST_ERR_UNSUPPORTED;
+  if (out_dtype == HST_F16)
+    return launch_grouped<GroupMode::kScaled, false, __half>(p, maps, args, 16384, workspace, workspace_bytes, s);
+  return launch_grouped<GroupMode::kScaled, false, __nv_bfloat16>(p, maps, args, 16384, workspace, workspace_bytes, s);
 }
 
 int hst_quantize_e4m3(int32_t dtype, int32_t tiles, const void* x, int64_t x_batch, int64_t x_row, int64_t x_col,
