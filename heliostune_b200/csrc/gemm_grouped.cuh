@@ -22,10 +22,11 @@
 //     not issued.
 //   * kScaled accumulates each 128-deep block in a TMEM buffer of its own; the epilogue warps read
 //     it, multiply by the block's scales and add it to FP32 registers, while the next block's UMMAs
-//     fill the other buffer. The rows are on the L side, where a row is a TMEM lane and its scale
-//     one register: with the rows on the R side the scales were 128 a thread and block, and their
-//     broadcast loads from shared memory, beside the UMMAs' operands, took three times the UMMAs'
-//     time (1.5 us a block of 256 rows against 0.5).
+//     fill another buffer. A tile's two 128-column halves go separate ways: each has its issuing
+//     warp, its two buffers and its four epilogue warps. The rows are on the L side, where a row is a
+//     TMEM lane and its scale one register: with the rows on the R side the scales were 128 a thread
+//     and block, and their broadcast loads from shared memory, beside the UMMAs' operands, took three
+//     times the UMMAs' time.
 //
 // Schedule: all (tile, K block) iterations of all groups in one line, cut into one equal share per
 // pair (GroupTable). A tile cut by a share's end leaves FP32 pieces in the workspace, which a second
@@ -50,17 +51,17 @@ constexpr int kMaxGroups = 1024;
 constexpr int kGroupLBytes = 16384;  // 128 L rows x 128 bytes of K (or 2 boxes of 64 x 64)
 constexpr int kGroupRaster = 8;      // row tiles before the next column tile
 
-// Warps: 0 loads, 1 issues the UMMAs; then the epilogue, and for kWeightGrad the masking warp. kScaled
-// holds 128 x 256 FP32 sums in the registers of 8 epilogue warps, which therefore form warpgroups
-// of their own (2 and 3 idle).
+// Warps: 0 loads, 1 issues the UMMAs (kScaled: and 2, one a half); then the epilogue, and for
+// kWeightGrad the masking warp. kScaled holds 128 x 256 FP32 sums in the registers of 8 epilogue
+// warps, which therefore form warpgroups of their own (3 idle).
 __host__ __device__ constexpr int group_first_epilogue_warp(GroupMode m) { return m == GroupMode::kScaled ? 4 : 2; }
 __host__ __device__ constexpr int group_epilogue_warps(GroupMode m) { return m == GroupMode::kScaled ? 8 : 4; }
 __host__ __device__ constexpr int group_threads(GroupMode m) {
   return 32 * (group_first_epilogue_warp(m) + group_epilogue_warps(m) + (m == GroupMode::kWeightGrad ? 1 : 0));
 }
 
-// Boxes of 128, 64, 32 and 16 rows on the side that needs them (kForward: R, kScaled: L), else one
-// (kScaled's R: 128 and 64; kWeightGrad: 64 x 64).
+// Boxes of 128, 64, 32 and 16 rows on the side that needs them (kForward: R, kScaled: L), else one in
+// [0] (kScaled's R: 64 rows; kWeightGrad: 64 x 64).
 struct GroupedMaps {
   CUtensorMap l[4];
   CUtensorMap r[4];
@@ -380,12 +381,47 @@ struct GroupWalk {
   }
 };
 
-__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* map, uint32_t bar_cluster_addr,
-                                                 int32_t x, int32_t y, int32_t z, uint64_t policy) {
+// Forms of the loads and of the barrier arrivals for a whole, converged warp: one elected lane
+// performs them. Their operands then come from code all lanes share and stay in uniform registers,
+// which TMA takes: from a branch of one lane a load cost about 130 cycles.
+__device__ __forceinline__ void elected_load_3d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar_cluster,
+                                                     int32_t x, int32_t y, int32_t z) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      ".L2::cache_hint [%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(smem_addr(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster_addr), "r"(x), "r"(y), "r"(z), "l"(policy)
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];\n\t}\n" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+__device__ __forceinline__ void elected_load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar_cluster,
+                                                     int32_t x, int32_t y) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];\n\t}\n" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(x), "r"(y)
+      : "memory");
+}
+// Into this CTA, completing on its own barrier.
+__device__ __forceinline__ void elected_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int32_t x, int32_t y) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];\n\t}\n" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void elected_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}\n" ::"r"(bar),
+      "r"(bytes)
+      : "memory");
+}
+__device__ __forceinline__ void elected_arrive_cluster_relaxed(uint32_t bar_cluster) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n\t}\n" ::"r"(bar_cluster)
       : "memory");
 }
 
@@ -433,14 +469,6 @@ __device__ __forceinline__ void umma_commit_elected(uint32_t bar) {
 // memory itself.
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
-// acc (two FP32 values) += p * s, both halves by the same pair of scales.
-__device__ __forceinline__ void fma_f32x2(uint64_t& acc, uint64_t p, uint64_t s) {
-  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(p), "l"(s));
-}
-__device__ __forceinline__ uint64_t pack_b32x2(uint32_t lo, uint32_t hi) {
-  return static_cast<uint64_t>(hi) << 32 | lo;
-}
 
 template <typename T>
 __device__ __forceinline__ T from_f32(float v);
@@ -586,7 +614,7 @@ __device__ __forceinline__ void registers_up() {
 // Shared memory: the ring, the barriers and the table.
 template <GroupMode MODE>
 struct GroupedShape {
-  static constexpr int kBarriers = 3 * kMaxStages + 2 * 2 + 1;
+  static constexpr int kBarriers = 3 * kMaxStages + 2 * 4 + 1;
   static constexpr int kBarrierBytes = kBarriers * 8 + 16;
   __host__ __device__ static constexpr int stage_bytes(int r_bytes) { return kGroupLBytes + r_bytes; }
   __host__ __device__ static constexpr int smem_bytes(int stages, int r_bytes, int groups, int pairs) {
@@ -607,6 +635,9 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
   constexpr int kSteps = 4;                    // UMMA K steps of a block: 128 bytes of K
   constexpr int kBlockK = kScaled ? 128 : 64;  // K values of a block
   constexpr bool kBf16 = !kScaled && std::is_same<T, __nv_bfloat16>::value;
+  constexpr int kIssuers = kScaled ? 2 : 1;    // warps issuing UMMAs, one a half of the tile
+  constexpr int kBufs = 2 * kIssuers;          // TMEM buffers; half h uses 2h and 2h + 1
+  constexpr int kBufCols = 512 / kBufs;
   constexpr uint32_t kIdescBase = (1u << 4) | (kBf16 ? (1u << 7) | (1u << 10) : 0u) | (L_MN ? 1u << 15 : 0u) |
                                   (kGrad ? 1u << 16 : 0u) | ((256u >> 4) << 24);
 
@@ -619,8 +650,8 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
   uint64_t* empty = full + kMaxStages;
   uint64_t* tail_full = empty + kMaxStages;  // kWeightGrad: this CTA's own part of a block to be masked
   uint64_t* tmem_full = tail_full + kMaxStages;
-  uint64_t* tmem_empty = tmem_full + 2;
-  uint64_t* mma_done = tmem_empty + 2;
+  uint64_t* tmem_empty = tmem_full + 4;
+  uint64_t* mma_done = tmem_empty + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* table_mem = reinterpret_cast<int*>(tmem_slot + 4);
@@ -634,14 +665,14 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], kGrad ? 2 : 1);  // kWeightGrad: both CTAs report each stage
-      mbar_init(&empty[s], 1);
+      mbar_init(&empty[s], kIssuers);
       mbar_init(&tail_full[s], 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < kBufs; ++b) {
       mbar_init(&tmem_full[b], 1);
-      mbar_init(&tmem_empty[b], 2 * kEpilogueWarps);  // the epilogue warps of both CTAs (leader's copy)
+      mbar_init(&tmem_empty[b], 8);  // four epilogue warps of each CTA (leader's copy)
     }
-    mbar_init(mma_done, 1);
+    mbar_init(mma_done, kIssuers);
     *abort_flag = 0;
     fence_mbarrier_init();
     tma_prefetch_map(&maps.l[0]);
@@ -664,11 +695,10 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
   }
 
   if (warp == 0) {
-    // ---------------- TMA producer (both CTAs): the warp walks, lane 0 issues ----------------
-    const uint64_t policy = l2_policy_evict_normal();
+    // ---------------- TMA producer (both CTAs) ----------------
     int stage = 0;
     uint32_t phase = 0;
-    uint32_t armed_mask = 0, armed_parity = 0;  // stages this thread has armed (leader)
+    uint32_t armed_mask = 0, armed_parity = 0;  // stages this warp has armed (leader)
     uint32_t tail_mask = 0, tail_parity = 0;    // tail barriers used; parity of their next use
     bool ok = true;
     GroupWalk<MODE> walk(args, table, pair);
@@ -677,70 +707,61 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
       const int half = s.width / 2;
       const int tail = kGrad ? (s.row_end - s.row0) - (s.blocks - 1) * 64 : 0;
       const int l0 = s.l0 + static_cast<int>(rank) * 128;
-      const int r0 = s.r0 + static_cast<int>(rank) * half;
-      const int box = group_box(half);
+      const int r0 = s.r0 + static_cast<int>(rank) * (kScaled ? 64 : half);
       // kScaled: rows the tile has in this CTA, and in both; what a box of them leaves of the stage
       // holds what it held (those lanes are not stored).
       const int left = s.row_end - s.l0;
       const int mine = min(128, left - static_cast<int>(rank) * 128);
       auto box_bytes = [](int rows) { return rows <= 0 ? 0u : (128u >> group_box(rows)) * 128u; };
-      const uint32_t r_bytes = kGrad ? static_cast<uint32_t>(half) * 128u : (128u >> box) * 128u;
+      const CUtensorMap* l_map = &maps.l[kScaled ? group_box(mine) : 0];
+      const CUtensorMap* r_map = &maps.r[MODE == GroupMode::kForward ? group_box(half) : 0];
+      const uint32_t r_bytes = MODE == GroupMode::kForward ? box_bytes(half) : static_cast<uint32_t>(half) * 128u;
       const uint32_t both_bytes = 2 * r_bytes + (kScaled ? box_bytes(left) + box_bytes(left - 128) : 2 * kGroupLBytes);
       for (int kb = s.kb0; kb < s.kb1; ++kb) {
         ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1u, abort_flag));
         if (!ok) break;
-        if (lane == 0) {
-          uint8_t* l_dst = ring + stage * stage_bytes;
-          uint8_t* r_dst = l_dst + kGroupLBytes;
-          const uint32_t leader_full = map_to_rank(smem_addr(&full[stage]), 0);
-          if (kGrad && kb == s.blocks - 1 && (tail & 15) != 0) {
-            // The group's last rows: into this CTA's own barrier, for the masking warp.
-            mbar_arrive_expect_tx(&tail_full[stage], kGroupLBytes + r_bytes);
-            tail_mask |= 1u << stage;
-            tail_parity ^= 1u << stage;
-            armed_mask &= ~(1u << stage);
+        const uint32_t l_dst = smem_addr(ring) + static_cast<uint32_t>(stage * stage_bytes);
+        const uint32_t r_dst = l_dst + kGroupLBytes;
+        const uint32_t leader_full = map_to_rank(smem_addr(&full[stage]), 0);
+        if (kGrad && kb == s.blocks - 1 && (tail & 15) != 0) {
+          // The group's last rows: into this CTA's own barrier, for the masking warp.
+          const uint32_t bar = smem_addr(&tail_full[stage]);
+          elected_expect_tx(bar, kGroupLBytes + r_bytes);
+          tail_mask |= 1u << stage;
+          tail_parity ^= 1u << stage;
+          armed_mask &= ~(1u << stage);
+          const int y = s.row0 + kb * 64;
+          for (int i = 0; i < 2; ++i) elected_load_2d(l_dst + i * 8192, l_map, bar, l0 + 64 * i, y);
+          for (int i = 0; i < half / 64; ++i) elected_load_2d(r_dst + i * 8192, r_map, bar, r0 + 64 * i, y);
+        } else {
+          if (rank == 0) {
+            elected_expect_tx(smem_addr(&full[stage]), both_bytes);
+            armed_mask |= 1u << stage;
+            armed_parity = (armed_parity & ~(1u << stage)) | (phase << stage);
+          } else if (kGrad) {
+            elected_arrive_cluster_relaxed(leader_full);
+          }
+          if constexpr (kGrad) {
             const int y = s.row0 + kb * 64;
-            for (int i = 0; i < 2; ++i) {
-              tma_load_2d(l_dst + i * 8192, &maps.l[0], &tail_full[stage], l0 + 64 * i, y, policy);
-            }
-            for (int i = 0; i < half / 64; ++i) {
-              tma_load_2d(r_dst + i * 8192, &maps.r[0], &tail_full[stage], r0 + 64 * i, y, policy);
-            }
+            for (int i = 0; i < 2; ++i) elected_load_2d_pair(l_dst + i * 8192, l_map, leader_full, l0 + 64 * i, y);
+            for (int i = 0; i < half / 64; ++i) elected_load_2d_pair(r_dst + i * 8192, r_map, leader_full, r0 + 64 * i, y);
           } else {
-            if (rank == 0) {
-              mbar_arrive_expect_tx(&full[stage], both_bytes);
-              armed_mask |= 1u << stage;
-              armed_parity = (armed_parity & ~(1u << stage)) | (phase << stage);
-            } else if (kGrad) {
-              mbar_arrive_cluster_relaxed(leader_full);
-            }
-            if constexpr (kGrad) {
-              const int y = s.row0 + kb * 64;
-              for (int i = 0; i < 2; ++i) {
-                tma_load_2d_pair(l_dst + i * 8192, &maps.l[0], leader_full, l0 + 64 * i, y, policy);
-              }
-              for (int i = 0; i < half / 64; ++i) {
-                tma_load_2d_pair(r_dst + i * 8192, &maps.r[0], leader_full, r0 + 64 * i, y, policy);
+            const int k0 = kb * kBlockK;
+            if constexpr (kScaled) {
+              if (mine > 0) elected_load_2d_pair(l_dst, l_map, leader_full, k0, l0);
+              for (int h = 0; h < s.width / 128; ++h) {
+                elected_load_3d_pair(r_dst + h * 8192, r_map, leader_full, k0, r0 + h * 128, s.group);
               }
             } else {
-              const int k0 = kb * kBlockK;
-              if constexpr (kScaled) {
-                if (mine > 0) tma_load_2d_pair(l_dst, &maps.l[group_box(mine)], leader_full, k0, l0, policy);
-                tma_load_3d_pair(r_dst, &maps.r[box], leader_full, k0, r0, s.group, policy);
+              if constexpr (L_MN) {
+                for (int i = 0; i < 2; ++i) elected_load_3d_pair(l_dst + i * 8192, l_map, leader_full, l0 + 64 * i, k0, s.group);
               } else {
-                if constexpr (L_MN) {
-                  for (int i = 0; i < 2; ++i) {
-                    tma_load_3d_pair(l_dst + i * 8192, &maps.l[0], leader_full, l0 + 64 * i, k0, s.group, policy);
-                  }
-                } else {
-                  tma_load_3d_pair(l_dst, &maps.l[0], leader_full, k0, l0, s.group, policy);
-                }
-                tma_load_2d_pair(r_dst, &maps.r[box], leader_full, k0, r0, policy);
+                elected_load_3d_pair(l_dst, l_map, leader_full, k0, l0, s.group);
               }
+              elected_load_2d_pair(r_dst, r_map, leader_full, k0, r0);
             }
           }
         }
-        __syncwarp();
         if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
@@ -760,24 +781,26 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
         }
       }
     }
-  } else if (warp == 1 && rank == 0) {
-    // ---------------- UMMA issuer (leader only): the warp walks, lane 0 issues ----------------
+  } else if (warp <= kIssuers && rank == 0) {
+    // ---------------- UMMA issuers (leader only) ----------------
+    const int side = warp - 1;  // kScaled: the half of the tile's columns
     int stage = 0;
     uint32_t phase = 0;
     int buf = 0;
     uint32_t buf_phase = 0;
     bool ok = true;
     const uint64_t l_desc0 = smem_desc(smem_addr(ring), L_MN ? 8192 : 16, 1024);
-    const uint64_t r_desc0 = smem_desc(smem_addr(ring) + kGroupLBytes, kGrad ? 8192 : 16, 1024);
+    const uint64_t r_desc0 = smem_desc(smem_addr(ring) + kGroupLBytes + side * 8192, kGrad ? 8192 : 16, 1024);
     constexpr int kLStep = (L_MN ? 2048 : 32) >> 4, kRStep = (kGrad ? 2048 : 32) >> 4;
     GroupWalk<MODE> walk(args, table, pair);
     GroupSegment s;
     while (ok && walk.next(args, table, s)) {
-      const uint32_t idesc = kIdescBase | (static_cast<uint32_t>(s.width >> 3) << 17);
+      const uint32_t idesc = kIdescBase | (static_cast<uint32_t>((kScaled ? 128 : s.width) >> 3) << 17);
+      const bool active = !kScaled || side * 128 < s.width;
       const int tail = kGrad ? (s.row_end - s.row0) - (s.blocks - 1) * 64 : 0;
       for (int kb = s.kb0; kb < s.kb1; ++kb) {
-        if (kScaled || kb == s.kb0) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&tmem_empty[buf], buf_phase ^ 1u, abort_flag));
+        if (active && (kScaled || kb == s.kb0)) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&tmem_empty[2 * side + buf], buf_phase ^ 1u, abort_flag));
           if (!ok) break;
           tc_fence_after_sync();
         }
@@ -790,15 +813,17 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
         tc_fence_after_sync();
         const uint64_t off = static_cast<uint64_t>(stage * (stage_bytes >> 4));
         const int steps = kGrad && kb == s.blocks - 1 ? (tail + 15) / 16 : kSteps;
-        umma_block_pair<kScaled, kLStep, kRStep>(tmem_base + static_cast<uint32_t>(buf * 256), l_desc0 + off, r_desc0 + off,
-                                                 idesc, !kScaled && kb != s.kb0, steps);
+        if (active) {
+          umma_block_pair<kScaled, kLStep, kRStep>(tmem_base + static_cast<uint32_t>((2 * side + buf) * kBufCols),
+                                                   l_desc0 + off, r_desc0 + off, idesc, !kScaled && kb != s.kb0, steps);
+        }
         umma_commit_elected(smem_addr(&empty[stage]));
         if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
         }
-        if (kScaled || kb + 1 == s.kb1) {
-          umma_commit_elected(smem_addr(&tmem_full[buf]));
+        if (active && (kScaled || kb + 1 == s.kb1)) {
+          umma_commit_elected(smem_addr(&tmem_full[2 * side + buf]));
           buf ^= 1;
           if (buf == 0) buf_phase ^= 1u;
         }
@@ -845,10 +870,11 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
     const int row = quarter * 32 + static_cast<int>(lane);  // TMEM lane
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
     T* out = static_cast<T*>(args.out);
+    const int side = kScaled ? (warp - kFirstEpilogue) / 4 : 0;  // the half of the tile's columns
     int buf = 0;
     uint32_t buf_phase = 0;
     auto wait_buf = [&]() {
-      const bool ready = __all_sync(0xffffffffu, mbar_wait(&tmem_full[buf], buf_phase, abort_flag));
+      const bool ready = __all_sync(0xffffffffu, mbar_wait(&tmem_full[2 * side + buf], buf_phase, abort_flag));
       if (!ready && lane == 0) raise_abort(args.status, abort_flag, kStatusEpilogueTimeout);
       if (ready) tc_fence_after_sync();
       return ready;
@@ -858,9 +884,9 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
       __syncwarp();
       if (lane == 0) {
         if (rank == 0) {
-          mbar_arrive_relaxed(&tmem_empty[buf]);
+          mbar_arrive_relaxed(&tmem_empty[2 * side + buf]);
         } else {
-          mbar_arrive_cluster_relaxed(map_to_rank(smem_addr(&tmem_empty[buf]), 0));
+          mbar_arrive_cluster_relaxed(map_to_rank(smem_addr(&tmem_empty[2 * side + buf]), 0));
         }
       }
       buf ^= 1;
@@ -875,7 +901,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
     if constexpr (!kScaled) {
       while (walk.next(args, table, s)) {
         if (!wait_buf()) break;
-        const uint32_t taddr = lane_base + static_cast<uint32_t>(buf * 256);
+        const uint32_t taddr = lane_base + static_cast<uint32_t>(buf * kBufCols);
         const int l32 = s.l0 + static_cast<int>(rank) * 128 + quarter * 32;  // the warp's first L row
         const bool whole = s.kb0 == 0 && s.kb1 == s.blocks;
         // 32 columns at a time, the next ones in flight while these are stored.
@@ -913,10 +939,10 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
         release_buf();
       }
     } else {
-      // Two warps share a TMEM quarter, each with 128 of the tile's 256 columns: one weight scale a
-      // block. The scales of four blocks are fetched while the four before are in use.
-      const int side = (warp - kFirstEpilogue) / 4;
+      // One weight scale a block for the 128 columns of a half. The scales of four blocks are fetched
+      // while the four before are in use.
       while (walk.next(args, table, s)) {
+        if (side * 128 >= s.width) continue;
         const int l32 = s.l0 + static_cast<int>(rank) * 128 + quarter * 32;
         const int col = s.r0 + side * 128;
         const bool live = l32 < s.row_end && col < args.cols;  // warp-uniform
@@ -935,9 +961,9 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
           for (int i = 0; i < 4; ++i) next_b[i] = sb[min(kb4 + i, s.blocks - 1) * args.ts_k];
         };
         if (live) fetch(s.kb0 & ~3);
-        uint64_t acc[64];
+        float acc[128];
 #pragma unroll
-        for (int j = 0; j < 64; ++j) acc[j] = 0;
+        for (int j = 0; j < 128; ++j) acc[j] = 0.f;
         bool ready = true;
         for (int kb = s.kb0; kb < s.kb1; ++kb) {
           if (live && (kb == s.kb0 || (kb & 3) == 0)) {
@@ -953,11 +979,11 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
           ready = wait_buf();
           if (!ready) break;
           if (live) {
-            const uint64_t scale2 = pack_b32x2(__float_as_uint(scale[0]), __float_as_uint(scale[0]));
+            const float now = scale[0];
             scale[0] = scale[1];
             scale[1] = scale[2];
             scale[2] = scale[3];
-            const uint32_t taddr = lane_base + static_cast<uint32_t>(buf * 256 + side * 128);
+            const uint32_t taddr = lane_base + static_cast<uint32_t>((2 * side + buf) * kBufCols);
             uint32_t v[2][32];
             tmem_ld_32x32b_x32(taddr, v[0]);
 #pragma unroll
@@ -970,9 +996,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
                 release_buf();
               }
 #pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                fma_f32x2(acc[16 * i + j], pack_b32x2(v[i & 1][2 * j], v[i & 1][2 * j + 1]), scale2);
-              }
+              for (int j = 0; j < 32; ++j) acc[32 * i + j] = fmaf(__uint_as_float(v[i & 1][j]), now, acc[32 * i + j]);
             }
           } else {
             release_buf();
@@ -986,18 +1010,15 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
           if (whole) {
             float f[32];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              f[2 * j] = __uint_as_float(static_cast<uint32_t>(acc[16 * i + j]));
-              f[2 * j + 1] = __uint_as_float(static_cast<uint32_t>(acc[16 * i + j] >> 32));
-            }
+            for (int j = 0; j < 32; ++j) f[j] = acc[32 * i + j];
             store_cols_32(out, l32, s.row_end - l32, col + 32 * i, args, f);
           } else {
             float* dst = piece_of(s) + (static_cast<size_t>((side * 128 + 32 * i) / 4) * 128 + row) * 4;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              st_global_v4(dst + static_cast<size_t>(j) * 512, static_cast<uint32_t>(acc[16 * i + 2 * j]),
-                           static_cast<uint32_t>(acc[16 * i + 2 * j] >> 32), static_cast<uint32_t>(acc[16 * i + 2 * j + 1]),
-                           static_cast<uint32_t>(acc[16 * i + 2 * j + 1] >> 32));
+              const int k = 32 * i + 4 * j;
+              st_global_v4(dst + static_cast<size_t>(j) * 512, __float_as_uint(acc[k]), __float_as_uint(acc[k + 1]),
+                           __float_as_uint(acc[k + 2]), __float_as_uint(acc[k + 3]));
             }
           }
         }

@@ -275,7 +275,7 @@ int hst_matmul_blockscaled(int32_t out_dtype, const void* a, int64_t lda, const 
   const CUtensorMapDataType type = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   GroupedMaps maps = {};
   for (int i = 0; i < 4; ++i) HST_TRY(encode_rows(&maps.l[i], type, 1, a, rows, k, lda, box_rows_of(i)));
-  for (int i = 0; i < 2; ++i) HST_TRY(encode_weights(&maps.r[i], type, 1, b, groups, n, k, b_group, ldb, box_rows_of(i)));
+  HST_TRY(encode_weights(&maps.r[0], type, 1, b, groups, n, k, b_group, ldb, 64));
   GroupedArgs args = {};
   args.ends = ends;
   args.out = y;
