@@ -1,12 +1,12 @@
 // Matrix products over rows grouped by expert, on CTA pairs (tcgen05.mma.cta_group::2).
 //
 // Group e owns rows [ends[e - 1], ends[e]) of a row matrix; `ends` lives on the GPU, so nothing
-// about the sizes is known on the host. Three products share this kernel:
+// about the sizes is known on the host. Three products, in four forms, share this kernel:
 //   kForward     y[t, :] = x[t, :] W[e(t)]           16-bit x [T, K], W [E, K, N] (either of its two
 //                                                    inner dimensions contiguous)
 //   kWeightGrad  D[e] = L[rows of e]^T R[rows of e]   16-bit L [T, Lc], R [T, Rc]
-//   kScaled      y[t, n] = sum_b sa[t, b] sb[e, n/128, b] sum_{k in block b} a[t, k] b[e, n, k]
-//                                                    E4M3 a [T, K], b [E, N, K], FP32 scales of 128
+//   kScaled and  y[t, n] = sum_b sa[t, b] sb[e, n/128, b] sum_{k in block b} a[t, k] b[e, n, k]
+//   kScaledFew                                       E4M3 a [T, K], b [E, N, K], FP32 scales of 128
 //                                                    (a) and 128 x 128 (b) values
 //
 // One pair of CTAs computes a 256 x width tile: CTA r owns 128 rows of the L operand and half of
@@ -24,9 +24,12 @@
 //     it, multiply by the block's scales and add it to FP32 registers, while the next block's UMMAs
 //     fill another buffer. A tile's two 128-column halves go separate ways: each has its issuing
 //     warp, its two buffers and its four epilogue warps. The rows are on the L side, where a row is a
-//     TMEM lane and its scale one register: with the rows on the R side the scales were 128 a thread
-//     and block, and their broadcast loads from shared memory, beside the UMMAs' operands, took three
-//     times the UMMAs' time.
+//     TMEM lane and its scale one register: on the R side the scales of 256 rows are 128 a thread and
+//     block, and their broadcast loads from shared memory, beside the UMMAs' operands, took three times
+//     the UMMAs' time.
+//   * kScaledFew is for few rows a group: as kForward, weights on the L side and at most 64 rows on
+//     the R side, in eight TMEM buffers. A block then costs 64 to 128 UMMA cycles instead of 512 and
+//     keeps all lanes busy, and the weights stream at the rate of HBM.
 //
 // Schedule: all (tile, K block) iterations of all groups in one line, cut into one equal share per
 // pair (GroupTable). A tile cut by a share's end leaves FP32 pieces in the workspace, which a second
@@ -45,7 +48,10 @@
 
 namespace hst {
 
-enum class GroupMode { kForward, kWeightGrad, kScaled };
+enum class GroupMode { kForward, kWeightGrad, kScaled, kScaledFew };
+__host__ __device__ constexpr bool group_scaled(GroupMode m) { return m == GroupMode::kScaled || m == GroupMode::kScaledFew; }
+// The rows are on the R side.
+__host__ __device__ constexpr bool group_rows_right(GroupMode m) { return m == GroupMode::kForward || m == GroupMode::kScaledFew; }
 
 constexpr int kMaxGroups = 1024;
 constexpr int kGroupLBytes = 16384;  // 128 L rows x 128 bytes of K (or 2 boxes of 64 x 64)
@@ -60,7 +66,7 @@ __host__ __device__ constexpr int group_threads(GroupMode m) {
   return 32 * (group_first_epilogue_warp(m) + group_epilogue_warps(m) + (m == GroupMode::kWeightGrad ? 1 : 0));
 }
 
-// Boxes of 128, 64, 32 and 16 rows on the side that needs them (kForward: R, kScaled: L), else one in
+// Boxes of 128, 64, 32 and 16 rows on the side that has the rows (kForward, kScaledFew: R; kScaled: L), else one in
 // [0] (kScaled's R: 64 rows; kWeightGrad: 64 x 64).
 struct GroupedMaps {
   CUtensorMap l[4];
@@ -74,7 +80,7 @@ struct GroupedArgs {
   int cols;             // columns of the output
   int lrows;            // kWeightGrad: rows of one group's output
   int k_blocks;         // K blocks of a tile (kWeightGrad: by group)
-  int width_cap;        // kForward: most rows in a tile (a multiple of 32)
+  int width_cap;        // rows on the R side: most of them in a tile (a multiple of 32)
   int stages;
   int r_bytes;          // bytes of the R operand's part of a stage
   int pairs;            // CTA pairs launched
@@ -86,7 +92,6 @@ struct GroupedArgs {
   int piece_floats;
   const float* row_scales;  // sa: strides below, in elements
   int64_t rs_row, rs_k;
-  int rs_vec;               // sa is stored by rows, four values at a time
   const float* tile_scales;  // sb
   int64_t ts_group, ts_n, ts_k;
 };
@@ -106,7 +111,7 @@ __host__ __device__ inline int group_box(int rows) { return rows > 64 ? 0 : (row
 template <GroupMode MODE>
 __host__ __device__ inline int group_row_tiles(const GroupedArgs& a, int rows) {
   if (rows <= 0) return 0;
-  if (MODE == GroupMode::kForward) return ceil_div(rows, group_width(rows, a.width_cap));
+  if (group_rows_right(MODE)) return ceil_div(rows, group_width(rows, a.width_cap));
   return ceil_div(MODE == GroupMode::kWeightGrad ? a.lrows : rows, 256);
 }
 
@@ -126,6 +131,7 @@ __host__ __device__ inline int group_blocks(const GroupedArgs& a, int rows) {
 struct GroupTable {
   const int* start;      // [groups + 1] first row of each group
   const int* tile_base;  // [groups + 1] first tile of each group
+  const int* row_tiles;  // [groups] tiles of a column of each group's output
   const int* col_base;   // [pairs + 1] first iteration of each column
   int groups;
   int tiles, shares, total;
@@ -152,7 +158,7 @@ struct GroupTable {
   }
 };
 
-constexpr __host__ __device__ int group_table_ints(int groups, int pairs) { return 2 * (groups + 1) + pairs + 1 + 4; }
+constexpr __host__ __device__ int group_table_ints(int groups, int pairs) { return 3 * (groups + 1) + pairs + 1 + 4; }
 
 // Builds the table in shared memory. Ends are taken as they would be if clamped to
 // [previous end, rows], so no value of `ends` leads out of the matrices. All threads of the block
@@ -161,7 +167,9 @@ template <GroupMode MODE>
 __device__ inline void build_group_rows(const GroupedArgs& a, int* mem) {
   int* start = mem;
   int* tile_base = start + a.groups + 1;
+  int* row_tiles = tile_base + a.groups + 1;
   const int lane = static_cast<int>(lane_id());
+  const int col_tiles = ceil_div(a.cols, 256);
   int row = 0, tiles = 0, total = 0;
   for (int g0 = 0; g0 < a.groups; g0 += 32) {
     const int g = g0 + lane;
@@ -175,7 +183,8 @@ __device__ inline void build_group_rows(const GroupedArgs& a, int* mem) {
     end = max(end, row);
     int begin = __shfl_up_sync(0xffffffffu, end, 1);
     if (lane == 0) begin = row;
-    const int mine = g < a.groups ? group_row_tiles<MODE>(a, end - begin) * ceil_div(a.cols, 256) : 0;
+    const int high = g < a.groups ? group_row_tiles<MODE>(a, end - begin) : 0;
+    const int mine = high * col_tiles;
     int sum = mine;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
@@ -186,6 +195,7 @@ __device__ inline void build_group_rows(const GroupedArgs& a, int* mem) {
     if (g < a.groups) {
       start[g] = begin;
       tile_base[g] = tiles + sum - mine;
+      row_tiles[g] = high;
     }
     row = __shfl_sync(0xffffffffu, end, 31);
     tiles += __shfl_sync(0xffffffffu, sum, 31);
@@ -193,7 +203,7 @@ __device__ inline void build_group_rows(const GroupedArgs& a, int* mem) {
   if (lane == 0) {
     start[a.groups] = row;
     tile_base[a.groups] = tiles;
-    int* head = mem + 2 * (a.groups + 1) + a.pairs + 1;
+    int* head = mem + 3 * (a.groups + 1) + a.pairs + 1;
     head[0] = tiles;
     head[1] = max(1, min(a.pairs, total / a.min_blocks));
     head[2] = total;
@@ -204,7 +214,8 @@ __device__ inline GroupTable group_table(const GroupedArgs& a, const int* mem) {
   GroupTable t;
   t.start = mem;
   t.tile_base = mem + a.groups + 1;
-  t.col_base = t.tile_base + a.groups + 1;
+  t.row_tiles = t.tile_base + a.groups + 1;
+  t.col_base = t.row_tiles + a.groups + 1;
   t.groups = a.groups;
   const int* head = t.col_base + a.pairs + 1;
   t.tiles = head[0];
@@ -219,7 +230,7 @@ __device__ inline GroupTable group_table(const GroupedArgs& a, const int* mem) {
 template <GroupMode MODE>
 __device__ inline void build_group_columns(const GroupedArgs& a, int* mem) {
   const GroupTable t = group_table(a, mem);
-  int* col_base = mem + 2 * (a.groups + 1);
+  int* col_base = mem + 3 * (a.groups + 1);
   if constexpr (MODE != GroupMode::kWeightGrad) {
     for (int c = static_cast<int>(threadIdx.x); c <= t.shares; c += static_cast<int>(blockDim.x)) {
       col_base[c] = t.column_first(c) * a.k_blocks;
@@ -272,24 +283,25 @@ struct GroupSegment {
   bool first;         // the share's first segment
 };
 
-// Tile `tile` of group `e`: where it lies.
+// Width of a tile of a group of `rows` rows whose first R column is r0.
 template <GroupMode MODE>
-__device__ inline void group_tile(const GroupedArgs& a, const GroupTable& t, int e, int tile, GroupSegment& s) {
-  s.group = e;
-  s.row0 = t.start[e];
-  s.row_end = t.start[e + 1];
-  const int rows = s.row_end - s.row0;
-  s.blocks = group_blocks<MODE>(a, rows);
+__device__ inline int tile_width(const GroupedArgs& a, int rows, int r0) {
+  if (group_rows_right(MODE)) return group_width(rows, a.width_cap);
+  return a.cols - r0 <= 128 ? 128 : 256;
+}
+
+// First L row and R column of tile `tile` of group `e`.
+template <GroupMode MODE>
+__device__ inline void tile_origin(const GroupedArgs& a, const GroupTable& t, int e, int tile, int& l0, int& r0) {
+  const int row0 = t.start[e];
   int pr, pc;
-  grouped_tile(tile - t.tile_base[e], group_row_tiles<MODE>(a, rows), ceil_div(a.cols, 256), kGroupRaster, pr, pc);
-  if (MODE == GroupMode::kForward) {
-    s.width = group_width(rows, a.width_cap);
-    s.r0 = s.row0 + pr * s.width;
-    s.l0 = pc * 256;
+  grouped_tile(tile - t.tile_base[e], t.row_tiles[e], ceil_div(a.cols, 256), kGroupRaster, pr, pc);
+  if (group_rows_right(MODE)) {
+    r0 = row0 + pr * group_width(t.start[e + 1] - row0, a.width_cap);
+    l0 = pc * 256;
   } else {
-    s.l0 = (MODE == GroupMode::kWeightGrad ? 0 : s.row0) + pr * 256;
-    s.r0 = pc * 256;
-    s.width = a.cols - s.r0 <= 128 ? 128 : 256;
+    l0 = (MODE == GroupMode::kWeightGrad ? 0 : row0) + pr * 256;
+    r0 = pc * 256;
   }
 }
 
@@ -302,9 +314,8 @@ struct GroupWalk {
   int v;           // first tile of the next batch, counted along the line
   int line;        // its first iteration
   int cur, count;  // the batch's next lane, and the end of its live lanes
-  int begin;       // this lane's tile: its first iteration,
-  int tile;        // its number
-  GroupSegment mine;
+  // This lane's tile: its group (negative, ~group, if it begins the stretch), origin and K blocks.
+  int group, l0, r0, kb0, kb1;
 
   // `guess`: a column near lo.
   __device__ GroupWalk(const GroupedArgs& a, const GroupTable& t, int lo_, int hi_, int guess)
@@ -332,7 +343,7 @@ struct GroupWalk {
     const int lane = static_cast<int>(lane_id());
     uint32_t live = 0;
     while (live == 0 && line < hi) {  // kWeightGrad: batches before lo are passed over
-      int blocks = 0, e = 0;
+      int blocks = 0, e = 0, tile = 0;
       if (v + lane < t.tiles) {
         const int c = t.column_of(v + lane);
         tile = t.tile_of(c, v + lane - t.column_first(c));
@@ -345,14 +356,14 @@ struct GroupWalk {
         const int o = __shfl_up_sync(0xffffffffu, scan, d);
         if (lane >= d) scan += o;
       }
-      begin = line + scan - blocks;
+      const int begin = line + scan - blocks;
       const bool mine_live = blocks > 0 && begin < hi && begin + blocks > lo;
       live = __ballot_sync(0xffffffffu, mine_live);
       if (mine_live) {
-        group_tile<MODE>(a, t, e, tile, mine);
-        mine.kb0 = max(lo - begin, 0);
-        mine.kb1 = min(blocks, hi - begin);
-        mine.first = begin <= lo;
+        tile_origin<MODE>(a, t, e, tile, l0, r0);
+        group = begin <= lo ? ~e : e;
+        kb0 = max(lo - begin, 0);
+        kb1 = min(blocks, hi - begin);
       }
       line += __shfl_sync(0xffffffffu, scan, 31);
       v += 32;
@@ -367,16 +378,17 @@ struct GroupWalk {
       if (cur >= count) return false;
     }
     const int from = cur++;
-    s.group = __shfl_sync(0xffffffffu, mine.group, from);
-    s.row0 = __shfl_sync(0xffffffffu, mine.row0, from);
-    s.row_end = __shfl_sync(0xffffffffu, mine.row_end, from);
-    s.l0 = __shfl_sync(0xffffffffu, mine.l0, from);
-    s.r0 = __shfl_sync(0xffffffffu, mine.r0, from);
-    s.width = __shfl_sync(0xffffffffu, mine.width, from);
-    s.kb0 = __shfl_sync(0xffffffffu, mine.kb0, from);
-    s.kb1 = __shfl_sync(0xffffffffu, mine.kb1, from);
-    s.blocks = __shfl_sync(0xffffffffu, mine.blocks, from);
-    s.first = __shfl_sync(0xffffffffu, static_cast<int>(mine.first), from) != 0;
+    const int g = __shfl_sync(0xffffffffu, group, from);
+    s.first = g < 0;
+    s.group = s.first ? ~g : g;
+    s.l0 = __shfl_sync(0xffffffffu, l0, from);
+    s.r0 = __shfl_sync(0xffffffffu, r0, from);
+    s.kb0 = __shfl_sync(0xffffffffu, kb0, from);
+    s.kb1 = __shfl_sync(0xffffffffu, kb1, from);
+    s.row0 = t.start[s.group];
+    s.row_end = t.start[s.group + 1];
+    s.blocks = group_blocks<MODE>(a, s.row_end - s.row0);
+    s.width = tile_width<MODE>(a, s.row_end - s.row0, s.r0);
     return true;
   }
 };
@@ -518,35 +530,6 @@ __device__ __forceinline__ void store_rows_across(T* out, const GroupedArgs& a, 
   }
 }
 
-// One lane's 16 consecutive output columns of its own row, in stores of 32, 16, 8 or 4 bytes (what
-// the rows' alignment allows); the ragged end value by value.
-template <typename T>
-__device__ __forceinline__ void store_cols_16(T* p, const float (&v)[16], int left, int vec) {
-  uint32_t w[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) w[j] = pack_f32<T>(v[2 * j], v[2 * j + 1]);
-  if (left >= 16 && vec == 32) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                 : "memory");
-  } else if (vec >= 16) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {  // rows are a multiple of 8 values: no part of a store is ragged
-      if (8 * j < left) reinterpret_cast<uint4*>(p)[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-    }
-  } else if (vec == 8) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (4 * j < left) reinterpret_cast<uint2*>(p)[j] = make_uint2(w[2 * j], w[2 * j + 1]);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (2 * j < left) reinterpret_cast<uint32_t*>(p)[j] = w[j];
-    }
-  }
-}
-
 // Transposes the warp's 32 x 32 matrix: v[i] of lane j becomes v[j] of lane i.
 __device__ __forceinline__ void warp_transpose(float (&v)[32]) {
   const uint32_t lane = lane_id();
@@ -568,35 +551,44 @@ __device__ __forceinline__ void warp_transpose(float (&v)[32]) {
   }
 }
 
-// The warp's 32 rows x 32 columns, one row a lane, `cols` an odd number: two-byte stores along the
-// rows, after a transpose, instead of 32 rows at a time (256 x 256 tiles: 32 sectors a store).
+// The warp's 32 rows x 64 output columns from column `col` on, one row a lane: `first` is the warp's
+// first row in the output, `rows` how many of the 32 exist. Rows of 16-byte alignment go through
+// 4 KB of the warp's shared memory (16-byte chunks, XORed with the row against bank conflicts), so that
+// a store covers four whole 128-byte lines: with one row a lane, a store touches 32 lines, and a
+// 128 x 256 tile took 6000 cycles. Other rows are transposed in registers and stored two bytes a lane.
+constexpr int kStageOutBytes = 4096;
 template <typename T>
-__device__ __forceinline__ void store_cols_odd(T* row0, int64_t ldo, float (&v)[32], int rows, int left) {
-  warp_transpose(v);
+__device__ __forceinline__ void store_cols_64(T* out, int64_t first, int rows, int col, const GroupedArgs& a, uint32_t stage,
+                                              float (&lo)[32], float (&hi)[32]) {
   const int lane = static_cast<int>(lane_id());
+  if (a.vec >= 16) {
+    const uint32_t mine = stage + lane * 128;
+    __syncwarp();  // the warp has read what was staged before
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    if (i < rows && lane < left) row0[static_cast<int64_t>(i) * ldo + lane] = from_f32<T>(v[i]);
-  }
-}
-
-// 32 columns of the warp's 32 rows from column `col` on, one row a lane: `first` is the warp's first
-// row in the output, `rows` how many of the 32 exist.
-template <typename T>
-__device__ __forceinline__ void store_cols_32(T* out, int64_t first, int rows, int col, const GroupedArgs& a, float (&v)[32]) {
-  const int left = a.cols - col;
-  if (a.vec == 2) {
-    store_cols_odd(out + first * a.cols + col, a.cols, v, rows, left);
-    return;
-  }
-  if (static_cast<int>(lane_id()) >= rows) return;
-  T* p = out + (first + lane_id()) * a.cols + col;
+    for (int j = 0; j < 8; ++j) {
+      const float* f = j < 4 ? &lo[8 * j] : &hi[8 * (j - 4)];
+      st_shared_v4(mine + ((j ^ (lane & 7)) << 4), pack_f32<T>(f[0], f[1]), pack_f32<T>(f[2], f[3]), pack_f32<T>(f[4], f[5]),
+                   pack_f32<T>(f[6], f[7]));
+    }
+    __syncwarp();
+    const int ch = lane & 7;
+    const bool inside = col + ch * 8 < a.cols;  // rows are whole chunks: none is ragged
+    T* p = out + (first + (lane >> 3)) * a.cols + col + ch * 8;
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float f[16];
+    for (int i = 0; i < 8; ++i) {
+      const int r = 4 * i + (lane >> 3);
+      const float4 v = ld_shared_f32x4(stage + r * 128 + ((ch ^ (r & 7)) << 4));
+      if (inside && r < rows) *reinterpret_cast<float4*>(p + static_cast<int64_t>(4 * i) * a.cols) = v;
+    }
+  } else {
+    T* p = out + first * a.cols + col + lane;
+    warp_transpose(lo);
+    warp_transpose(hi);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) f[j] = v[16 * h + j];
-    store_cols_16(p + 16 * h, f, left - 16 * h, a.vec);
+    for (int i = 0; i < 32; ++i) {
+      if (i < rows && col + lane < a.cols) p[static_cast<int64_t>(i) * a.cols] = from_f32<T>(lo[i]);
+      if (i < rows && col + lane + 32 < a.cols) p[static_cast<int64_t>(i) * a.cols + 32] = from_f32<T>(hi[i]);
+    }
   }
 }
 
@@ -611,14 +603,15 @@ __device__ __forceinline__ void registers_up() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
 }
 
-// Shared memory: the ring, the barriers and the table.
+// Shared memory: the ring, the staged output rows, the barriers and the table.
 template <GroupMode MODE>
 struct GroupedShape {
-  static constexpr int kBarriers = 3 * kMaxStages + 2 * 4 + 1;
+  static constexpr int kBarriers = 3 * kMaxStages + 2 * 8 + 1;
   static constexpr int kBarrierBytes = kBarriers * 8 + 16;
+  static constexpr int kOutBytes = group_rows_right(MODE) ? 0 : group_epilogue_warps(MODE) * kStageOutBytes;
   __host__ __device__ static constexpr int stage_bytes(int r_bytes) { return kGroupLBytes + r_bytes; }
   __host__ __device__ static constexpr int smem_bytes(int stages, int r_bytes, int groups, int pairs) {
-    return 1024 + stages * stage_bytes(r_bytes) + kBarrierBytes + group_table_ints(groups, pairs) * 4;
+    return 1024 + stages * stage_bytes(r_bytes) + kOutBytes + kBarrierBytes + group_table_ints(groups, pairs) * 4;
   }
 };
 
@@ -628,16 +621,18 @@ template <GroupMode MODE, bool L_MN, typename T>
 __global__ void __launch_bounds__(group_threads(MODE), 1)
     grouped_gemm_kernel(const __grid_constant__ GroupedMaps maps, const __grid_constant__ GroupedArgs args) {
   using S = GroupedShape<MODE>;
-  constexpr bool kScaled = MODE == GroupMode::kScaled;
+  constexpr bool kScaled = group_scaled(MODE);
+  constexpr bool kWide = MODE == GroupMode::kScaled;
+  constexpr bool kFew = MODE == GroupMode::kScaledFew;
   constexpr bool kGrad = MODE == GroupMode::kWeightGrad;
   constexpr int kFirstEpilogue = group_first_epilogue_warp(MODE);
   constexpr int kEpilogueWarps = group_epilogue_warps(MODE);
   constexpr int kSteps = 4;                    // UMMA K steps of a block: 128 bytes of K
   constexpr int kBlockK = kScaled ? 128 : 64;  // K values of a block
   constexpr bool kBf16 = !kScaled && std::is_same<T, __nv_bfloat16>::value;
-  constexpr int kIssuers = kScaled ? 2 : 1;    // warps issuing UMMAs, one a half of the tile
-  constexpr int kBufs = 2 * kIssuers;          // TMEM buffers; half h uses 2h and 2h + 1
-  constexpr int kBufCols = 512 / kBufs;
+  constexpr int kIssuers = kWide ? 2 : 1;  // warps issuing UMMAs, one a half of the tile
+  constexpr int kBufs = kFew ? 8 : 2;      // TMEM buffers of an issuer
+  constexpr int kBufCols = 512 / (kBufs * kIssuers);
   constexpr uint32_t kIdescBase = (1u << 4) | (kBf16 ? (1u << 7) | (1u << 10) : 0u) | (L_MN ? 1u << 15 : 0u) |
                                   (kGrad ? 1u << 16 : 0u) | ((256u >> 4) << 24);
 
@@ -646,12 +641,13 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
       reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   const int stages = args.stages;
   const int stage_bytes = S::stage_bytes(args.r_bytes);
-  uint64_t* full = reinterpret_cast<uint64_t*>(ring + stages * stage_bytes);
+  uint8_t* out_stage = ring + stages * stage_bytes;
+  uint64_t* full = reinterpret_cast<uint64_t*>(out_stage + S::kOutBytes);
   uint64_t* empty = full + kMaxStages;
   uint64_t* tail_full = empty + kMaxStages;  // kWeightGrad: this CTA's own part of a block to be masked
   uint64_t* tmem_full = tail_full + kMaxStages;
-  uint64_t* tmem_empty = tmem_full + 4;
-  uint64_t* mma_done = tmem_empty + 4;
+  uint64_t* tmem_empty = tmem_full + 8;
+  uint64_t* mma_done = tmem_empty + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* table_mem = reinterpret_cast<int*>(tmem_slot + 4);
@@ -668,7 +664,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
       mbar_init(&empty[s], kIssuers);
       mbar_init(&tail_full[s], 1);
     }
-    for (int b = 0; b < kBufs; ++b) {
+    for (int b = 0; b < kBufs * kIssuers; ++b) {
       mbar_init(&tmem_full[b], 1);
       mbar_init(&tmem_empty[b], 8);  // four epilogue warps of each CTA (leader's copy)
     }
@@ -690,8 +686,8 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
   const GroupTable table = group_table(args, table_mem);
-  if constexpr (kScaled) {
-    if (warp < kFirstEpilogue) registers_down<56>();
+  if constexpr (kWide) {
+    if (warp < kFirstEpilogue) registers_down<40>();
   }
 
   if (warp == 0) {
@@ -707,16 +703,16 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
       const int half = s.width / 2;
       const int tail = kGrad ? (s.row_end - s.row0) - (s.blocks - 1) * 64 : 0;
       const int l0 = s.l0 + static_cast<int>(rank) * 128;
-      const int r0 = s.r0 + static_cast<int>(rank) * (kScaled ? 64 : half);
+      const int r0 = s.r0 + static_cast<int>(rank) * (kWide ? 64 : half);
       // kScaled: rows the tile has in this CTA, and in both; what a box of them leaves of the stage
       // holds what it held (those lanes are not stored).
       const int left = s.row_end - s.l0;
       const int mine = min(128, left - static_cast<int>(rank) * 128);
       auto box_bytes = [](int rows) { return rows <= 0 ? 0u : (128u >> group_box(rows)) * 128u; };
-      const CUtensorMap* l_map = &maps.l[kScaled ? group_box(mine) : 0];
-      const CUtensorMap* r_map = &maps.r[MODE == GroupMode::kForward ? group_box(half) : 0];
-      const uint32_t r_bytes = MODE == GroupMode::kForward ? box_bytes(half) : static_cast<uint32_t>(half) * 128u;
-      const uint32_t both_bytes = 2 * r_bytes + (kScaled ? box_bytes(left) + box_bytes(left - 128) : 2 * kGroupLBytes);
+      const CUtensorMap* l_map = &maps.l[kWide ? group_box(mine) : 0];
+      const CUtensorMap* r_map = &maps.r[group_rows_right(MODE) ? group_box(half) : 0];
+      const uint32_t r_bytes = group_rows_right(MODE) ? box_bytes(half) : static_cast<uint32_t>(half) * 128u;
+      const uint32_t both_bytes = 2 * r_bytes + (kWide ? box_bytes(left) + box_bytes(left - 128) : 2 * kGroupLBytes);
       for (int kb = s.kb0; kb < s.kb1; ++kb) {
         ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1u, abort_flag));
         if (!ok) break;
@@ -747,7 +743,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
             for (int i = 0; i < half / 64; ++i) elected_load_2d_pair(r_dst + i * 8192, r_map, leader_full, r0 + 64 * i, y);
           } else {
             const int k0 = kb * kBlockK;
-            if constexpr (kScaled) {
+            if constexpr (kWide) {
               if (mine > 0) elected_load_2d_pair(l_dst, l_map, leader_full, k0, l0);
               for (int h = 0; h < s.width / 128; ++h) {
                 elected_load_3d_pair(r_dst + h * 8192, r_map, leader_full, k0, r0 + h * 128, s.group);
@@ -795,12 +791,12 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
     GroupWalk<MODE> walk(args, table, pair);
     GroupSegment s;
     while (ok && walk.next(args, table, s)) {
-      const uint32_t idesc = kIdescBase | (static_cast<uint32_t>((kScaled ? 128 : s.width) >> 3) << 17);
-      const bool active = !kScaled || side * 128 < s.width;
+      const uint32_t idesc = kIdescBase | (static_cast<uint32_t>((kWide ? 128 : s.width) >> 3) << 17);
+      const bool active = !kWide || side * 128 < s.width;
       const int tail = kGrad ? (s.row_end - s.row0) - (s.blocks - 1) * 64 : 0;
       for (int kb = s.kb0; kb < s.kb1; ++kb) {
         if (active && (kScaled || kb == s.kb0)) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&tmem_empty[2 * side + buf], buf_phase ^ 1u, abort_flag));
+          ok = __all_sync(0xffffffffu, mbar_wait(&tmem_empty[kBufs * side + buf], buf_phase ^ 1u, abort_flag));
           if (!ok) break;
           tc_fence_after_sync();
         }
@@ -814,7 +810,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
         const uint64_t off = static_cast<uint64_t>(stage * (stage_bytes >> 4));
         const int steps = kGrad && kb == s.blocks - 1 ? (tail + 15) / 16 : kSteps;
         if (active) {
-          umma_block_pair<kScaled, kLStep, kRStep>(tmem_base + static_cast<uint32_t>((2 * side + buf) * kBufCols),
+          umma_block_pair<kScaled, kLStep, kRStep>(tmem_base + static_cast<uint32_t>((kBufs * side + buf) * kBufCols),
                                                    l_desc0 + off, r_desc0 + off, idesc, !kScaled && kb != s.kb0, steps);
         }
         umma_commit_elected(smem_addr(&empty[stage]));
@@ -823,9 +819,11 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
           phase ^= 1u;
         }
         if (active && (kScaled || kb + 1 == s.kb1)) {
-          umma_commit_elected(smem_addr(&tmem_full[2 * side + buf]));
-          buf ^= 1;
-          if (buf == 0) buf_phase ^= 1u;
+          umma_commit_elected(smem_addr(&tmem_full[kBufs * side + buf]));
+          if (++buf == kBufs) {
+            buf = 0;
+            buf_phase ^= 1u;
+          }
         }
       }
     }
@@ -865,32 +863,29 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
     }
   } else if (warp >= kFirstEpilogue && warp < kFirstEpilogue + kEpilogueWarps) {
     // ---------------- epilogue (both CTAs, own 128 TMEM lanes) ----------------
-    if constexpr (kScaled) registers_up<224>();
+    if constexpr (kWide) registers_up<232>();
     const int quarter = warp & 3;
     const int row = quarter * 32 + static_cast<int>(lane);  // TMEM lane
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
     T* out = static_cast<T*>(args.out);
-    const int side = kScaled ? (warp - kFirstEpilogue) / 4 : 0;  // the half of the tile's columns
+    const int side = kWide ? (warp - kFirstEpilogue) / 4 : 0;  // the half of the tile's columns
     int buf = 0;
     uint32_t buf_phase = 0;
     auto wait_buf = [&]() {
-      const bool ready = __all_sync(0xffffffffu, mbar_wait(&tmem_full[2 * side + buf], buf_phase, abort_flag));
+      const bool ready = __all_sync(0xffffffffu, mbar_wait(&tmem_full[kBufs * side + buf], buf_phase, abort_flag));
       if (!ready && lane == 0) raise_abort(args.status, abort_flag, kStatusEpilogueTimeout);
       if (ready) tc_fence_after_sync();
       return ready;
     };
+    const uint32_t leader_empty = map_to_rank(smem_addr(&tmem_empty[kBufs * side]), 0);
     auto release_buf = [&]() {
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) {
-        if (rank == 0) {
-          mbar_arrive_relaxed(&tmem_empty[2 * side + buf]);
-        } else {
-          mbar_arrive_cluster_relaxed(map_to_rank(smem_addr(&tmem_empty[2 * side + buf]), 0));
-        }
+      elected_arrive_cluster_relaxed(leader_empty + static_cast<uint32_t>(buf) * 8);
+      if (++buf == kBufs) {
+        buf = 0;
+        buf_phase ^= 1u;
       }
-      buf ^= 1;
-      if (buf == 0) buf_phase ^= 1u;
     };
     auto piece_of = [&](const GroupSegment& s) {
       return args.partials +
@@ -904,99 +899,93 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
         const uint32_t taddr = lane_base + static_cast<uint32_t>(buf * kBufCols);
         const int l32 = s.l0 + static_cast<int>(rank) * 128 + quarter * 32;  // the warp's first L row
         const bool whole = s.kb0 == 0 && s.kb1 == s.blocks;
-        // 32 columns at a time, the next ones in flight while these are stored.
-        uint32_t v[2][32];
-        tmem_ld_32x32b_x32(taddr, v[0]);
-        tmem_ld_wait();
-        tmem_ld_fence_regs(v[0]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int c = 32 * i;
-          if (c >= s.width) break;
-          uint32_t(&now)[32] = v[i & 1];
-          if (c + 32 < s.width) {
-            tmem_ld_32x32b_x32(taddr + c + 32, v[(i & 1) ^ 1]);
-          }
-          if (!whole) {
+        if (!whole) {
+#pragma unroll 1
+          for (int c = 0; c < s.width; c += 32) {
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(taddr + c, v);
+            tmem_ld_wait();
             float* dst = piece_of(s) + (static_cast<size_t>(c / 4) * 128 + row) * 4;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              st_global_v4(dst + static_cast<size_t>(j) * 512, now[4 * j], now[4 * j + 1], now[4 * j + 2], now[4 * j + 3]);
-            }
-          } else {
-            float f[32];
-#pragma unroll
-            for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(now[j]);
-            if constexpr (kGrad) {
-              store_cols_32(out, static_cast<int64_t>(s.group) * args.lrows + l32, args.lrows - l32, s.r0 + c, args, f);
-            } else {
-              store_rows_across(out, args, f, s.r0 + c, min(s.row_end, s.r0 + s.width), l32);
+              st_global_v4(dst + static_cast<size_t>(j) * 512, v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
             }
           }
+        } else if constexpr (kGrad) {
+          const uint32_t stage_out = smem_addr(out_stage) + static_cast<uint32_t>(warp - kFirstEpilogue) * kStageOutBytes;
+#pragma unroll 1
+          for (int c = 0; c < s.width; c += 64) {
+            uint32_t v[2][32];
+            tmem_ld_32x32b_x32(taddr + c, v[0]);
+            tmem_ld_32x32b_x32(taddr + c + 32, v[1]);
+            tmem_ld_wait();
+            float f[2][32];
+#pragma unroll
+            for (int j = 0; j < 64; ++j) f[j / 32][j % 32] = __uint_as_float(v[j / 32][j % 32]);
+            store_cols_64(out, static_cast<int64_t>(s.group) * args.lrows + l32, args.lrows - l32, s.r0 + c, args, stage_out,
+                          f[0], f[1]);
+          }
+        } else {
+          // 32 columns at a time, the next ones in flight while these are stored.
+          uint32_t v[2][32];
+          tmem_ld_32x32b_x32(taddr, v[0]);
           tmem_ld_wait();
-          tmem_ld_fence_regs(v[(i & 1) ^ 1]);
+          tmem_ld_fence_regs(v[0]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (32 * i >= s.width) break;
+            if (32 * i + 32 < s.width) tmem_ld_32x32b_x32(taddr + 32 * i + 32, v[(i & 1) ^ 1]);
+            float f[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) f[j] = __uint_as_float(v[i & 1][j]);
+            store_rows_across(out, args, f, s.r0 + 32 * i, min(s.row_end, s.r0 + s.width), l32);
+            tmem_ld_wait();
+            tmem_ld_fence_regs(v[(i & 1) ^ 1]);
+          }
         }
         release_buf();
       }
-    } else {
-      // One weight scale a block for the 128 columns of a half. The scales of four blocks are fetched
-      // while the four before are in use.
+    } else if constexpr (kWide) {
+      // One weight scale a block for the 128 columns of a half; both scales are loaded a block ahead.
       while (walk.next(args, table, s)) {
         if (side * 128 >= s.width) continue;
         const int l32 = s.l0 + static_cast<int>(rank) * 128 + quarter * 32;
         const int col = s.r0 + side * 128;
         const bool live = l32 < s.row_end && col < args.cols;  // warp-uniform
-        const float* sa = args.row_scales + static_cast<int64_t>(min(l32 + static_cast<int>(lane), args.rows - 1)) * args.rs_row;
-        const float* sb = args.tile_scales + s.group * args.ts_group + (min(col, args.cols - 1) >> 7) * args.ts_n;
-        float scale[4], next_a[4], next_b[4];
-        auto fetch = [&](int kb4) {  // the scales of blocks kb4 to kb4 + 3
-          if (args.rs_vec && kb4 + 4 <= s.blocks) {
-            const float4 f = *reinterpret_cast<const float4*>(sa + kb4);
-            next_a[0] = f.x; next_a[1] = f.y; next_a[2] = f.z; next_a[3] = f.w;
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) next_a[i] = sa[min(kb4 + i, s.blocks - 1) * args.rs_k];
-          }
-#pragma unroll
-          for (int i = 0; i < 4; ++i) next_b[i] = sb[min(kb4 + i, s.blocks - 1) * args.ts_k];
-        };
-        if (live) fetch(s.kb0 & ~3);
+        const float* sa = args.row_scales + static_cast<int64_t>(min(l32 + static_cast<int>(lane), args.rows - 1)) * args.rs_row +
+                          s.kb0 * args.rs_k;
+        const float* sb = args.tile_scales + s.group * args.ts_group + (min(col, args.cols - 1) >> 7) * args.ts_n + s.kb0 * args.ts_k;
+        float next_a = *sa, next_b = *sb;
         float acc[128];
 #pragma unroll
         for (int j = 0; j < 128; ++j) acc[j] = 0.f;
         bool ready = true;
         for (int kb = s.kb0; kb < s.kb1; ++kb) {
-          if (live && (kb == s.kb0 || (kb & 3) == 0)) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) scale[i] = next_a[i] * next_b[i];
-            for (int i = kb & 3; i > 0; --i) {  // a segment that begins inside four blocks
-              scale[0] = scale[1];
-              scale[1] = scale[2];
-              scale[2] = scale[3];
-            }
-            if ((kb | 3) + 1 < s.kb1) fetch((kb | 3) + 1);
+          const float now = next_a * next_b;
+          if (kb + 1 < s.kb1) {
+            sa += args.rs_k;
+            sb += args.ts_k;
+            next_a = *sa;
+            next_b = *sb;
           }
           ready = wait_buf();
           if (!ready) break;
           if (live) {
-            const float now = scale[0];
-            scale[0] = scale[1];
-            scale[1] = scale[2];
-            scale[2] = scale[3];
-            const uint32_t taddr = lane_base + static_cast<uint32_t>((2 * side + buf) * kBufCols);
-            uint32_t v[2][32];
-            tmem_ld_32x32b_x32(taddr, v[0]);
+            const uint32_t taddr = lane_base + static_cast<uint32_t>((kBufs * side + buf) * kBufCols);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int h = 0; h < 2; ++h) {
+              uint32_t v[2][32];
+              tmem_ld_32x32b_x32(taddr + 64 * h, v[0]);
+              tmem_ld_32x32b_x32(taddr + 64 * h + 32, v[1]);
               tmem_ld_wait();
-              tmem_ld_fence_regs(v[i & 1]);
-              if (i < 3) {
-                tmem_ld_32x32b_x32(taddr + 32 * (i + 1), v[(i + 1) & 1]);
-              } else {
-                release_buf();
-              }
+              tmem_ld_fence_regs(v[0]);
+              tmem_ld_fence_regs(v[1]);
+              if (h == 1) release_buf();
+              // (FP32 pairs, fma.rn.f32x2, measured twice the time of single FMAs here.)
 #pragma unroll
-              for (int j = 0; j < 32; ++j) acc[32 * i + j] = fmaf(__uint_as_float(v[i & 1][j]), now, acc[32 * i + j]);
+              for (int j = 0; j < 64; ++j) {
+                acc[64 * h + j] = fmaf(__uint_as_float(v[j / 32][j % 32]), now, acc[64 * h + j]);
+              }
             }
           } else {
             release_buf();
@@ -1005,20 +994,85 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
         if (!ready) break;
         if (!live) continue;
         const bool whole = s.kb0 == 0 && s.kb1 == s.blocks;
+        if (whole) {
+          const uint32_t stage_out = smem_addr(out_stage) + static_cast<uint32_t>(warp - kFirstEpilogue) * kStageOutBytes;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (whole) {
-            float f[32];
+          for (int h = 0; h < 2; ++h) {
+            float f[2][32];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) f[j] = acc[32 * i + j];
-            store_cols_32(out, l32, s.row_end - l32, col + 32 * i, args, f);
-          } else {
-            float* dst = piece_of(s) + (static_cast<size_t>((side * 128 + 32 * i) / 4) * 128 + row) * 4;
+            for (int j = 0; j < 64; ++j) f[j / 32][j % 32] = acc[64 * h + j];
+            store_cols_64(out, l32, s.row_end - l32, col + 64 * h, args, stage_out, f[0], f[1]);
+          }
+        } else {
+          float* dst = piece_of(s) + (static_cast<size_t>(side * 32) * 128 + row) * 4;
+          if (l32 + static_cast<int>(lane) < s.row_end) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int k = 32 * i + 4 * j;
-              st_global_v4(dst + static_cast<size_t>(j) * 512, __float_as_uint(acc[k]), __float_as_uint(acc[k + 1]),
-                           __float_as_uint(acc[k + 2]), __float_as_uint(acc[k + 3]));
+            for (int j = 0; j < 32; ++j) {
+              st_global_v4(dst + static_cast<size_t>(j) * 512, __float_as_uint(acc[4 * j]), __float_as_uint(acc[4 * j + 1]),
+                           __float_as_uint(acc[4 * j + 2]), __float_as_uint(acc[4 * j + 3]));
+            }
+          }
+        }
+      }
+    } else {
+      // kScaledFew: lane j holds the scales of rows j and j + 32, times this CTA's weight scale.
+      while (walk.next(args, table, s)) {
+        const int l32 = s.l0 + static_cast<int>(rank) * 128 + quarter * 32;
+        const int nb = min((s.l0 >> 7) + static_cast<int>(rank), (args.cols - 1) >> 7);
+        const float* sb = args.tile_scales + s.group * args.ts_group + nb * args.ts_n + s.kb0 * args.ts_k;
+        const float* sa = args.row_scales + static_cast<int64_t>(min(s.r0 + static_cast<int>(lane), args.rows - 1)) * args.rs_row +
+                          s.kb0 * args.rs_k;
+        const float* sa32 =
+            args.row_scales + static_cast<int64_t>(min(s.r0 + 32 + static_cast<int>(lane), args.rows - 1)) * args.rs_row +
+            s.kb0 * args.rs_k;
+        const bool second = s.width > 32;
+        float acc[64];
+#pragma unroll
+        for (int j = 0; j < 64; ++j) acc[j] = 0.f;
+        float next_a = *sa, next_a32 = second ? *sa32 : 0.f, next_b = *sb;
+        bool ready = true;
+        for (int kb = s.kb0; kb < s.kb1; ++kb) {
+          const float now = next_a * next_b, now32 = next_a32 * next_b;
+          if (kb + 1 < s.kb1) {
+            sa += args.rs_k;
+            sb += args.ts_k;
+            next_a = *sa;
+            next_b = *sb;
+            if (second) {
+              sa32 += args.rs_k;
+              next_a32 = *sa32;
+            }
+          }
+          ready = wait_buf();
+          if (!ready) break;
+          const uint32_t taddr = lane_base + static_cast<uint32_t>(buf * kBufCols);
+          uint32_t v[2][32];
+          tmem_ld_32x32b_x32(taddr, v[0]);
+          if (second) tmem_ld_32x32b_x32(taddr + 32, v[1]);
+          tmem_ld_wait();
+          tmem_ld_fence_regs(v[0]);
+          tmem_ld_fence_regs(v[1]);
+          release_buf();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) acc[j] = fmaf(__uint_as_float(v[0][j]), __shfl_sync(0xffffffffu, now, j), acc[j]);
+          if (second) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              acc[32 + j] = fmaf(__uint_as_float(v[1][j]), __shfl_sync(0xffffffffu, now32, j), acc[32 + j]);
+            }
+          }
+        }
+        if (!ready) break;
+        const int row_end = min(s.row_end, s.r0 + s.width);
+        if (s.kb0 == 0 && s.kb1 == s.blocks) {
+          store_rows_across(out, args, acc, s.r0, row_end, l32);
+        } else {
+          float* dst = piece_of(s) + static_cast<size_t>(row) * 4;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            if (s.r0 + 4 * j < row_end) {
+              st_global_v4(dst + static_cast<size_t>(j) * 512, __float_as_uint(acc[4 * j]), __float_as_uint(acc[4 * j + 1]),
+                           __float_as_uint(acc[4 * j + 2]), __float_as_uint(acc[4 * j + 3]));
             }
           }
         }
@@ -1036,13 +1090,19 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
 }
 
 constexpr int kFinishThreads = 128;
-constexpr int kFinishCols = 32;  // columns of a piece one block joins
+constexpr int kFinishCols = 32;  // columns of a piece one block joins (kWeightGrad, kScaled: 64)
+template <GroupMode MODE>
+__host__ __device__ constexpr int finish_cols() {
+  return group_rows_right(MODE) ? kFinishCols : 2 * kFinishCols;
+}
 
 // Joins the tiles that shares cut: block (p, CTA half, chunk of columns) takes the tile in which share
 // p + 1 begins, if that is the first share to begin inside it, and adds its FP32 pieces in K order.
 // Then all blocks write the zeros nobody else writes.
 template <GroupMode MODE, typename T>
 __global__ void __launch_bounds__(kFinishThreads) grouped_finish_kernel(const __grid_constant__ GroupedArgs args) {
+  constexpr int kCols = finish_cols<MODE>();
+  __shared__ __align__(128) uint8_t out_stage[group_rows_right(MODE) ? 16 : kFinishThreads / 32 * kStageOutBytes];
   extern __shared__ int finish_table[];
   if (threadIdx.x < 32) build_group_rows<MODE>(args, finish_table);
   __syncthreads();
@@ -1059,33 +1119,40 @@ __global__ void __launch_bounds__(kFinishThreads) grouped_finish_kernel(const __
     GroupSegment s;
     walk.next(args, table, s);
     const int begin = cut - s.kb0, end = begin + s.blocks;
-    const int c = static_cast<int>(blockIdx.z) * kFinishCols;
+    const int c = static_cast<int>(blockIdx.z) * kCols;
     if (cut > begin && table.share_begin(p - 1) <= begin && c < s.width) {
       const int row = static_cast<int>(threadIdx.x);
-      float v[kFinishCols];
+      float v[kCols / 32][32];
 #pragma unroll
-      for (int j = 0; j < kFinishCols; ++j) v[j] = 0.f;
-      for (int o = p - 1; o < table.shares && table.share_begin(o) < end; ++o) {
+      for (int j = 0; j < kCols; ++j) v[j / 32][j % 32] = 0.f;
+      // Columns and rows that hold values of the output (what else a piece has was not written).
+      const bool mine = MODE != GroupMode::kScaled || s.l0 + rank * 128 + row < s.row_end;
+      const int live_cols = group_rows_right(MODE) ? min(s.width, s.row_end - s.r0) : min(s.width, args.cols - s.r0);
+      for (int o = p - 1; mine && o < table.shares && table.share_begin(o) < end; ++o) {
         const int piece = table.share_begin(o) >= begin ? 0 : 1;
         const float* src = args.partials +
                            (static_cast<size_t>(o * 2 + piece) * 2 + rank) * static_cast<size_t>(args.piece_floats) +
                            (static_cast<size_t>(c / 4) * 128 + row) * 4;
 #pragma unroll
-        for (int j = 0; j < kFinishCols / 4; ++j) {
-          const float4 f = *reinterpret_cast<const float4*>(src + j * 512);
-          v[4 * j] += f.x;
-          v[4 * j + 1] += f.y;
-          v[4 * j + 2] += f.z;
-          v[4 * j + 3] += f.w;
+        for (int j = 0; j < kCols / 4; ++j) {
+          if (c + 4 * j < live_cols) {
+            const float4 f = *reinterpret_cast<const float4*>(src + j * 512);
+            float* sum = &v[j / 8][4 * (j % 8)];
+            sum[0] += f.x;
+            sum[1] += f.y;
+            sum[2] += f.z;
+            sum[3] += f.w;
+          }
         }
       }
       const int l32 = s.l0 + rank * 128 + (row & ~31);
-      if constexpr (MODE == GroupMode::kForward) {
-        store_rows_across(out, args, v, s.r0 + c, min(s.row_end, s.r0 + s.width), l32);
+      if constexpr (group_rows_right(MODE)) {
+        store_rows_across(out, args, v[0], s.r0 + c, min(s.row_end, s.r0 + s.width), l32);
       } else {
         const bool grad = MODE == GroupMode::kWeightGrad;
-        store_cols_32(out, grad ? static_cast<int64_t>(s.group) * args.lrows + l32 : l32,
-                      (grad ? args.lrows : s.row_end) - l32, s.r0 + c, args, v);
+        store_cols_64(out, grad ? static_cast<int64_t>(s.group) * args.lrows + l32 : l32,
+                      (grad ? args.lrows : s.row_end) - l32, s.r0 + c, args,
+                      smem_addr(out_stage) + (threadIdx.x >> 5) * kStageOutBytes, v[0], v[kCols / 32 - 1]);
       }
     }
   }

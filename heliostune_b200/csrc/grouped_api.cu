@@ -18,7 +18,7 @@ struct GroupedProblem {
   int64_t cols;      // output columns
   int64_t lrows;     // kWeightGrad: rows of one output
   int64_t k_blocks;  // forward, scaled
-  int width_cap;     // columns of a piece; kForward: most rows in a tile
+  int width_cap;     // columns of a piece; rows on the R side: most of them in a tile
 };
 
 int check_groups(const char* what, int64_t rows, int32_t groups, const void* ends) {
@@ -48,7 +48,7 @@ template <GroupMode MODE>
 int64_t max_iterations(const GroupedProblem& p) {
   const int64_t cols = cdiv(p.cols, 256);
   if (MODE == GroupMode::kWeightGrad) return cols * cdiv(p.lrows, 256) * (p.rows / 64 + p.groups);
-  return cols * std::min(p.rows / (MODE == GroupMode::kForward ? p.width_cap : 256) + p.groups, p.rows) * p.k_blocks;
+  return cols * std::min(p.rows / (group_rows_right(MODE) ? p.width_cap : 256) + p.groups, p.rows) * p.k_blocks;
 }
 
 // Iterations a share has at least: below it, joining a tile's pieces costs more than another pair
@@ -114,7 +114,7 @@ int launch_grouped(const GroupedProblem& p, const GroupedMaps& maps, GroupedArgs
   }
   cudaLaunchConfig_t lc = {};
   lc.gridDim = dim3(static_cast<unsigned>(std::max(1, args.pairs - 1)), 2,
-                    static_cast<unsigned>(args.piece_floats / 128 / kFinishCols));
+                    static_cast<unsigned>(cdiv(args.piece_floats / 128, finish_cols<MODE>())));
   lc.blockDim = dim3(kFinishThreads);
   lc.dynamicSmemBytes = static_cast<size_t>(group_table_ints(p.groups, args.pairs)) * 4;
   lc.stream = stream;
@@ -163,8 +163,10 @@ GroupedProblem forward_problem(int64_t rows, int groups, int64_t n, int64_t k) {
 GroupedProblem grad_problem(int64_t rows, int groups, int64_t lcols, int64_t rcols) {
   return GroupedProblem{rows, groups, rcols, lcols, 0, 256};
 }
+// Up to 64 rows a group on average the rows go on the R side (kScaledFew).
+bool scaled_few(int64_t rows, int groups) { return rows <= int64_t(64) * groups; }
 GroupedProblem scaled_problem(int64_t rows, int groups, int64_t n, int64_t k) {
-  return GroupedProblem{rows, groups, n, 0, cdiv(k, 128), 256};
+  return GroupedProblem{rows, groups, n, 0, cdiv(k, 128), scaled_few(rows, groups) ? width_cap(rows, 64) : 256};
 }
 
 }  // namespace
@@ -189,7 +191,8 @@ int hst_grouped_workspace_size(int32_t op, int64_t rows, int32_t groups, int64_t
       *bytes = workspace_bytes<GroupMode::kWeightGrad>(grad_problem(rows, groups, k, n), sms);
       return HST_OK;
     case HST_GROUPED_SCALED:
-      *bytes = workspace_bytes<GroupMode::kScaled>(scaled_problem(rows, groups, n, k), sms);
+      *bytes = scaled_few(rows, groups) ? workspace_bytes<GroupMode::kScaledFew>(scaled_problem(rows, groups, n, k), sms)
+                                        : workspace_bytes<GroupMode::kScaled>(scaled_problem(rows, groups, n, k), sms);
       return HST_OK;
     default:
       return fail(HST_ERR_INVALID, "unknown grouped product %d", op);
@@ -274,22 +277,29 @@ int hst_matmul_blockscaled(int32_t out_dtype, const void* a, int64_t lda, const 
   const GroupedProblem p = scaled_problem(rows, groups, n, k);
   const CUtensorMapDataType type = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   GroupedMaps maps = {};
-  for (int i = 0; i < 4; ++i) HST_TRY(encode_rows(&maps.l[i], type, 1, a, rows, k, lda, box_rows_of(i)));
-  HST_TRY(encode_weights(&maps.r[0], type, 1, b, groups, n, k, b_group, ldb, 64));
+  const bool few = scaled_few(rows, groups);
+  for (int i = 0; i < 4; ++i) HST_TRY(encode_rows(few ? &maps.r[i] : &maps.l[i], type, 1, a, rows, k, lda, box_rows_of(i)));
+  HST_TRY(encode_weights(few ? &maps.l[0] : &maps.r[0], type, 1, b, groups, n, k, b_group, ldb, few ? 128 : 64));
   GroupedArgs args = {};
   args.ends = ends;
   args.out = y;
   args.row_scales = a_scales;
   args.rs_row = sa_row;
   args.rs_k = sa_block;
-  args.rs_vec = sa_block == 1 && sa_row % 4 == 0 && (reinterpret_cast<uintptr_t>(a_scales) & 15) == 0;
   args.tile_scales = b_scales;
   args.ts_group = sb_group;
   args.ts_n = sb_row;
   args.ts_k = sb_block;
-  if (out_dtype == HST_F16)
-    return launch_grouped<GroupMode::kScaled, false, __half>(p, maps, args, 16384, workspace, workspace_bytes, s);
-  return launch_grouped<GroupMode::kScaled, false, __nv_bfloat16>(p, maps, args, 16384, workspace, workspace_bytes, s);
+  const int r_bytes = few ? box_rows_of(group_box(p.width_cap / 2)) * 128 : 16384;
+#define HST_SCALED_CASE(FEW_, MODE_, DT_, T_) \
+  if (few == FEW_ && out_dtype == DT_)        \
+    return launch_grouped<GroupMode::MODE_, false, T_>(p, maps, args, r_bytes, workspace, workspace_bytes, s);
+  HST_SCALED_CASE(true, kScaledFew, HST_F16, __half)
+  HST_SCALED_CASE(true, kScaledFew, HST_BF16, __nv_bfloat16)
+  HST_SCALED_CASE(false, kScaled, HST_F16, __half)
+  HST_SCALED_CASE(false, kScaled, HST_BF16, __nv_bfloat16)
+#undef HST_SCALED_CASE
+  return HST_ERR_UNSUPPORTED;
 }
 
 int hst_quantize_e4m3(int32_t dtype, int32_t tiles, const void* x, int64_t x_batch, int64_t x_row, int64_t x_col,
