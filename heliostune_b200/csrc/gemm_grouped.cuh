@@ -132,18 +132,24 @@ struct GroupTable {
   const int* start;      // [groups + 1] first row of each group
   const int* tile_base;  // [groups + 1] first tile of each group
   const int* row_tiles;  // [groups] tiles of a column of each group's output
-  const int* col_base;   // [pairs + 1] first iteration of each column
+  const int* width;      // [groups] rows on the R side: width of each group's tiles
+  const int* col_tile;   // [shares + 1] first tile of each column, along the line
+  const int* col_base;   // [shares + 1] first iteration of each column
   int groups;
   int tiles, shares, total;
-  int per_column, extra;  // tiles / shares and tiles % shares
+  int per_column;             // tiles / shares
+  int per_share, more_share;  // total / shares and total % shares
 
-  __device__ int column_first(int c) const { return c * per_column + c * extra / shares; }
+  // Column c gets tiles / shares tiles, and the part-filled row's are spread over the columns.
+  __device__ static int column_first(int c, int tiles, int shares) {
+    return c * (tiles / shares) + c * (tiles % shares) / shares;
+  }
+  __device__ int share_begin(int p) const { return p * per_share + min(p, more_share); }
   // The column of the line's tile v: the last c with column_first(c) = floor(c * tiles / shares) <= v.
   __device__ int column_of(int v) const { return ((v + 1) * shares - 1) / tiles; }
   __device__ int tile_of(int c, int t) const {
-    return t < per_column ? t * shares + c : per_column * shares + c * extra / shares;
+    return t < per_column ? t * shares + c : per_column * shares + col_tile[c] - c * per_column;
   }
-  __device__ int share_begin(int p) const { return p * (total / shares) + min(p, total % shares); }
   __device__ int group_of(int tile) const {
     int e = 0, top = groups - 1;  // last group whose first tile is <= tile; groups without tiles come before it
     while (e < top) {
@@ -158,16 +164,20 @@ struct GroupTable {
   }
 };
 
-constexpr __host__ __device__ int group_table_ints(int groups, int pairs) { return 3 * (groups + 1) + pairs + 1 + 4; }
+constexpr int kTableHead = 8;
+constexpr __host__ __device__ int group_table_ints(int groups, int pairs) {
+  return kTableHead + 4 * (groups + 1) + 2 * (pairs + 1);
+}
 
 // Builds the table in shared memory. Ends are taken as they would be if clamped to
 // [previous end, rows], so no value of `ends` leads out of the matrices. All threads of the block
 // (128 or more); the caller synchronises before and after, and reads it with group_table.
 template <GroupMode MODE>
 __device__ inline void build_group_rows(const GroupedArgs& a, int* mem) {
-  int* start = mem;
+  int* start = mem + kTableHead;
   int* tile_base = start + a.groups + 1;
   int* row_tiles = tile_base + a.groups + 1;
+  int* width = row_tiles + a.groups + 1;
   const int lane = static_cast<int>(lane_id());
   const int col_tiles = ceil_div(a.cols, 256);
   int row = 0, tiles = 0, total = 0;
@@ -196,6 +206,7 @@ __device__ inline void build_group_rows(const GroupedArgs& a, int* mem) {
       start[g] = begin;
       tile_base[g] = tiles + sum - mine;
       row_tiles[g] = high;
+      width[g] = group_rows_right(MODE) && high > 0 ? group_width(end - begin, a.width_cap) : 0;
     }
     row = __shfl_sync(0xffffffffu, end, 31);
     tiles += __shfl_sync(0xffffffffu, sum, 31);
@@ -203,26 +214,31 @@ __device__ inline void build_group_rows(const GroupedArgs& a, int* mem) {
   if (lane == 0) {
     start[a.groups] = row;
     tile_base[a.groups] = tiles;
-    int* head = mem + 3 * (a.groups + 1) + a.pairs + 1;
-    head[0] = tiles;
-    head[1] = max(1, min(a.pairs, total / a.min_blocks));
-    head[2] = total;
+    const int shares = max(1, min(a.pairs, total / a.min_blocks));
+    mem[0] = tiles;
+    mem[1] = shares;
+    mem[2] = total;
+    mem[3] = tiles / shares;
+    mem[4] = total / shares;
+    mem[5] = total % shares;
   }
 }
 
 __device__ inline GroupTable group_table(const GroupedArgs& a, const int* mem) {
   GroupTable t;
-  t.start = mem;
-  t.tile_base = mem + a.groups + 1;
+  t.start = mem + kTableHead;
+  t.tile_base = t.start + a.groups + 1;
   t.row_tiles = t.tile_base + a.groups + 1;
-  t.col_base = t.row_tiles + a.groups + 1;
+  t.width = t.row_tiles + a.groups + 1;
+  t.col_tile = t.width + a.groups + 1;
+  t.col_base = t.col_tile + a.pairs + 1;
   t.groups = a.groups;
-  const int* head = t.col_base + a.pairs + 1;
-  t.tiles = head[0];
-  t.shares = head[1];
-  t.total = head[2];
-  t.per_column = t.tiles / t.shares;
-  t.extra = t.tiles % t.shares;
+  t.tiles = mem[0];
+  t.shares = mem[1];
+  t.total = mem[2];
+  t.per_column = mem[3];
+  t.per_share = mem[4];
+  t.more_share = mem[5];
   return t;
 }
 
@@ -230,12 +246,15 @@ __device__ inline GroupTable group_table(const GroupedArgs& a, const int* mem) {
 template <GroupMode MODE>
 __device__ inline void build_group_columns(const GroupedArgs& a, int* mem) {
   const GroupTable t = group_table(a, mem);
-  int* col_base = mem + 3 * (a.groups + 1);
-  if constexpr (MODE != GroupMode::kWeightGrad) {
-    for (int c = static_cast<int>(threadIdx.x); c <= t.shares; c += static_cast<int>(blockDim.x)) {
-      col_base[c] = t.column_first(c) * a.k_blocks;
-    }
-  } else {
+  int* col_tile = mem + kTableHead + 4 * (a.groups + 1);
+  int* col_base = col_tile + a.pairs + 1;
+  for (int c = static_cast<int>(threadIdx.x); c <= t.shares; c += static_cast<int>(blockDim.x)) {
+    const int first = GroupTable::column_first(c, t.tiles, t.shares);
+    col_tile[c] = first;
+    if (MODE != GroupMode::kWeightGrad) col_base[c] = first * a.k_blocks;
+  }
+  if constexpr (MODE == GroupMode::kWeightGrad) {
+    __syncthreads();
     // K blocks differ by group: one warp sums a column, its lanes over the groups; then a scan.
     const int lane = static_cast<int>(lane_id());
     const int whole = t.per_column * t.shares;  // tiles of the full rows
@@ -249,7 +268,7 @@ __device__ inline void build_group_columns(const GroupedArgs& a, int* mem) {
         sum += count * group_blocks<MODE>(a, t.start[e + 1] - t.start[e]);
       }
       sum = __reduce_add_sync(0xffffffffu, sum);
-      if (t.column_first(c + 1) - t.column_first(c) > t.per_column) {
+      if (t.col_tile[c + 1] - t.col_tile[c] > t.per_column) {
         const int e = t.group_of(t.tile_of(c, t.per_column));
         sum += group_blocks<MODE>(a, t.start[e + 1] - t.start[e]);
       }
@@ -283,10 +302,10 @@ struct GroupSegment {
   bool first;         // the share's first segment
 };
 
-// Width of a tile of a group of `rows` rows whose first R column is r0.
+// Width of a tile of group e whose first R column is r0.
 template <GroupMode MODE>
-__device__ inline int tile_width(const GroupedArgs& a, int rows, int r0) {
-  if (group_rows_right(MODE)) return group_width(rows, a.width_cap);
+__device__ inline int tile_width(const GroupedArgs& a, const GroupTable& t, int e, int r0) {
+  if (group_rows_right(MODE)) return t.width[e];
   return a.cols - r0 <= 128 ? 128 : 256;
 }
 
@@ -297,7 +316,7 @@ __device__ inline void tile_origin(const GroupedArgs& a, const GroupTable& t, in
   int pr, pc;
   grouped_tile(tile - t.tile_base[e], t.row_tiles[e], ceil_div(a.cols, 256), kGroupRaster, pr, pc);
   if (group_rows_right(MODE)) {
-    r0 = row0 + pr * group_width(t.start[e + 1] - row0, a.width_cap);
+    r0 = row0 + pr * t.width[e];
     l0 = pc * 256;
   } else {
     l0 = (MODE == GroupMode::kWeightGrad ? 0 : row0) + pr * 256;
@@ -326,7 +345,7 @@ struct GroupWalk {
     int c = guess;
     while (t.col_base[c] > lo) --c;
     while (t.col_base[c + 1] <= lo) ++c;
-    v = t.column_first(c);
+    v = t.col_tile[c];
     line = t.col_base[c];
     if constexpr (MODE != GroupMode::kWeightGrad) {
       const int n = (lo - line) / a.k_blocks;
@@ -346,7 +365,7 @@ struct GroupWalk {
       int blocks = 0, e = 0, tile = 0;
       if (v + lane < t.tiles) {
         const int c = t.column_of(v + lane);
-        tile = t.tile_of(c, v + lane - t.column_first(c));
+        tile = t.tile_of(c, v + lane - t.col_tile[c]);
         e = t.group_of(tile);
         blocks = group_blocks<MODE>(a, t.start[e + 1] - t.start[e]);
       }
@@ -388,7 +407,7 @@ struct GroupWalk {
     s.row0 = t.start[s.group];
     s.row_end = t.start[s.group + 1];
     s.blocks = group_blocks<MODE>(a, s.row_end - s.row0);
-    s.width = tile_width<MODE>(a, s.row_end - s.row0, s.r0);
+    s.width = tile_width<MODE>(a, t, s.group, s.r0);
     return true;
   }
 };
@@ -1109,15 +1128,18 @@ __global__ void __launch_bounds__(kFinishThreads) grouped_finish_kernel(const __
   build_group_columns<MODE>(args, finish_table);
   __syncthreads();
   const GroupTable table = group_table(args, finish_table);
-  wait_for_primary();
   T* out = static_cast<T*>(args.out);
   const int p = static_cast<int>(blockIdx.x) + 1;
   const int rank = static_cast<int>(blockIdx.y);
+  GroupSegment s = {};
+  int cut = 0;
   if (p < table.shares) {
-    const int cut = table.share_begin(p);
+    cut = table.share_begin(p);
     GroupWalk<MODE> walk(args, table, cut, cut + 1, p);
-    GroupSegment s;
     walk.next(args, table, s);
+  }
+  wait_for_primary();  // the pieces; all before it comes from `ends` alone
+  if (p < table.shares) {
     const int begin = cut - s.kb0, end = begin + s.blocks;
     const int c = static_cast<int>(blockIdx.z) * kCols;
     if (cut > begin && table.share_begin(p - 1) <= begin && c < s.width) {
