@@ -20,7 +20,15 @@ from __future__ import annotations
 import torch
 
 from heliostune_b200 import _native
-from heliostune_b200.grouped import _DTYPES, MAX_GROUPS, _check_ends, _readable, _row_stride, _workspace
+from heliostune_b200.grouped import (
+    _DTYPES,
+    MAX_GROUPS,
+    _check_ends,
+    _padded_copy,
+    _readable_rows,
+    _stack_strides,
+    _workspace,
+)
 from heliostune_b200.kernel import _device_guard, _stream
 
 #: Values that share a scale along a row (and, for tiles, along a column).
@@ -38,29 +46,32 @@ def _refuse_gradient(what: str, *tensors: torch.Tensor) -> None:
 
 def _quantize(x: torch.Tensor, tiles: bool) -> tuple[torch.Tensor, torch.Tensor]:
     what = "quantize_tiles" if tiles else "quantize_rows"
-    if x.device.type != "cuda":
+    if not x.is_cuda:
         raise ValueError(f"{what} expects a CUDA tensor")
     if x.dtype not in _DTYPES:
         raise ValueError(f"{what} serves torch.float16 or torch.bfloat16, got {x.dtype}")
     _refuse_gradient(what, x)
-    batch = x.shape[:-2]
-    rows, cols = int(x.shape[-2]), int(x.shape[-1])
+    *batch, rows, cols = x.shape
+    device = x.device
     # Rows of q start on 16 bytes, so that the products read them in place.
     width = -(-cols // 16) * 16
-    q = torch.empty((*batch, rows, width), device=x.device, dtype=torch.float8_e4m3fn)[..., :cols]
+    q = torch.empty((*batch, rows, width), device=device, dtype=torch.float8_e4m3fn)
+    if width != cols:
+        q = q[..., :cols]
     if tiles:
-        scales = torch.empty((*batch, _blocks(rows), _blocks(cols)), device=x.device, dtype=torch.float32)
+        scales = torch.empty((*batch, _blocks(rows), _blocks(cols)), device=device, dtype=torch.float32)
     else:
         # Stored [blocks, rows]: the products read one block's scales of neighbouring rows together.
-        scales = torch.empty((_blocks(cols), rows), device=x.device, dtype=torch.float32).T
-    count = int(batch[0]) if batch else 1
-    lead = (x.stride(0), q.stride(0), scales.stride(0)) if batch else (0, 0, 0)
-    with _device_guard(x.device):
+        scales = torch.empty((_blocks(cols), rows), device=device, dtype=torch.float32).T
+    *x_batch, x_row, x_col = x.stride()
+    *q_batch, q_row, _ = q.stride()
+    *s_batch, s_row, s_col = scales.stride()
+    count, lead = (batch[0], (x_batch[0], q_batch[0], s_batch[0])) if batch else (1, (0, 0, 0))
+    with _device_guard(device):
         _native.check(
             _native.library().hst_quantize_e4m3(
-                _DTYPES[x.dtype], int(tiles), x.data_ptr(), lead[0], x.stride(-2), x.stride(-1), q.data_ptr(), lead[1],
-                q.stride(-2), scales.data_ptr(), lead[2], scales.stride(-2), scales.stride(-1), count, rows, cols,
-                _stream(x.device),
+                _DTYPES[x.dtype], tiles, x.data_ptr(), lead[0], x_row, x_col, q.data_ptr(), lead[1], q_row,
+                scales.data_ptr(), lead[2], s_row, s_col, count, rows, cols, _stream(device),
             )
         )  # fmt: skip
     return q, scales
@@ -84,12 +95,12 @@ def quantize_tiles(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     return _quantize(weight, True)
 
 
-def _check_scales(name: str, scales: torch.Tensor, shape: tuple[int, ...], device: torch.device) -> None:
-    if tuple(scales.shape) != shape:
+def _check_scales(name: str, scales: torch.Tensor, shape: tuple[int, ...], device: int) -> None:
+    if scales.shape != shape:
         raise ValueError(f"{name} must have shape {shape}, got {tuple(scales.shape)}")
     if scales.dtype != torch.float32:
         raise ValueError(f"{name} must have dtype torch.float32")
-    if scales.device != device:
+    if scales.get_device() != device:
         raise ValueError(f"{name} must be on the device of the operands")
 
 
@@ -112,35 +123,44 @@ def matmul_blockscaled(
         raise ValueError("matmul_blockscaled expects a [T, K] and b [N, K], or b [E, N, K] with group_ends [E]")
     if a.shape[1] != b.shape[-1]:
         raise ValueError(f"incompatible shapes: a {tuple(a.shape)} and b {tuple(b.shape)}")
-    if a.device.type != "cuda" or b.device != a.device:
+    if not a.is_cuda or not b.is_cuda or b.get_device() != a.get_device():
         raise ValueError("a and b must be on the same CUDA device")
     if a.dtype != torch.float8_e4m3fn or b.dtype != torch.float8_e4m3fn:
         raise ValueError("a and b must have dtype torch.float8_e4m3fn")
     if out_dtype not in _DTYPES:
         raise ValueError(f"out_dtype must be torch.float16 or torch.bfloat16, got {out_dtype}")
-    rows, k, n = int(a.shape[0]), int(a.shape[1]), int(b.shape[-2])
+    (rows, k), n, device = a.shape, b.shape[-2], a.device
+    index = a.get_device()
     groups = 1
     lead: tuple[int, ...] = ()
+    ends = None
     if group_ends is not None:
-        groups = int(b.shape[0])
+        groups = b.shape[0]
         lead = (groups,)
         if not 1 <= groups <= MAX_GROUPS:
             raise ValueError(f"matmul_blockscaled serves 1 to {MAX_GROUPS} experts, got {groups}")
-        _check_ends(group_ends, groups, a.device)
-    _check_scales("a_scales", a_scales, (rows, _blocks(k)), a.device)
-    _check_scales("b_scales", b_scales, (*lead, _blocks(n), _blocks(k)), a.device)
+        _check_ends(group_ends, groups, index)
+        ends = group_ends.data_ptr()
+    _check_scales("a_scales", a_scales, (rows, _blocks(k)), index)
+    _check_scales("b_scales", b_scales, (*lead, _blocks(n), _blocks(k)), index)
     _refuse_gradient("matmul_blockscaled", a, a_scales, b, b_scales)
-    y = torch.empty((rows, n), device=a.device, dtype=out_dtype)
-    a, b = _readable(a), _readable(b)
-    workspace = _workspace(_native.GROUPED_SCALED, rows, groups, n, k, a.device)
-    with _device_guard(a.device):
+    y = torch.empty((rows, n), device=device, dtype=out_dtype)
+    a, a_pointer, a_row = _readable_rows(a, 16)
+    b_pointer = b.data_ptr()
+    strides = b.stride() if lead else (0, *b.stride())
+    found = _stack_strides(strides, (groups, n, k), 16) if b_pointer % 16 == 0 else None
+    if found is None:
+        b = _padded_copy(b)
+        b_pointer, found = b.data_ptr(), (b.stride(0), b.stride(-2))
+    sa_row, sa_block = a_scales.stride()
+    sb_group, sb_row, sb_block = b_scales.stride() if lead else (0, *b_scales.stride())
+    workspace, nbytes = _workspace(_native.GROUPED_SCALED, rows, groups, n, k, device)
+    with _device_guard(device):
         _native.check(
             _native.library().hst_matmul_blockscaled(
-                _DTYPES[out_dtype], a.data_ptr(), _row_stride(a), a_scales.data_ptr(), a_scales.stride(0),
-                a_scales.stride(1), b.data_ptr(), b.stride(0), _row_stride(b), b_scales.data_ptr(),
-                b_scales.stride(0), b_scales.stride(-2), b_scales.stride(-1),
-                None if group_ends is None else group_ends.data_ptr(), groups, y.data_ptr(), rows, n, k,
-                workspace.data_ptr(), workspace.numel(), _stream(a.device),
+                _DTYPES[out_dtype], a_pointer, a_row, a_scales.data_ptr(), sa_row, sa_block, b_pointer, *found,
+                b_scales.data_ptr(), sb_group, sb_row, sb_block, ends, groups, y.data_ptr(), rows, n, k,
+                workspace.data_ptr(), nbytes, _stream(device),
             )
         )  # fmt: skip
     return y

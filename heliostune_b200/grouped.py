@@ -42,95 +42,110 @@ def _workspace_bytes(op: int, rows: int, groups: int, n: int, k: int, device: in
     return size.value
 
 
-def _workspace(op: int, rows: int, groups: int, n: int, k: int, device: torch.device) -> torch.Tensor:
-    """The FP32 pieces of tiles shared between CTA pairs; a tensor of this call alone."""
+def _workspace(op: int, rows: int, groups: int, n: int, k: int, device: torch.device) -> tuple[torch.Tensor, int]:
+    """The FP32 pieces of tiles shared between CTA pairs, a tensor of this call alone, and its bytes."""
     index = device.index if device.index is not None else torch.cuda.current_device()
-    return torch.empty(_workspace_bytes(op, rows, groups, n, k, index), device=device, dtype=torch.uint8)
+    nbytes = _workspace_bytes(op, rows, groups, n, k, index)
+    return torch.empty(nbytes, device=device, dtype=torch.uint8), nbytes
 
 
-def _aligned_rows(t: torch.Tensor) -> bool:
-    """Whether a tensor map can describe ``t`` (2-D, or 3-D with one matrix per group): unit stride
-    in the last dimension, the others multiples of 16 bytes that do not overlap, and the base too."""
-    unit = 16 // t.element_size()
-    if t.data_ptr() % 16 != 0 or (t.shape[-1] > 1 and t.stride(-1) != 1):
-        return False
-    if t.shape[-2] > 1 and (t.stride(-2) % unit != 0 or t.stride(-2) < t.shape[-1]):
-        return False
-    if t.ndim == 3 and t.shape[0] > 1:
-        return t.stride(0) % unit == 0 and t.stride(0) >= _row_stride(t) * t.shape[1]
-    return True
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    unit = 16 // t.element_size()
-    return t.stride(-2) if t.shape[-2] > 1 else -(-t.shape[-1] // unit) * unit
-
-
-def _readable(t: torch.Tensor) -> torch.Tensor:
-    """``t``, or a copy with 16-byte aligned rows where a tensor map cannot describe it."""
-    if _aligned_rows(t):
-        return t
+def _padded_copy(t: torch.Tensor) -> torch.Tensor:
+    """``t`` with rows of a multiple of 16 bytes, one after the other."""
     unit = 16 // t.element_size()
     width = -(-t.shape[-1] // unit) * unit
     padded = torch.empty((*t.shape[:-1], width), device=t.device, dtype=t.dtype)[..., : t.shape[-1]]
     return padded.copy_(t)
 
 
-def _check_ends(group_ends: torch.Tensor, groups: int, device: torch.device) -> None:
+def _readable_rows(t: torch.Tensor, unit: int) -> tuple[torch.Tensor, int, int]:
+    """A row matrix a tensor map can describe -- unit column stride, rows and base aligned to 16 bytes
+    (``unit`` values) -- with its address and row stride: ``t`` itself, or a copy."""
+    pointer, (row, column), (rows, columns) = t.data_ptr(), t.stride(), t.shape
+    if rows == 1:
+        row = -(-columns // unit) * unit
+    if (column == 1 or columns == 1) and row % unit == 0 and row >= columns and pointer % 16 == 0:
+        return t, pointer, row
+    copy = _padded_copy(t)
+    return copy, copy.data_ptr(), copy.stride(0)
+
+
+def _stack_strides(strides: tuple[int, int, int], shape: tuple[int, int, int], unit: int) -> tuple[int, int] | None:
+    """Group and row stride of a stack of row matrices a tensor map can describe, None if it cannot."""
+    (group, row, column), (groups, rows, columns) = strides, shape
+    if rows == 1:
+        row = -(-columns // unit) * unit
+    if groups == 1:
+        group = row * rows
+    if (column == 1 or columns == 1) and row % unit == 0 and row >= columns and group % unit == 0 and group >= row * rows:
+        return group, row
+    return None
+
+
+def _readable_weights(weight: torch.Tensor) -> tuple[torch.Tensor, int, int, int, int]:
+    """``weight [E, K, N]`` with its address, group and row stride and layout: itself in either layout, or
+    a copy."""
+    pointer, (group, inner, outer), (groups, k, n) = weight.data_ptr(), weight.stride(), weight.shape
+    if pointer % 16 == 0:
+        found = _stack_strides((group, inner, outer), (groups, k, n), 8)
+        if found is not None:
+            return weight, pointer, *found, _native.HST_WEIGHT_KN
+        found = _stack_strides((group, outer, inner), (groups, n, k), 8)
+        if found is not None:
+            return weight, pointer, *found, _native.HST_WEIGHT_NK
+    if inner == 1 and outer != 1:
+        copy = _padded_copy(weight.transpose(1, 2))
+        return copy, copy.data_ptr(), copy.stride(0), copy.stride(1), _native.HST_WEIGHT_NK
+    copy = _padded_copy(weight)
+    return copy, copy.data_ptr(), copy.stride(0), copy.stride(1), _native.HST_WEIGHT_KN
+
+
+def _check_ends(group_ends: torch.Tensor, groups: int, device: int) -> None:
     if group_ends.ndim != 1 or group_ends.shape[0] != groups:
         raise ValueError(f"group_ends must have one entry for each of {groups} weights, got {tuple(group_ends.shape)}")
     if group_ends.dtype != torch.int32:
         raise ValueError("group_ends must have dtype torch.int32")
-    if group_ends.device != device:
+    if group_ends.get_device() != device:
         raise ValueError("group_ends must be on the device of the operands")
     if not group_ends.is_contiguous():
         raise ValueError("group_ends must be contiguous")
 
 
 def _check_operands(what: str, x: torch.Tensor, other: torch.Tensor, names: tuple[str, str]) -> None:
-    if x.device.type != "cuda" or other.device != x.device:
+    if not x.is_cuda or not other.is_cuda or other.get_device() != x.get_device():
         raise ValueError(f"{names[0]} and {names[1]} must be on the same CUDA device")
     if x.dtype not in _DTYPES or other.dtype != x.dtype:
         raise ValueError(f"{what} serves torch.float16 or torch.bfloat16, the same for {names[0]} and {names[1]}")
 
 
 def _forward(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tensor) -> torch.Tensor:
-    groups, k, n = (int(v) for v in weight.shape)
-    rows = int(x.shape[0])
-    y = torch.empty((rows, n), device=x.device, dtype=x.dtype)
-    x = _readable(x)
-    # The layout whose last dimension is contiguous; a weight with neither is copied.
-    transposed = weight.transpose(1, 2)
-    if not _aligned_rows(weight) and _aligned_rows(transposed):
-        layout, stored = _native.HST_WEIGHT_NK, transposed
-    elif weight.stride(1) == 1 and weight.stride(2) != 1:
-        layout, stored = _native.HST_WEIGHT_NK, _readable(transposed)
-    else:
-        layout, stored = _native.HST_WEIGHT_KN, _readable(weight)
-    workspace = _workspace(_native.GROUPED_FORWARD, rows, groups, n, k, x.device)
-    with _device_guard(x.device):
+    groups, k, n = weight.shape
+    rows, device = x.shape[0], x.device
+    y = torch.empty((rows, n), device=device, dtype=x.dtype)
+    x, x_pointer, x_row = _readable_rows(x, 8)
+    weight, w_pointer, w_group, w_row, layout = _readable_weights(weight)
+    workspace, nbytes = _workspace(_native.GROUPED_FORWARD, rows, groups, n, k, device)
+    with _device_guard(device):
         _native.check(
             _native.library().hst_grouped_matmul(
-                _DTYPES[x.dtype], x.data_ptr(), _row_stride(x), stored.data_ptr(), stored.stride(0),
-                _row_stride(stored), layout, group_ends.data_ptr(), groups, y.data_ptr(), rows, n, k,
-                workspace.data_ptr(), workspace.numel(), _stream(x.device),
+                _DTYPES[x.dtype], x_pointer, x_row, w_pointer, w_group, w_row, layout, group_ends.data_ptr(), groups,
+                y.data_ptr(), rows, n, k, workspace.data_ptr(), nbytes, _stream(device),
             )
         )  # fmt: skip
     return y
 
 
 def _weight_grad(left: torch.Tensor, right: torch.Tensor, group_ends: torch.Tensor) -> torch.Tensor:
-    groups, rows = int(group_ends.shape[0]), int(left.shape[0])
-    lcols, rcols = int(left.shape[1]), int(right.shape[1])
-    out = torch.empty((groups, lcols, rcols), device=left.device, dtype=left.dtype)
-    left, right = _readable(left), _readable(right)
-    workspace = _workspace(_native.GROUPED_WEIGHT_GRAD, rows, groups, rcols, lcols, left.device)
-    with _device_guard(left.device):
+    groups = group_ends.shape[0]
+    (rows, lcols), rcols, device = left.shape, right.shape[1], left.device
+    out = torch.empty((groups, lcols, rcols), device=device, dtype=left.dtype)
+    left, l_pointer, l_row = _readable_rows(left, 8)
+    right, r_pointer, r_row = _readable_rows(right, 8)
+    workspace, nbytes = _workspace(_native.GROUPED_WEIGHT_GRAD, rows, groups, rcols, lcols, device)
+    with _device_guard(device):
         _native.check(
             _native.library().hst_grouped_weight_grad(
-                _DTYPES[left.dtype], left.data_ptr(), _row_stride(left), right.data_ptr(), _row_stride(right),
-                group_ends.data_ptr(), groups, out.data_ptr(), rows, lcols, rcols, workspace.data_ptr(),
-                workspace.numel(), _stream(left.device),
+                _DTYPES[left.dtype], l_pointer, l_row, r_pointer, r_row, group_ends.data_ptr(), groups, out.data_ptr(),
+                rows, lcols, rcols, workspace.data_ptr(), nbytes, _stream(device),
             )
         )  # fmt: skip
     return out
@@ -146,7 +161,7 @@ def grouped_weight_grad(x: torch.Tensor, dy: torch.Tensor, group_ends: torch.Ten
     groups = int(group_ends.shape[0]) if group_ends.ndim == 1 else 0
     if not 1 <= groups <= MAX_GROUPS:
         raise ValueError(f"grouped_weight_grad serves 1 to {MAX_GROUPS} experts, got {groups}")
-    _check_ends(group_ends, groups, x.device)
+    _check_ends(group_ends, groups, x.get_device())
     if torch.is_grad_enabled() and (x.requires_grad or dy.requires_grad):
         raise ValueError("grouped_weight_grad has no gradient; detach its inputs")
     return _weight_grad(x, dy, group_ends)
@@ -186,7 +201,7 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tens
     _check_operands("grouped_matmul", x, weight, ("x", "weight"))
     if not 1 <= weight.shape[0] <= MAX_GROUPS:
         raise ValueError(f"grouped_matmul serves 1 to {MAX_GROUPS} experts, got {weight.shape[0]}")
-    _check_ends(group_ends, int(weight.shape[0]), x.device)
+    _check_ends(group_ends, weight.shape[0], x.get_device())
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         return _GroupedMatmul.apply(x, weight, group_ends)
     return _forward(x, weight, group_ends)
