@@ -86,6 +86,7 @@ EXPORTED_SYMBOLS = (
     "hst_grouped_weight_grad",
     "hst_matmul_blockscaled",
     "hst_quantize_e4m3",
+    "hst_pack_rows",
 )
 
 
@@ -215,6 +216,10 @@ def _declare(lib: ctypes.CDLL) -> None:
         ),
         "hst_quantize_e4m3": (
             [_i32, _i32, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _ptr],
+            ctypes.c_int,
+        ),
+        "hst_pack_rows": (
+            [_i32, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _ptr],
             ctypes.c_int,
         ),
         "hst_matmul_split_k_noalloc": (

@@ -150,7 +150,7 @@ def matmul_blockscaled(
     strides = b.stride() if lead else (0, *b.stride())
     found = _stack_strides(strides, (groups, n, k), 16) if b_pointer % 16 == 0 else None
     if found is None:
-        b = _padded_copy(b)
+        b = _padded_copy(b, group_ends, rows)
         b_pointer, found = b.data_ptr(), (b.stride(0), b.stride(-2))
     sa_row, sa_block = a_scales.stride()
     sb_group, sb_row, sb_block = b_scales.stride() if lead else (0, *b_scales.stride())

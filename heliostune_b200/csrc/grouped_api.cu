@@ -4,6 +4,7 @@
 
 #include "gemm_grouped.cuh"
 #include "host.h"
+#include "pack.cuh"
 #include "quantize.cuh"
 
 namespace hst {
@@ -328,12 +329,48 @@ int hst_quantize_e4m3(int32_t dtype, int32_t tiles, const void* x, int64_t x_bat
     else quantize_tiles_any_kernel<__nv_bfloat16><<<grid, kQuantThreads, 0, st>>>(a);
   } else {
     const int64_t units = rows * col_blocks;
-    const unsigned vec_grid = static_cast<unsigned>(cdiv(units, kQuantThreads / 16 * kQuantUnroll));
+    const unsigned vec_grid = static_cast<unsigned>(cdiv(rows, kQuantRows) * cdiv(col_blocks, kQuantBlocks));
     const unsigned any_grid = static_cast<unsigned>(cdiv(units, kQuantThreads / 32));
     if (vec && dtype == HST_F16) quantize_rows_kernel<__half><<<vec_grid, kQuantThreads, 0, st>>>(a);
     else if (vec) quantize_rows_kernel<__nv_bfloat16><<<vec_grid, kQuantThreads, 0, st>>>(a);
     else if (dtype == HST_F16) quantize_rows_any_kernel<__half><<<any_grid, kQuantThreads, 0, st>>>(a);
     else quantize_rows_any_kernel<__nv_bfloat16><<<any_grid, kQuantThreads, 0, st>>>(a);
+  }
+  HST_CUDA(cudaGetLastError());
+  return HST_OK;
+}
+
+int hst_pack_rows(int32_t value_bytes, const void* src, int64_t s_group, int64_t s_row, int64_t s_col, void* dst,
+                  int64_t d_group, int64_t d_row, const int32_t* ends, int64_t total_rows, int64_t groups, int64_t rows,
+                  int64_t cols, void* stream) {
+  if (value_bytes != 1 && value_bytes != 2) return fail(HST_ERR_INVALID, "values of %d bytes", value_bytes);
+  HST_TRY(check_extents("the packed copy", rows, cols));
+  if (groups < 0 || groups > kMaxGroups || total_rows < 0 || total_rows > kMaxExtent)
+    return fail(HST_ERR_INVALID, "the packed copy serves at most %d matrices", kMaxGroups);
+  if (groups == 0 || rows == 0 || cols == 0) return HST_OK;
+  if (src == nullptr || dst == nullptr) return fail(HST_ERR_INVALID, "null pointer");
+  const int64_t e = value_bytes;
+  if ((reinterpret_cast<uintptr_t>(dst) & 15) != 0 || d_row * e % 16 != 0 || d_row < cols || d_group * e % 16 != 0)
+    return fail(HST_ERR_INVALID, "the packed copy's rows must be 16-byte aligned and hold all columns");
+  PackArgs a = {static_cast<const uint8_t*>(src), s_group * e, s_row * e, s_col * e, static_cast<uint8_t*>(dst), d_group * e,
+                d_row * e, ends, static_cast<int>(total_rows), rows, static_cast<int>(cdiv(cols * e, 16)), cols * e};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (s_col == 1 || cols == 1) {
+    const dim3 grid(static_cast<unsigned>(cdiv(rows * a.chunks, kPackThreads * kPackPerThread)), static_cast<unsigned>(groups));
+    // The common alignment of every row's start and of its length.
+    const uint64_t bits = reinterpret_cast<uintptr_t>(src) | static_cast<uint64_t>(a.row_bytes) |
+                          (rows > 1 ? static_cast<uint64_t>(a.s_row) : 0) | (groups > 1 ? static_cast<uint64_t>(a.s_group) : 0);
+    if (bits % 16 == 0) pack_rows_kernel<uint4><<<grid, kPackThreads, 0, st>>>(a);
+    else if (bits % 8 == 0) pack_rows_kernel<uint2><<<grid, kPackThreads, 0, st>>>(a);
+    else if (bits % 4 == 0) pack_rows_kernel<uint32_t><<<grid, kPackThreads, 0, st>>>(a);
+    else if (bits % 2 == 0) pack_rows_kernel<uint16_t><<<grid, kPackThreads, 0, st>>>(a);
+    else pack_rows_kernel<uint8_t><<<grid, kPackThreads, 0, st>>>(a);
+  } else {
+    const int64_t tiles = cdiv(rows, 32) * cdiv(cols, 32);
+    if (tiles > INT32_MAX) return fail(HST_ERR_UNSUPPORTED, "the packed copy is too large");
+    const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(groups));
+    if (value_bytes == 2) pack_any_kernel<uint16_t><<<grid, kPackThreads, 0, st>>>(a);
+    else pack_any_kernel<uint8_t><<<grid, kPackThreads, 0, st>>>(a);
   }
   HST_CUDA(cudaGetLastError());
   return HST_OK;

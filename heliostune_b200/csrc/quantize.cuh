@@ -8,9 +8,10 @@
 // and then NaN on top, so a NaN or an infinity in a block makes its scale one as well.
 //
 // Bound: HBM, 3 bytes a value. One pass: a block's values stay in registers between the maximum and
-// the conversion. Rows: a half-warp holds a block as 16 bytes a lane and each thread loads four
-// blocks before it uses the first; tiles: a CTA of 256 threads holds the 32 KB tile as eight 16-byte
-// loads a thread.
+// the conversion. Rows: a half-warp holds a block as 16 bytes a lane, each thread loads four blocks
+// before it uses the first, and a CTA takes 8 rows x 8 blocks, so that the scales, stored by blocks,
+// go out as 32-byte sectors. Tiles: a CTA of 256 threads holds the 32 KB tile as eight 16-byte loads a
+// thread.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -21,7 +22,7 @@
 namespace hst {
 
 constexpr int kQuantThreads = 256;
-constexpr int kQuantUnroll = 4;
+constexpr int kQuantRows = 8, kQuantBlocks = 8;  // rows and 128-value blocks of a CTA
 constexpr float kE4m3Max = 448.f;
 constexpr float kAmaxFloor = 7.8886090522101181e-31f;  // 2^-100
 
@@ -76,36 +77,42 @@ __device__ __forceinline__ uint8_t quantize1(uint32_t bits, float inv) {
 // multiple of 8 columns; q's rows 8-byte aligned.
 template <typename T>
 __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const QuantizeArgs a) {
+  __shared__ float staged[kQuantRows * kQuantBlocks];
   const int half_lane = threadIdx.x & 15, half_warp = threadIdx.x >> 4;
-  constexpr int kHalfWarps = kQuantThreads / 16;
-  const uint32_t units = static_cast<uint32_t>(a.rows) * static_cast<uint32_t>(a.col_blocks);
-  const uint32_t first = blockIdx.x * (kHalfWarps * kQuantUnroll) + half_warp;
+  const int block_tiles = (a.col_blocks + kQuantBlocks - 1) / kQuantBlocks;
+  const int row_tile = static_cast<int>(blockIdx.x) / block_tiles;
+  const int row0 = row_tile * kQuantRows, cb0 = (static_cast<int>(blockIdx.x) - row_tile * block_tiles) * kQuantBlocks;
+  const int cb = half_warp % kQuantBlocks;  // this half-warp's block of four rows
+  const int col = (cb0 + cb) * 128 + half_lane * 8;
+  constexpr int kStep = kQuantThreads / 16 / kQuantBlocks;
+  const int first = half_warp / kQuantBlocks;
   const uint16_t* x = static_cast<const uint16_t*>(a.x);
-  uint4 v[kQuantUnroll];
-  uint32_t row[kQuantUnroll], cb[kQuantUnroll];
+  uint4 v[kQuantRows / kStep];
 #pragma unroll
-  for (int i = 0; i < kQuantUnroll; ++i) {
-    const uint32_t u = min(first + i * kHalfWarps, units - 1);
-    row[i] = u / static_cast<uint32_t>(a.col_blocks);
-    cb[i] = u - row[i] * static_cast<uint32_t>(a.col_blocks);
-    const int col = static_cast<int>(cb[i]) * 128 + half_lane * 8;
+  for (int i = 0; i < kQuantRows / kStep; ++i) {
+    const int row = row0 + first + i * kStep;
     v[i] = make_uint4(0, 0, 0, 0);
-    if (col < a.cols) v[i] = __ldcs(reinterpret_cast<const uint4*>(x + row[i] * a.x_row + col));
+    if (row < a.rows && col < a.cols) v[i] = __ldcs(reinterpret_cast<const uint4*>(x + row * a.x_row + col));
   }
 #pragma unroll
-  for (int i = 0; i < kQuantUnroll; ++i) {
+  for (int i = 0; i < kQuantRows / kStep; ++i) {
+    const int r = first + i * kStep;
     uint32_t m = absmax8(0, v[i]);
 #pragma unroll
     for (int d = 8; d >= 1; d /= 2) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, d));
     const float amax = amax_of<T>(m);
     const float inv = kE4m3Max / amax;
-    if (first + i * kHalfWarps >= units) continue;
-    const int col = static_cast<int>(cb[i]) * 128 + half_lane * 8;
-    if (col < a.cols) {
-      *reinterpret_cast<uint2*>(a.q + row[i] * a.q_row + col) =
+    if (row0 + r < a.rows && col < a.cols) {
+      *reinterpret_cast<uint2*>(a.q + (row0 + r) * a.q_row + col) =
           make_uint2(quantize4<T>(v[i].x, v[i].y, inv), quantize4<T>(v[i].z, v[i].w, inv));
     }
-    if (half_lane == 0) a.scales[row[i] * a.s_row + cb[i] * a.s_col] = amax / kE4m3Max;
+    if (half_lane == 0) staged[cb * kQuantRows + r] = amax / kE4m3Max;
+  }
+  __syncthreads();
+  const int t = static_cast<int>(threadIdx.x);
+  if (t < kQuantRows * kQuantBlocks) {
+    const int r = row0 + t % kQuantRows, c = cb0 + t / kQuantRows;
+    if (r < a.rows && c < a.col_blocks) a.scales[r * a.s_row + c * a.s_col] = staged[t];
   }
 }
 

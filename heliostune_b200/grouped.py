@@ -49,12 +49,22 @@ def _workspace(op: int, rows: int, groups: int, n: int, k: int, device: torch.de
     return torch.empty(nbytes, device=device, dtype=torch.uint8), nbytes
 
 
-def _padded_copy(t: torch.Tensor) -> torch.Tensor:
-    """``t`` with rows of a multiple of 16 bytes, one after the other."""
+def _padded_copy(t: torch.Tensor, group_ends: torch.Tensor | None = None, total_rows: int = 0) -> torch.Tensor:
+    """``t`` (one matrix or a stack) with rows of a multiple of 16 bytes, one after the other. With the
+    ends of a product over ``total_rows`` rows, the matrices of groups without rows are left out."""
     unit = 16 // t.element_size()
-    width = -(-t.shape[-1] // unit) * unit
-    padded = torch.empty((*t.shape[:-1], width), device=t.device, dtype=t.dtype)[..., : t.shape[-1]]
-    return padded.copy_(t)
+    *lead, rows, columns = t.shape
+    copy = torch.empty((*lead, rows, -(-columns // unit) * unit), device=t.device, dtype=t.dtype)[..., :columns]
+    groups, s_group, d_group = (lead[0], t.stride(0), copy.stride(0)) if lead else (1, 0, 0)
+    with _device_guard(t.device):
+        _native.check(
+            _native.library().hst_pack_rows(
+                t.element_size(), t.data_ptr(), s_group, t.stride(-2), t.stride(-1), copy.data_ptr(), d_group,
+                copy.stride(-2), None if group_ends is None else group_ends.data_ptr(), total_rows, groups, rows,
+                columns, _stream(t.device),
+            )
+        )  # fmt: skip
+    return copy
 
 
 def _readable_rows(t: torch.Tensor, unit: int) -> tuple[torch.Tensor, int, int]:
@@ -81,9 +91,11 @@ def _stack_strides(strides: tuple[int, int, int], shape: tuple[int, int, int], u
     return None
 
 
-def _readable_weights(weight: torch.Tensor) -> tuple[torch.Tensor, int, int, int, int]:
+def _readable_weights(
+    weight: torch.Tensor, group_ends: torch.Tensor, total_rows: int
+) -> tuple[torch.Tensor, int, int, int, int]:
     """``weight [E, K, N]`` with its address, group and row stride and layout: itself in either layout, or
-    a copy."""
+    a copy of the weights that have rows."""
     pointer, (group, inner, outer), (groups, k, n) = weight.data_ptr(), weight.stride(), weight.shape
     if pointer % 16 == 0:
         found = _stack_strides((group, inner, outer), (groups, k, n), 8)
@@ -93,9 +105,9 @@ def _readable_weights(weight: torch.Tensor) -> tuple[torch.Tensor, int, int, int
         if found is not None:
             return weight, pointer, *found, _native.HST_WEIGHT_NK
     if inner == 1 and outer != 1:
-        copy = _padded_copy(weight.transpose(1, 2))
+        copy = _padded_copy(weight.transpose(1, 2), group_ends, total_rows)
         return copy, copy.data_ptr(), copy.stride(0), copy.stride(1), _native.HST_WEIGHT_NK
-    copy = _padded_copy(weight)
+    copy = _padded_copy(weight, group_ends, total_rows)
     return copy, copy.data_ptr(), copy.stride(0), copy.stride(1), _native.HST_WEIGHT_KN
 
 
@@ -122,7 +134,7 @@ def _forward(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tensor) ->
     rows, device = x.shape[0], x.device
     y = torch.empty((rows, n), device=device, dtype=x.dtype)
     x, x_pointer, x_row = _readable_rows(x, 8)
-    weight, w_pointer, w_group, w_row, layout = _readable_weights(weight)
+    weight, w_pointer, w_group, w_row, layout = _readable_weights(weight, group_ends, rows)
     workspace, nbytes = _workspace(_native.GROUPED_FORWARD, rows, groups, n, k, device)
     with _device_guard(device):
         _native.check(

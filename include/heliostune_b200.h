@@ -227,6 +227,15 @@ int hst_matmul_blockscaled(int32_t out_dtype, const void* a, int64_t lda, const 
                            int64_t rows, int64_t n, int64_t k, void* workspace,
                            size_t workspace_bytes, void* stream);
 
+/* Copies row matrices into rows of a multiple of 16 bytes, for operands the products above cannot
+ * read in place: src [groups, rows, cols] of 1- or 2-byte values with any strides, dst with unit column
+ * stride, 16-byte aligned base, rows and groups (strides in values). With `ends` (those of the
+ * product, over total_rows rows) the matrices of groups without rows are not copied; the product does
+ * not read them. Null `ends`: all are. */
+int hst_pack_rows(int32_t value_bytes, const void* src, int64_t s_group, int64_t s_row, int64_t s_col,
+                  void* dst, int64_t d_group, int64_t d_row, const int32_t* ends, int64_t total_rows,
+                  int64_t groups, int64_t rows, int64_t cols, void* stream);
+
 /* E4M3 with FP32 scales: for every block amax = max(max |x|, 2^-100), scale = amax / 448 and
  * q = e4m3(x * (448 / amax)), the quotients and the product rounded to FP32, q to nearest even.
  * A block is 128 consecutive values of a row (tiles = 0, one matrix) or 128 x 128 values of a
