@@ -154,13 +154,14 @@ def matmul_blockscaled(
         b_pointer, found = b.data_ptr(), (b.stride(0), b.stride(-2))
     sa_row, sa_block = a_scales.stride()
     sb_group, sb_row, sb_block = b_scales.stride() if lead else (0, *b_scales.stride())
-    workspace, nbytes = _workspace(_native.GROUPED_SCALED, rows, groups, n, k, device)
+    workspace, ws_pointer, ws_bytes = _workspace(_native.GROUPED_SCALED, rows, groups, n, k, device)
     with _device_guard(device):
         _native.check(
             _native.library().hst_matmul_blockscaled(
                 _DTYPES[out_dtype], a_pointer, a_row, a_scales.data_ptr(), sa_row, sa_block, b_pointer, *found,
                 b_scales.data_ptr(), sb_group, sb_row, sb_block, ends, groups, y.data_ptr(), rows, n, k,
-                workspace.data_ptr(), nbytes, _stream(device),
+                ws_pointer, ws_bytes, _stream(device),
             )
         )  # fmt: skip
+    del workspace  # stream-ordered reuse by the caching allocator is safe on this stream
     return y

@@ -33,10 +33,12 @@
 //
 // Schedule: all (tile, K block) iterations of all groups in one line, cut into one equal share per
 // pair (GroupTable). A tile cut by a share's end leaves FP32 pieces in the workspace, which a second
-// small kernel (grouped_finish_kernel, a programmatic dependent) adds in K order. No CTA ever waits
-// for another pair, no atomics: results are bitwise reproducible, and the two kernels can be captured
-// and replayed. The second kernel also writes the zeros of rows past the last group and of the weight
-// gradients of empty groups.
+// small kernel (grouped_finish_kernel, a programmatic dependent) adds in K order. Where no tile has
+// more than 16 K blocks (args.whole) the shares end at tiles instead: the second launch and the pieces
+// cost more than the imbalance (8 groups, 421 rows, 520 x 1000: 19 us a product with them, 12 without).
+// No CTA ever waits for another pair, no atomics: results are bitwise reproducible, and the kernels can
+// be captured and replayed. Whichever kernel is last also writes the zeros of rows past the last group
+// and of the weight gradients of empty groups.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -85,6 +87,7 @@ struct GroupedArgs {
   int r_bytes;          // bytes of the R operand's part of a stage
   int pairs;            // CTA pairs launched
   int min_blocks;       // iterations a share has at least
+  int whole;            // shares end at tiles: nothing is cut
   int vec;              // bytes of a store the output rows' alignment allows: 32, 16, 8, 4 or 2
   int* status;
   void* out;            // [rows, cols], or [groups, lrows, cols], contiguous
@@ -128,33 +131,47 @@ __host__ __device__ inline int group_blocks(const GroupedArgs& a, int rows) {
 // column c, give or take a part of a tile, so at any moment the pairs work on neighbouring tiles: with
 // contiguous runs of the group-by-group order instead, the 74 weight panels in use passed L2's size
 // (8194 x 14336 x 4096 over 8 groups: 1007 us, 577 ns a block, against 0.28 for the UMMAs alone).
+//
+// In shared memory: eight integers (below), then [groups + 1] first row and first tile of each group,
+// tiles in a column of its output and width of its tiles (rows on the R side), then [pairs + 1] first
+// tile of each column along the line and its first iteration. The view keeps one address: the issuing
+// warps have no registers for six.
+constexpr int kTableHead = 8;
 struct GroupTable {
-  const int* start;      // [groups + 1] first row of each group
-  const int* tile_base;  // [groups + 1] first tile of each group
-  const int* row_tiles;  // [groups] tiles of a column of each group's output
-  const int* width;      // [groups] rows on the R side: width of each group's tiles
-  const int* col_tile;   // [shares + 1] first tile of each column, along the line
-  const int* col_base;   // [shares + 1] first iteration of each column
-  int groups;
-  int tiles, shares, total;
-  int per_column;             // tiles / shares
-  int per_share, more_share;  // total / shares and total % shares
+  int* mem;
+  int groups, pairs, whole;
+
+  __device__ int& tiles() const { return mem[0]; }
+  __device__ int& shares() const { return mem[1]; }
+  __device__ int& total() const { return mem[2]; }       // iterations
+  __device__ int& per_column() const { return mem[3]; }  // tiles / shares
+  __device__ int& per_share() const { return mem[4]; }   // total / shares, and what remains
+  __device__ int& more_share() const { return mem[5]; }
+  __device__ int& start(int e) const { return mem[kTableHead + e]; }
+  __device__ int& tile_base(int e) const { return mem[kTableHead + groups + 1 + e]; }
+  __device__ int& row_tiles(int e) const { return mem[kTableHead + 2 * (groups + 1) + e]; }
+  __device__ int& width(int e) const { return mem[kTableHead + 3 * (groups + 1) + e]; }
+  __device__ int& col_tile(int c) const { return mem[kTableHead + 4 * (groups + 1) + c]; }
+  __device__ int& col_base(int c) const { return mem[kTableHead + 4 * (groups + 1) + pairs + 1 + c]; }
 
   // Column c gets tiles / shares tiles, and the part-filled row's are spread over the columns.
   __device__ static int column_first(int c, int tiles, int shares) {
     return c * (tiles / shares) + c * (tiles % shares) / shares;
   }
-  __device__ int share_begin(int p) const { return p * per_share + min(p, more_share); }
+  __device__ int share_begin(int p) const {
+    return whole ? col_base(p) : p * per_share() + min(p, more_share());
+  }
   // The column of the line's tile v: the last c with column_first(c) = floor(c * tiles / shares) <= v.
-  __device__ int column_of(int v) const { return ((v + 1) * shares - 1) / tiles; }
+  __device__ int column_of(int v) const { return ((v + 1) * shares() - 1) / tiles(); }
   __device__ int tile_of(int c, int t) const {
-    return t < per_column ? t * shares + c : per_column * shares + col_tile[c] - c * per_column;
+    const int high = per_column(), wide = shares();
+    return t < high ? t * wide + c : high * wide + col_tile(c) - c * high;
   }
   __device__ int group_of(int tile) const {
     int e = 0, top = groups - 1;  // last group whose first tile is <= tile; groups without tiles come before it
     while (e < top) {
       const int mid = (e + top + 1) >> 1;
-      if (tile_base[mid] <= tile) {
+      if (tile_base(mid) <= tile) {
         e = mid;
       } else {
         top = mid - 1;
@@ -164,20 +181,14 @@ struct GroupTable {
   }
 };
 
-constexpr int kTableHead = 8;
 constexpr __host__ __device__ int group_table_ints(int groups, int pairs) {
   return kTableHead + 4 * (groups + 1) + 2 * (pairs + 1);
 }
 
-// Builds the table in shared memory. Ends are taken as they would be if clamped to
-// [previous end, rows], so no value of `ends` leads out of the matrices. All threads of the block
-// (128 or more); the caller synchronises before and after, and reads it with group_table.
+// Builds the groups' part. Ends are taken as they would be if clamped to [previous end, rows], so no
+// value of `ends` leads out of the matrices. One warp; a barrier before the second step.
 template <GroupMode MODE>
-__device__ inline void build_group_rows(const GroupedArgs& a, int* mem) {
-  int* start = mem + kTableHead;
-  int* tile_base = start + a.groups + 1;
-  int* row_tiles = tile_base + a.groups + 1;
-  int* width = row_tiles + a.groups + 1;
+__device__ inline void build_group_rows(const GroupedArgs& a, const GroupTable& t) {
   const int lane = static_cast<int>(lane_id());
   const int col_tiles = ceil_div(a.cols, 256);
   int row = 0, tiles = 0, total = 0;
@@ -203,90 +214,70 @@ __device__ inline void build_group_rows(const GroupedArgs& a, int* mem) {
     }
     total += __reduce_add_sync(0xffffffffu, mine * group_blocks<MODE>(a, end - begin));
     if (g < a.groups) {
-      start[g] = begin;
-      tile_base[g] = tiles + sum - mine;
-      row_tiles[g] = high;
-      width[g] = group_rows_right(MODE) && high > 0 ? group_width(end - begin, a.width_cap) : 0;
+      t.start(g) = begin;
+      t.tile_base(g) = tiles + sum - mine;
+      t.row_tiles(g) = high;
+      t.width(g) = group_rows_right(MODE) && high > 0 ? group_width(end - begin, a.width_cap) : 0;
     }
     row = __shfl_sync(0xffffffffu, end, 31);
     tiles += __shfl_sync(0xffffffffu, sum, 31);
   }
   if (lane == 0) {
-    start[a.groups] = row;
-    tile_base[a.groups] = tiles;
-    const int shares = max(1, min(a.pairs, total / a.min_blocks));
-    mem[0] = tiles;
-    mem[1] = shares;
-    mem[2] = total;
-    mem[3] = tiles / shares;
-    mem[4] = total / shares;
-    mem[5] = total % shares;
+    t.start(a.groups) = row;
+    t.tile_base(a.groups) = tiles;
+    const int shares = max(1, min(a.pairs, a.whole ? tiles : total / a.min_blocks));
+    t.tiles() = tiles;
+    t.shares() = shares;
+    t.total() = total;
+    t.per_column() = tiles / shares;
+    t.per_share() = total / shares;
+    t.more_share() = total % shares;
   }
 }
 
-__device__ inline GroupTable group_table(const GroupedArgs& a, const int* mem) {
-  GroupTable t;
-  t.start = mem + kTableHead;
-  t.tile_base = t.start + a.groups + 1;
-  t.row_tiles = t.tile_base + a.groups + 1;
-  t.width = t.row_tiles + a.groups + 1;
-  t.col_tile = t.width + a.groups + 1;
-  t.col_base = t.col_tile + a.pairs + 1;
-  t.groups = a.groups;
-  t.tiles = mem[0];
-  t.shares = mem[1];
-  t.total = mem[2];
-  t.per_column = mem[3];
-  t.per_share = mem[4];
-  t.more_share = mem[5];
-  return t;
-}
-
-// Second step, after a barrier; all threads, and a barrier before the table is used.
+// Second step, the columns' part: all threads, and a barrier before the table is used.
 template <GroupMode MODE>
-__device__ inline void build_group_columns(const GroupedArgs& a, int* mem) {
-  const GroupTable t = group_table(a, mem);
-  int* col_tile = mem + kTableHead + 4 * (a.groups + 1);
-  int* col_base = col_tile + a.pairs + 1;
-  for (int c = static_cast<int>(threadIdx.x); c <= t.shares; c += static_cast<int>(blockDim.x)) {
-    const int first = GroupTable::column_first(c, t.tiles, t.shares);
-    col_tile[c] = first;
-    if (MODE != GroupMode::kWeightGrad) col_base[c] = first * a.k_blocks;
+__device__ inline void build_group_columns(const GroupedArgs& a, const GroupTable& t) {
+  const int shares = t.shares(), tiles = t.tiles();
+  for (int c = static_cast<int>(threadIdx.x); c <= shares; c += static_cast<int>(blockDim.x)) {
+    const int first = GroupTable::column_first(c, tiles, shares);
+    t.col_tile(c) = first;
+    if (MODE != GroupMode::kWeightGrad) t.col_base(c) = first * a.k_blocks;
   }
   if constexpr (MODE == GroupMode::kWeightGrad) {
     __syncthreads();
     // K blocks differ by group: one warp sums a column, its lanes over the groups; then a scan.
     const int lane = static_cast<int>(lane_id());
-    const int whole = t.per_column * t.shares;  // tiles of the full rows
-    for (int c = static_cast<int>(threadIdx.x >> 5); c < t.shares; c += static_cast<int>(blockDim.x >> 5)) {
+    const int whole = t.per_column() * shares;  // tiles of the full rows
+    for (int c = static_cast<int>(threadIdx.x >> 5); c < shares; c += static_cast<int>(blockDim.x >> 5)) {
       int sum = 0;
       for (int e = lane; e < a.groups; e += 32) {
-        const int lo = min(t.tile_base[e], whole), hi = min(t.tile_base[e + 1], whole);
+        const int lo = min(t.tile_base(e), whole), hi = min(t.tile_base(e + 1), whole);
         if (hi <= lo) continue;
         // Tiles of column c below x: those with number * shares + c < x.
-        const int count = (hi - c + t.shares - 1) / t.shares - (lo - c + t.shares - 1) / t.shares;
-        sum += count * group_blocks<MODE>(a, t.start[e + 1] - t.start[e]);
+        const int count = (hi - c + shares - 1) / shares - (lo - c + shares - 1) / shares;
+        sum += count * group_blocks<MODE>(a, t.start(e + 1) - t.start(e));
       }
       sum = __reduce_add_sync(0xffffffffu, sum);
-      if (t.col_tile[c + 1] - t.col_tile[c] > t.per_column) {
-        const int e = t.group_of(t.tile_of(c, t.per_column));
-        sum += group_blocks<MODE>(a, t.start[e + 1] - t.start[e]);
+      if (t.col_tile(c + 1) - t.col_tile(c) > t.per_column()) {
+        const int e = t.group_of(t.tile_of(c, t.per_column()));
+        sum += group_blocks<MODE>(a, t.start(e + 1) - t.start(e));
       }
-      if (lane == 0) col_base[c] = sum;
+      if (lane == 0) t.col_base(c) = sum;
     }
     __syncthreads();
     if (threadIdx.x >= 32) return;
     int before = 0;
-    for (int c0 = 0; c0 <= t.shares; c0 += 32) {
+    for (int c0 = 0; c0 <= shares; c0 += 32) {
       const int c = c0 + lane;
-      const int sum = c < t.shares ? col_base[c] : 0;
+      const int sum = c < shares ? t.col_base(c) : 0;
       int scan = sum;
 #pragma unroll
       for (int d = 1; d < 32; d *= 2) {
         const int o = __shfl_up_sync(0xffffffffu, scan, d);
         if (lane >= d) scan += o;
       }
-      if (c <= t.shares) col_base[c] = before + scan - sum;
+      if (c <= shares) t.col_base(c) = before + scan - sum;
       before += __shfl_sync(0xffffffffu, scan, 31);
     }
   }
@@ -305,18 +296,18 @@ struct GroupSegment {
 // Width of a tile of group e whose first R column is r0.
 template <GroupMode MODE>
 __device__ inline int tile_width(const GroupedArgs& a, const GroupTable& t, int e, int r0) {
-  if (group_rows_right(MODE)) return t.width[e];
+  if (group_rows_right(MODE)) return t.width(e);
   return a.cols - r0 <= 128 ? 128 : 256;
 }
 
 // First L row and R column of tile `tile` of group `e`.
 template <GroupMode MODE>
 __device__ inline void tile_origin(const GroupedArgs& a, const GroupTable& t, int e, int tile, int& l0, int& r0) {
-  const int row0 = t.start[e];
+  const int row0 = t.start(e);
   int pr, pc;
-  grouped_tile(tile - t.tile_base[e], t.row_tiles[e], ceil_div(a.cols, 256), kGroupRaster, pr, pc);
+  grouped_tile(tile - t.tile_base(e), t.row_tiles(e), ceil_div(a.cols, 256), kGroupRaster, pr, pc);
   if (group_rows_right(MODE)) {
-    r0 = row0 + pr * t.width[e];
+    r0 = row0 + pr * t.width(e);
     l0 = pc * 256;
   } else {
     l0 = (MODE == GroupMode::kWeightGrad ? 0 : row0) + pr * 256;
@@ -343,10 +334,10 @@ struct GroupWalk {
     line = hi;
     if (lo >= hi) return;
     int c = guess;
-    while (t.col_base[c] > lo) --c;
-    while (t.col_base[c + 1] <= lo) ++c;
-    v = t.col_tile[c];
-    line = t.col_base[c];
+    while (t.col_base(c) > lo) --c;
+    while (t.col_base(c + 1) <= lo) ++c;
+    v = t.col_tile(c);
+    line = t.col_base(c);
     if constexpr (MODE != GroupMode::kWeightGrad) {
       const int n = (lo - line) / a.k_blocks;
       v += n;
@@ -355,19 +346,19 @@ struct GroupWalk {
   }
   // The share of `pair`.
   __device__ GroupWalk(const GroupedArgs& a, const GroupTable& t, int pair)
-      : GroupWalk(a, t, pair < t.shares ? t.share_begin(pair) : 0, pair < t.shares ? t.share_begin(pair + 1) : 0,
-                  min(pair, t.shares - 1)) {}
+      : GroupWalk(a, t, pair < t.shares() ? t.share_begin(pair) : 0, pair < t.shares() ? t.share_begin(pair + 1) : 0,
+                  min(pair, t.shares() - 1)) {}
 
   __device__ void refill(const GroupedArgs& a, const GroupTable& t) {
     const int lane = static_cast<int>(lane_id());
     uint32_t live = 0;
     while (live == 0 && line < hi) {  // kWeightGrad: batches before lo are passed over
       int blocks = 0, e = 0, tile = 0;
-      if (v + lane < t.tiles) {
+      if (v + lane < t.tiles()) {
         const int c = t.column_of(v + lane);
-        tile = t.tile_of(c, v + lane - t.col_tile[c]);
+        tile = t.tile_of(c, v + lane - t.col_tile(c));
         e = t.group_of(tile);
-        blocks = group_blocks<MODE>(a, t.start[e + 1] - t.start[e]);
+        blocks = group_blocks<MODE>(a, t.start(e + 1) - t.start(e));
       }
       int scan = blocks;
 #pragma unroll
@@ -404,8 +395,8 @@ struct GroupWalk {
     s.r0 = __shfl_sync(0xffffffffu, r0, from);
     s.kb0 = __shfl_sync(0xffffffffu, kb0, from);
     s.kb1 = __shfl_sync(0xffffffffu, kb1, from);
-    s.row0 = t.start[s.group];
-    s.row_end = t.start[s.group + 1];
+    s.row0 = t.start(s.group);
+    s.row_end = t.start(s.group + 1);
     s.blocks = group_blocks<MODE>(a, s.row_end - s.row0);
     s.width = tile_width<MODE>(a, t, s.group, s.r0);
     return true;
@@ -611,8 +602,31 @@ __device__ __forceinline__ void store_cols_64(T* out, int64_t first, int rows, i
   }
 }
 
-// Takes `regs` registers a thread from, or gives them to, the calling warpgroup. The kernel is
-// launched with 384 x 168; 128 x 56 + 256 x 224 is the same number.
+// What no tile covers: rows past the last group, or the outputs of groups without rows. Thread `mine`
+// of `step`.
+template <GroupMode MODE, typename T>
+__device__ inline void write_zeros(const GroupedArgs& a, const GroupTable& t, T* out, int64_t mine, int64_t step) {
+  auto zero = [&](T* p, int64_t count) {
+    if ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && count % 8 == 0) {
+      for (int64_t i = mine; i < count / 8; i += step) reinterpret_cast<uint4*>(p)[i] = make_uint4(0, 0, 0, 0);
+    } else {
+      for (int64_t i = mine; i < count; i += step) p[i] = from_f32<T>(0.f);
+    }
+  };
+  if constexpr (MODE == GroupMode::kWeightGrad) {
+    const int64_t size = static_cast<int64_t>(a.lrows) * a.cols;
+    for (int g = 0; g < a.groups; ++g) {
+      if (t.start(g + 1) == t.start(g)) zero(out + g * size, size);
+    }
+  } else {
+    const int64_t from = t.start(a.groups);
+    if (from < a.rows) zero(out + from * a.cols, (a.rows - from) * a.cols);
+  }
+}
+
+// Takes registers from, or gives them to, the calling warpgroup: REGS a thread then. The kernel is
+// launched with 384 x 168 = 64512; 128 x 80 + 256 x 208 are 63488, and neither side spills (with 40 and
+// 232, or 56 and 224, the issuing warps did: 46 us against 43 for 257 x 12800 x 4096).
 template <int REGS>
 __device__ __forceinline__ void registers_down() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
@@ -669,7 +683,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
   uint64_t* mma_done = tmem_empty + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* table_mem = reinterpret_cast<int*>(tmem_slot + 4);
+  const GroupTable table = {reinterpret_cast<int*>(tmem_slot + 4), args.groups, args.pairs, args.whole};
 
   const int warp = threadIdx.x >> 5;
   const uint32_t lane = lane_id();
@@ -697,16 +711,15 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
     tmem_alloc_pair(tmem_slot, 512);
     tmem_relinquish_pair();
   }
-  if (warp == 2) build_group_rows<MODE>(args, table_mem);
+  if (warp == 2) build_group_rows<MODE>(args, table);
   __syncthreads();
-  build_group_columns<MODE>(args, table_mem);
+  build_group_columns<MODE>(args, table);
   tc_fence_before_sync();
   cluster_sync();  // both CTAs' barriers exist before either signals the other
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot;
-  const GroupTable table = group_table(args, table_mem);
   if constexpr (kWide) {
-    if (warp < kFirstEpilogue) registers_down<40>();
+    if (warp < kFirstEpilogue) registers_down<80>();
   }
 
   if (warp == 0) {
@@ -882,7 +895,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
     }
   } else if (warp >= kFirstEpilogue && warp < kFirstEpilogue + kEpilogueWarps) {
     // ---------------- epilogue (both CTAs, own 128 TMEM lanes) ----------------
-    if constexpr (kWide) registers_up<232>();
+    if constexpr (kWide) registers_up<208>();
     const int quarter = warp & 3;
     const int row = quarter * 32 + static_cast<int>(lane);  // TMEM lane
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
@@ -1097,6 +1110,11 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
         }
       }
     }
+    if (args.whole) {
+      const int64_t thread = (warp - kFirstEpilogue) * 32 + static_cast<int>(lane);
+      write_zeros<MODE>(args, table, out, blockIdx.x * (kEpilogueWarps * 32) + thread,
+                        static_cast<int64_t>(gridDim.x) * (kEpilogueWarps * 32));
+    }
   }
 
   tc_fence_before_sync();
@@ -1123,23 +1141,23 @@ __global__ void __launch_bounds__(kFinishThreads) grouped_finish_kernel(const __
   constexpr int kCols = finish_cols<MODE>();
   __shared__ __align__(128) uint8_t out_stage[group_rows_right(MODE) ? 16 : kFinishThreads / 32 * kStageOutBytes];
   extern __shared__ int finish_table[];
-  if (threadIdx.x < 32) build_group_rows<MODE>(args, finish_table);
+  const GroupTable table = {finish_table, args.groups, args.pairs, args.whole};
+  if (threadIdx.x < 32) build_group_rows<MODE>(args, table);
   __syncthreads();
-  build_group_columns<MODE>(args, finish_table);
+  build_group_columns<MODE>(args, table);
   __syncthreads();
-  const GroupTable table = group_table(args, finish_table);
   T* out = static_cast<T*>(args.out);
   const int p = static_cast<int>(blockIdx.x) + 1;
   const int rank = static_cast<int>(blockIdx.y);
   GroupSegment s = {};
   int cut = 0;
-  if (p < table.shares) {
+  if (p < table.shares()) {
     cut = table.share_begin(p);
     GroupWalk<MODE> walk(args, table, cut, cut + 1, p);
     walk.next(args, table, s);
   }
   wait_for_primary();  // the pieces; all before it comes from `ends` alone
-  if (p < table.shares) {
+  if (p < table.shares()) {
     const int begin = cut - s.kb0, end = begin + s.blocks;
     const int c = static_cast<int>(blockIdx.z) * kCols;
     if (cut > begin && table.share_begin(p - 1) <= begin && c < s.width) {
@@ -1150,7 +1168,7 @@ __global__ void __launch_bounds__(kFinishThreads) grouped_finish_kernel(const __
       // Columns and rows that hold values of the output (what else a piece has was not written).
       const bool mine = MODE != GroupMode::kScaled || s.l0 + rank * 128 + row < s.row_end;
       const int live_cols = group_rows_right(MODE) ? min(s.width, s.row_end - s.r0) : min(s.width, args.cols - s.r0);
-      for (int o = p - 1; mine && o < table.shares && table.share_begin(o) < end; ++o) {
+      for (int o = p - 1; mine && o < table.shares() && table.share_begin(o) < end; ++o) {
         const int piece = table.share_begin(o) >= begin ? 0 : 1;
         const float* src = args.partials +
                            (static_cast<size_t>(o * 2 + piece) * 2 + rank) * static_cast<size_t>(args.piece_floats) +
@@ -1178,26 +1196,9 @@ __global__ void __launch_bounds__(kFinishThreads) grouped_finish_kernel(const __
       }
     }
   }
-  // Zeros: rows past the last group, or the outputs of groups without rows.
-  const int64_t step = static_cast<int64_t>(gridDim.x) * gridDim.y * gridDim.z * kFinishThreads;
-  const int64_t mine =
-      ((static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * kFinishThreads + threadIdx.x;
-  auto zero = [&](T* p, int64_t count) {
-    if ((reinterpret_cast<uintptr_t>(p) & 15) == 0 && count % 8 == 0) {
-      for (int64_t i = mine; i < count / 8; i += step) reinterpret_cast<uint4*>(p)[i] = make_uint4(0, 0, 0, 0);
-    } else {
-      for (int64_t i = mine; i < count; i += step) p[i] = from_f32<T>(0.f);
-    }
-  };
-  if constexpr (MODE == GroupMode::kWeightGrad) {
-    const int64_t size = static_cast<int64_t>(args.lrows) * args.cols;
-    for (int g = 0; g < args.groups; ++g) {
-      if (table.start[g + 1] == table.start[g]) zero(out + g * size, size);
-    }
-  } else {
-    const int64_t from = table.start[args.groups];
-    if (from < args.rows) zero(out + from * args.cols, (args.rows - from) * args.cols);
-  }
+  write_zeros<MODE>(args, table, out,
+                    ((static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * kFinishThreads + threadIdx.x,
+                    static_cast<int64_t>(gridDim.x) * gridDim.y * gridDim.z * kFinishThreads);
 }
 
 }  // namespace hst

@@ -56,13 +56,35 @@ int64_t max_iterations(const GroupedProblem& p) {
 // saves.
 constexpr int kMinBlocks = 4;
 
+// K blocks of the deepest tile there can be.
+template <GroupMode MODE>
+int64_t deepest_tile(const GroupedProblem& p) {
+  return MODE == GroupMode::kWeightGrad ? cdiv(p.rows, 64) : p.k_blocks;
+}
+
+// Shares end at tiles up to this depth (gemm_grouped.cuh, the schedule). Measured either side: at 8 and
+// 16 blocks whole tiles take 3 to 7 us less, at 32 they take up to 4 us more where the tiles fill part
+// of a wave.
+constexpr int kWholeBlocks = 16;
+template <GroupMode MODE>
+bool whole_tiles(const GroupedProblem& p) {
+  return deepest_tile<MODE>(p) <= kWholeBlocks;
+}
+
 template <GroupMode MODE>
 int plan_pairs(const GroupedProblem& p, int sms) {
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms / 2, max_iterations<MODE>(p) / kMinBlocks)));
+  int64_t most = max_iterations<MODE>(p) / kMinBlocks;
+  if (whole_tiles<MODE>(p)) {
+    const int64_t cols = cdiv(p.cols, 256);
+    most = MODE == GroupMode::kWeightGrad ? cols * cdiv(p.lrows, 256) * std::min<int64_t>(p.groups, p.rows)
+                                          : max_iterations<MODE>(p) / std::max<int64_t>(1, p.k_blocks);
+  }
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms / 2, most)));
 }
 
 template <GroupMode MODE>
 size_t workspace_bytes(const GroupedProblem& p, int sms) {
+  if (whole_tiles<MODE>(p)) return 0;
   return static_cast<size_t>(plan_pairs<MODE>(p, sms)) * 4 * 128 * p.width_cap * sizeof(float);
 }
 
@@ -77,7 +99,7 @@ int launch_grouped(const GroupedProblem& p, const GroupedMaps& maps, GroupedArgs
   HST_TRY(device_state(&dev));
   if (max_iterations<MODE>(p) > INT32_MAX) return fail(HST_ERR_UNSUPPORTED, "the grouped product has too many tiles");
   const size_t need = workspace_bytes<MODE>(p, dev->sm_count);
-  if (workspace_size < need || workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)
+  if (need > 0 && (workspace_size < need || workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0))
     return fail(HST_ERR_WORKSPACE, "workspace of %zu bytes, 16-byte aligned, needed; got %zu", need, workspace_size);
   args.groups = p.groups;
   args.rows = static_cast<int>(p.rows);
@@ -88,6 +110,7 @@ int launch_grouped(const GroupedProblem& p, const GroupedMaps& maps, GroupedArgs
   args.r_bytes = r_bytes;
   args.pairs = plan_pairs<MODE>(p, dev->sm_count);
   args.min_blocks = kMinBlocks;
+  args.whole = whole_tiles<MODE>(p);
   args.vec = 32;
   while (args.vec > 2 && (p.cols * 2 % args.vec != 0 || reinterpret_cast<uintptr_t>(args.out) % args.vec != 0)) args.vec /= 2;
   args.status = dev->status;
@@ -96,7 +119,7 @@ int launch_grouped(const GroupedProblem& p, const GroupedMaps& maps, GroupedArgs
   int stages = kMaxStages;
   while (stages > 2 && S::smem_bytes(stages, r_bytes, p.groups, args.pairs) > kMaxDynamicSmem) --stages;
   args.stages = stages;
-  if (p.rows > 0) {
+  {
     static std::atomic<uint64_t> smem_done{0};
     HST_TRY(allow_smem(grouped_gemm_kernel<MODE, L_MN, T>, smem_done));
     cudaLaunchConfig_t lc = {};
@@ -113,6 +136,7 @@ int launch_grouped(const GroupedProblem& p, const GroupedMaps& maps, GroupedArgs
     lc.numAttrs = 1;
     HST_CUDA(cudaLaunchKernelEx(&lc, grouped_gemm_kernel<MODE, L_MN, T>, maps, args));
   }
+  if (args.whole) return HST_OK;
   cudaLaunchConfig_t lc = {};
   lc.gridDim = dim3(static_cast<unsigned>(std::max(1, args.pairs - 1)), 2,
                     static_cast<unsigned>(cdiv(args.piece_floats / 128, finish_cols<MODE>())));
@@ -123,7 +147,7 @@ int launch_grouped(const GroupedProblem& p, const GroupedMaps& maps, GroupedArgs
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   lc.attrs = attr;
-  lc.numAttrs = p.rows > 0 ? 1 : 0;
+  lc.numAttrs = 1;
   HST_CUDA(cudaLaunchKernelEx(&lc, grouped_finish_kernel<MODE, T>, args));
   return HST_OK;
 }

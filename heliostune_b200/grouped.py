@@ -11,7 +11,8 @@ the same kernel on the transposed view, ``dweight[e] = x[e].T @ dy[e]`` its own
 (:func:`grouped_weight_grad`).
 
 Nothing is read back from the GPU: the sizes stay there, and a call can be captured into a CUDA
-graph and replayed with other ends. Rows past the last end belong to no expert: their outputs and
+graph and replayed with other ends. (A backward pass is captured, as with any torch operator, while no
+eager graph of the same leaves is alive: their gradient nodes would tie the capture to the eager stream.) Rows past the last end belong to no expert: their outputs and
 input gradients are zero, and they enter no weight gradient. An expert without rows gets a zero
 weight gradient. Each end is taken clamped to ``[previous end, T]``.
 
@@ -42,11 +43,17 @@ def _workspace_bytes(op: int, rows: int, groups: int, n: int, k: int, device: in
     return size.value
 
 
-def _workspace(op: int, rows: int, groups: int, n: int, k: int, device: torch.device) -> tuple[torch.Tensor, int]:
-    """The FP32 pieces of tiles shared between CTA pairs, a tensor of this call alone, and its bytes."""
+def _workspace(
+    op: int, rows: int, groups: int, n: int, k: int, device: torch.device
+) -> tuple[torch.Tensor | None, int | None, int]:
+    """The FP32 pieces of tiles shared between CTA pairs: a tensor of this call alone (None for products
+    without any), its address and its bytes."""
     index = device.index if device.index is not None else torch.cuda.current_device()
     nbytes = _workspace_bytes(op, rows, groups, n, k, index)
-    return torch.empty(nbytes, device=device, dtype=torch.uint8), nbytes
+    if nbytes == 0:
+        return None, None, 0
+    buffer = torch.empty(nbytes, device=device, dtype=torch.uint8)
+    return buffer, buffer.data_ptr(), nbytes
 
 
 def _padded_copy(t: torch.Tensor, group_ends: torch.Tensor | None = None, total_rows: int = 0) -> torch.Tensor:
@@ -135,14 +142,15 @@ def _forward(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tensor) ->
     y = torch.empty((rows, n), device=device, dtype=x.dtype)
     x, x_pointer, x_row = _readable_rows(x, 8)
     weight, w_pointer, w_group, w_row, layout = _readable_weights(weight, group_ends, rows)
-    workspace, nbytes = _workspace(_native.GROUPED_FORWARD, rows, groups, n, k, device)
+    workspace, ws_pointer, ws_bytes = _workspace(_native.GROUPED_FORWARD, rows, groups, n, k, device)
     with _device_guard(device):
         _native.check(
             _native.library().hst_grouped_matmul(
                 _DTYPES[x.dtype], x_pointer, x_row, w_pointer, w_group, w_row, layout, group_ends.data_ptr(), groups,
-                y.data_ptr(), rows, n, k, workspace.data_ptr(), nbytes, _stream(device),
+                y.data_ptr(), rows, n, k, ws_pointer, ws_bytes, _stream(device),
             )
         )  # fmt: skip
+    del workspace  # stream-ordered reuse by the caching allocator is safe on this stream
     return y
 
 
@@ -152,14 +160,15 @@ def _weight_grad(left: torch.Tensor, right: torch.Tensor, group_ends: torch.Tens
     out = torch.empty((groups, lcols, rcols), device=device, dtype=left.dtype)
     left, l_pointer, l_row = _readable_rows(left, 8)
     right, r_pointer, r_row = _readable_rows(right, 8)
-    workspace, nbytes = _workspace(_native.GROUPED_WEIGHT_GRAD, rows, groups, rcols, lcols, device)
+    workspace, ws_pointer, ws_bytes = _workspace(_native.GROUPED_WEIGHT_GRAD, rows, groups, rcols, lcols, device)
     with _device_guard(device):
         _native.check(
             _native.library().hst_grouped_weight_grad(
                 _DTYPES[left.dtype], l_pointer, l_row, r_pointer, r_row, group_ends.data_ptr(), groups, out.data_ptr(),
-                rows, lcols, rcols, workspace.data_ptr(), nbytes, _stream(device),
+                rows, lcols, rcols, ws_pointer, ws_bytes, _stream(device),
             )
         )  # fmt: skip
+    del workspace
     return out
 
 

@@ -193,8 +193,9 @@ int hst_gated_mlp_stream(int32_t block_m, int32_t block_k, int32_t num_stages, i
  * Operands: 16-byte aligned bases and strides. Outputs are contiguous and written whole: rows past
  * the last group, and the weight gradients of groups without rows, are zero. FP32 accumulation, one
  * rounding, bitwise reproducible. The caller gives a 16-byte aligned workspace of
- * hst_grouped_workspace_size bytes (no initialisation needed); calls that share one must not overlap
- * on the GPU. Each product is two launches on the stream and can be captured. */
+ * hst_grouped_workspace_size bytes (0 for shallow products, no initialisation needed); calls that share
+ * one must not overlap on the GPU. Each product is one or two launches on the stream and can be
+ * captured. */
 #define HST_GROUPED_FORWARD 0      /* hst_grouped_matmul: n, k */
 #define HST_GROUPED_WEIGHT_GRAD 1  /* hst_grouped_weight_grad: n = rcols, k = lcols */
 #define HST_GROUPED_SCALED 2       /* hst_matmul_blockscaled: n, k */

@@ -243,7 +243,7 @@ def test_extents_and_strides_that_tma_cannot_read(rows: int, n: int, k: int) -> 
     "rows,ends",
     ((1, [0, 1]), (9, [3, 3, 8]), (96, [40, 41, 96]), (300, [0, 255, 255, 300]), (700, [256, 513, 700]), (40, [0, 0, 0]), (1111, [600, 600, 1100])),
 )
-@pytest.mark.parametrize("n,k", ((136, 264), (520, 1040)))
+@pytest.mark.parametrize("n,k", ((136, 264), (520, 1040), (264, 2192)))  # 2192: more than 16 K blocks, tiles are cut
 def test_grouped(rows: int, ends: list[int], n: int, k: int) -> None:
     a, sa, b, sb = _operands(rows, n, k, seed=rows + n, groups=len(ends))
     y = blockscale.matmul_blockscaled(a, sa, b, sb, _ends(ends), out_dtype=torch.float16)
@@ -313,10 +313,11 @@ def test_empty_extents_and_refusals() -> None:
 
 @gpu
 @pytest.mark.parametrize("rows", (3, 700))
-def test_captured_and_concurrent_calls(rows: int) -> None:
+@pytest.mark.parametrize("k", (1040, 2320))
+def test_captured_and_concurrent_calls(rows: int, k: int) -> None:
     g = torch.Generator(device="cuda").manual_seed(5)
-    x = torch.randn((rows, 1040), generator=g, device="cuda").bfloat16()
-    w = (torch.randn((520, 1040), generator=g, device="cuda") / 32).bfloat16()
+    x = torch.randn((rows, k), generator=g, device="cuda").bfloat16()
+    w = (torch.randn((520, k), generator=g, device="cuda") / 32).bfloat16()
     b, sb = blockscale.quantize_tiles(w)
 
     def step() -> torch.Tensor:

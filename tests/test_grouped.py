@@ -149,7 +149,7 @@ ROWS = (
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("layout", ("kn", "nk"))
 @pytest.mark.parametrize("rows,ends", ROWS)
-@pytest.mark.parametrize("k,n", ((64, 256), (200, 264), (1000, 72)))
+@pytest.mark.parametrize("k,n", ((64, 256), (200, 264), (1000, 72), (1096, 264)))  # 1096: more than 16 K blocks, tiles are cut
 def test_forward_and_gradients(dtype: torch.dtype, layout: str, rows: int, ends: list[int], k: int, n: int) -> None:
     x, w, dy = _operands(rows, len(ends), k, n, dtype, layout, seed=rows + k)
     x.requires_grad_()
@@ -342,7 +342,7 @@ def test_repeats_are_bitwise_identical() -> None:
 @gpu
 def test_two_streams_at_once() -> None:
     ends = [100, 300, 640]
-    x, w, dy = _operands(640, 3, 1032, 520, torch.float16, "kn", seed=15)
+    x, w, dy = _operands(640, 3, 2056, 520, torch.float16, "kn", seed=15)
     e = _ends(ends)
     expected = grouped.grouped_matmul(x, w, e), grouped.grouped_weight_grad(x, dy, e)
     streams = torch.cuda.Stream(), torch.cuda.Stream()
@@ -357,9 +357,10 @@ def test_two_streams_at_once() -> None:
 
 
 @gpu
-def test_captured_steps_follow_new_ends_and_inputs() -> None:
+@pytest.mark.parametrize("k", (264, 1544))
+def test_captured_steps_follow_new_ends_and_inputs(k: int) -> None:
     """Two graphs of a training step, replayed in turn with other ends and inputs than they were captured with."""
-    x, w, dy = _operands(300, 3, 264, 200, torch.float16, "kn", seed=16)
+    x, w, dy = _operands(300, 3, k, 200, torch.float16, "kn", seed=16)
     ends = _ends([100, 200, 300])
     x.requires_grad_()
     w.requires_grad_()
@@ -391,16 +392,28 @@ def test_captured_steps_follow_new_ends_and_inputs() -> None:
 
 
 @gpu
+def test_outputs_past_32_bit_offsets() -> None:
+    """70000 x 32776 outputs, 2.3e9 values: the last rows of the last group."""
+    rows, n, k = 70_000, 32_776, 64
+    x, w, _ = _operands(rows, 2, k, n, torch.float16, "nk", seed=19)
+    y = grouped.grouped_matmul(x, w, _ends([33, rows - 3]))
+    last = slice(rows - 40, rows - 3)
+    _assert_close(y[last], x[last].double() @ w[1].double(), x[last].double().abs() @ w[1].double().abs(), k)
+    assert bool((y[rows - 3 :] == 0).all())
+
+
+@gpu
 def test_the_workspace_is_checked_and_its_contents_do_not_matter() -> None:
-    x, w, dy = _operands(120, 2, 520, 264, torch.float16, "kn", seed=17)
+    x, w, dy = _operands(120, 2, 2056, 264, torch.float16, "kn", seed=17)
     ends = _ends([50, 120])
     lib = _native.library()
-    size = grouped._workspace_bytes(_native.GROUPED_FORWARD, 120, 2, 264, 520, 0)
+    assert grouped._workspace_bytes(_native.GROUPED_FORWARD, 120, 2, 264, 520, 0) == 0
+    size = grouped._workspace_bytes(_native.GROUPED_FORWARD, 120, 2, 264, 2056, 0)
     y = torch.empty((120, 264), device="cuda", dtype=torch.float16)
 
     def call(workspace: torch.Tensor) -> int:
         return lib.hst_grouped_matmul(
-            0, x.data_ptr(), 520, w.data_ptr(), 520 * 264, 264, 0, ends.data_ptr(), 2, y.data_ptr(), 120, 264, 520,
+            0, x.data_ptr(), 2056, w.data_ptr(), 2056 * 264, 264, 0, ends.data_ptr(), 2, y.data_ptr(), 120, 264, 2056,
             workspace.data_ptr(), workspace.numel(), torch.cuda.current_stream().cuda_stream,
         )  # fmt: skip
 
