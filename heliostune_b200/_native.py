@@ -49,11 +49,6 @@ FAMILY_PAIR = 4
 
 HST_F16 = 0
 HST_BF16 = 1
-HST_WEIGHT_KN = 0
-HST_WEIGHT_NK = 1
-GROUPED_FORWARD = 0
-GROUPED_WEIGHT_GRAD = 1
-GROUPED_SCALED = 2
 
 #: Every symbol include/heliostune_b200.h declares.
 EXPORTED_SYMBOLS = (
@@ -81,12 +76,13 @@ EXPORTED_SYMBOLS = (
     "hst_ipc_close",
     "hst_pair_stream_k_tiles",
     "hst_rmsnorm_matmul_stream",
-    "hst_grouped_workspace_size",
+    "hst_grouped_matmul_workspace",
     "hst_grouped_matmul",
+    "hst_grouped_weight_grad_workspace",
     "hst_grouped_weight_grad",
+    "hst_matmul_blockscaled_workspace",
     "hst_matmul_blockscaled",
     "hst_quantize_e4m3",
-    "hst_pack_rows",
 )
 
 
@@ -197,29 +193,33 @@ def _declare(lib: ctypes.CDLL) -> None:
             [ctypes.POINTER(ctypes.c_void_p), _i32, _i32, _i32, ctypes.c_uint64, ctypes.c_uint64, _ptr],
             ctypes.c_int,
         ),
-        "hst_grouped_workspace_size": (
-            [_i32, _i64, _i32, _i64, _i64, ctypes.c_int, ctypes.POINTER(_size)],
+        "hst_grouped_matmul_workspace": (
+            [_ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _i32, _i64, _i64, _i64, ctypes.c_int, ctypes.POINTER(_size)],
             ctypes.c_int,
         ),
         "hst_grouped_matmul": (
-            [_i32, _ptr, _i64, _ptr, _i64, _i64, _i32, _ptr, _i32, _ptr, _i64, _i64, _i64, _ptr, _size, _ptr],
+            [_i32, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _i32, _ptr, _i64, _i64, _i64, _ptr, _size, _ptr],
+            ctypes.c_int,
+        ),
+        "hst_grouped_weight_grad_workspace": (
+            [_ptr, _i64, _i64, _ptr, _i64, _i64, _i32, _i64, _i64, _i64, ctypes.c_int, ctypes.POINTER(_size)],
             ctypes.c_int,
         ),
         "hst_grouped_weight_grad": (
-            [_i32, _ptr, _i64, _ptr, _i64, _ptr, _i32, _ptr, _i64, _i64, _i64, _ptr, _size, _ptr],
+            [_i32, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i32, _ptr, _i64, _i64, _i64, _ptr, _size, _ptr],
+            ctypes.c_int,
+        ),
+        "hst_matmul_blockscaled_workspace": (
+            [_ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _i32, _i64, _i64, _i64, ctypes.c_int, ctypes.POINTER(_size)],
             ctypes.c_int,
         ),
         "hst_matmul_blockscaled": (
-            [_i32, _ptr, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _i32, _ptr,
+            [_i32, _ptr, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _i64, _ptr, _i32, _ptr,
              _i64, _i64, _i64, _ptr, _size, _ptr],
             ctypes.c_int,
         ),
         "hst_quantize_e4m3": (
             [_i32, _i32, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _i64, _i64, _ptr],
-            ctypes.c_int,
-        ),
-        "hst_pack_rows": (
-            [_i32, _ptr, _i64, _i64, _i64, _ptr, _i64, _i64, _ptr, _i64, _i64, _i64, _i64, _ptr],
             ctypes.c_int,
         ),
         "hst_matmul_split_k_noalloc": (

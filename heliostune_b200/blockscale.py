@@ -20,15 +20,7 @@ from __future__ import annotations
 import torch
 
 from heliostune_b200 import _native
-from heliostune_b200.grouped import (
-    _DTYPES,
-    MAX_GROUPS,
-    _check_ends,
-    _padded_copy,
-    _readable_rows,
-    _stack_strides,
-    _workspace,
-)
+from heliostune_b200.grouped import _DTYPES, MAX_GROUPS, _check_ends, _workspace
 from heliostune_b200.kernel import _device_guard, _stream
 
 #: Values that share a scale along a row (and, for tiles, along a column).
@@ -145,22 +137,20 @@ def matmul_blockscaled(
     _check_scales("b_scales", b_scales, (*lead, _blocks(n), _blocks(k)), index)
     _refuse_gradient("matmul_blockscaled", a, a_scales, b, b_scales)
     y = torch.empty((rows, n), device=device, dtype=out_dtype)
-    a, a_pointer, a_row = _readable_rows(a, 16)
-    b_pointer = b.data_ptr()
-    strides = b.stride() if lead else (0, *b.stride())
-    found = _stack_strides(strides, (groups, n, k), 16) if b_pointer % 16 == 0 else None
-    if found is None:
-        b = _padded_copy(b, group_ends, rows)
-        b_pointer, found = b.data_ptr(), (b.stride(0), b.stride(-2))
-    sa_row, sa_block = a_scales.stride()
-    sb_group, sb_row, sb_block = b_scales.stride() if lead else (0, *b_scales.stride())
-    workspace, ws_pointer, ws_bytes = _workspace(_native.GROUPED_SCALED, rows, groups, n, k, device)
+    a_pointer, a_strides, b_pointer = a.data_ptr(), a.stride(), b.data_ptr()
+    b_strides = b.stride() if lead else (0, *b.stride())
+    sb_strides = b_scales.stride() if lead else (0, *b_scales.stride())
+    workspace, ws_pointer, ws_bytes = _workspace(
+        "hst_matmul_blockscaled",
+        device,
+        (a_pointer & 15, *a_strides, b_pointer & 15, *b_strides, groups, rows, n, k),
+    )
     with _device_guard(device):
         _native.check(
             _native.library().hst_matmul_blockscaled(
-                _DTYPES[out_dtype], a_pointer, a_row, a_scales.data_ptr(), sa_row, sa_block, b_pointer, *found,
-                b_scales.data_ptr(), sb_group, sb_row, sb_block, ends, groups, y.data_ptr(), rows, n, k,
-                ws_pointer, ws_bytes, _stream(device),
+                _DTYPES[out_dtype], a_pointer, *a_strides, a_scales.data_ptr(), *a_scales.stride(), b_pointer, *b_strides,
+                b_scales.data_ptr(), *sb_strides, ends, groups, y.data_ptr(), rows, n, k, ws_pointer, ws_bytes,
+                _stream(device),
             )
         )  # fmt: skip
     del workspace  # stream-ordered reuse by the caching allocator is safe on this stream

@@ -36,12 +36,68 @@ int check_extents(const char* what, int64_t a, int64_t b) {
   return HST_OK;
 }
 
-// A row-major operand TMA can read: 16-byte aligned base and strides, rows no shorter than `cols`.
-int check_operand(const char* what, const void* p, int64_t ld, int64_t cols, int64_t elem) {
-  if (p == nullptr) return fail(HST_ERR_INVALID, "%s is null", what);
-  if ((reinterpret_cast<uintptr_t>(p) & 15) != 0 || ld * elem % 16 != 0 || ld < cols)
-    return fail(HST_ERR_INVALID, "%s must be row-major with 16-byte aligned rows of at least %lld values", what,
-                (long long)cols);
+// A stack of matrices [groups, rows, cols] with strides in values.
+struct Stack {
+  const void* ptr;
+  int64_t elem;  // bytes of a value
+  int64_t groups, rows, cols;
+  int64_t s_group, s_row, s_col;
+
+  int64_t unit() const { return 16 / elem; }
+  int64_t packed_row() const { return round_up(cols, unit()); }
+  size_t packed_bytes() const { return static_cast<size_t>(round_up(groups * rows * packed_row() * elem, 256)); }
+  // Strides of dimensions of one entry do not matter; a tensor map wants some.
+  void settle() {
+    if (cols == 1) s_col = 1;
+    if (rows == 1) s_row = packed_row();
+    if (groups == 1) s_group = s_row * rows;
+  }
+  // Whether a tensor map can describe it: unit column stride, and the base, the rows (at least as long as
+  // the columns) and the groups aligned to 16 bytes, none overlapping the next.
+  bool readable() const {
+    return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0 && s_col == 1 && s_row % unit() == 0 && s_row >= cols &&
+           s_group % unit() == 0 && s_group >= s_row * rows;
+  }
+};
+
+Stack make_stack(const void* ptr, int64_t elem, int64_t groups, int64_t rows, int64_t cols, int64_t s_group, int64_t s_row,
+                 int64_t s_col) {
+  Stack s = {ptr, elem, groups, rows, cols, s_group, s_row, s_col};
+  s.settle();
+  return s;
+}
+
+size_t pack_bytes(const Stack& s) { return s.readable() ? 0 : s.packed_bytes(); }
+
+// Copies a stack that is not readable to `dst`, the weights of empty groups left out where `ends` tells
+// of them, and describes the copy.
+int pack(Stack* s, void* dst, const int32_t* ends, int64_t total_rows, cudaStream_t stream) {
+  const int64_t e = s->elem;
+  PackArgs a = {static_cast<const uint8_t*>(s->ptr), s->s_group * e, s->s_row * e, s->s_col * e, static_cast<uint8_t*>(dst),
+                s->rows * s->packed_row() * e, s->packed_row() * e, ends, static_cast<int>(total_rows), s->rows,
+                static_cast<int>(cdiv(s->cols * e, 16)), s->cols * e};
+  if (s->s_col == 1) {
+    const dim3 grid(static_cast<unsigned>(cdiv(s->rows * a.chunks, kPackThreads * kPackPerThread)), static_cast<unsigned>(s->groups));
+    // The common alignment of every row's start and of its length.
+    const uint64_t bits = reinterpret_cast<uintptr_t>(s->ptr) | static_cast<uint64_t>(a.row_bytes) |
+                          static_cast<uint64_t>(a.s_row) | static_cast<uint64_t>(a.s_group);
+    if (bits % 16 == 0) pack_rows_kernel<uint4><<<grid, kPackThreads, 0, stream>>>(a);
+    else if (bits % 8 == 0) pack_rows_kernel<uint2><<<grid, kPackThreads, 0, stream>>>(a);
+    else if (bits % 4 == 0) pack_rows_kernel<uint32_t><<<grid, kPackThreads, 0, stream>>>(a);
+    else if (bits % 2 == 0) pack_rows_kernel<uint16_t><<<grid, kPackThreads, 0, stream>>>(a);
+    else pack_rows_kernel<uint8_t><<<grid, kPackThreads, 0, stream>>>(a);
+  } else {
+    const int64_t tiles = cdiv(s->rows, 32) * cdiv(s->cols, 32);
+    if (tiles > INT32_MAX) return fail(HST_ERR_UNSUPPORTED, "an operand to be copied is too large");
+    const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(s->groups));
+    if (e == 2) pack_any_kernel<uint16_t><<<grid, kPackThreads, 0, stream>>>(a);
+    else pack_any_kernel<uint8_t><<<grid, kPackThreads, 0, stream>>>(a);
+  }
+  HST_CUDA(cudaGetLastError());
+  s->ptr = dst;
+  s->s_col = 1;
+  s->s_row = s->packed_row();
+  s->s_group = s->s_row * s->rows;
   return HST_OK;
 }
 
@@ -82,25 +138,21 @@ int plan_pairs(const GroupedProblem& p, int sms) {
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sms / 2, most)));
 }
 
+// Bytes of the pieces, at the start of the workspace; packed operands follow.
 template <GroupMode MODE>
-size_t workspace_bytes(const GroupedProblem& p, int sms) {
+size_t piece_bytes(const GroupedProblem& p, int sms) {
   if (whole_tiles<MODE>(p)) return 0;
   return static_cast<size_t>(plan_pairs<MODE>(p, sms)) * 4 * 128 * p.width_cap * sizeof(float);
 }
 
 int width_cap(int64_t rows, int most) { return static_cast<int>(std::min<int64_t>(most, round_up(std::max<int64_t>(rows, 1), 32))); }
 
-// The two launches of one product. `maps` and the operand fields of `args` are set by the caller.
+// The launches of one product. `maps` and the operand fields of `args` are set by the caller.
 template <GroupMode MODE, bool L_MN, typename T>
-int launch_grouped(const GroupedProblem& p, const GroupedMaps& maps, GroupedArgs args, int r_bytes, void* workspace,
-                   size_t workspace_size, cudaStream_t stream) {
+int launch_grouped(const GroupedProblem& p, const GroupedMaps& maps, GroupedArgs args, int r_bytes, const DeviceState* dev,
+                   void* workspace, cudaStream_t stream) {
   using S = GroupedShape<MODE>;
-  DeviceState* dev = nullptr;
-  HST_TRY(device_state(&dev));
   if (max_iterations<MODE>(p) > INT32_MAX) return fail(HST_ERR_UNSUPPORTED, "the grouped product has too many tiles");
-  const size_t need = workspace_bytes<MODE>(p, dev->sm_count);
-  if (need > 0 && (workspace_size < need || workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0))
-    return fail(HST_ERR_WORKSPACE, "workspace of %zu bytes, 16-byte aligned, needed; got %zu", need, workspace_size);
   args.groups = p.groups;
   args.rows = static_cast<int>(p.rows);
   args.cols = static_cast<int>(p.cols);
@@ -152,23 +204,53 @@ int launch_grouped(const GroupedProblem& p, const GroupedMaps& maps, GroupedArgs
   return HST_OK;
 }
 
-// A row matrix [rows, cols] of `elem`-byte values in boxes of 128 bytes x `box_rows`.
-int encode_rows(CUtensorMap* map, CUtensorMapDataType type, int64_t elem, const void* base, int64_t rows, int64_t cols,
-                int64_t ld, int box_rows) {
-  const uint64_t dims[2] = {static_cast<uint64_t>(cols), static_cast<uint64_t>(rows)};
-  const uint64_t strides[1] = {static_cast<uint64_t>(ld * elem)};
-  const uint32_t box[2] = {static_cast<uint32_t>(128 / elem), static_cast<uint32_t>(box_rows)};
-  return encode_tiled(map, type, 2, base, dims, strides, box);
+// A row matrix in boxes of 128 bytes x `box_rows`.
+int encode_rows(CUtensorMap* map, CUtensorMapDataType type, const Stack& s, int box_rows) {
+  const uint64_t dims[2] = {static_cast<uint64_t>(s.cols), static_cast<uint64_t>(s.rows)};
+  const uint64_t strides[1] = {static_cast<uint64_t>(s.s_row * s.elem)};
+  const uint32_t box[2] = {static_cast<uint32_t>(128 / s.elem), static_cast<uint32_t>(box_rows)};
+  return encode_tiled(map, type, 2, s.ptr, dims, strides, box);
 }
 
-// Weights [groups, outer, inner].
-int encode_weights(CUtensorMap* map, CUtensorMapDataType type, int64_t elem, const void* base, int64_t groups,
-                   int64_t outer, int64_t inner, int64_t stride, int64_t ld, int box_rows) {
-  const uint64_t dims[3] = {static_cast<uint64_t>(inner), static_cast<uint64_t>(outer), static_cast<uint64_t>(groups)};
-  if (groups == 1) stride = outer * ld;  // not used; the map wants one
-  const uint64_t strides[2] = {static_cast<uint64_t>(ld * elem), static_cast<uint64_t>(stride * elem)};
-  const uint32_t box[3] = {static_cast<uint32_t>(128 / elem), static_cast<uint32_t>(box_rows), 1};
-  return encode_tiled(map, type, 3, base, dims, strides, box);
+// A stack of weights, in boxes within one of them.
+int encode_weights(CUtensorMap* map, CUtensorMapDataType type, const Stack& s, int box_rows) {
+  const uint64_t dims[3] = {static_cast<uint64_t>(s.cols), static_cast<uint64_t>(s.rows), static_cast<uint64_t>(s.groups)};
+  const uint64_t strides[2] = {static_cast<uint64_t>(s.s_row * s.elem), static_cast<uint64_t>(s.s_group * s.elem)};
+  const uint32_t box[3] = {static_cast<uint32_t>(128 / s.elem), static_cast<uint32_t>(box_rows), 1};
+  return encode_tiled(map, type, 3, s.ptr, dims, strides, box);
+}
+
+// Checks the workspace for `pieces` bytes and two operands, and copies those that need it behind the
+// pieces.
+int place_operands(size_t pieces, Stack* first, const int32_t* first_ends, Stack* second, const int32_t* second_ends,
+                   int64_t total_rows, void* workspace, size_t workspace_size, cudaStream_t stream) {
+  pieces = static_cast<size_t>(round_up(static_cast<int64_t>(pieces), 256));
+  const size_t first_bytes = pack_bytes(*first), need = pieces + first_bytes + pack_bytes(*second);
+  if (need > 0 && (workspace_size < need || workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0))
+    return fail(HST_ERR_WORKSPACE, "workspace of %zu bytes, 16-byte aligned, needed; got %zu", need, workspace_size);
+  uint8_t* at = static_cast<uint8_t*>(workspace) + pieces;
+  if (!first->readable()) HST_TRY(pack(first, at, first_ends, total_rows, stream));
+  if (!second->readable()) HST_TRY(pack(second, at + first_bytes, second_ends, total_rows, stream));
+  return HST_OK;
+}
+
+// Weights W [groups, k, n] as stored: [k, n] or [n, k] matrices, whichever a tensor map can describe; of
+// neither, the one whose rows are contiguous.
+Stack stored_weights(const void* w, int64_t groups, int64_t k, int64_t n, int64_t w_group, int64_t w_k, int64_t w_n, bool* kn) {
+  const Stack by_k = make_stack(w, 2, groups, k, n, w_group, w_k, w_n);
+  const Stack by_n = make_stack(w, 2, groups, n, k, w_group, w_n, w_k);
+  *kn = by_k.readable() || (!by_n.readable() && (w_n == 1 || w_k != 1));
+  return *kn ? by_k : by_n;
+}
+
+int total_bytes(size_t pieces, const Stack& a, const Stack& b, size_t* bytes) {
+  *bytes = static_cast<size_t>(round_up(static_cast<int64_t>(pieces), 256)) + pack_bytes(a) + pack_bytes(b);
+  return HST_OK;
+}
+
+int device_sms(int device, int* sms) {
+  HST_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device));
+  return HST_OK;
 }
 
 CUtensorMapDataType map_type(int32_t dtype) {
@@ -194,6 +276,10 @@ GroupedProblem scaled_problem(int64_t rows, int groups, int64_t n, int64_t k) {
   return GroupedProblem{rows, groups, n, 0, cdiv(k, 128), scaled_few(rows, groups) ? width_cap(rows, 64) : 256};
 }
 
+size_t scaled_piece_bytes(const GroupedProblem& p, int sms) {
+  return scaled_few(p.rows, p.groups) ? piece_bytes<GroupMode::kScaledFew>(p, sms) : piece_bytes<GroupMode::kScaled>(p, sms);
+}
+
 }  // namespace
 }  // namespace hst
 
@@ -201,56 +287,49 @@ using namespace hst;
 
 extern "C" {
 
-int hst_grouped_workspace_size(int32_t op, int64_t rows, int32_t groups, int64_t n, int64_t k, int device,
-                               size_t* bytes) {
+int hst_grouped_matmul_workspace(const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t w_group, int64_t w_k,
+                                 int64_t w_n, int32_t groups, int64_t rows, int64_t n, int64_t k, int device,
+                                 size_t* bytes) {
   if (bytes == nullptr) return fail(HST_ERR_INVALID, "bytes is null");
-  if (groups < 1 || groups > kMaxGroups || rows < 0 || n < 0 || k < 0 || rows > kMaxExtent || n > kMaxExtent || k > kMaxExtent)
-    return fail(HST_ERR_INVALID, "bad grouped product");
+  *bytes = 0;
+  HST_TRY(check_groups("the grouped matmul", rows, groups, bytes));
+  HST_TRY(check_extents("the grouped matmul", n, k));
+  if (rows == 0 || n == 0 || k == 0) return HST_OK;
   int sms = 0;
-  HST_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
-  switch (op) {
-    case HST_GROUPED_FORWARD:
-      *bytes = workspace_bytes<GroupMode::kForward>(forward_problem(rows, groups, n, k), sms);
-      return HST_OK;
-    case HST_GROUPED_WEIGHT_GRAD:
-      *bytes = workspace_bytes<GroupMode::kWeightGrad>(grad_problem(rows, groups, k, n), sms);
-      return HST_OK;
-    case HST_GROUPED_SCALED:
-      *bytes = scaled_few(rows, groups) ? workspace_bytes<GroupMode::kScaledFew>(scaled_problem(rows, groups, n, k), sms)
-                                        : workspace_bytes<GroupMode::kScaled>(scaled_problem(rows, groups, n, k), sms);
-      return HST_OK;
-    default:
-      return fail(HST_ERR_INVALID, "unknown grouped product %d", op);
-  }
+  HST_TRY(device_sms(device, &sms));
+  bool kn = false;
+  return total_bytes(piece_bytes<GroupMode::kForward>(forward_problem(rows, groups, n, k), sms),
+                     make_stack(x, 2, 1, rows, k, 0, x_row, x_col), stored_weights(w, groups, k, n, w_group, w_k, w_n, &kn), bytes);
 }
 
-int hst_grouped_matmul(int32_t dtype, const void* x, int64_t ldx, const void* w, int64_t w_group, int64_t ldw,
-                       int32_t w_layout, const int32_t* ends, int32_t groups, void* y, int64_t rows, int64_t n,
+int hst_grouped_matmul(int32_t dtype, const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t w_group,
+                       int64_t w_k, int64_t w_n, const int32_t* ends, int32_t groups, void* y, int64_t rows, int64_t n,
                        int64_t k, void* workspace, size_t workspace_bytes, void* stream) {
   if (dtype != HST_F16 && dtype != HST_BF16) return fail(HST_ERR_INVALID, "unknown data type %d", dtype);
-  if (w_layout != HST_WEIGHT_KN && w_layout != HST_WEIGHT_NK) return fail(HST_ERR_INVALID, "unknown weight layout %d", w_layout);
   HST_TRY(check_groups("the grouped matmul", rows, groups, ends));
   HST_TRY(check_extents("the grouped matmul", n, k));
   if (rows == 0 || n == 0) return HST_OK;
   if (y == nullptr) return fail(HST_ERR_INVALID, "y is null");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (k == 0) return zero_output(y, rows * n, s);
-  const bool kn = w_layout == HST_WEIGHT_KN;
-  const int64_t outer = kn ? k : n, inner = kn ? n : k;
-  HST_TRY(check_operand("x", x, ldx, k, 2));
-  HST_TRY(check_operand("w", w, ldw, inner, 2));
-  if (groups > 1 && (w_group % 8 != 0 || w_group < 8)) return fail(HST_ERR_INVALID, "w's group stride must be a positive multiple of 8");
+  if (x == nullptr || w == nullptr) return fail(HST_ERR_INVALID, "x or w is null");
+  DeviceState* dev = nullptr;
+  HST_TRY(device_state(&dev));
   const GroupedProblem p = forward_problem(rows, groups, n, k);
+  bool kn = false;
+  Stack xs = make_stack(x, 2, 1, rows, k, 0, x_row, x_col);
+  Stack ws = stored_weights(w, groups, k, n, w_group, w_k, w_n, &kn);
+  HST_TRY(place_operands(piece_bytes<GroupMode::kForward>(p, dev->sm_count), &xs, nullptr, &ws, ends, rows, workspace,
+                         workspace_bytes, s));
   GroupedMaps maps = {};
-  HST_TRY(encode_weights(&maps.l[0], map_type(dtype), 2, w, groups, outer, inner, w_group, ldw, kn ? 64 : 128));
-  for (int i = 0; i < 4; ++i) HST_TRY(encode_rows(&maps.r[i], map_type(dtype), 2, x, rows, k, ldx, box_rows_of(i)));
+  HST_TRY(encode_weights(&maps.l[0], map_type(dtype), ws, kn ? 64 : 128));
+  for (int i = 0; i < 4; ++i) HST_TRY(encode_rows(&maps.r[i], map_type(dtype), xs, box_rows_of(i)));
   GroupedArgs args = {};
   args.ends = ends;
   args.out = y;
   const int r_bytes = box_rows_of(group_box(p.width_cap / 2)) * 128;
 #define HST_GROUPED_CASE(KN_, DT_, T_) \
-  if (kn == KN_ && dtype == DT_)       \
-    return launch_grouped<GroupMode::kForward, KN_, T_>(p, maps, args, r_bytes, workspace, workspace_bytes, s);
+  if (kn == KN_ && dtype == DT_) return launch_grouped<GroupMode::kForward, KN_, T_>(p, maps, args, r_bytes, dev, workspace, s);
   HST_GROUPED_CASE(true, HST_F16, __half)
   HST_GROUPED_CASE(false, HST_F16, __half)
   HST_GROUPED_CASE(true, HST_BF16, __nv_bfloat16)
@@ -259,8 +338,23 @@ int hst_grouped_matmul(int32_t dtype, const void* x, int64_t ldx, const void* w,
   return HST_ERR_UNSUPPORTED;
 }
 
-int hst_grouped_weight_grad(int32_t dtype, const void* left, int64_t ldl, const void* right, int64_t ldr,
-                            const int32_t* ends, int32_t groups, void* out, int64_t rows, int64_t lcols,
+int hst_grouped_weight_grad_workspace(const void* left, int64_t l_row, int64_t l_col, const void* right, int64_t r_row,
+                                      int64_t r_col, int32_t groups, int64_t rows, int64_t lcols, int64_t rcols, int device,
+                                      size_t* bytes) {
+  if (bytes == nullptr) return fail(HST_ERR_INVALID, "bytes is null");
+  *bytes = 0;
+  HST_TRY(check_groups("the grouped weight gradient", rows, groups, bytes));
+  HST_TRY(check_extents("the grouped weight gradient", lcols, rcols));
+  if (rows == 0 || lcols == 0 || rcols == 0) return HST_OK;
+  int sms = 0;
+  HST_TRY(device_sms(device, &sms));
+  return total_bytes(piece_bytes<GroupMode::kWeightGrad>(grad_problem(rows, groups, lcols, rcols), sms),
+                     make_stack(left, 2, 1, rows, lcols, 0, l_row, l_col), make_stack(right, 2, 1, rows, rcols, 0, r_row, r_col),
+                     bytes);
+}
+
+int hst_grouped_weight_grad(int32_t dtype, const void* left, int64_t l_row, int64_t l_col, const void* right, int64_t r_row,
+                            int64_t r_col, const int32_t* ends, int32_t groups, void* out, int64_t rows, int64_t lcols,
                             int64_t rcols, void* workspace, size_t workspace_bytes, void* stream) {
   if (dtype != HST_F16 && dtype != HST_BF16) return fail(HST_ERR_INVALID, "unknown data type %d", dtype);
   HST_TRY(check_groups("the grouped weight gradient", rows, groups, ends));
@@ -269,25 +363,42 @@ int hst_grouped_weight_grad(int32_t dtype, const void* left, int64_t ldl, const 
   if (out == nullptr) return fail(HST_ERR_INVALID, "out is null");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (rows == 0) return zero_output(out, lcols * rcols * groups, s);
-  HST_TRY(check_operand("left", left, ldl, lcols, 2));
-  HST_TRY(check_operand("right", right, ldr, rcols, 2));
+  if (left == nullptr || right == nullptr) return fail(HST_ERR_INVALID, "left or right is null");
+  DeviceState* dev = nullptr;
+  HST_TRY(device_state(&dev));
   const GroupedProblem p = grad_problem(rows, groups, lcols, rcols);
+  Stack ls = make_stack(left, 2, 1, rows, lcols, 0, l_row, l_col), rs = make_stack(right, 2, 1, rows, rcols, 0, r_row, r_col);
+  HST_TRY(place_operands(piece_bytes<GroupMode::kWeightGrad>(p, dev->sm_count), &ls, nullptr, &rs, nullptr, rows, workspace,
+                         workspace_bytes, s));
   GroupedMaps maps = {};
-  HST_TRY(encode_rows(&maps.l[0], map_type(dtype), 2, left, rows, lcols, ldl, 64));
-  HST_TRY(encode_rows(&maps.r[0], map_type(dtype), 2, right, rows, rcols, ldr, 64));
+  HST_TRY(encode_rows(&maps.l[0], map_type(dtype), ls, 64));
+  HST_TRY(encode_rows(&maps.r[0], map_type(dtype), rs, 64));
   GroupedArgs args = {};
   args.ends = ends;
   args.out = out;
-  if (dtype == HST_F16)
-    return launch_grouped<GroupMode::kWeightGrad, true, __half>(p, maps, args, 16384, workspace, workspace_bytes, s);
-  return launch_grouped<GroupMode::kWeightGrad, true, __nv_bfloat16>(p, maps, args, 16384, workspace, workspace_bytes, s);
+  if (dtype == HST_F16) return launch_grouped<GroupMode::kWeightGrad, true, __half>(p, maps, args, 16384, dev, workspace, s);
+  return launch_grouped<GroupMode::kWeightGrad, true, __nv_bfloat16>(p, maps, args, 16384, dev, workspace, s);
 }
 
-int hst_matmul_blockscaled(int32_t out_dtype, const void* a, int64_t lda, const float* a_scales, int64_t sa_row,
-                           int64_t sa_block, const void* b, int64_t b_group, int64_t ldb, const float* b_scales,
-                           int64_t sb_group, int64_t sb_row, int64_t sb_block, const int32_t* ends, int32_t groups,
-                           void* y, int64_t rows, int64_t n, int64_t k, void* workspace, size_t workspace_bytes,
-                           void* stream) {
+int hst_matmul_blockscaled_workspace(const void* a, int64_t a_row, int64_t a_col, const void* b, int64_t b_group,
+                                     int64_t b_row, int64_t b_col, int32_t groups, int64_t rows, int64_t n, int64_t k,
+                                     int device, size_t* bytes) {
+  if (bytes == nullptr) return fail(HST_ERR_INVALID, "bytes is null");
+  *bytes = 0;
+  HST_TRY(check_groups("the block-scaled matmul", rows, groups, bytes));
+  HST_TRY(check_extents("the block-scaled matmul", n, k));
+  if (rows == 0 || n == 0 || k == 0) return HST_OK;
+  int sms = 0;
+  HST_TRY(device_sms(device, &sms));
+  return total_bytes(scaled_piece_bytes(scaled_problem(rows, groups, n, k), sms), make_stack(a, 1, 1, rows, k, 0, a_row, a_col),
+                     make_stack(b, 1, groups, n, k, b_group, b_row, b_col), bytes);
+}
+
+int hst_matmul_blockscaled(int32_t out_dtype, const void* a, int64_t a_row, int64_t a_col, const float* a_scales,
+                           int64_t sa_row, int64_t sa_block, const void* b, int64_t b_group, int64_t b_row, int64_t b_col,
+                           const float* b_scales, int64_t sb_group, int64_t sb_row, int64_t sb_block, const int32_t* ends,
+                           int32_t groups, void* y, int64_t rows, int64_t n, int64_t k, void* workspace,
+                           size_t workspace_bytes, void* stream) {
   if (out_dtype != HST_F16 && out_dtype != HST_BF16) return fail(HST_ERR_INVALID, "unknown data type %d", out_dtype);
   HST_TRY(check_groups("the block-scaled matmul", rows, groups, ends));
   HST_TRY(check_extents("the block-scaled matmul", n, k));
@@ -295,16 +406,18 @@ int hst_matmul_blockscaled(int32_t out_dtype, const void* a, int64_t lda, const 
   if (y == nullptr) return fail(HST_ERR_INVALID, "y is null");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (k == 0) return zero_output(y, rows * n, s);
-  HST_TRY(check_operand("a", a, lda, k, 1));
-  HST_TRY(check_operand("b", b, ldb, k, 1));
+  if (a == nullptr || b == nullptr) return fail(HST_ERR_INVALID, "a or b is null");
   if (a_scales == nullptr || b_scales == nullptr) return fail(HST_ERR_INVALID, "scales are null");
-  if (groups > 1 && (b_group % 16 != 0 || b_group < 16)) return fail(HST_ERR_INVALID, "b's group stride must be a positive multiple of 16");
+  DeviceState* dev = nullptr;
+  HST_TRY(device_state(&dev));
   const GroupedProblem p = scaled_problem(rows, groups, n, k);
+  Stack as = make_stack(a, 1, 1, rows, k, 0, a_row, a_col), bs = make_stack(b, 1, groups, n, k, b_group, b_row, b_col);
+  HST_TRY(place_operands(scaled_piece_bytes(p, dev->sm_count), &as, nullptr, &bs, ends, rows, workspace, workspace_bytes, s));
   const CUtensorMapDataType type = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   GroupedMaps maps = {};
   const bool few = scaled_few(rows, groups);
-  for (int i = 0; i < 4; ++i) HST_TRY(encode_rows(few ? &maps.r[i] : &maps.l[i], type, 1, a, rows, k, lda, box_rows_of(i)));
-  HST_TRY(encode_weights(few ? &maps.l[0] : &maps.r[0], type, 1, b, groups, n, k, b_group, ldb, few ? 128 : 64));
+  for (int i = 0; i < 4; ++i) HST_TRY(encode_rows(few ? &maps.r[i] : &maps.l[i], type, as, box_rows_of(i)));
+  HST_TRY(encode_weights(few ? &maps.l[0] : &maps.r[0], type, bs, few ? 128 : 64));
   GroupedArgs args = {};
   args.ends = ends;
   args.out = y;
@@ -318,7 +431,7 @@ int hst_matmul_blockscaled(int32_t out_dtype, const void* a, int64_t lda, const 
   const int r_bytes = few ? box_rows_of(group_box(p.width_cap / 2)) * 128 : 16384;
 #define HST_SCALED_CASE(FEW_, MODE_, DT_, T_) \
   if (few == FEW_ && out_dtype == DT_)        \
-    return launch_grouped<GroupMode::MODE_, false, T_>(p, maps, args, r_bytes, workspace, workspace_bytes, s);
+    return launch_grouped<GroupMode::MODE_, false, T_>(p, maps, args, r_bytes, dev, workspace, s);
   HST_SCALED_CASE(true, kScaledFew, HST_F16, __half)
   HST_SCALED_CASE(true, kScaledFew, HST_BF16, __nv_bfloat16)
   HST_SCALED_CASE(false, kScaled, HST_F16, __half)
@@ -359,42 +472,6 @@ int hst_quantize_e4m3(int32_t dtype, int32_t tiles, const void* x, int64_t x_bat
     else if (vec) quantize_rows_kernel<__nv_bfloat16><<<vec_grid, kQuantThreads, 0, st>>>(a);
     else if (dtype == HST_F16) quantize_rows_any_kernel<__half><<<any_grid, kQuantThreads, 0, st>>>(a);
     else quantize_rows_any_kernel<__nv_bfloat16><<<any_grid, kQuantThreads, 0, st>>>(a);
-  }
-  HST_CUDA(cudaGetLastError());
-  return HST_OK;
-}
-
-int hst_pack_rows(int32_t value_bytes, const void* src, int64_t s_group, int64_t s_row, int64_t s_col, void* dst,
-                  int64_t d_group, int64_t d_row, const int32_t* ends, int64_t total_rows, int64_t groups, int64_t rows,
-                  int64_t cols, void* stream) {
-  if (value_bytes != 1 && value_bytes != 2) return fail(HST_ERR_INVALID, "values of %d bytes", value_bytes);
-  HST_TRY(check_extents("the packed copy", rows, cols));
-  if (groups < 0 || groups > kMaxGroups || total_rows < 0 || total_rows > kMaxExtent)
-    return fail(HST_ERR_INVALID, "the packed copy serves at most %d matrices", kMaxGroups);
-  if (groups == 0 || rows == 0 || cols == 0) return HST_OK;
-  if (src == nullptr || dst == nullptr) return fail(HST_ERR_INVALID, "null pointer");
-  const int64_t e = value_bytes;
-  if ((reinterpret_cast<uintptr_t>(dst) & 15) != 0 || d_row * e % 16 != 0 || d_row < cols || d_group * e % 16 != 0)
-    return fail(HST_ERR_INVALID, "the packed copy's rows must be 16-byte aligned and hold all columns");
-  PackArgs a = {static_cast<const uint8_t*>(src), s_group * e, s_row * e, s_col * e, static_cast<uint8_t*>(dst), d_group * e,
-                d_row * e, ends, static_cast<int>(total_rows), rows, static_cast<int>(cdiv(cols * e, 16)), cols * e};
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (s_col == 1 || cols == 1) {
-    const dim3 grid(static_cast<unsigned>(cdiv(rows * a.chunks, kPackThreads * kPackPerThread)), static_cast<unsigned>(groups));
-    // The common alignment of every row's start and of its length.
-    const uint64_t bits = reinterpret_cast<uintptr_t>(src) | static_cast<uint64_t>(a.row_bytes) |
-                          (rows > 1 ? static_cast<uint64_t>(a.s_row) : 0) | (groups > 1 ? static_cast<uint64_t>(a.s_group) : 0);
-    if (bits % 16 == 0) pack_rows_kernel<uint4><<<grid, kPackThreads, 0, st>>>(a);
-    else if (bits % 8 == 0) pack_rows_kernel<uint2><<<grid, kPackThreads, 0, st>>>(a);
-    else if (bits % 4 == 0) pack_rows_kernel<uint32_t><<<grid, kPackThreads, 0, st>>>(a);
-    else if (bits % 2 == 0) pack_rows_kernel<uint16_t><<<grid, kPackThreads, 0, st>>>(a);
-    else pack_rows_kernel<uint8_t><<<grid, kPackThreads, 0, st>>>(a);
-  } else {
-    const int64_t tiles = cdiv(rows, 32) * cdiv(cols, 32);
-    if (tiles > INT32_MAX) return fail(HST_ERR_UNSUPPORTED, "the packed copy is too large");
-    const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(groups));
-    if (value_bytes == 2) pack_any_kernel<uint16_t><<<grid, kPackThreads, 0, st>>>(a);
-    else pack_any_kernel<uint8_t><<<grid, kPackThreads, 0, st>>>(a);
   }
   HST_CUDA(cudaGetLastError());
   return HST_OK;

@@ -37,85 +37,24 @@ _DTYPES = {torch.float16: _native.HST_F16, torch.bfloat16: _native.HST_BF16}
 
 
 @functools.lru_cache(maxsize=4096)
-def _workspace_bytes(op: int, rows: int, groups: int, n: int, k: int, device: int) -> int:
+def _workspace_bytes(product: str, device: int, operands: tuple[int, ...]) -> int:
+    """Bytes of workspace, by everything the native planner reads: alignments, strides, extents, device."""
     size = ctypes.c_size_t(0)
-    _native.check(_native.library().hst_grouped_workspace_size(op, rows, groups, n, k, device, ctypes.byref(size)))
+    _native.check(getattr(_native.library(), f"{product}_workspace")(*operands, device, ctypes.byref(size)))
     return size.value
 
 
 def _workspace(
-    op: int, rows: int, groups: int, n: int, k: int, device: torch.device
+    product: str, device: torch.device, operands: tuple[int, ...]
 ) -> tuple[torch.Tensor | None, int | None, int]:
-    """The FP32 pieces of tiles shared between CTA pairs: a tensor of this call alone (None for products
-    without any), its address and its bytes."""
+    """The workspace of one call -- FP32 pieces of tiles shared between CTA pairs, copies of operands a tensor
+    map cannot describe -- as a tensor (None if there is none), its address and its bytes."""
     index = device.index if device.index is not None else torch.cuda.current_device()
-    nbytes = _workspace_bytes(op, rows, groups, n, k, index)
+    nbytes = _workspace_bytes(product, index, operands)
     if nbytes == 0:
         return None, None, 0
     buffer = torch.empty(nbytes, device=device, dtype=torch.uint8)
     return buffer, buffer.data_ptr(), nbytes
-
-
-def _padded_copy(t: torch.Tensor, group_ends: torch.Tensor | None = None, total_rows: int = 0) -> torch.Tensor:
-    """``t`` (one matrix or a stack) with rows of a multiple of 16 bytes, one after the other. With the
-    ends of a product over ``total_rows`` rows, the matrices of groups without rows are left out."""
-    unit = 16 // t.element_size()
-    *lead, rows, columns = t.shape
-    copy = torch.empty((*lead, rows, -(-columns // unit) * unit), device=t.device, dtype=t.dtype)[..., :columns]
-    groups, s_group, d_group = (lead[0], t.stride(0), copy.stride(0)) if lead else (1, 0, 0)
-    with _device_guard(t.device):
-        _native.check(
-            _native.library().hst_pack_rows(
-                t.element_size(), t.data_ptr(), s_group, t.stride(-2), t.stride(-1), copy.data_ptr(), d_group,
-                copy.stride(-2), None if group_ends is None else group_ends.data_ptr(), total_rows, groups, rows,
-                columns, _stream(t.device),
-            )
-        )  # fmt: skip
-    return copy
-
-
-def _readable_rows(t: torch.Tensor, unit: int) -> tuple[torch.Tensor, int, int]:
-    """A row matrix a tensor map can describe -- unit column stride, rows and base aligned to 16 bytes
-    (``unit`` values) -- with its address and row stride: ``t`` itself, or a copy."""
-    pointer, (row, column), (rows, columns) = t.data_ptr(), t.stride(), t.shape
-    if rows == 1:
-        row = -(-columns // unit) * unit
-    if (column == 1 or columns == 1) and row % unit == 0 and row >= columns and pointer % 16 == 0:
-        return t, pointer, row
-    copy = _padded_copy(t)
-    return copy, copy.data_ptr(), copy.stride(0)
-
-
-def _stack_strides(strides: tuple[int, int, int], shape: tuple[int, int, int], unit: int) -> tuple[int, int] | None:
-    """Group and row stride of a stack of row matrices a tensor map can describe, None if it cannot."""
-    (group, row, column), (groups, rows, columns) = strides, shape
-    if rows == 1:
-        row = -(-columns // unit) * unit
-    if groups == 1:
-        group = row * rows
-    if (column == 1 or columns == 1) and row % unit == 0 and row >= columns and group % unit == 0 and group >= row * rows:
-        return group, row
-    return None
-
-
-def _readable_weights(
-    weight: torch.Tensor, group_ends: torch.Tensor, total_rows: int
-) -> tuple[torch.Tensor, int, int, int, int]:
-    """``weight [E, K, N]`` with its address, group and row stride and layout: itself in either layout, or
-    a copy of the weights that have rows."""
-    pointer, (group, inner, outer), (groups, k, n) = weight.data_ptr(), weight.stride(), weight.shape
-    if pointer % 16 == 0:
-        found = _stack_strides((group, inner, outer), (groups, k, n), 8)
-        if found is not None:
-            return weight, pointer, *found, _native.HST_WEIGHT_KN
-        found = _stack_strides((group, outer, inner), (groups, n, k), 8)
-        if found is not None:
-            return weight, pointer, *found, _native.HST_WEIGHT_NK
-    if inner == 1 and outer != 1:
-        copy = _padded_copy(weight.transpose(1, 2), group_ends, total_rows)
-        return copy, copy.data_ptr(), copy.stride(0), copy.stride(1), _native.HST_WEIGHT_NK
-    copy = _padded_copy(weight, group_ends, total_rows)
-    return copy, copy.data_ptr(), copy.stride(0), copy.stride(1), _native.HST_WEIGHT_KN
 
 
 def _check_ends(group_ends: torch.Tensor, groups: int, device: int) -> None:
@@ -140,13 +79,14 @@ def _forward(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tensor) ->
     groups, k, n = weight.shape
     rows, device = x.shape[0], x.device
     y = torch.empty((rows, n), device=device, dtype=x.dtype)
-    x, x_pointer, x_row = _readable_rows(x, 8)
-    weight, w_pointer, w_group, w_row, layout = _readable_weights(weight, group_ends, rows)
-    workspace, ws_pointer, ws_bytes = _workspace(_native.GROUPED_FORWARD, rows, groups, n, k, device)
+    x_pointer, x_strides, w_pointer, w_strides = x.data_ptr(), x.stride(), weight.data_ptr(), weight.stride()
+    workspace, ws_pointer, ws_bytes = _workspace(
+        "hst_grouped_matmul", device, (x_pointer & 15, *x_strides, w_pointer & 15, *w_strides, groups, rows, n, k)
+    )
     with _device_guard(device):
         _native.check(
             _native.library().hst_grouped_matmul(
-                _DTYPES[x.dtype], x_pointer, x_row, w_pointer, w_group, w_row, layout, group_ends.data_ptr(), groups,
+                _DTYPES[x.dtype], x_pointer, *x_strides, w_pointer, *w_strides, group_ends.data_ptr(), groups,
                 y.data_ptr(), rows, n, k, ws_pointer, ws_bytes, _stream(device),
             )
         )  # fmt: skip
@@ -158,14 +98,17 @@ def _weight_grad(left: torch.Tensor, right: torch.Tensor, group_ends: torch.Tens
     groups = group_ends.shape[0]
     (rows, lcols), rcols, device = left.shape, right.shape[1], left.device
     out = torch.empty((groups, lcols, rcols), device=device, dtype=left.dtype)
-    left, l_pointer, l_row = _readable_rows(left, 8)
-    right, r_pointer, r_row = _readable_rows(right, 8)
-    workspace, ws_pointer, ws_bytes = _workspace(_native.GROUPED_WEIGHT_GRAD, rows, groups, rcols, lcols, device)
+    l_pointer, l_strides, r_pointer, r_strides = left.data_ptr(), left.stride(), right.data_ptr(), right.stride()
+    workspace, ws_pointer, ws_bytes = _workspace(
+        "hst_grouped_weight_grad",
+        device,
+        (l_pointer & 15, *l_strides, r_pointer & 15, *r_strides, groups, rows, lcols, rcols),
+    )
     with _device_guard(device):
         _native.check(
             _native.library().hst_grouped_weight_grad(
-                _DTYPES[left.dtype], l_pointer, l_row, r_pointer, r_row, group_ends.data_ptr(), groups, out.data_ptr(),
-                rows, lcols, rcols, ws_pointer, ws_bytes, _stream(device),
+                _DTYPES[left.dtype], l_pointer, *l_strides, r_pointer, *r_strides, group_ends.data_ptr(), groups,
+                out.data_ptr(), rows, lcols, rcols, ws_pointer, ws_bytes, _stream(device),
             )
         )  # fmt: skip
     del workspace

@@ -182,60 +182,53 @@ int hst_gated_mlp_stream(int32_t block_m, int32_t block_k, int32_t num_stages, i
 #define HST_F16 0
 #define HST_BF16 1
 
-/* Layout of one group's weight: [k, n] or [n, k], its last dimension contiguous. */
-#define HST_WEIGHT_KN 0
-#define HST_WEIGHT_NK 1
-
 /* Products over rows grouped by expert (no reference counterpart). Group g owns rows
  * [ends[g - 1], ends[g]) (ends[-1] = 0) of a row matrix; `ends` is int32 on the GPU and read there,
  * so nothing is known of the sizes on the host. Each end is taken clamped to [previous end, rows]:
  * no value leads out of the matrices. 1 to 1024 groups; a null `ends` with one group is all rows.
- * Operands: 16-byte aligned bases and strides. Outputs are contiguous and written whole: rows past
- * the last group, and the weight gradients of groups without rows, are zero. FP32 accumulation, one
- * rounding, bitwise reproducible. The caller gives a 16-byte aligned workspace of
- * hst_grouped_workspace_size bytes (0 for shallow products, no initialisation needed); calls that share
- * one must not overlap on the GPU. Each product is one or two launches on the stream and can be
- * captured. */
-#define HST_GROUPED_FORWARD 0      /* hst_grouped_matmul: n, k */
-#define HST_GROUPED_WEIGHT_GRAD 1  /* hst_grouped_weight_grad: n = rcols, k = lcols */
-#define HST_GROUPED_SCALED 2       /* hst_matmul_blockscaled: n, k */
-int hst_grouped_workspace_size(int32_t op, int64_t rows, int32_t groups, int64_t n, int64_t k,
-                               int device, size_t* bytes);
+ * Operands have any strides (in values); those a TMA tensor map cannot describe -- another column
+ * stride than 1, or a base, rows or groups not aligned to 16 bytes -- are copied into the workspace
+ * first, a stack of weights without those of groups that have no rows. Outputs are contiguous and
+ * written whole: rows past the last group, and the weight gradients of groups without rows, are zero.
+ * FP32 accumulation, one rounding, bitwise reproducible. The caller gives a 16-byte aligned workspace
+ * of the bytes that the function's _workspace form reports for the same operands (inspected for
+ * alignment only; 0 for shallow products of aligned operands; no initialisation needed). Calls that
+ * share one must not overlap on the GPU. The launches, all on the stream, can be captured. */
 
-/* y[t, :] = x[t, :] W[g(t)]: x [rows, k] (row stride ldx), w [groups, k, n] or [groups, n, k]
- * (w_layout; group stride w_group, row stride ldw), y [rows, n], all of `dtype`. The input
- * gradient is the same call with dy for x and the other layout. */
-int hst_grouped_matmul(int32_t dtype, const void* x, int64_t ldx, const void* w, int64_t w_group,
-                       int64_t ldw, int32_t w_layout, const int32_t* ends, int32_t groups, void* y,
-                       int64_t rows, int64_t n, int64_t k, void* workspace, size_t workspace_bytes,
-                       void* stream);
+/* y[t, :] = x[t, :] W[g(t)]: x [rows, k], w [groups, k, n] (w_k and w_n the strides of its inner
+ * dimensions: [groups, n, k] storage is read in place too), y [rows, n], all of `dtype`. The input
+ * gradient is the same call with dy for x and the weights' inner dimensions exchanged. */
+int hst_grouped_matmul_workspace(const void* x, int64_t x_row, int64_t x_col, const void* w,
+                                 int64_t w_group, int64_t w_k, int64_t w_n, int32_t groups,
+                                 int64_t rows, int64_t n, int64_t k, int device, size_t* bytes);
+int hst_grouped_matmul(int32_t dtype, const void* x, int64_t x_row, int64_t x_col, const void* w,
+                       int64_t w_group, int64_t w_k, int64_t w_n, const int32_t* ends, int32_t groups,
+                       void* y, int64_t rows, int64_t n, int64_t k, void* workspace,
+                       size_t workspace_bytes, void* stream);
 
 /* out[g] = left[rows of g]^T right[rows of g]: left [rows, lcols], right [rows, rcols], out
  * [groups, lcols, rcols], all of `dtype`. The weight gradient of hst_grouped_matmul. */
-int hst_grouped_weight_grad(int32_t dtype, const void* left, int64_t ldl, const void* right,
-                            int64_t ldr, const int32_t* ends, int32_t groups, void* out, int64_t rows,
-                            int64_t lcols, int64_t rcols, void* workspace, size_t workspace_bytes,
-                            void* stream);
+int hst_grouped_weight_grad_workspace(const void* left, int64_t l_row, int64_t l_col, const void* right,
+                                      int64_t r_row, int64_t r_col, int32_t groups, int64_t rows,
+                                      int64_t lcols, int64_t rcols, int device, size_t* bytes);
+int hst_grouped_weight_grad(int32_t dtype, const void* left, int64_t l_row, int64_t l_col,
+                            const void* right, int64_t r_row, int64_t r_col, const int32_t* ends,
+                            int32_t groups, void* out, int64_t rows, int64_t lcols, int64_t rcols,
+                            void* workspace, size_t workspace_bytes, void* stream);
 
 /* y[t, j] = sum over blocks c of 128 values of k: a_scales[t, c] * b_scales[g, j / 128, c] *
  * sum over the block of a[t, i] * b[g, j, i]. a [rows, k] and b [groups, n, k] E4M3, FP32 scales
- * with the strides given (elements), y [rows, n] of out_dtype. The block sums and their scaled sum
+ * with the strides given (in values), y [rows, n] of out_dtype. The block sums and their scaled sum
  * are FP32. For a plain product pass one group and a null `ends`. */
-int hst_matmul_blockscaled(int32_t out_dtype, const void* a, int64_t lda, const float* a_scales,
-                           int64_t sa_row, int64_t sa_block, const void* b, int64_t b_group,
-                           int64_t ldb, const float* b_scales, int64_t sb_group, int64_t sb_row,
-                           int64_t sb_block, const int32_t* ends, int32_t groups, void* y,
-                           int64_t rows, int64_t n, int64_t k, void* workspace,
+int hst_matmul_blockscaled_workspace(const void* a, int64_t a_row, int64_t a_col, const void* b,
+                                     int64_t b_group, int64_t b_row, int64_t b_col, int32_t groups,
+                                     int64_t rows, int64_t n, int64_t k, int device, size_t* bytes);
+int hst_matmul_blockscaled(int32_t out_dtype, const void* a, int64_t a_row, int64_t a_col,
+                           const float* a_scales, int64_t sa_row, int64_t sa_block, const void* b,
+                           int64_t b_group, int64_t b_row, int64_t b_col, const float* b_scales,
+                           int64_t sb_group, int64_t sb_row, int64_t sb_block, const int32_t* ends,
+                           int32_t groups, void* y, int64_t rows, int64_t n, int64_t k, void* workspace,
                            size_t workspace_bytes, void* stream);
-
-/* Copies row matrices into rows of a multiple of 16 bytes, for operands the products above cannot
- * read in place: src [groups, rows, cols] of 1- or 2-byte values with any strides, dst with unit column
- * stride, 16-byte aligned base, rows and groups (strides in values). With `ends` (those of the
- * product, over total_rows rows) the matrices of groups without rows are not copied; the product does
- * not read them. Null `ends`: all are. */
-int hst_pack_rows(int32_t value_bytes, const void* src, int64_t s_group, int64_t s_row, int64_t s_col,
-                  void* dst, int64_t d_group, int64_t d_row, const int32_t* ends, int64_t total_rows,
-                  int64_t groups, int64_t rows, int64_t cols, void* stream);
 
 /* E4M3 with FP32 scales: for every block amax = max(max |x|, 2^-100), scale = amax / 448 and
  * q = e4m3(x * (448 / amax)), the quotients and the product rounded to FP32, q to nearest even.

@@ -9,6 +9,8 @@ subnormal step, 2^-25.
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
@@ -99,31 +101,27 @@ def test_the_library_refuses_bad_calls_before_any_cuda_work() -> None:
     _native.build_library()
     lib = _native.library()
 
-    def matmul(dtype=0, layout=0, groups=2, rows=4, n=8, k=16, x=16, ldx=16, w=16, stride=128, ldw=8, ends=16, y=16):  # type: ignore[no-untyped-def]
-        return lib.hst_grouped_matmul(dtype, x, ldx, w, stride, ldw, layout, ends, groups, y, rows, n, k, None, 0, None)
+    def matmul(dtype=0, groups=2, rows=4, n=8, k=16, x=16, w=16, ends=16, y=16):  # type: ignore[no-untyped-def]
+        return lib.hst_grouped_matmul(dtype, x, k, 1, w, k * n, n, 1, ends, groups, y, rows, n, k, None, 0, None)
 
     for kwargs, message in (
         ({"dtype": 7}, b"data type"),
-        ({"layout": 2}, b"layout"),
         ({"groups": 0}, b"1 to 1024"),
         ({"groups": 1025}, b"1 to 1024"),
         ({"ends": None}, b"ends are null"),
         ({"rows": -1}, b"row count"),
         ({"n": -1}, b"extents"),
+        ({"k": 2**31}, b"extents"),
         ({"y": None}, b"y is null"),
-        ({"x": 8}, b"x must be"),
-        ({"ldx": 12}, b"x must be"),
-        ({"ldx": 8}, b"x must be"),
-        ({"w": None}, b"w is null"),
-        ({"ldw": 4}, b"w must be"),
-        ({"stride": 0}, b"group stride"),
-        ({"stride": 12}, b"group stride"),
+        ({"x": None}, b"x or w is null"),
+        ({"w": None}, b"x or w is null"),
     ):
         assert matmul(**kwargs) == _native.HST_ERR_INVALID, kwargs
         assert message in lib.hst_last_error(), kwargs
     assert matmul(rows=0) == _native.HST_OK
-    assert lib.hst_grouped_weight_grad(0, 16, 12, 16, 8, 16, 2, 16, 4, 16, 8, None, 0, None) == _native.HST_ERR_INVALID
-    assert b"left must be" in lib.hst_last_error()
+    assert lib.hst_grouped_weight_grad(0, None, 8, 1, 16, 8, 1, 16, 2, 16, 4, 8, 8, None, 0, None) == _native.HST_ERR_INVALID
+    assert b"left or right is null" in lib.hst_last_error()
+    assert lib.hst_grouped_weight_grad(3, 16, 8, 1, 16, 8, 1, 16, 2, 16, 4, 8, 8, None, 0, None) == _native.HST_ERR_INVALID
 
 
 # ------------------------------------------------------------------------------------------
@@ -407,16 +405,21 @@ def test_the_workspace_is_checked_and_its_contents_do_not_matter() -> None:
     x, w, dy = _operands(120, 2, 2056, 264, torch.float16, "kn", seed=17)
     ends = _ends([50, 120])
     lib = _native.library()
-    assert grouped._workspace_bytes(_native.GROUPED_FORWARD, 120, 2, 264, 520, 0) == 0
-    size = grouped._workspace_bytes(_native.GROUPED_FORWARD, 120, 2, 264, 2056, 0)
     y = torch.empty((120, 264), device="cuda", dtype=torch.float16)
+
+    def needed(k: int) -> int:
+        size = ctypes.c_size_t(1)
+        assert lib.hst_grouped_matmul_workspace(16, 2056, 1, 16, 2056 * 264, 264, 1, 2, 120, 264, k, 0, ctypes.byref(size)) == 0
+        return size.value
 
     def call(workspace: torch.Tensor) -> int:
         return lib.hst_grouped_matmul(
-            0, x.data_ptr(), 2056, w.data_ptr(), 2056 * 264, 264, 0, ends.data_ptr(), 2, y.data_ptr(), 120, 264, 2056,
+            0, x.data_ptr(), 2056, 1, w.data_ptr(), 2056 * 264, 264, 1, ends.data_ptr(), 2, y.data_ptr(), 120, 264, 2056,
             workspace.data_ptr(), workspace.numel(), torch.cuda.current_stream().cuda_stream,
         )  # fmt: skip
 
+    assert needed(520) == 0
+    size = needed(2056)
     assert call(torch.empty(size - 1, device="cuda", dtype=torch.uint8)) == _native.HST_ERR_WORKSPACE
     for fill in (0, 255):
         assert call(torch.full((size,), fill, device="cuda", dtype=torch.uint8)) == _native.HST_OK
