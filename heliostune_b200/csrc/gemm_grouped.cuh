@@ -61,9 +61,10 @@ constexpr int kGroupRaster = 8;      // row tiles before the next column tile
 
 // Warps: 0 loads, 1 issues the UMMAs (kScaled: and 2, one a half); then the epilogue, and for
 // kWeightGrad the masking warp. kScaled holds 128 x 256 FP32 sums in the registers of 8 epilogue
-// warps, which therefore form warpgroups of their own (3 idle).
+// warps, which therefore form warpgroups of their own (3 idle); kWeightGrad has 8 because a group of few
+// rows is little but epilogue (32 groups of 64 rows, 2048 x 2816: 102 us against 108 with four).
 __host__ __device__ constexpr int group_first_epilogue_warp(GroupMode m) { return m == GroupMode::kScaled ? 4 : 2; }
-__host__ __device__ constexpr int group_epilogue_warps(GroupMode m) { return m == GroupMode::kScaled ? 8 : 4; }
+__host__ __device__ constexpr int group_epilogue_warps(GroupMode m) { return m == GroupMode::kScaled || m == GroupMode::kWeightGrad ? 8 : 4; }
 __host__ __device__ constexpr int group_threads(GroupMode m) {
   return 32 * (group_first_epilogue_warp(m) + group_epilogue_warps(m) + (m == GroupMode::kWeightGrad ? 1 : 0));
 }
@@ -487,8 +488,9 @@ __device__ __forceinline__ void umma_commit_elected(uint32_t bar) {
       : "memory");
 }
 
-// Lets the finish kernel launch as soon as every CTA of this grid runs; it waits for the grid's
-// memory itself.
+// Lets the finish kernel launch as soon as every CTA of this grid runs; it waits for the grid's memory
+// itself. (This kernel is no dependent of what precedes it: that gained 2% and would have the finish
+// kernel read `ends` before they are written.)
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
@@ -707,7 +709,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
     }
     for (int b = 0; b < kBufs * kIssuers; ++b) {
       mbar_init(&tmem_full[b], 1);
-      mbar_init(&tmem_empty[b], 8);  // four epilogue warps of each CTA (leader's copy)
+      mbar_init(&tmem_empty[b], 2 * kEpilogueWarps / kIssuers);  // its epilogue warps in both CTAs (leader's copy)
     }
     mbar_init(mma_done, kIssuers);
     *abort_flag = 0;
@@ -908,7 +910,9 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
     const int row = quarter * 32 + static_cast<int>(lane);  // TMEM lane
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
     T* out = static_cast<T*>(args.out);
-    const int side = kWide ? (warp - kFirstEpilogue) / 4 : 0;  // the half of the tile's columns
+    // The half of the tile's columns; kWeightGrad's halves share the buffers.
+    const int half = kEpilogueWarps == 8 ? (warp - kFirstEpilogue) / 4 : 0;
+    const int side = kWide ? half : 0;
     int buf = 0;
     uint32_t buf_phase = 0;
     auto wait_buf = [&]() {
@@ -939,9 +943,10 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
         const uint32_t taddr = lane_base + static_cast<uint32_t>(buf * kBufCols);
         const int l32 = s.l0 + static_cast<int>(rank) * 128 + quarter * 32;  // the warp's first L row
         const bool whole = s.kb0 == 0 && s.kb1 == s.blocks;
+        const int c_begin = kGrad ? half * (s.width / 2) : 0, c_end = kGrad ? c_begin + s.width / 2 : s.width;
         if (!whole) {
 #pragma unroll 1
-          for (int c = 0; c < s.width; c += 32) {
+          for (int c = c_begin; c < c_end; c += 32) {
             uint32_t v[32];
             tmem_ld_32x32b_x32(taddr + c, v);
             tmem_ld_wait();
@@ -954,7 +959,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
         } else if constexpr (kGrad) {
           const uint32_t stage_out = smem_addr(out_stage) + static_cast<uint32_t>(warp - kFirstEpilogue) * kStageOutBytes;
 #pragma unroll 1
-          for (int c = 0; c < s.width; c += 64) {
+          for (int c = c_begin; c < c_end; c += 64) {
             uint32_t v[2][32];
             tmem_ld_32x32b_x32(taddr + c, v[0]);
             tmem_ld_32x32b_x32(taddr + c + 32, v[1]);
