@@ -243,31 +243,31 @@ __device__ inline void build_group_columns(const GroupedArgs& a, const GroupTabl
   for (int c = static_cast<int>(threadIdx.x); c <= shares; c += static_cast<int>(blockDim.x)) {
     const int first = GroupTable::column_first(c, tiles, shares);
     t.col_tile(c) = first;
-    if (MODE != GroupMode::kWeightGrad) t.col_base(c) = first * a.k_blocks;
+    t.col_base(c) = MODE == GroupMode::kWeightGrad ? 0 : first * a.k_blocks;
   }
   if constexpr (MODE == GroupMode::kWeightGrad) {
+    // K blocks differ by group: the threads share out (column, group), then one warp scans the sums.
     __syncthreads();
-    // K blocks differ by group: one warp sums a column, its lanes over the groups; then a scan.
-    const int lane = static_cast<int>(lane_id());
-    const int whole = t.per_column() * shares;  // tiles of the full rows
-    for (int c = static_cast<int>(threadIdx.x >> 5); c < shares; c += static_cast<int>(blockDim.x >> 5)) {
+    const int high = t.per_column(), whole = high * shares;  // tiles of the full rows
+    const int slices = max(1, static_cast<int>(blockDim.x) / shares);
+    for (int i = static_cast<int>(threadIdx.x); i < slices * shares; i += static_cast<int>(blockDim.x)) {
+      const int c = i % shares, slice = i / shares;
       int sum = 0;
-      for (int e = lane; e < a.groups; e += 32) {
-        const int lo = min(t.tile_base(e), whole), hi = min(t.tile_base(e + 1), whole);
+      for (int e = slice; e < a.groups; e += slices) {
+        const int lo = t.tile_base(e), hi = t.tile_base(e + 1);
         if (hi <= lo) continue;
-        // Tiles of column c below x: those with number * shares + c < x.
-        const int count = (hi - c + shares - 1) / shares - (lo - c + shares - 1) / shares;
+        // Tiles of column c below x (x <= whole): those with number * shares + c < x.
+        int count = (min(hi, whole) - c + shares - 1) / shares - (min(lo, whole) - c + shares - 1) / shares;
+        // The column's tile of the part-filled row, if it has one.
+        const int last = whole + t.col_tile(c) - c * high;
+        if (t.col_tile(c + 1) - t.col_tile(c) > high && lo <= last && last < hi) ++count;
         sum += count * group_blocks<MODE>(a, t.start(e + 1) - t.start(e));
       }
-      sum = __reduce_add_sync(0xffffffffu, sum);
-      if (t.col_tile(c + 1) - t.col_tile(c) > t.per_column()) {
-        const int e = t.group_of(t.tile_of(c, t.per_column()));
-        sum += group_blocks<MODE>(a, t.start(e + 1) - t.start(e));
-      }
-      if (lane == 0) t.col_base(c) = sum;
+      if (sum > 0) atomicAdd(&t.col_base(c), sum);
     }
     __syncthreads();
     if (threadIdx.x >= 32) return;
+    const int lane = static_cast<int>(lane_id());
     int before = 0;
     for (int c0 = 0; c0 <= shares; c0 += 32) {
       const int c = c0 + lane;
