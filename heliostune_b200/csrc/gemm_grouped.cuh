@@ -13,9 +13,9 @@
 // the R operand's `width` columns. Each weight is read once for up to 256 rows, so few rows a group
 // are bound by HBM, many by the tensor cores.
 //   * kForward puts the weights on the L side (M = 256 output columns) and the rows on the R side,
-//     whose width is a run-time field of the UMMA descriptor (32..256): a group's rows are cut into
-//     equal widths, and raggedness costs round_up(rows / tiles, 32) columns of tensor-core time
-//     instead of the next multiple of 256.
+//     whose width is a run-time field of the UMMA descriptor (32..256): a group's rows, rounded up to
+//     a multiple of 32, are cut into widths that differ by at most one 32, so raggedness costs up to
+//     31 columns of tensor-core time a group instead of the next multiple of 256.
 //   * kWeightGrad reduces over the rows, 64 at a time. Rows past the group's end in its last block
 //     belong to other groups: one more warp zeroes those of the last 16-row UMMA step in shared
 //     memory (both operands, so that NaN or infinity there stays out), and the steps past them are
@@ -102,12 +102,9 @@ struct GroupedArgs {
 
 __host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-// Width of a group's tiles when its rows are on the R side: equal parts of at most `cap`, rounded
-// up to the UMMA's step of 32.
-__host__ __device__ inline int group_width(int rows, int cap) {
-  const int tiles = ceil_div(rows, cap);
-  return ceil_div(ceil_div(rows, tiles), 32) * 32;
-}
+// Rows on the R side: units of 32 rows (the UMMA's step) in a group, and tiles of at most `cap` rows.
+__host__ __device__ inline int group_units(int rows) { return ceil_div(rows, 32); }
+__host__ __device__ inline int group_tiles_right(int rows, int cap) { return ceil_div(group_units(rows), cap / 32); }
 
 // Index among the boxes (128, 64, 32, 16 rows) of the smallest that holds `rows`.
 __host__ __device__ inline int group_box(int rows) { return rows > 64 ? 0 : (rows > 32 ? 1 : (rows > 16 ? 2 : 3)); }
@@ -115,7 +112,7 @@ __host__ __device__ inline int group_box(int rows) { return rows > 64 ? 0 : (row
 template <GroupMode MODE>
 __host__ __device__ inline int group_row_tiles(const GroupedArgs& a, int rows) {
   if (rows <= 0) return 0;
-  if (group_rows_right(MODE)) return ceil_div(rows, group_width(rows, a.width_cap));
+  if (group_rows_right(MODE)) return group_tiles_right(rows, a.width_cap);
   return ceil_div(MODE == GroupMode::kWeightGrad ? a.lrows : rows, 256);
 }
 
@@ -134,7 +131,8 @@ __host__ __device__ inline int group_blocks(const GroupedArgs& a, int rows) {
 // (8194 x 14336 x 4096 over 8 groups: 1007 us, 577 ns a block, against 0.28 for the UMMAs alone).
 //
 // In shared memory: eight integers (below), then [groups + 1] first row and first tile of each group,
-// tiles in a column of its output and width of its tiles (rows on the R side), then [pairs + 1] first
+// tiles in a column of its output and the units of 32 rows of its smaller tiles (rows on the R side: the
+// first group_units mod tiles of them have one more), then [pairs + 1] first
 // tile of each column along the line and its first iteration. The view keeps one address: the issuing
 // warps have no registers for six.
 constexpr int kTableHead = 8;
@@ -151,7 +149,7 @@ struct GroupTable {
   __device__ int& start(int e) const { return mem[kTableHead + e]; }
   __device__ int& tile_base(int e) const { return mem[kTableHead + groups + 1 + e]; }
   __device__ int& row_tiles(int e) const { return mem[kTableHead + 2 * (groups + 1) + e]; }
-  __device__ int& width(int e) const { return mem[kTableHead + 3 * (groups + 1) + e]; }
+  __device__ int& units(int e) const { return mem[kTableHead + 3 * (groups + 1) + e]; }
   __device__ int& col_tile(int c) const { return mem[kTableHead + 4 * (groups + 1) + c]; }
   __device__ int& col_base(int c) const { return mem[kTableHead + 4 * (groups + 1) + pairs + 1 + c]; }
 
@@ -218,7 +216,7 @@ __device__ inline void build_group_rows(const GroupedArgs& a, const GroupTable& 
       t.start(g) = begin;
       t.tile_base(g) = tiles + sum - mine;
       t.row_tiles(g) = high;
-      t.width(g) = group_rows_right(MODE) && high > 0 ? group_width(end - begin, a.width_cap) : 0;
+      t.units(g) = group_rows_right(MODE) && high > 0 ? group_units(end - begin) / high : 0;
     }
     row = __shfl_sync(0xffffffffu, end, 31);
     tiles += __shfl_sync(0xffffffffu, sum, 31);
@@ -294,11 +292,17 @@ struct GroupSegment {
   bool first;         // the share's first segment
 };
 
+// Tiles of group e, rows on the R side, that have a unit more than the others.
+__device__ inline int larger_tiles(const GroupTable& t, int e) {
+  return group_units(t.start(e + 1) - t.start(e)) - t.units(e) * t.row_tiles(e);
+}
+
 // Width of a tile of group e whose first R column is r0.
 template <GroupMode MODE>
 __device__ inline int tile_width(const GroupedArgs& a, const GroupTable& t, int e, int r0) {
-  if (group_rows_right(MODE)) return t.width(e);
-  return a.cols - r0 <= 128 ? 128 : 256;
+  if (!group_rows_right(MODE)) return a.cols - r0 <= 128 ? 128 : 256;
+  const int units = t.units(e);
+  return 32 * (r0 - t.start(e) < 32 * (units + 1) * larger_tiles(t, e) ? units + 1 : units);
 }
 
 // First L row and R column of tile `tile` of group `e`.
@@ -308,7 +312,7 @@ __device__ inline void tile_origin(const GroupedArgs& a, const GroupTable& t, in
   int pr, pc;
   grouped_tile(tile - t.tile_base(e), t.row_tiles(e), ceil_div(a.cols, 256), kGroupRaster, pr, pc);
   if (group_rows_right(MODE)) {
-    r0 = row0 + pr * t.width(e);
+    r0 = row0 + 32 * (pr * t.units(e) + min(pr, larger_tiles(t, e)));
     l0 = pc * 256;
   } else {
     l0 = (MODE == GroupMode::kWeightGrad ? 0 : row0) + pr * 256;
