@@ -123,33 +123,44 @@ __host__ __device__ inline int group_blocks(const GroupedArgs& a, int rows) {
 
 // The tiles of all groups, numbered group by group, and how the pairs share them.
 //
-// The tiles are dealt to `shares` columns like cards (tile t * shares + c is number t of column c; the
-// last, part-filled row is spread evenly over the columns), the columns are put end to end into one
-// line of (tile, K block) iterations, and the line is cut into equal shares. Share c then runs along
-// column c, give or take a part of a tile, so at any moment the pairs work on neighbouring tiles: with
-// contiguous runs of the group-by-group order instead, the 74 weight panels in use passed L2's size
-// (8194 x 14336 x 4096 over 8 groups: 1007 us, 577 ns a block, against 0.28 for the UMMAs alone).
+// kForward and the scaled products (every tile has the same K blocks): the tiles are dealt to `shares`
+// columns like cards (tile t * shares + c is number t of column c; the last, part-filled row is spread
+// evenly over the columns), the columns are put end to end into one line of (tile, K block)
+// iterations, and the line is cut into equal shares. Share c then runs along column c, give or take a
+// part of a tile, so at any moment the pairs work on neighbouring tiles: with contiguous runs of the
+// group-by-group order instead, the 74 weight panels in use passed L2's size (8194 x 14336 x 4096 over
+// 8 groups: 1007 us against 811, before the steps that followed).
 //
-// In shared memory: eight integers (below), then [groups + 1] first row and first tile of each group,
-// tiles in a column of its output and the units of 32 rows of its smaller tiles (rows on the R side: the
-// first group_units mod tiles of them have one more), then [pairs + 1] first
-// tile of each column along the line and its first iteration. The view keeps one address: the issuing
-// warps have no registers for six.
+// kWeightGrad (K blocks by group, the same number of tiles in each): of every group with rows, each
+// pair takes its tiles / pairs whole tiles, all pairs at the same group at the same time; what remains
+// of the groups, put end to end, is the line that is cut into equal shares. (Dealt as above, heavy and
+// light columns put the pairs into different groups, whose rows together do not stay in L2: 823 MB
+// read from DRAM for 160 MB of operands, 16384 x 2048 x 2816 over 32 ragged groups.)
+//
+// In shared memory: eight integers (below), then [groups + 1] of first row and three more (below), then
+// [pairs + 1] first tile of each column along the line and its first iteration. The view keeps one
+// address: the issuing warps have no registers for six.
 constexpr int kTableHead = 8;
 struct GroupTable {
   int* mem;
   int groups, pairs, whole;
 
-  __device__ int& tiles() const { return mem[0]; }
+  __device__ int& tiles() const { return mem[0]; }       // kWeightGrad: of the line
   __device__ int& shares() const { return mem[1]; }
-  __device__ int& total() const { return mem[2]; }       // iterations
+  __device__ int& total() const { return mem[2]; }       // iterations of the line
   __device__ int& per_column() const { return mem[3]; }  // tiles / shares
   __device__ int& per_share() const { return mem[4]; }   // total / shares, and what remains
   __device__ int& more_share() const { return mem[5]; }
+  __device__ int& used() const { return mem[6]; }        // kWeightGrad: groups with rows
   __device__ int& start(int e) const { return mem[kTableHead + e]; }
+  // First tile of a group, tiles in a column of its output, and the units of 32 rows of its smaller
+  // tiles (rows on the R side: the first group_units mod tiles of them have one more).
   __device__ int& tile_base(int e) const { return mem[kTableHead + groups + 1 + e]; }
   __device__ int& row_tiles(int e) const { return mem[kTableHead + 2 * (groups + 1) + e]; }
   __device__ int& units(int e) const { return mem[kTableHead + 3 * (groups + 1) + e]; }
+  // kWeightGrad, in their place: the r-th group with rows, and the K blocks of a tile of those before it.
+  __device__ int& used_group(int r) const { return tile_base(r); }
+  __device__ int& blocks_before(int r) const { return row_tiles(r); }
   __device__ int& col_tile(int c) const { return mem[kTableHead + 4 * (groups + 1) + c]; }
   __device__ int& col_base(int c) const { return mem[kTableHead + 4 * (groups + 1) + pairs + 1 + c]; }
 
@@ -158,7 +169,7 @@ struct GroupTable {
     return c * (tiles / shares) + c * (tiles % shares) / shares;
   }
   __device__ int share_begin(int p) const {
-    return whole ? col_base(p) : p * per_share() + min(p, more_share());
+    return whole ? col_base(p) : p * per_share() + min(p, more_share());  // kWeightGrad: never `whole` here
   }
   // The column of the line's tile v: the last c with column_first(c) = floor(c * tiles / shares) <= v.
   __device__ int column_of(int v) const { return ((v + 1) * shares() - 1) / tiles(); }
@@ -184,13 +195,24 @@ constexpr __host__ __device__ int group_table_ints(int groups, int pairs) {
   return kTableHead + 4 * (groups + 1) + 2 * (pairs + 1);
 }
 
+// Tiles of a group's weight gradient, and those each pair takes of it; what is over goes to the line.
+struct GradTiles {
+  int all, each, over;
+  __device__ explicit GradTiles(const GroupedArgs& a) {
+    all = ceil_div(a.lrows, 256) * ceil_div(a.cols, 256);
+    each = all / a.pairs;
+    over = all - each * a.pairs;
+  }
+};
+
 // Builds the groups' part. Ends are taken as they would be if clamped to [previous end, rows], so no
 // value of `ends` leads out of the matrices. One warp; a barrier before the second step.
 template <GroupMode MODE>
 __device__ inline void build_group_rows(const GroupedArgs& a, const GroupTable& t) {
+  constexpr bool kGrad = MODE == GroupMode::kWeightGrad;
   const int lane = static_cast<int>(lane_id());
   const int col_tiles = ceil_div(a.cols, 256);
-  int row = 0, tiles = 0, total = 0;
+  int row = 0, tiles = 0, total = 0;  // kGrad: groups with rows, and K blocks of a tile of each
   for (int g0 = 0; g0 < a.groups; g0 += 32) {
     const int g = g0 + lane;
     int end = 0;
@@ -203,30 +225,52 @@ __device__ inline void build_group_rows(const GroupedArgs& a, const GroupTable& 
     end = max(end, row);
     int begin = __shfl_up_sync(0xffffffffu, end, 1);
     if (lane == 0) begin = row;
-    const int high = g < a.groups ? group_row_tiles<MODE>(a, end - begin) : 0;
-    const int mine = high * col_tiles;
+    const int rows = g < a.groups ? end - begin : 0;
+    const int high = kGrad ? (rows > 0 ? 1 : 0) : group_row_tiles<MODE>(a, rows);
+    const int mine = kGrad ? group_blocks<MODE>(a, rows) : high * col_tiles;
     int sum = mine;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
       const int o = __shfl_up_sync(0xffffffffu, sum, d);
       if (lane >= d) sum += o;
     }
-    total += __reduce_add_sync(0xffffffffu, mine * group_blocks<MODE>(a, end - begin));
-    if (g < a.groups) {
-      t.start(g) = begin;
-      t.tile_base(g) = tiles + sum - mine;
-      t.row_tiles(g) = high;
-      t.units(g) = group_rows_right(MODE) && high > 0 ? group_units(end - begin) / high : 0;
+    if (g < a.groups) t.start(g) = begin;
+    if constexpr (kGrad) {
+      const uint32_t with_rows = __ballot_sync(0xffffffffu, high != 0);
+      if (high != 0) {
+        const int r = tiles + __popc(with_rows & ((1u << lane) - 1));
+        t.used_group(r) = g;
+        t.blocks_before(r) = total + sum - mine;
+      }
+      tiles += __popc(with_rows);
+      total += __shfl_sync(0xffffffffu, sum, 31);
+    } else {
+      if (g < a.groups) {
+        t.tile_base(g) = tiles + sum - mine;
+        t.row_tiles(g) = high;
+        t.units(g) = group_rows_right(MODE) && high > 0 ? group_units(rows) / high : 0;
+      }
+      tiles += __shfl_sync(0xffffffffu, sum, 31);
     }
     row = __shfl_sync(0xffffffffu, end, 31);
-    tiles += __shfl_sync(0xffffffffu, sum, 31);
   }
   if (lane == 0) {
     t.start(a.groups) = row;
-    t.tile_base(a.groups) = tiles;
-    const int shares = max(1, min(a.pairs, a.whole ? tiles : total / a.min_blocks));
+    if constexpr (kGrad) {
+      const GradTiles n(a);
+      t.blocks_before(tiles) = total;
+      t.used() = tiles;
+      tiles *= n.over;
+      total *= n.over;
+      // Where every pair takes whole tiles there is work for all.
+      t.shares() = n.each > 0 ? a.pairs : max(1, min(a.pairs, a.whole ? tiles : total / a.min_blocks));
+    } else {
+      t.tile_base(a.groups) = tiles;
+      total = tiles * a.k_blocks;
+      t.shares() = max(1, min(a.pairs, a.whole ? tiles : total / a.min_blocks));
+    }
+    const int shares = t.shares();
     t.tiles() = tiles;
-    t.shares() = shares;
     t.total() = total;
     t.per_column() = tiles / shares;
     t.per_share() = total / shares;
@@ -237,47 +281,12 @@ __device__ inline void build_group_rows(const GroupedArgs& a, const GroupTable& 
 // Second step, the columns' part: all threads, and a barrier before the table is used.
 template <GroupMode MODE>
 __device__ inline void build_group_columns(const GroupedArgs& a, const GroupTable& t) {
-  const int shares = t.shares(), tiles = t.tiles();
-  for (int c = static_cast<int>(threadIdx.x); c <= shares; c += static_cast<int>(blockDim.x)) {
-    const int first = GroupTable::column_first(c, tiles, shares);
-    t.col_tile(c) = first;
-    t.col_base(c) = MODE == GroupMode::kWeightGrad ? 0 : first * a.k_blocks;
-  }
-  if constexpr (MODE == GroupMode::kWeightGrad) {
-    // K blocks differ by group: the threads share out (column, group), then one warp scans the sums.
-    __syncthreads();
-    const int high = t.per_column(), whole = high * shares;  // tiles of the full rows
-    const int slices = max(1, static_cast<int>(blockDim.x) / shares);
-    for (int i = static_cast<int>(threadIdx.x); i < slices * shares; i += static_cast<int>(blockDim.x)) {
-      const int c = i % shares, slice = i / shares;
-      int sum = 0;
-      for (int e = slice; e < a.groups; e += slices) {
-        const int lo = t.tile_base(e), hi = t.tile_base(e + 1);
-        if (hi <= lo) continue;
-        // Tiles of column c below x (x <= whole): those with number * shares + c < x.
-        int count = (min(hi, whole) - c + shares - 1) / shares - (min(lo, whole) - c + shares - 1) / shares;
-        // The column's tile of the part-filled row, if it has one.
-        const int last = whole + t.col_tile(c) - c * high;
-        if (t.col_tile(c + 1) - t.col_tile(c) > high && lo <= last && last < hi) ++count;
-        sum += count * group_blocks<MODE>(a, t.start(e + 1) - t.start(e));
-      }
-      if (sum > 0) atomicAdd(&t.col_base(c), sum);
-    }
-    __syncthreads();
-    if (threadIdx.x >= 32) return;
-    const int lane = static_cast<int>(lane_id());
-    int before = 0;
-    for (int c0 = 0; c0 <= shares; c0 += 32) {
-      const int c = c0 + lane;
-      const int sum = c < shares ? t.col_base(c) : 0;
-      int scan = sum;
-#pragma unroll
-      for (int d = 1; d < 32; d *= 2) {
-        const int o = __shfl_up_sync(0xffffffffu, scan, d);
-        if (lane >= d) scan += o;
-      }
-      if (c <= shares) t.col_base(c) = before + scan - sum;
-      before += __shfl_sync(0xffffffffu, scan, 31);
+  if constexpr (MODE != GroupMode::kWeightGrad) {
+    const int shares = t.shares(), tiles = t.tiles();
+    for (int c = static_cast<int>(threadIdx.x); c <= shares; c += static_cast<int>(blockDim.x)) {
+      const int first = GroupTable::column_first(c, tiles, shares);
+      t.col_tile(c) = first;
+      t.col_base(c) = first * a.k_blocks;
     }
   }
 }
@@ -309,88 +318,131 @@ __device__ inline int tile_width(const GroupedArgs& a, const GroupTable& t, int 
 template <GroupMode MODE>
 __device__ inline void tile_origin(const GroupedArgs& a, const GroupTable& t, int e, int tile, int& l0, int& r0) {
   const int row0 = t.start(e);
+  const bool grad = MODE == GroupMode::kWeightGrad;  // `tile` counts within the group
   int pr, pc;
-  grouped_tile(tile - t.tile_base(e), t.row_tiles(e), ceil_div(a.cols, 256), kGroupRaster, pr, pc);
+  grouped_tile(grad ? tile : tile - t.tile_base(e), grad ? ceil_div(a.lrows, 256) : t.row_tiles(e), ceil_div(a.cols, 256),
+               kGroupRaster, pr, pc);
   if (group_rows_right(MODE)) {
     r0 = row0 + 32 * (pr * t.units(e) + min(pr, larger_tiles(t, e)));
     l0 = pc * 256;
   } else {
-    l0 = (MODE == GroupMode::kWeightGrad ? 0 : row0) + pr * 256;
+    l0 = (grad ? 0 : row0) + pr * 256;
     r0 = pc * 256;
   }
 }
 
-// The tiles of one stretch [lo, hi) of the line in order, by a whole warp: each lane works out one
-// tile of a batch of 32, since a tile's place takes about a dozen divisions (one at a time, they cost
-// the UMMA issuer half a microsecond a tile).
+// The tiles of one share, or of one stretch [lo, hi) of the line, in order, by a whole warp: each lane
+// works out one tile of a batch of 32, since a tile's place takes about a dozen divisions (one at a
+// time, they cost the UMMA issuer half a microsecond a tile).
 template <GroupMode MODE>
 struct GroupWalk {
   int lo, hi;
-  int v;           // first tile of the next batch, counted along the line
-  int line;        // its first iteration
+  int v, v_end;    // first tile of the next batch, counted along the line, and the end
+  int ahead;       // kWeightGrad: whole tiles still to come before those of the line,
+  int done;        // and those behind
   int cur, count;  // the batch's next lane, and the end of its live lanes
   // This lane's tile: its group (negative, ~group, if it begins the stretch), origin and K blocks.
   int group, l0, r0, kb0, kb1;
 
-  // `guess`: a column near lo.
+  // A stretch of the line; `guess`: a column near lo.
   __device__ GroupWalk(const GroupedArgs& a, const GroupTable& t, int lo_, int hi_, int guess)
-      : lo(lo_), hi(hi_), cur(0), count(0) {
-    v = 0;
-    line = hi;
+      : lo(lo_), hi(hi_), v(0), v_end(0), ahead(0), done(0), cur(0), count(0) {
     if (lo >= hi) return;
-    int c = guess;
-    while (t.col_base(c) > lo) --c;
-    while (t.col_base(c + 1) <= lo) ++c;
-    v = t.col_tile(c);
-    line = t.col_base(c);
-    if constexpr (MODE != GroupMode::kWeightGrad) {
-      const int n = (lo - line) / a.k_blocks;
-      v += n;
-      line += n * a.k_blocks;
+    if constexpr (MODE == GroupMode::kWeightGrad) {
+      const int over = GradTiles(a).over;
+      int r = 0, top = t.used() - 1;  // last group with rows that begins at or before lo
+      while (r < top) {
+        const int mid = (r + top + 1) >> 1;
+        if (over * t.blocks_before(mid) <= lo) {
+          r = mid;
+        } else {
+          top = mid - 1;
+        }
+      }
+      v = r * over + (lo - over * t.blocks_before(r)) / (t.blocks_before(r + 1) - t.blocks_before(r));
+    } else {
+      int c = guess;
+      while (t.col_base(c) > lo) --c;
+      while (t.col_base(c + 1) <= lo) ++c;
+      v = t.col_tile(c) + (lo - t.col_base(c)) / a.k_blocks;
     }
+    v_end = t.tiles();
   }
   // The share of `pair`.
   __device__ GroupWalk(const GroupedArgs& a, const GroupTable& t, int pair)
-      : GroupWalk(a, t, pair < t.shares() ? t.share_begin(pair) : 0, pair < t.shares() ? t.share_begin(pair + 1) : 0,
-                  min(pair, t.shares() - 1)) {}
+      : GroupWalk(a, t, line_begin(a, t, pair), line_begin(a, t, pair + 1), min(pair, t.shares() - 1)) {
+    if constexpr (MODE == GroupMode::kWeightGrad) {
+      if (pair < t.shares()) ahead = t.used() * GradTiles(a).each;
+      if (a.whole) {  // shares of whole tiles
+        const int per = t.per_column(), more = t.tiles() - per * t.shares();
+        lo = 0;
+        hi = t.total();
+        v = pair * per + min(pair, more);
+        v_end = pair < t.shares() ? v + per + (pair < more ? 1 : 0) : v;
+      }
+    }
+  }
+  __device__ static int line_begin(const GroupedArgs& a, const GroupTable& t, int p) {
+    if (MODE == GroupMode::kWeightGrad && a.whole) return 0;
+    return p <= t.shares() ? t.share_begin(p) : t.total();
+  }
 
-  __device__ void refill(const GroupedArgs& a, const GroupTable& t) {
+  __device__ void refill(const GroupedArgs& a, const GroupTable& t, int pair) {
     const int lane = static_cast<int>(lane_id());
-    uint32_t live = 0;
-    while (live == 0 && line < hi) {  // kWeightGrad: batches before lo are passed over
-      int blocks = 0, e = 0, tile = 0;
-      if (v + lane < t.tiles()) {
-        const int c = t.column_of(v + lane);
-        tile = t.tile_of(c, v + lane - t.col_tile(c));
-        e = t.group_of(tile);
+    bool live = false;
+    int e = 0, tile = 0, begin = 0, blocks = 0;
+    if constexpr (MODE == GroupMode::kWeightGrad) {
+      const GradTiles n(a);
+      const int i = done + lane;
+      if (i < ahead) {  // whole tiles: number i % each of the pair's in a group
+        const int r = i / n.each;
+        e = t.used_group(r);
+        tile = (i - r * n.each) * a.pairs + pair;
         blocks = group_blocks<MODE>(a, t.start(e + 1) - t.start(e));
+        begin = lo;
+        live = true;
+      } else if (v + i - ahead < v_end) {
+        const int at = v + i - ahead, r = at / n.over;
+        e = t.used_group(r);
+        tile = n.each * a.pairs + at - r * n.over;
+        blocks = group_blocks<MODE>(a, t.start(e + 1) - t.start(e));
+        begin = n.over * t.blocks_before(r) + (at - r * n.over) * blocks;
+        live = begin < hi;
       }
-      int scan = blocks;
-#pragma unroll
-      for (int d = 1; d < 32; d *= 2) {
-        const int o = __shfl_up_sync(0xffffffffu, scan, d);
-        if (lane >= d) scan += o;
+      if (live) {
+        const bool line = i >= ahead;
+        group = line && begin <= lo ? ~e : e;
+        kb0 = line ? max(lo - begin, 0) : 0;
+        kb1 = line ? min(blocks, hi - begin) : blocks;
       }
-      const int begin = line + scan - blocks;
-      const bool mine_live = blocks > 0 && begin < hi && begin + blocks > lo;
-      live = __ballot_sync(0xffffffffu, mine_live);
-      if (mine_live) {
-        tile_origin<MODE>(a, t, e, tile, l0, r0);
+      done += 32;
+    } else {
+      const int at = v + done + lane;
+      if (at < v_end) {
+        const int c = t.column_of(at);
+        tile = t.tile_of(c, at - t.col_tile(c));
+        e = t.group_of(tile);
+        blocks = a.k_blocks;
+        begin = at * blocks;
+        live = begin < hi;
+      }
+      if (live) {
         group = begin <= lo ? ~e : e;
         kb0 = max(lo - begin, 0);
         kb1 = min(blocks, hi - begin);
       }
-      line += __shfl_sync(0xffffffffu, scan, 31);
-      v += 32;
+      done += 32;
     }
-    cur = live != 0 ? __ffs(static_cast<int>(live)) - 1 : 0;
-    count = 32 - __clz(static_cast<int>(live));
+    if (live) tile_origin<MODE>(a, t, e, tile, l0, r0);
+    cur = 0;
+    count = __popc(__ballot_sync(0xffffffffu, live));  // the live lanes come first
   }
 
-  __device__ bool next(const GroupedArgs& a, const GroupTable& t, GroupSegment& s) {
+  __device__ bool next(const GroupedArgs& a, const GroupTable& t, int pair, GroupSegment& s) {
     if (cur >= count) {
-      refill(a, t);
-      if (cur >= count) return false;
+      if (done > 0 && count < 32) return false;
+      refill(a, t, pair);
+      if (count == 0) return false;
     }
     const int from = cur++;
     const int g = __shfl_sync(0xffffffffu, group, from);
@@ -745,7 +797,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
     bool ok = true;
     GroupWalk<MODE> walk(args, table, pair);
     GroupSegment s;
-    while (ok && walk.next(args, table, s)) {
+    while (ok && walk.next(args, table, pair, s)) {
       const int half = s.width / 2;
       const int tail = kGrad ? (s.row_end - s.row0) - (s.blocks - 1) * 64 : 0;
       const int l0 = s.l0 + static_cast<int>(rank) * 128;
@@ -836,7 +888,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
     constexpr int kLStep = (L_MN ? 2048 : 32) >> 4, kRStep = (kGrad ? 2048 : 32) >> 4;
     GroupWalk<MODE> walk(args, table, pair);
     GroupSegment s;
-    while (ok && walk.next(args, table, s)) {
+    while (ok && walk.next(args, table, pair, s)) {
       const uint32_t idesc = kIdescBase | (static_cast<uint32_t>((kWide ? 128 : s.width) >> 3) << 17);
       const bool active = !kWide || side * 128 < s.width;
       const int tail = kGrad ? (s.row_end - s.row0) - (s.blocks - 1) * 64 : 0;
@@ -882,7 +934,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
     uint32_t parity = 0;  // bit s: parity of the next use of tail_full[s]
     GroupWalk<MODE> walk(args, table, pair);
     GroupSegment s;
-    while (walk.next(args, table, s)) {
+    while (walk.next(args, table, pair, s)) {
       const int blocks = s.kb1 - s.kb0;
       const int tail = (s.row_end - s.row0) - (s.blocks - 1) * 64;
       if (s.kb1 == s.blocks && (tail & 15) != 0) {
@@ -942,7 +994,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
     GroupWalk<MODE> walk(args, table, pair);
     GroupSegment s;
     if constexpr (!kScaled) {
-      while (walk.next(args, table, s)) {
+      while (walk.next(args, table, pair, s)) {
         if (!wait_buf()) break;
         const uint32_t taddr = lane_base + static_cast<uint32_t>(buf * kBufCols);
         const int l32 = s.l0 + static_cast<int>(rank) * 128 + quarter * 32;  // the warp's first L row
@@ -996,7 +1048,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
       }
     } else if constexpr (kWide) {
       // One weight scale a block for the 128 columns of a half; both scales are loaded a block ahead.
-      while (walk.next(args, table, s)) {
+      while (walk.next(args, table, pair, s)) {
         if (side * 128 >= s.width) continue;
         const int l32 = s.l0 + static_cast<int>(rank) * 128 + quarter * 32;
         const int col = s.r0 + side * 128;
@@ -1064,7 +1116,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
       }
     } else {
       // kScaledFew: lane j holds the scales of rows j and j + 32, times this CTA's weight scale.
-      while (walk.next(args, table, s)) {
+      while (walk.next(args, table, pair, s)) {
         const int l32 = s.l0 + static_cast<int>(rank) * 128 + quarter * 32;
         const int nb = min((s.l0 >> 7) + static_cast<int>(rank), (args.cols - 1) >> 7);
         const float* sb = args.tile_scales + s.group * args.ts_group + nb * args.ts_n + s.kb0 * args.ts_k;
@@ -1167,13 +1219,14 @@ __global__ void __launch_bounds__(kFinishThreads) grouped_finish_kernel(const __
   const int rank = static_cast<int>(blockIdx.y);
   GroupSegment s = {};
   int cut = 0;
-  if (p < table.shares()) {
+  const bool joins = p < table.shares() && table.share_begin(p) < table.total();
+  if (joins) {
     cut = table.share_begin(p);
     GroupWalk<MODE> walk(args, table, cut, cut + 1, p);
-    walk.next(args, table, s);
+    walk.next(args, table, 0, s);
   }
   wait_for_primary();  // the pieces; all before it comes from `ends` alone
-  if (p < table.shares()) {
+  if (joins) {
     const int begin = cut - s.kb0, end = begin + s.blocks;
     const int c = static_cast<int>(blockIdx.z) * kCols;
     if (cut > begin && table.share_begin(p - 1) <= begin && c < s.width) {

@@ -186,6 +186,14 @@ def test_long_sums_and_many_tiles_are_joined_across_pairs() -> None:
 
 
 @gpu
+@pytest.mark.parametrize("k,n", ((2312, 2056), (2304, 2048)))  # 90 and 72 tiles a group: more and fewer than the pairs of SMs
+@pytest.mark.parametrize("ends", ([300, 300, 1700], [0, 1100, 1101], [1500, 1500, 1500]))
+def test_weight_gradients_of_many_tiles(k: int, n: int, ends: list[int]) -> None:
+    x, _, dy = _operands(1703, 1, k, n, torch.float16, "kn", seed=20)
+    _check_weight_grad(grouped.grouped_weight_grad(x, dy, _ends(ends)), x, dy, ends)
+
+
+@gpu
 def test_many_groups() -> None:
     groups = grouped.MAX_GROUPS
     counts = torch.randint(0, 4, (groups,), generator=torch.Generator().manual_seed(1))
