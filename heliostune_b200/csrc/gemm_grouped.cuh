@@ -22,11 +22,11 @@
 //     not issued.
 //   * kScaled accumulates each 128-deep block in a TMEM buffer of its own; the epilogue warps read
 //     it, multiply by the block's scales and add it to FP32 registers, while the next block's UMMAs
-//     fill another buffer. A tile's two 128-column halves go separate ways: each has its issuing
-//     warp, its two buffers and its four epilogue warps. The rows are on the L side, where a row is a
-//     TMEM lane and its scale one register: on the R side the scales of 256 rows are 128 a thread and
-//     block, and their broadcast loads from shared memory, beside the UMMAs' operands, took three times
-//     the UMMAs' time.
+//     fill the other buffer. The rows are on the L side, where a row is a TMEM lane and its scale one
+//     register: on the R side the scales of 256 rows are 128 a thread and block, and their broadcast
+//     loads from shared memory, beside the UMMAs' operands, took three times the UMMAs' time. Bound now
+//     by the way of a block through the two buffers (UMMAs 512 cycles, hand-over, 128 columns a thread
+//     read and added, hand-back): 8192 x 14336 x 4096 in 470 us, 350 without the reading and adding.
 //   * kScaledFew is for few rows a group: as kForward, weights on the L side and at most 64 rows on
 //     the R side, in eight TMEM buffers. A block then costs 64 to 128 UMMA cycles instead of 512 and
 //     keeps all lanes busy, and the weights stream at the rate of HBM.
@@ -59,9 +59,9 @@ constexpr int kMaxGroups = 1024;
 constexpr int kGroupLBytes = 16384;  // 128 L rows x 128 bytes of K (or 2 boxes of 64 x 64)
 constexpr int kGroupRaster = 8;      // row tiles before the next column tile
 
-// Warps: 0 loads, 1 issues the UMMAs (kScaled: and 2, one a half); then the epilogue, and for
-// kWeightGrad the masking warp. kScaled holds 128 x 256 FP32 sums in the registers of 8 epilogue
-// warps, which therefore form warpgroups of their own (3 idle); kWeightGrad has 8 because a group of few
+// Warps: 0 loads, 1 issues the UMMAs; then the epilogue, and for kWeightGrad the masking warp. kScaled
+// holds 128 x 256 FP32 sums in the registers of 8 epilogue warps, which therefore form warpgroups of
+// their own (2 and 3 idle); kWeightGrad has 8 because a group of few
 // rows is little but epilogue (32 groups of 64 rows, 2048 x 2816: 102 us against 108 with four).
 __host__ __device__ constexpr int group_first_epilogue_warp(GroupMode m) { return m == GroupMode::kScaled ? 4 : 2; }
 __host__ __device__ constexpr int group_epilogue_warps(GroupMode m) { return m == GroupMode::kScaled || m == GroupMode::kWeightGrad ? 8 : 4; }
@@ -70,7 +70,7 @@ __host__ __device__ constexpr int group_threads(GroupMode m) {
 }
 
 // Boxes of 128, 64, 32 and 16 rows on the side that has the rows (kForward, kScaledFew: R; kScaled: L), else one in
-// [0] (kScaled's R: 64 rows; kWeightGrad: 64 x 64).
+// [0] (kScaled's R: 128 rows and, in [1], 64; kWeightGrad: 64 x 64).
 struct GroupedMaps {
   CUtensorMap l[4];
   CUtensorMap r[4];
@@ -729,9 +729,8 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
   constexpr int kSteps = 4;                    // UMMA K steps of a block: 128 bytes of K
   constexpr int kBlockK = kScaled ? 128 : 64;  // K values of a block
   constexpr bool kBf16 = !kScaled && std::is_same<T, __nv_bfloat16>::value;
-  constexpr int kIssuers = kWide ? 2 : 1;  // warps issuing UMMAs, one a half of the tile
-  constexpr int kBufs = kFew ? 8 : 2;      // TMEM buffers of an issuer
-  constexpr int kBufCols = 512 / (kBufs * kIssuers);
+  constexpr int kBufs = kFew ? 8 : 2;  // TMEM buffers
+  constexpr int kBufCols = 512 / kBufs;
   constexpr uint32_t kIdescBase = (1u << 4) | (kBf16 ? (1u << 7) | (1u << 10) : 0u) | (L_MN ? 1u << 15 : 0u) |
                                   (kGrad ? 1u << 16 : 0u) | ((256u >> 4) << 24);
 
@@ -760,14 +759,14 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(&full[s], kGrad ? 2 : 1);  // kWeightGrad: both CTAs report each stage
-      mbar_init(&empty[s], kIssuers);
+      mbar_init(&empty[s], 1);
       mbar_init(&tail_full[s], 1);
     }
-    for (int b = 0; b < kBufs * kIssuers; ++b) {
+    for (int b = 0; b < kBufs; ++b) {
       mbar_init(&tmem_full[b], 1);
-      mbar_init(&tmem_empty[b], 2 * kEpilogueWarps / kIssuers);  // its epilogue warps in both CTAs (leader's copy)
+      mbar_init(&tmem_empty[b], 2 * kEpilogueWarps);  // the epilogue warps of both CTAs (leader's copy)
     }
-    mbar_init(mma_done, kIssuers);
+    mbar_init(mma_done, 1);
     *abort_flag = 0;
     fence_mbarrier_init();
     tma_prefetch_map(&maps.l[0]);
@@ -801,14 +800,14 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
       const int half = s.width / 2;
       const int tail = kGrad ? (s.row_end - s.row0) - (s.blocks - 1) * 64 : 0;
       const int l0 = s.l0 + static_cast<int>(rank) * 128;
-      const int r0 = s.r0 + static_cast<int>(rank) * (kWide ? 64 : half);
+      const int r0 = s.r0 + static_cast<int>(rank) * half;
       // kScaled: rows the tile has in this CTA, and in both; what a box of them leaves of the stage
       // holds what it held (those lanes are not stored).
       const int left = s.row_end - s.l0;
       const int mine = min(128, left - static_cast<int>(rank) * 128);
       auto box_bytes = [](int rows) { return rows <= 0 ? 0u : (128u >> group_box(rows)) * 128u; };
       const CUtensorMap* l_map = &maps.l[kWide ? group_box(mine) : 0];
-      const CUtensorMap* r_map = &maps.r[group_rows_right(MODE) ? group_box(half) : 0];
+      const CUtensorMap* r_map = &maps.r[kGrad ? 0 : group_box(half)];
       const uint32_t r_bytes = group_rows_right(MODE) ? box_bytes(half) : static_cast<uint32_t>(half) * 128u;
       const uint32_t both_bytes = 2 * r_bytes + (kWide ? box_bytes(left) + box_bytes(left - 128) : 2 * kGroupLBytes);
       for (int kb = s.kb0; kb < s.kb1; ++kb) {
@@ -843,9 +842,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
             const int k0 = kb * kBlockK;
             if constexpr (kWide) {
               if (mine > 0) elected_load_2d_pair(l_dst, l_map, leader_full, k0, l0);
-              for (int h = 0; h < s.width / 128; ++h) {
-                elected_load_3d_pair(r_dst + h * 8192, r_map, leader_full, k0, r0 + h * 128, s.group);
-              }
+              elected_load_3d_pair(r_dst, r_map, leader_full, k0, r0, s.group);
             } else {
               if constexpr (L_MN) {
                 for (int i = 0; i < 2; ++i) elected_load_3d_pair(l_dst + i * 8192, l_map, leader_full, l0 + 64 * i, k0, s.group);
@@ -875,26 +872,24 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
         }
       }
     }
-  } else if (warp <= kIssuers && rank == 0) {
-    // ---------------- UMMA issuers (leader only) ----------------
-    const int side = warp - 1;  // kScaled: the half of the tile's columns
+  } else if (warp == 1 && rank == 0) {
+    // ---------------- UMMA issuer (leader only) ----------------
     int stage = 0;
     uint32_t phase = 0;
     int buf = 0;
     uint32_t buf_phase = 0;
     bool ok = true;
     const uint64_t l_desc0 = smem_desc(smem_addr(ring), L_MN ? 8192 : 16, 1024);
-    const uint64_t r_desc0 = smem_desc(smem_addr(ring) + kGroupLBytes + side * 8192, kGrad ? 8192 : 16, 1024);
+    const uint64_t r_desc0 = smem_desc(smem_addr(ring) + kGroupLBytes, kGrad ? 8192 : 16, 1024);
     constexpr int kLStep = (L_MN ? 2048 : 32) >> 4, kRStep = (kGrad ? 2048 : 32) >> 4;
     GroupWalk<MODE> walk(args, table, pair);
     GroupSegment s;
     while (ok && walk.next(args, table, pair, s)) {
-      const uint32_t idesc = kIdescBase | (static_cast<uint32_t>((kWide ? 128 : s.width) >> 3) << 17);
-      const bool active = !kWide || side * 128 < s.width;
+      const uint32_t idesc = kIdescBase | (static_cast<uint32_t>(s.width >> 3) << 17);
       const int tail = kGrad ? (s.row_end - s.row0) - (s.blocks - 1) * 64 : 0;
       for (int kb = s.kb0; kb < s.kb1; ++kb) {
-        if (active && (kScaled || kb == s.kb0)) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&tmem_empty[kBufs * side + buf], buf_phase ^ 1u, abort_flag));
+        if (kScaled || kb == s.kb0) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&tmem_empty[buf], buf_phase ^ 1u, abort_flag));
           if (!ok) break;
           tc_fence_after_sync();
         }
@@ -907,17 +902,15 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
         tc_fence_after_sync();
         const uint64_t off = static_cast<uint64_t>(stage * (stage_bytes >> 4));
         const int steps = kGrad && kb == s.blocks - 1 ? (tail + 15) / 16 : kSteps;
-        if (active) {
-          umma_block_pair<kScaled, kLStep, kRStep>(tmem_base + static_cast<uint32_t>((kBufs * side + buf) * kBufCols),
-                                                   l_desc0 + off, r_desc0 + off, idesc, !kScaled && kb != s.kb0, steps);
-        }
+        umma_block_pair<kScaled, kLStep, kRStep>(tmem_base + static_cast<uint32_t>(buf * kBufCols), l_desc0 + off, r_desc0 + off,
+                                                 idesc, !kScaled && kb != s.kb0, steps);
         umma_commit_elected(smem_addr(&empty[stage]));
         if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
         }
-        if (active && (kScaled || kb + 1 == s.kb1)) {
-          umma_commit_elected(smem_addr(&tmem_full[kBufs * side + buf]));
+        if (kScaled || kb + 1 == s.kb1) {
+          umma_commit_elected(smem_addr(&tmem_full[buf]));
           if (++buf == kBufs) {
             buf = 0;
             buf_phase ^= 1u;
@@ -966,18 +959,16 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
     const int row = quarter * 32 + static_cast<int>(lane);  // TMEM lane
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
     T* out = static_cast<T*>(args.out);
-    // The half of the tile's columns; kWeightGrad's halves share the buffers.
-    const int half = kEpilogueWarps == 8 ? (warp - kFirstEpilogue) / 4 : 0;
-    const int side = kWide ? half : 0;
+    const int half = kEpilogueWarps == 8 ? (warp - kFirstEpilogue) / 4 : 0;  // of the tile's columns
     int buf = 0;
     uint32_t buf_phase = 0;
     auto wait_buf = [&]() {
-      const bool ready = __all_sync(0xffffffffu, mbar_wait(&tmem_full[kBufs * side + buf], buf_phase, abort_flag));
+      const bool ready = __all_sync(0xffffffffu, mbar_wait(&tmem_full[buf], buf_phase, abort_flag));
       if (!ready && lane == 0) raise_abort(args.status, abort_flag, kStatusEpilogueTimeout);
       if (ready) tc_fence_after_sync();
       return ready;
     };
-    const uint32_t leader_empty = map_to_rank(smem_addr(&tmem_empty[kBufs * side]), 0);
+    const uint32_t leader_empty = map_to_rank(smem_addr(tmem_empty), 0);
     auto release_buf = [&]() {
       tc_fence_before_sync();
       __syncwarp();
@@ -1049,9 +1040,8 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
     } else if constexpr (kWide) {
       // One weight scale a block for the 128 columns of a half; both scales are loaded a block ahead.
       while (walk.next(args, table, pair, s)) {
-        if (side * 128 >= s.width) continue;
         const int l32 = s.l0 + static_cast<int>(rank) * 128 + quarter * 32;
-        const int col = s.r0 + side * 128;
+        const int col = s.r0 + half * 128;
         const bool live = l32 < s.row_end && col < args.cols;  // warp-uniform
         const float* sa = args.row_scales + static_cast<int64_t>(min(l32 + static_cast<int>(lane), args.rows - 1)) * args.rs_row +
                           s.kb0 * args.rs_k;
@@ -1072,7 +1062,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
           ready = wait_buf();
           if (!ready) break;
           if (live) {
-            const uint32_t taddr = lane_base + static_cast<uint32_t>((kBufs * side + buf) * kBufCols);
+            const uint32_t taddr = lane_base + static_cast<uint32_t>(buf * kBufCols + half * 128);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               uint32_t v[2][32];
@@ -1104,7 +1094,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
             store_cols_64(out, l32, s.row_end - l32, col + 64 * h, args, stage_out, f[0], f[1]);
           }
         } else {
-          float* dst = piece_of(s) + (static_cast<size_t>(side * 32) * 128 + row) * 4;
+          float* dst = piece_of(s) + (static_cast<size_t>(half * 32) * 128 + row) * 4;
           if (l32 + static_cast<int>(lane) < s.row_end) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) {

@@ -417,7 +417,8 @@ int hst_matmul_blockscaled(int32_t out_dtype, const void* a, int64_t a_row, int6
   GroupedMaps maps = {};
   const bool few = scaled_few(rows, groups);
   for (int i = 0; i < 4; ++i) HST_TRY(encode_rows(few ? &maps.r[i] : &maps.l[i], type, as, box_rows_of(i)));
-  HST_TRY(encode_weights(few ? &maps.l[0] : &maps.r[0], type, bs, few ? 128 : 64));
+  HST_TRY(encode_weights(few ? &maps.l[0] : &maps.r[0], type, bs, 128));
+  if (!few) HST_TRY(encode_weights(&maps.r[1], type, bs, 64));
   GroupedArgs args = {};
   args.ends = ends;
   args.out = y;
