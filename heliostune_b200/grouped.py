@@ -12,9 +12,10 @@ the same kernel on the transposed view, ``dweight[e] = x[e].T @ dy[e]`` its own
 
 Nothing is read back from the GPU: the sizes stay there, and a call can be captured into a CUDA
 graph and replayed with other ends. (A backward pass is captured, as with any torch operator, while no
-eager graph of the same leaves is alive: their gradient nodes would tie the capture to the eager stream.) Rows past the last end belong to no expert: their outputs and
-input gradients are zero, and they enter no weight gradient. An expert without rows gets a zero
-weight gradient. Each end is taken clamped to ``[previous end, T]``.
+eager graph of the same leaves is alive: their gradient nodes would tie the capture to the eager
+stream.) Rows past the last end belong to no expert: their outputs and input gradients are zero, and
+they enter no weight gradient. An expert without rows gets a zero weight gradient. Each end is taken
+clamped to ``[previous end, T]``.
 
 The heliostune reference has no counterpart (its products have one weight).
 """
@@ -134,7 +135,11 @@ def grouped_weight_grad(x: torch.Tensor, dy: torch.Tensor, group_ends: torch.Ten
 class _GroupedMatmul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, group_ends):  # type: ignore[no-untyped-def]
-        ctx.save_for_backward(x, weight, group_ends)
+        # Each gradient reads the other operand: what is frozen keeps nothing alive.
+        need_x, need_weight, _ = ctx.needs_input_grad
+        ctx.save_for_backward(x if need_weight else None, weight if need_x else None, group_ends)
+        # [E, N, K] storage: its gradient gets the same layout, so that it adds up in place.
+        ctx.weight_by_n = weight.stride(1) == 1 and weight.stride(2) != 1
         return _forward(x, weight, group_ends)
 
     @staticmethod
@@ -145,8 +150,7 @@ class _GroupedMatmul(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             dx = _forward(dy, weight.transpose(1, 2), group_ends)
         if ctx.needs_input_grad[1]:
-            if weight.stride(1) == 1 and weight.stride(2) != 1:
-                # [E, N, K] storage: the gradient in the same layout, so that it adds up in place.
+            if ctx.weight_by_n:
                 dweight = _weight_grad(dy, x, group_ends).transpose(1, 2)
             else:
                 dweight = _weight_grad(x, dy, group_ends)

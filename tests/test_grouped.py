@@ -312,6 +312,28 @@ def test_only_the_gradients_asked_for_and_no_second_derivative() -> None:
 
 
 @gpu
+def test_a_frozen_operand_keeps_the_other_out_of_the_graph() -> None:
+    ends = _ends([4, 9])
+    x, w, _ = _operands(9, 2, 32, 16, torch.float16, "kn", seed=13)
+
+    def saved(x: torch.Tensor, w: torch.Tensor) -> set[int]:
+        kept: set[int] = set()
+
+        def keep(t: torch.Tensor) -> torch.Tensor:
+            kept.add(t.data_ptr())
+            return t
+
+        with torch.autograd.graph.saved_tensors_hooks(keep, lambda t: t):
+            grouped.grouped_matmul(x, w, ends)
+        return kept
+
+    leaf_x, leaf_w = x.clone().requires_grad_(), w.clone().requires_grad_()
+    assert saved(leaf_x, w) == {w.data_ptr(), ends.data_ptr()}
+    assert saved(x, leaf_w) == {x.data_ptr(), ends.data_ptr()}
+    assert saved(leaf_x, leaf_w) == {leaf_x.data_ptr(), leaf_w.data_ptr(), ends.data_ptr()}
+
+
+@gpu
 def test_bad_arguments_are_rejected() -> None:
     x, w, dy = _operands(9, 2, 32, 16, torch.float16, "kn", seed=13)
     ends = _ends([4, 9])
