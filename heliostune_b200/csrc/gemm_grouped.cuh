@@ -33,9 +33,10 @@
 //
 // Schedule: all (tile, K block) iterations of all groups in one line, cut into one equal share per
 // pair (GroupTable). A tile cut by a share's end leaves FP32 pieces in the workspace, which a second
-// small kernel (grouped_finish_kernel, a programmatic dependent) adds in K order. Where no tile has
-// more than 16 K blocks (args.whole) the shares end at tiles instead: the second launch and the pieces
-// cost more than the imbalance (8 groups, 421 rows, 520 x 1000: 19 us a product with them, 12 without).
+// small kernel (grouped_finish_kernel, a programmatic dependent) adds in K order. Where ending the
+// shares at tiles idles the last pairs for a few K blocks only (GroupedArgs::idle_limit), they end there
+// instead: writing, reading and adding the pieces costs more (8192 x 2048 x 2048 over 16 groups: 72 us
+// cut, 63 whole; 421 x 520 x 1000 over 8: 16 and 10).
 // No CTA ever waits for another pair, no atomics: results are bitwise reproducible, and the kernels can
 // be captured and replayed. Whichever kernel is last also writes the zeros of rows past the last group
 // and of the weight gradients of empty groups.
@@ -88,7 +89,8 @@ struct GroupedArgs {
   int r_bytes;          // bytes of the R operand's part of a stage
   int pairs;            // CTA pairs launched
   int min_blocks;       // iterations a share has at least
-  int whole;            // shares end at tiles: nothing is cut
+  int idle_limit;       // shares end at tiles if that idles a pair for at most so many K blocks (GroupTable)
+  int whole;            // they do whatever the ends are: no finish kernel follows
   int vec;              // bytes of a store the output rows' alignment allows: 32, 16, 8, 4 or 2
   int* status;
   void* out;            // [rows, cols], or [groups, lrows, cols], contiguous
@@ -143,7 +145,7 @@ __host__ __device__ inline int group_blocks(const GroupedArgs& a, int rows) {
 constexpr int kTableHead = 8;
 struct GroupTable {
   int* mem;
-  int groups, pairs, whole;
+  int groups, pairs;
 
   __device__ int& tiles() const { return mem[0]; }       // kWeightGrad: of the line
   __device__ int& shares() const { return mem[1]; }
@@ -152,6 +154,7 @@ struct GroupTable {
   __device__ int& per_share() const { return mem[4]; }   // total / shares, and what remains
   __device__ int& more_share() const { return mem[5]; }
   __device__ int& used() const { return mem[6]; }        // kWeightGrad: groups with rows
+  __device__ int& whole() const { return mem[7]; }       // the shares end at tiles
   __device__ int& start(int e) const { return mem[kTableHead + e]; }
   // First tile of a group, tiles in a column of its output, and the units of 32 rows of its smaller
   // tiles (rows on the R side: the first group_units mod tiles of them have one more).
@@ -169,7 +172,7 @@ struct GroupTable {
     return c * (tiles / shares) + c * (tiles % shares) / shares;
   }
   __device__ int share_begin(int p) const {
-    return whole ? col_base(p) : p * per_share() + min(p, more_share());  // kWeightGrad: never `whole` here
+    return whole() ? col_base(p) : p * per_share() + min(p, more_share());  // kWeightGrad: never whole here
   }
   // The column of the line's tile v: the last c with column_first(c) = floor(c * tiles / shares) <= v.
   __device__ int column_of(int v) const { return ((v + 1) * shares() - 1) / tiles(); }
@@ -205,6 +208,21 @@ struct GradTiles {
   }
 };
 
+// How the line is shared: by whole tiles or by K blocks, and among how many pairs. `all`: there is
+// work for every pair already (the whole tiles of kWeightGrad).
+struct GroupShares {
+  int shares;
+  bool whole;
+  __host__ __device__ GroupShares(const GroupedArgs& a, int tiles, int total, int deepest, bool all) {
+    const int by_tiles = all ? a.pairs : at_least_one(a.pairs, tiles);
+    const int by_blocks = all ? a.pairs : at_least_one(a.pairs, total / a.min_blocks);
+    const int64_t idle = static_cast<int64_t>(ceil_div(tiles, by_tiles)) * deepest - total / by_blocks;
+    whole = a.whole != 0 || idle <= a.idle_limit;
+    shares = whole ? by_tiles : by_blocks;
+  }
+  __host__ __device__ static int at_least_one(int pairs, int work) { return work < 1 ? 1 : (work < pairs ? work : pairs); }
+};
+
 // Builds the groups' part. Ends are taken as they would be if clamped to [previous end, rows], so no
 // value of `ends` leads out of the matrices. One warp; a barrier before the second step.
 template <GroupMode MODE>
@@ -213,6 +231,7 @@ __device__ inline void build_group_rows(const GroupedArgs& a, const GroupTable& 
   const int lane = static_cast<int>(lane_id());
   const int col_tiles = ceil_div(a.cols, 256);
   int row = 0, tiles = 0, total = 0;  // kGrad: groups with rows, and K blocks of a tile of each
+  int deepest = kGrad ? 0 : a.k_blocks;
   for (int g0 = 0; g0 < a.groups; g0 += 32) {
     const int g = g0 + lane;
     int end = 0;
@@ -243,6 +262,7 @@ __device__ inline void build_group_rows(const GroupedArgs& a, const GroupTable& 
         t.blocks_before(r) = total + sum - mine;
       }
       tiles += __popc(with_rows);
+      deepest = max(deepest, __reduce_max_sync(0xffffffffu, mine));
       total += __shfl_sync(0xffffffffu, sum, 31);
     } else {
       if (g < a.groups) {
@@ -262,14 +282,14 @@ __device__ inline void build_group_rows(const GroupedArgs& a, const GroupTable& 
       t.used() = tiles;
       tiles *= n.over;
       total *= n.over;
-      // Where every pair takes whole tiles there is work for all.
-      t.shares() = n.each > 0 ? a.pairs : max(1, min(a.pairs, a.whole ? tiles : total / a.min_blocks));
     } else {
       t.tile_base(a.groups) = tiles;
       total = tiles * a.k_blocks;
-      t.shares() = max(1, min(a.pairs, a.whole ? tiles : total / a.min_blocks));
     }
-    const int shares = t.shares();
+    const GroupShares plan(a, tiles, total, deepest, kGrad && GradTiles(a).each > 0);
+    const int shares = plan.shares;
+    t.whole() = plan.whole;
+    t.shares() = shares;
     t.tiles() = tiles;
     t.total() = total;
     t.per_column() = tiles / shares;
@@ -373,7 +393,7 @@ struct GroupWalk {
       : GroupWalk(a, t, line_begin(a, t, pair), line_begin(a, t, pair + 1), min(pair, t.shares() - 1)) {
     if constexpr (MODE == GroupMode::kWeightGrad) {
       if (pair < t.shares()) ahead = t.used() * GradTiles(a).each;
-      if (a.whole) {  // shares of whole tiles
+      if (t.whole()) {  // shares of whole tiles
         const int per = t.per_column(), more = t.tiles() - per * t.shares();
         lo = 0;
         hi = t.total();
@@ -383,7 +403,7 @@ struct GroupWalk {
     }
   }
   __device__ static int line_begin(const GroupedArgs& a, const GroupTable& t, int p) {
-    if (MODE == GroupMode::kWeightGrad && a.whole) return 0;
+    if (MODE == GroupMode::kWeightGrad && t.whole()) return 0;
     return p <= t.shares() ? t.share_begin(p) : t.total();
   }
 
@@ -748,7 +768,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
   uint64_t* mma_done = tmem_empty + 8;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const GroupTable table = {reinterpret_cast<int*>(tmem_slot + 4), args.groups, args.pairs, args.whole};
+  const GroupTable table = {reinterpret_cast<int*>(tmem_slot + 4), args.groups, args.pairs};
 
   const int warp = threadIdx.x >> 5;
   const uint32_t lane = lane_id();
@@ -1199,7 +1219,7 @@ __global__ void __launch_bounds__(kFinishThreads) grouped_finish_kernel(const __
   constexpr int kCols = finish_cols<MODE>();
   __shared__ __align__(128) uint8_t out_stage[group_rows_right(MODE) ? 16 : kFinishThreads / 32 * kStageOutBytes];
   extern __shared__ int finish_table[];
-  const GroupTable table = {finish_table, args.groups, args.pairs, args.whole};
+  const GroupTable table = {finish_table, args.groups, args.pairs};
   if (threadIdx.x < 32) build_group_rows<MODE>(args, table);
   __syncthreads();
   build_group_columns<MODE>(args, table);
@@ -1209,7 +1229,7 @@ __global__ void __launch_bounds__(kFinishThreads) grouped_finish_kernel(const __
   const int rank = static_cast<int>(blockIdx.y);
   GroupSegment s = {};
   int cut = 0;
-  const bool joins = p < table.shares() && table.share_begin(p) < table.total();
+  const bool joins = !table.whole() && p < table.shares() && table.share_begin(p) < table.total();
   if (joins) {
     cut = table.share_begin(p);
     GroupWalk<MODE> walk(args, table, cut, cut + 1, p);

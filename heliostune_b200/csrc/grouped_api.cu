@@ -109,7 +109,8 @@ int64_t max_iterations(const GroupedProblem& p) {
 }
 
 // Iterations a share has at least: below it, joining a tile's pieces costs more than another pair
-// saves.
+// saves (421 rows over 8 groups, 520 x 1000, all three products with every tile cut: 75.5, 71.9, 63.6, 63.2
+// and 73.9 us with 1, 2, 4, 8 and 16).
 constexpr int kMinBlocks = 4;
 
 // K blocks of the deepest tile there can be.
@@ -118,13 +119,27 @@ int64_t deepest_tile(const GroupedProblem& p) {
   return MODE == GroupMode::kWeightGrad ? cdiv(p.rows, 64) : p.k_blocks;
 }
 
-// Shares end at tiles up to this depth (gemm_grouped.cuh, the schedule). Measured either side: at 8 and
-// 16 blocks whole tiles take 3 to 7 us less, at 32 they take up to 4 us more where the tiles fill part
-// of a wave.
+// K blocks a pair may idle before tiles are cut (GroupShares), from both sides measured (us):
+//   forward, 256 wide   1300 x 2560 x 4096, 28 blocks: 30.7 whole, 32.9 cut; 1300 x 4096 x 4096, 45: 43.2 and 43.0
+//   forward, 32 wide    16 x 1536 x 4096, 19: 11.4 and 13.5; 16 x 2560 x 4096, 31: 15.1 and 13.9
+//   weight gradient     2048 rows, 520 x 1000, 27: 21.3 and 26.4; 4096 rows, 54: 34.7 and 28.7
+//   scaled              512 x 4096 x 4096, 18: 22.8 and 28.4; 2048 x 4096 x 9728, 28: 92.3 and 92.7; 257 x 8192 x 12800,
+//                       42: 70.9 and 60.7
+//   scaled, few rows    1 x 2176 x 12800, 6: 11.6 and 14.8; 128 x 4096 x 2816 over 32 groups, 8: 84.6 and 76.6
+// What is cut is written and read as FP32, so that narrow tiles cost less to cut.
+template <GroupMode MODE>
+int idle_limit(const GroupedProblem& p) {
+  if (MODE == GroupMode::kForward) return 24 + 3 * p.width_cap / 32;
+  if (MODE == GroupMode::kWeightGrad) return 40;
+  return MODE == GroupMode::kScaled ? 24 : 7;
+}
+
+// Whether the shares end at tiles whatever the ends are: no tile can be deeper than the limit, or than
+// 16 blocks (1 x 2048 x 12800 and 16 x 2176 x 4096 with few rows: 11 us whole, 13 to 15 cut).
 constexpr int kWholeBlocks = 16;
 template <GroupMode MODE>
 bool whole_tiles(const GroupedProblem& p) {
-  return deepest_tile<MODE>(p) <= kWholeBlocks;
+  return deepest_tile<MODE>(p) <= std::max(kWholeBlocks, idle_limit<MODE>(p));
 }
 
 template <GroupMode MODE>
@@ -152,7 +167,9 @@ template <GroupMode MODE, bool L_MN, typename T>
 int launch_grouped(const GroupedProblem& p, const GroupedMaps& maps, GroupedArgs args, int r_bytes, const DeviceState* dev,
                    void* workspace, cudaStream_t stream) {
   using S = GroupedShape<MODE>;
-  if (max_iterations<MODE>(p) > INT32_MAX) return fail(HST_ERR_UNSUPPORTED, "the grouped product has too many tiles");
+  // The schedule counts iterations, and tiles times pairs, in 32 bits.
+  if (max_iterations<MODE>(p) * (MODE == GroupMode::kWeightGrad ? 1 : cdiv(dev->sm_count / 2, p.k_blocks)) > INT32_MAX)
+    return fail(HST_ERR_UNSUPPORTED, "the grouped product has too many tiles");
   args.groups = p.groups;
   args.rows = static_cast<int>(p.rows);
   args.cols = static_cast<int>(p.cols);
@@ -162,7 +179,12 @@ int launch_grouped(const GroupedProblem& p, const GroupedMaps& maps, GroupedArgs
   args.r_bytes = r_bytes;
   args.pairs = plan_pairs<MODE>(p, dev->sm_count);
   args.min_blocks = kMinBlocks;
+  args.idle_limit = idle_limit<MODE>(p);
   args.whole = whole_tiles<MODE>(p);
+  if (args.ends == nullptr && MODE != GroupMode::kWeightGrad && args.whole == 0) {  // one group: its tiles are known
+    const int tiles = group_row_tiles<MODE>(args, args.rows) * ceil_div(args.cols, 256);
+    args.whole = GroupShares(args, tiles, tiles * args.k_blocks, args.k_blocks, false).whole;
+  }
   args.vec = 32;
   while (args.vec > 2 && (p.cols * 2 % args.vec != 0 || reinterpret_cast<uintptr_t>(args.out) % args.vec != 0)) args.vec /= 2;
   args.status = dev->status;
@@ -270,7 +292,8 @@ GroupedProblem forward_problem(int64_t rows, int groups, int64_t n, int64_t k) {
 GroupedProblem grad_problem(int64_t rows, int groups, int64_t lcols, int64_t rcols) {
   return GroupedProblem{rows, groups, rcols, lcols, 0, 256};
 }
-// Up to 64 rows a group on average the rows go on the R side (kScaledFew).
+// Up to 64 rows a group on average the rows go on the R side (kScaledFew; K = 4096, N = 12800: 64 rows 25.4 us
+// there and 28.9 on the L side, 96 rows 35.0 and 30.9).
 bool scaled_few(int64_t rows, int groups) { return rows <= int64_t(64) * groups; }
 GroupedProblem scaled_problem(int64_t rows, int groups, int64_t n, int64_t k) {
   return GroupedProblem{rows, groups, n, 0, cdiv(k, 128), scaled_few(rows, groups) ? width_cap(rows, 64) : 256};

@@ -211,7 +211,7 @@ def test_quantisers_take_any_strides_and_stacks() -> None:
 @gpu
 @pytest.mark.parametrize("out_dtype", DTYPES)
 @pytest.mark.parametrize("rows", (1, 2, 31, 33, 64, 65, 127, 128, 200, 256, 257, 600))
-@pytest.mark.parametrize("n,k", ((128, 128), (136, 264), (520, 1040), (72, 4096), (1000, 16)))
+@pytest.mark.parametrize("n,k", ((128, 128), (136, 264), (520, 1040), (72, 4096), (1000, 16), (201, 4368)))
 def test_dense(out_dtype: torch.dtype, rows: int, n: int, k: int) -> None:
     a, sa, b, sb = _operands(rows, n, k, seed=rows + n + k)
     y = blockscale.matmul_blockscaled(a, sa, b, sb, out_dtype=out_dtype)
@@ -241,7 +241,7 @@ def test_extents_and_strides_that_tma_cannot_read(rows: int, n: int, k: int) -> 
     "rows,ends",
     ((1, [0, 1]), (9, [3, 3, 8]), (96, [40, 41, 96]), (300, [0, 255, 255, 300]), (700, [256, 513, 700]), (40, [0, 0, 0]), (1111, [600, 600, 1100])),
 )
-@pytest.mark.parametrize("n,k", ((136, 264), (520, 1040), (264, 2192)))  # 2192: more than 16 K blocks, tiles are cut
+@pytest.mark.parametrize("n,k", ((136, 264), (520, 1040), (264, 2192), (264, 4368)))  # the last: tiles are cut
 def test_grouped(rows: int, ends: list[int], n: int, k: int) -> None:
     a, sa, b, sb = _operands(rows, n, k, seed=rows + n, groups=len(ends))
     y = blockscale.matmul_blockscaled(a, sa, b, sb, _ends(ends), out_dtype=torch.float16)

@@ -147,7 +147,7 @@ ROWS = (
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("layout", ("kn", "nk"))
 @pytest.mark.parametrize("rows,ends", ROWS)
-@pytest.mark.parametrize("k,n", ((64, 256), (200, 264), (1000, 72), (1096, 264)))  # 1096: more than 16 K blocks, tiles are cut
+@pytest.mark.parametrize("k,n", ((64, 256), (200, 264), (1000, 72), (1096, 264)))
 def test_forward_and_gradients(dtype: torch.dtype, layout: str, rows: int, ends: list[int], k: int, n: int) -> None:
     x, w, dy = _operands(rows, len(ends), k, n, dtype, layout, seed=rows + k)
     x.requires_grad_()
@@ -183,6 +183,44 @@ def test_long_sums_and_many_tiles_are_joined_across_pairs() -> None:
     x, w, dy = _operands(9001, 3, 136, 520, torch.float16, "nk", seed=4)
     _check_weight_grad(grouped.grouped_weight_grad(x, dy, _ends(ends)), x, dy, ends)
     _check_forward(grouped.grouped_matmul(x, w, _ends(ends)), x, w, ends)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ("kn", "nk"))
+@pytest.mark.parametrize("rows,ends", ((1, [0, 1]), (70, [33, 33, 70]), (300, [0, 255, 255, 290]), (700, [256, 513, 700]), (40, [0, 0])))
+@pytest.mark.parametrize("n", (264, 72, 1001))
+def test_deep_tiles_are_cut_and_joined(dtype: torch.dtype, layout: str, rows: int, ends: list[int], n: int) -> None:
+    x, w, _ = _operands(rows, len(ends), 4176, n, dtype, layout, seed=rows + n)
+    _check_forward(grouped.grouped_matmul(x, w, _ends(ends)), x, w, ends)
+
+
+@gpu
+@pytest.mark.parametrize("ends", ([4600, 4600, 4650], [0, 3100, 6100, 6101], [6200]))
+@pytest.mark.parametrize("k,n", ((200, 264), (301, 77), (72, 1000)))
+def test_deep_weight_gradients_are_cut_and_joined(ends: list[int], k: int, n: int) -> None:
+    x, _, dy = _operands(6200, 1, k, n, torch.bfloat16, "kn", seed=k)
+    _check_weight_grad(grouped.grouped_weight_grad(x, dy, _ends(ends)), x, dy, ends)
+
+
+@gpu
+def test_a_replay_cuts_tiles_where_its_ends_ask_for_it() -> None:
+    # 66 K blocks, 19 column tiles: of two groups 38 tiles (whole), of one 19 (cut: a pair would idle for 49 blocks).
+    x, w, _ = _operands(300, 3, 4168, 4736, torch.bfloat16, "kn", seed=23)
+    ends = _ends([0, 0, 0])
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        grouped.grouped_matmul(x, w, ends)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        y = grouped.grouped_matmul(x, w, ends)
+    for values in ([200, 200, 300], [0, 1, 1], [100, 200, 300], [0, 0, 0], [0, 256, 256]):
+        ends.copy_(_ends(values))
+        graph.replay()
+        torch.cuda.synchronize()
+        _check_forward(y, x, w, values)
+        assert torch.equal(y, grouped.grouped_matmul(x, w, ends))
 
 
 @gpu
@@ -385,7 +423,7 @@ def test_two_streams_at_once() -> None:
 
 
 @gpu
-@pytest.mark.parametrize("k", (264, 1544))
+@pytest.mark.parametrize("k", (264, 4168))
 def test_captured_steps_follow_new_ends_and_inputs(k: int) -> None:
     """Two graphs of a training step, replayed in turn with other ends and inputs than they were captured with."""
     x, w, dy = _operands(300, 3, k, 200, torch.float16, "kn", seed=16)
@@ -432,24 +470,24 @@ def test_outputs_past_32_bit_offsets() -> None:
 
 @gpu
 def test_the_workspace_is_checked_and_its_contents_do_not_matter() -> None:
-    x, w, dy = _operands(120, 2, 2056, 264, torch.float16, "kn", seed=17)
+    x, w, dy = _operands(120, 2, 4104, 264, torch.float16, "kn", seed=17)
     ends = _ends([50, 120])
     lib = _native.library()
     y = torch.empty((120, 264), device="cuda", dtype=torch.float16)
 
     def needed(k: int) -> int:
         size = ctypes.c_size_t(1)
-        assert lib.hst_grouped_matmul_workspace(16, 2056, 1, 16, 2056 * 264, 264, 1, 2, 120, 264, k, 0, ctypes.byref(size)) == 0
+        assert lib.hst_grouped_matmul_workspace(16, 4104, 1, 16, 4104 * 264, 264, 1, 2, 120, 264, k, 0, ctypes.byref(size)) == 0
         return size.value
 
     def call(workspace: torch.Tensor) -> int:
         return lib.hst_grouped_matmul(
-            0, x.data_ptr(), 2056, 1, w.data_ptr(), 2056 * 264, 264, 1, ends.data_ptr(), 2, y.data_ptr(), 120, 264, 2056,
+            0, x.data_ptr(), 4104, 1, w.data_ptr(), 4104 * 264, 264, 1, ends.data_ptr(), 2, y.data_ptr(), 120, 264, 4104,
             workspace.data_ptr(), workspace.numel(), torch.cuda.current_stream().cuda_stream,
         )  # fmt: skip
 
     assert needed(520) == 0
-    size = needed(2056)
+    size = needed(4104)
     assert call(torch.empty(size - 1, device="cuda", dtype=torch.uint8)) == _native.HST_ERR_WORKSPACE
     for fill in (0, 255):
         assert call(torch.full((size,), fill, device="cuda", dtype=torch.uint8)) == _native.HST_OK
