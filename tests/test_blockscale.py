@@ -9,6 +9,8 @@ output by ``eps / 2``.
 
 from __future__ import annotations
 
+from concurrent.futures import ThreadPoolExecutor
+
 import pytest
 import torch
 
@@ -102,6 +104,12 @@ def test_inputs_are_checked_before_any_cuda_work() -> None:
 
 
 def test_the_library_refuses_bad_calls_before_any_cuda_work() -> None:
+    # In a thread of its own: the library keeps the last error of each.
+    with ThreadPoolExecutor(1) as thread:
+        thread.submit(_refused_calls).result()
+
+
+def _refused_calls() -> None:
     _native.build_library()
     lib = _native.library()
 
