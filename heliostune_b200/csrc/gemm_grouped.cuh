@@ -1261,12 +1261,12 @@ __global__ void __launch_bounds__(kFinishThreads) grouped_finish_kernel(const __
                           (static_cast<int64_t>(c / 4) * 128 + row) * 4;
       for (int o = p - 1; mine && o <= last; o += kBatch) {
         float4 f[kBatch][kCols / 4];
-        auto add = [&](int i, int j) {
+        auto add = [&](const float4& g, int j) {
           float* sum = &v[j / 8][4 * (j % 8)];
-          sum[0] += f[i][j].x;
-          sum[1] += f[i][j].y;
-          sum[2] += f[i][j].z;
-          sum[3] += f[i][j].w;
+          sum[0] += g.x;
+          sum[1] += g.y;
+          sum[2] += g.z;
+          sum[3] += g.w;
         };
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
@@ -1275,7 +1275,7 @@ __global__ void __launch_bounds__(kFinishThreads) grouped_finish_kernel(const __
             for (int j = 0; j < kCols / 4; ++j) {
               if (c + 4 * j < live_cols) {
                 f[i][j] = *reinterpret_cast<const float4*>(src + j * 512);
-                if (kBatch == 1) add(i, j);
+                if (kBatch == 1) add(f[i][j], j);
               }
             }
             src = next;
@@ -1288,7 +1288,7 @@ __global__ void __launch_bounds__(kFinishThreads) grouped_finish_kernel(const __
             if (o + i <= last) {
 #pragma unroll
               for (int j = 0; j < kCols / 4; ++j) {
-                if (c + 4 * j < live_cols) add(i, j);
+                if (c + 4 * j < live_cols) add(f[i][j], j);
               }
             }
           }
