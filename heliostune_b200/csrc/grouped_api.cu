@@ -36,6 +36,13 @@ int check_extents(const char* what, int64_t a, int64_t b) {
   return HST_OK;
 }
 
+// Whether a pointer starts on a multiple of its values' size; what does not would fault on the GPU.
+int check_aligned(const char* name, const void* ptr, int bytes) {
+  if (reinterpret_cast<uintptr_t>(ptr) % bytes != 0)
+    return fail(HST_ERR_INVALID, "%s must be aligned to %d bytes", name, bytes);
+  return HST_OK;
+}
+
 // A stack of matrices [groups, rows, cols] with strides in values.
 struct Stack {
   const void* ptr;
@@ -336,6 +343,10 @@ int hst_grouped_matmul(int32_t dtype, const void* x, int64_t x_row, int64_t x_co
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (k == 0) return zero_output(y, rows * n, s);
   if (x == nullptr || w == nullptr) return fail(HST_ERR_INVALID, "x or w is null");
+  HST_TRY(check_aligned("x", x, 2));
+  HST_TRY(check_aligned("w", w, 2));
+  HST_TRY(check_aligned("ends", ends, 4));
+  HST_TRY(check_aligned("y", y, 2));
   DeviceState* dev = nullptr;
   HST_TRY(device_state(&dev));
   const GroupedProblem p = forward_problem(rows, groups, n, k);
@@ -387,6 +398,10 @@ int hst_grouped_weight_grad(int32_t dtype, const void* left, int64_t l_row, int6
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (rows == 0) return zero_output(out, lcols * rcols * groups, s);
   if (left == nullptr || right == nullptr) return fail(HST_ERR_INVALID, "left or right is null");
+  HST_TRY(check_aligned("left", left, 2));
+  HST_TRY(check_aligned("right", right, 2));
+  HST_TRY(check_aligned("ends", ends, 4));
+  HST_TRY(check_aligned("out", out, 2));
   DeviceState* dev = nullptr;
   HST_TRY(device_state(&dev));
   const GroupedProblem p = grad_problem(rows, groups, lcols, rcols);
@@ -431,6 +446,10 @@ int hst_matmul_blockscaled(int32_t out_dtype, const void* a, int64_t a_row, int6
   if (k == 0) return zero_output(y, rows * n, s);
   if (a == nullptr || b == nullptr) return fail(HST_ERR_INVALID, "a or b is null");
   if (a_scales == nullptr || b_scales == nullptr) return fail(HST_ERR_INVALID, "scales are null");
+  HST_TRY(check_aligned("a_scales", a_scales, 4));
+  HST_TRY(check_aligned("b_scales", b_scales, 4));
+  HST_TRY(check_aligned("ends", ends, 4));
+  HST_TRY(check_aligned("y", y, 2));
   DeviceState* dev = nullptr;
   HST_TRY(device_state(&dev));
   const GroupedProblem p = scaled_problem(rows, groups, n, k);
@@ -473,6 +492,8 @@ int hst_quantize_e4m3(int32_t dtype, int32_t tiles, const void* x, int64_t x_bat
   if (!tiles && batch > 1) return fail(HST_ERR_INVALID, "row scales are for one matrix");
   if (rows == 0 || cols == 0 || batch == 0) return HST_OK;
   if (x == nullptr || q == nullptr || scales == nullptr) return fail(HST_ERR_INVALID, "null pointer");
+  HST_TRY(check_aligned("x", x, 2));
+  HST_TRY(check_aligned("scales", scales, 4));
   if (q_row < cols) return fail(HST_ERR_INVALID, "q's rows are shorter than its columns");
   const int64_t col_blocks = cdiv(cols, 128), row_blocks = cdiv(rows, 128);
   if (rows * col_blocks > INT32_MAX || (tiles && row_blocks > 65535))

@@ -193,7 +193,8 @@ int hst_gated_mlp_stream(int32_t block_m, int32_t block_k, int32_t num_stages, i
  * FP32 accumulation, one rounding, bitwise reproducible. The caller gives a 16-byte aligned workspace
  * of the bytes that the function's _workspace form reports for the same operands (inspected for
  * alignment only; 0 for shallow products of aligned operands; no initialisation needed). Calls that
- * share one must not overlap on the GPU. The launches, all on the stream, can be captured. */
+ * share one must not overlap on the GPU. The launches, all on the stream, can be captured. Every
+ * pointer is a multiple of its values' size. */
 
 /* y[t, :] = x[t, :] W[g(t)]: x [rows, k], w [groups, k, n] (w_k and w_n the strides of its inner
  * dimensions: [groups, n, k] storage is read in place too), y [rows, n], all of `dtype`. The input

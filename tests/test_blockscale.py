@@ -127,6 +127,10 @@ def _refused_calls() -> None:
         ({"b": None}, b"a or b is null"),
         ({"sa": None}, b"scales"),
         ({"y": None}, b"y is null"),
+        ({"sa": 18}, b"a_scales must be aligned to 4"),
+        ({"sb": 18}, b"b_scales must be aligned to 4"),
+        ({"ends": 18}, b"ends must be aligned to 4"),
+        ({"y": 17}, b"y must be aligned to 2"),
     ):
         assert scaled(**kwargs) == _native.HST_ERR_INVALID, kwargs
         assert message in lib.hst_last_error(), kwargs
@@ -141,6 +145,8 @@ def _refused_calls() -> None:
         ({"tiles": 1, "batch": 65536}, b"65535"),
         ({"x": None}, b"null"),
         ({"q_row": 127}, b"shorter"),
+        ({"x": 17}, b"x must be aligned to 2"),
+        ({"s": 18}, b"scales must be aligned to 4"),
     ):
         assert quantize(**kwargs) == _native.HST_ERR_INVALID, kwargs
         assert message in lib.hst_last_error(), kwargs

@@ -122,12 +122,18 @@ def _refused_calls() -> None:
         ({"y": None}, b"y is null"),
         ({"x": None}, b"x or w is null"),
         ({"w": None}, b"x or w is null"),
+        ({"x": 17}, b"x must be aligned to 2"),
+        ({"w": 17}, b"w must be aligned to 2"),
+        ({"y": 17}, b"y must be aligned to 2"),
+        ({"ends": 18}, b"ends must be aligned to 4"),
     ):
         assert matmul(**kwargs) == _native.HST_ERR_INVALID, kwargs
         assert message in lib.hst_last_error(), kwargs
     assert matmul(rows=0) == _native.HST_OK
     assert lib.hst_grouped_weight_grad(0, None, 8, 1, 16, 8, 1, 16, 2, 16, 4, 8, 8, None, 0, None) == _native.HST_ERR_INVALID
     assert b"left or right is null" in lib.hst_last_error()
+    assert lib.hst_grouped_weight_grad(0, 17, 8, 1, 16, 8, 1, 16, 2, 16, 4, 8, 8, None, 0, None) == _native.HST_ERR_INVALID
+    assert b"left must be aligned" in lib.hst_last_error()
     assert lib.hst_grouped_weight_grad(3, 16, 8, 1, 16, 8, 1, 16, 2, 16, 4, 8, 8, None, 0, None) == _native.HST_ERR_INVALID
 
 
