@@ -47,22 +47,23 @@ def _quantize(x: torch.Tensor, tiles: bool) -> tuple[torch.Tensor, torch.Tensor]
     device = x.device
     # Rows of q start on 16 bytes, so that the products read them in place.
     width = -(-cols // 16) * 16
-    q = torch.empty((*batch, rows, width), device=device, dtype=torch.float8_e4m3fn)
+    q = x.new_empty((*batch, rows, width), dtype=torch.float8_e4m3fn)
     if width != cols:
         q = q[..., :cols]
+    blocks = _blocks(cols)
+    s_batch, s_row, s_col = _blocks(rows) * blocks, blocks, 1
     if tiles:
-        scales = torch.empty((*batch, _blocks(rows), _blocks(cols)), device=device, dtype=torch.float32)
+        scales = x.new_empty((*batch, _blocks(rows), blocks), dtype=torch.float32)
     else:
         # Stored [blocks, rows]: the products read one block's scales of neighbouring rows together.
-        scales = torch.empty((_blocks(cols), rows), device=device, dtype=torch.float32).T
+        s_row, s_col = 1, rows
+        scales = x.new_empty_strided((rows, blocks), (s_row, s_col), dtype=torch.float32)
     *x_batch, x_row, x_col = x.stride()
-    *q_batch, q_row, _ = q.stride()
-    *s_batch, s_row, s_col = scales.stride()
-    count, lead = (batch[0], (x_batch[0], q_batch[0], s_batch[0])) if batch else (1, (0, 0, 0))
+    count, lead = (batch[0], (x_batch[0], rows * width, s_batch)) if batch else (1, (0, 0, 0))
     with _device_guard(device):
         _native.check(
             _native.library().hst_quantize_e4m3(
-                _DTYPES[x.dtype], tiles, x.data_ptr(), lead[0], x_row, x_col, q.data_ptr(), lead[1], q_row,
+                _DTYPES[x.dtype], tiles, x.data_ptr(), lead[0], x_row, x_col, q.data_ptr(), lead[1], width,
                 scales.data_ptr(), lead[2], s_row, s_col, count, rows, cols, _stream(device),
             )
         )  # fmt: skip
@@ -136,7 +137,7 @@ def matmul_blockscaled(
     _check_scales("a_scales", a_scales, (rows, _blocks(k)), index)
     _check_scales("b_scales", b_scales, (*lead, _blocks(n), _blocks(k)), index)
     _refuse_gradient("matmul_blockscaled", a, a_scales, b, b_scales)
-    y = torch.empty((rows, n), device=device, dtype=out_dtype)
+    y = a.new_empty((rows, n), dtype=out_dtype)
     a_pointer, a_strides, b_pointer = a.data_ptr(), a.stride(), b.data_ptr()
     b_strides = b.stride() if lead else (0, *b.stride())
     sb_strides = b_scales.stride() if lead else (0, *b_scales.stride())

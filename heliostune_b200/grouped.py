@@ -79,7 +79,7 @@ def _check_operands(what: str, x: torch.Tensor, other: torch.Tensor, names: tupl
 def _forward(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tensor) -> torch.Tensor:
     groups, k, n = weight.shape
     rows, device = x.shape[0], x.device
-    y = torch.empty((rows, n), device=device, dtype=x.dtype)
+    y = x.new_empty((rows, n))
     x_pointer, x_strides, w_pointer, w_strides = x.data_ptr(), x.stride(), weight.data_ptr(), weight.stride()
     workspace, ws_pointer, ws_bytes = _workspace(
         "hst_grouped_matmul", device, (x_pointer & 15, *x_strides, w_pointer & 15, *w_strides, groups, rows, n, k)
@@ -98,7 +98,7 @@ def _forward(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tensor) ->
 def _weight_grad(left: torch.Tensor, right: torch.Tensor, group_ends: torch.Tensor) -> torch.Tensor:
     groups = group_ends.shape[0]
     (rows, lcols), rcols, device = left.shape, right.shape[1], left.device
-    out = torch.empty((groups, lcols, rcols), device=device, dtype=left.dtype)
+    out = left.new_empty((groups, lcols, rcols))
     l_pointer, l_strides, r_pointer, r_strides = left.data_ptr(), left.stride(), right.data_ptr(), right.stride()
     workspace, ws_pointer, ws_bytes = _workspace(
         "hst_grouped_weight_grad",
