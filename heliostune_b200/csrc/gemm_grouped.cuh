@@ -128,10 +128,11 @@ __host__ __device__ inline int group_blocks(const GroupedArgs& a, int rows) {
 // kForward and the scaled products (every tile has the same K blocks): the tiles are dealt to `shares`
 // columns like cards (tile t * shares + c is number t of column c; the last, part-filled row is spread
 // evenly over the columns), the columns are put end to end into one line of (tile, K block)
-// iterations, and the line is cut into equal shares. Share c then runs along column c, give or take a
-// part of a tile, so at any moment the pairs work on neighbouring tiles: with contiguous runs of the
-// group-by-group order instead, the 74 weight panels in use passed L2's size (8194 x 14336 x 4096 over
-// 8 groups: 1007 us against 811, before the steps that followed).
+// iterations, and the line is cut into equal shares (or every pair takes its column, GroupShares). Share
+// c then runs along column c, give or take a part of a tile, so at any moment the pairs work on
+// neighbouring tiles: with contiguous runs of the group-by-group order instead, the 74 weight panels in
+// use passed L2's size (8194 x 14336 x 4096 over 8 groups: 1007 us against 811, before the steps that
+// followed).
 //
 // kWeightGrad (K blocks by group, the same number of tiles in each): of every group with rows, each
 // pair takes its tiles / pairs whole tiles, all pairs at the same group at the same time; what remains

@@ -142,7 +142,7 @@ int idle_limit(const GroupedProblem& p) {
 }
 
 // Whether the shares end at tiles whatever the ends are: no tile can be deeper than the limit, or than
-// 16 blocks (1 x 2048 x 12800 and 16 x 2176 x 4096 with few rows: 11 us whole, 13 to 15 cut).
+// 16 blocks (at 17, few rows in 8 bits: 1 x 2176 x 12800 11.6 us whole and 14.8 cut, 16 x 2176 x 4096 11.5 and 13.5).
 constexpr int kWholeBlocks = 16;
 template <GroupMode MODE>
 bool whole_tiles(const GroupedProblem& p) {
