@@ -1247,7 +1247,7 @@ class CpuBaseline:
         )
         shapes = len(self.workloads)
         return {
-            "value": round(flops / seconds / 1e12, 4),
+            "value": float(f"{flops / seconds / 1e12:.6g}"),  # digits, not decimals: tiny shapes on a busy host are under 1e-4
             "unit": "TFLOP/s",
             "cores": torch.get_num_threads(),
             "os_cpu_count": os.cpu_count(),
