@@ -20,7 +20,7 @@ from __future__ import annotations
 import torch
 
 from heliostune_b200 import _native
-from heliostune_b200.grouped import _DTYPES, MAX_GROUPS, _check_ends, _workspace
+from heliostune_b200.grouped import _DTYPES, MAX_GROUPS, _check_ends, _refuse_tangents, _workspace
 from heliostune_b200.kernel import _device_guard, _stream
 
 #: Values that share a scale along a row (and, for tiles, along a column).
@@ -34,15 +34,16 @@ def _blocks(extent: int) -> int:
 def _refuse_gradient(what: str, *tensors: torch.Tensor) -> None:
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise ValueError(f"{what} has no gradient; detach its inputs or run it under torch.no_grad()")
+    _refuse_tangents(what, *tensors)
 
 
 def _quantize(x: torch.Tensor, tiles: bool) -> tuple[torch.Tensor, torch.Tensor]:
     what = "quantize_tiles" if tiles else "quantize_rows"
+    _refuse_gradient(what, x)
     if not x.is_cuda:
         raise ValueError(f"{what} expects a CUDA tensor")
     if x.dtype not in _DTYPES:
         raise ValueError(f"{what} serves torch.float16 or torch.bfloat16, got {x.dtype}")
-    _refuse_gradient(what, x)
     *batch, rows, cols = x.shape
     device = x.device
     # Rows of q start on 16 bytes, so that the products read them in place.
@@ -112,6 +113,7 @@ def matmul_blockscaled(
     ``b_scales [ceil(N / 128), ceil(K / 128)]`` FP32 with any strides; ``y [T, N]`` is ``out_dtype`` (FP16 or
     BF16). With ``group_ends [E]``, ``b`` is ``[E, N, K]``, ``b_scales [E, ...]``, and each row of ``a`` meets
     its expert's weight; rows past the last end are zero."""
+    _refuse_gradient("matmul_blockscaled", a, a_scales, b, b_scales)
     if a.ndim != 2 or b.ndim != (2 if group_ends is None else 3):
         raise ValueError("matmul_blockscaled expects a [T, K] and b [N, K], or b [E, N, K] with group_ends [E]")
     if a.shape[1] != b.shape[-1]:
@@ -136,7 +138,6 @@ def matmul_blockscaled(
         ends = group_ends.data_ptr()
     _check_scales("a_scales", a_scales, (rows, _blocks(k)), index)
     _check_scales("b_scales", b_scales, (*lead, _blocks(n), _blocks(k)), index)
-    _refuse_gradient("matmul_blockscaled", a, a_scales, b, b_scales)
     y = a.new_empty((rows, n), dtype=out_dtype)
     a_pointer, a_strides, b_pointer = a.data_ptr(), a.stride(), b.data_ptr()
     b_strides = b.stride() if lead else (0, *b.stride())

@@ -26,6 +26,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from heliostune_b200 import _native
@@ -56,6 +57,12 @@ def _workspace(
         return None, None, 0
     buffer = torch.empty(nbytes, device=device, dtype=torch.uint8)
     return buffer, buffer.data_ptr(), nbytes
+
+
+def _refuse_tangents(what: str, *tensors: torch.Tensor) -> None:
+    """Refuses operands with a forward-mode gradient: the result would come without one, and without an error."""
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError(f"{what} has no forward-mode gradient; take its operands' primals")
 
 
 def _check_ends(group_ends: torch.Tensor, groups: int, device: int) -> None:
@@ -120,6 +127,7 @@ def grouped_weight_grad(x: torch.Tensor, dy: torch.Tensor, group_ends: torch.Ten
     """``out[e] = x[rows of e].T @ dy[rows of e]``, ``[E, K, N]``: the weight gradient of
     :func:`grouped_matmul`, with FP32 sums over the rows and one rounding. ``x [T, K]`` and ``dy [T, N]``
     are FP16 or BF16 with any strides (copied once where their rows are not 16-byte aligned)."""
+    _refuse_tangents("grouped_weight_grad", x, dy)
     if x.ndim != 2 or dy.ndim != 2 or x.shape[0] != dy.shape[0]:
         raise ValueError(f"grouped_weight_grad expects x [T, K] and dy [T, N], got {tuple(x.shape)} and {tuple(dy.shape)}")
     _check_operands("grouped_weight_grad", x, dy, ("x", "dy"))
@@ -161,7 +169,8 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tens
     """``y[t] = x[t] @ weight[e(t)]`` with FP32 accumulation: ``x [T, K]``, ``weight [E, K, N]`` (either of
     its last two dimensions contiguous), both FP16 or both BF16, ``y [T, N]`` of their type; 1 to
     :data:`MAX_GROUPS` experts. Any strides are served; operands whose rows are not 16-byte aligned
-    are copied once. Differentiable in ``x`` and ``weight`` (once)."""
+    are copied once. Differentiable in ``x`` and ``weight`` (once, in reverse mode)."""
+    _refuse_tangents("grouped_matmul", x, weight)
     if x.ndim != 2 or weight.ndim != 3:
         raise ValueError("grouped_matmul expects x [T, K] and weight [E, K, N]")
     if x.shape[1] != weight.shape[1]:

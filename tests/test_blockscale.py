@@ -13,6 +13,7 @@ from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from heliostune_b200 import _native, blockscale, grouped
 from tests.test_grouped import _bounds, _ends
@@ -101,6 +102,19 @@ def test_inputs_are_checked_before_any_cuda_work() -> None:
         blockscale.quantize_rows(s)
     with pytest.raises(ValueError, match=r"weight \[N, K\]"):
         blockscale.quantize_tiles(s[0])
+
+
+def test_operands_with_a_forward_gradient_are_refused() -> None:
+    a = torch.zeros((4, 128), dtype=torch.float8_e4m3fn)
+    s = torch.zeros((4, 1))
+    x = torch.zeros((4, 128), dtype=torch.float16)
+    with forward_ad.dual_level():
+        for quantize in (blockscale.quantize_rows, blockscale.quantize_tiles):
+            with torch.no_grad(), pytest.raises(ValueError, match="no forward-mode gradient"):
+                quantize(forward_ad.make_dual(x, x))
+        for args in ((a, forward_ad.make_dual(s, s), a, s[:1]), (a, s, a, forward_ad.make_dual(s, s)[:1])):
+            with pytest.raises(ValueError, match="no forward-mode gradient"):
+                blockscale.matmul_blockscaled(*args)
 
 
 def test_the_library_refuses_bad_calls_before_any_cuda_work() -> None:

@@ -14,6 +14,7 @@ from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from heliostune_b200 import _native, grouped
 
@@ -96,6 +97,37 @@ def test_inputs_are_checked_before_any_cuda_work() -> None:
         grouped.grouped_weight_grad(x, x[:3], ends)
     with pytest.raises(ValueError, match="same CUDA device"):
         grouped.grouped_weight_grad(x, x, ends)
+
+
+def test_operands_with_a_forward_gradient_are_refused() -> None:
+    """A dual tensor does not require grad: its tangent would be lost without an error."""
+    x = torch.zeros((4, 16), dtype=torch.float16)
+    w = torch.zeros((2, 16, 8), dtype=torch.float16)
+    ends = torch.zeros(2, dtype=torch.int32)
+    with forward_ad.dual_level():
+        for args in ((forward_ad.make_dual(x, x), w), (x, forward_ad.make_dual(w, w))):
+            with pytest.raises(ValueError, match="grouped_matmul has no forward-mode gradient"):
+                grouped.grouped_matmul(*args, ends)
+        with pytest.raises(ValueError, match="grouped_weight_grad has no forward-mode gradient"):
+            grouped.grouped_weight_grad(x, forward_ad.make_dual(x, x), ends)
+        with pytest.raises(ValueError, match="same CUDA device"):  # as before
+            grouped.grouped_matmul(x, w, ends)
+
+
+@gpu
+def test_a_forward_gradient_is_refused_on_the_gpu_and_its_primal_taken() -> None:
+    x, w, dy = _operands(9, 2, 32, 16, torch.float16, "kn", seed=31)
+    ends = _ends([4, 9])
+    expected = grouped.grouped_matmul(x, w, ends)
+    with forward_ad.dual_level():
+        for grad in (torch.no_grad(), torch.enable_grad()):
+            with grad:
+                for args in ((forward_ad.make_dual(x, x), w), (x, forward_ad.make_dual(w, w))):
+                    with pytest.raises(ValueError, match="forward-mode"):
+                        grouped.grouped_matmul(*args, ends)
+        assert torch.equal(grouped.grouped_matmul(forward_ad.unpack_dual(forward_ad.make_dual(x, x)).primal, w, ends), expected)
+        with pytest.raises(ValueError, match="forward-mode"):
+            grouped.grouped_weight_grad(forward_ad.make_dual(x, x), dy, ends)
 
 
 def test_the_library_refuses_bad_calls_before_any_cuda_work() -> None:
