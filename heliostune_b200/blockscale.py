@@ -20,7 +20,9 @@ from __future__ import annotations
 import torch
 
 from heliostune_b200 import _native
-from heliostune_b200.grouped import _DTYPES, MAX_GROUPS, _check_ends, _refuse_tangents, _workspace
+from heliostune_b200.grouped import (
+    _DTYPES, MAX_GROUPS, _check_ends, _operator, _refuse_gradient, _workspace,
+)  # fmt: skip
 from heliostune_b200.kernel import _device_guard, _stream
 
 #: Values that share a scale along a row (and, for tiles, along a column).
@@ -31,34 +33,36 @@ def _blocks(extent: int) -> int:
     return -(-extent // BLOCK)
 
 
-def _refuse_gradient(what: str, *tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise ValueError(f"{what} has no gradient; detach its inputs or run it under torch.no_grad()")
-    _refuse_tangents(what, *tensors)
-
-
-def _quantize(x: torch.Tensor, tiles: bool) -> tuple[torch.Tensor, torch.Tensor]:
-    what = "quantize_tiles" if tiles else "quantize_rows"
-    _refuse_gradient(what, x)
+def _outputs(what: str, x: torch.Tensor, tiles: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    """Checks ``x`` and allocates its values and scales."""
+    if tiles and x.ndim not in (2, 3):
+        raise ValueError("quantize_tiles expects weight [N, K] or [E, N, K]")
+    if not tiles and x.ndim != 2:
+        raise ValueError("quantize_rows expects x [T, K]")
     if not x.is_cuda:
         raise ValueError(f"{what} expects a CUDA tensor")
     if x.dtype not in _DTYPES:
         raise ValueError(f"{what} serves torch.float16 or torch.bfloat16, got {x.dtype}")
     *batch, rows, cols = x.shape
-    device = x.device
     # Rows of q start on 16 bytes, so that the products read them in place.
     width = -(-cols // 16) * 16
     q = x.new_empty((*batch, rows, width), dtype=torch.float8_e4m3fn)
     if width != cols:
         q = q[..., :cols]
-    blocks = _blocks(cols)
-    s_batch, s_row, s_col = _blocks(rows) * blocks, blocks, 1
     if tiles:
-        scales = x.new_empty((*batch, _blocks(rows), blocks), dtype=torch.float32)
-    else:
-        # Stored [blocks, rows]: the products read one block's scales of neighbouring rows together.
-        s_row, s_col = 1, rows
-        scales = x.new_empty_strided((rows, blocks), (s_row, s_col), dtype=torch.float32)
+        return q, x.new_empty((*batch, _blocks(rows), _blocks(cols)), dtype=torch.float32)
+    # Stored [blocks, rows]: the products read one block's scales of neighbouring rows together.
+    return q, x.new_empty_strided((rows, _blocks(cols)), (1, rows), dtype=torch.float32)
+
+
+def _quantize(what: str, x: torch.Tensor, tiles: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    _refuse_gradient(what, x)
+    q, scales = _outputs(what, x, tiles)
+    *batch, rows, cols = x.shape
+    device = x.device
+    width = -(-cols // 16) * 16
+    blocks = _blocks(cols)
+    s_batch, s_row, s_col = (_blocks(rows) * blocks, blocks, 1) if tiles else (0, 1, rows)
     *x_batch, x_row, x_col = x.stride()
     count, lead = (batch[0], (x_batch[0], rows * width, s_batch)) if batch else (1, (0, 0, 0))
     with _device_guard(device):
@@ -71,22 +75,30 @@ def _quantize(x: torch.Tensor, tiles: bool) -> tuple[torch.Tensor, torch.Tensor]
     return q, scales
 
 
+_quantize_rows = _operator(
+    "quantize_rows(Tensor x) -> (Tensor, Tensor)",
+    lambda x: _quantize("quantize_rows", x, False),
+    lambda x: _outputs("quantize_rows", x, False),
+)
+_quantize_tiles = _operator(
+    "quantize_tiles(Tensor weight) -> (Tensor, Tensor)",
+    lambda weight: _quantize("quantize_tiles", weight, True),
+    lambda weight: _outputs("quantize_tiles", weight, True),
+)
+
+
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """``(q, scales)`` of ``x [T, K]`` (FP16 or BF16, any strides): ``q [T, K]`` in ``torch.float8_e4m3fn``
     and FP32 ``scales [T, ceil(K / 128)]``, one for each 128 consecutive values of a row. The scales are
     the transposed view of ``[blocks, T]`` storage."""
-    if x.ndim != 2:
-        raise ValueError("quantize_rows expects x [T, K]")
-    return _quantize(x, False)
+    return _quantize_rows(x)
 
 
 def quantize_tiles(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """``(q, scales)`` of ``weight [N, K]`` or ``[E, N, K]`` (FP16 or BF16, any strides): ``q`` of its shape
     in ``torch.float8_e4m3fn`` and FP32 ``scales [..., ceil(N / 128), ceil(K / 128)]``, one for each
     128 x 128 tile."""
-    if weight.ndim not in (2, 3):
-        raise ValueError("quantize_tiles expects weight [N, K] or [E, N, K]")
-    return _quantize(weight, True)
+    return _quantize_tiles(weight)
 
 
 def _check_scales(name: str, scales: torch.Tensor, shape: tuple[int, ...], device: int) -> None:
@@ -96,6 +108,89 @@ def _check_scales(name: str, scales: torch.Tensor, shape: tuple[int, ...], devic
         raise ValueError(f"{name} must have dtype torch.float32")
     if scales.get_device() != device:
         raise ValueError(f"{name} must be on the device of the operands")
+
+
+def _check_product(
+    a: torch.Tensor,
+    a_scales: torch.Tensor,
+    b: torch.Tensor,
+    b_scales: torch.Tensor,
+    group_ends: torch.Tensor | None,
+    out_dtype: torch.dtype,
+) -> None:
+    if a.ndim != 2 or b.ndim != (2 if group_ends is None else 3):
+        raise ValueError("matmul_blockscaled expects a [T, K] and b [N, K], or b [E, N, K] with group_ends [E]")
+    if a.shape[1] != b.shape[-1]:
+        raise ValueError(f"incompatible shapes: a {tuple(a.shape)} and b {tuple(b.shape)}")
+    index = a.get_device()
+    if not a.is_cuda or not b.is_cuda or b.get_device() != index:
+        raise ValueError("a and b must be on the same CUDA device")
+    if a.dtype != torch.float8_e4m3fn or b.dtype != torch.float8_e4m3fn:
+        raise ValueError("a and b must have dtype torch.float8_e4m3fn")
+    if out_dtype not in _DTYPES:
+        raise ValueError(f"out_dtype must be torch.float16 or torch.bfloat16, got {out_dtype}")
+    (rows, k), n = a.shape, b.shape[-2]
+    lead: tuple[int, ...] = ()
+    if group_ends is not None:
+        lead = (b.shape[0],)
+        if not 1 <= b.shape[0] <= MAX_GROUPS:
+            raise ValueError(f"matmul_blockscaled serves 1 to {MAX_GROUPS} experts, got {b.shape[0]}")
+        _check_ends(group_ends, b.shape[0], index)
+    _check_scales("a_scales", a_scales, (rows, _blocks(k)), index)
+    _check_scales("b_scales", b_scales, (*lead, _blocks(n), _blocks(k)), index)
+
+
+def _product_kernel(
+    a: torch.Tensor,
+    a_scales: torch.Tensor,
+    b: torch.Tensor,
+    b_scales: torch.Tensor,
+    group_ends: torch.Tensor | None,
+    out_dtype: torch.dtype,
+) -> torch.Tensor:
+    _refuse_gradient("matmul_blockscaled", a, a_scales, b, b_scales)
+    _check_product(a, a_scales, b, b_scales, group_ends, out_dtype)
+    (rows, k), n, device = a.shape, b.shape[-2], a.device
+    y = a.new_empty((rows, n), dtype=out_dtype)
+    a_pointer, a_strides, b_pointer, b_strides, sb_strides = a.data_ptr(), a.stride(), b.data_ptr(), b.stride(), b_scales.stride()
+    if group_ends is None:
+        groups, ends, b_strides, sb_strides = 1, None, (0, *b_strides), (0, *sb_strides)
+    else:
+        groups, ends = b.shape[0], group_ends.data_ptr()
+    workspace, ws_pointer, ws_bytes = _workspace(
+        "hst_matmul_blockscaled",
+        device,
+        (a_pointer & 15, *a_strides, b_pointer & 15, *b_strides, groups, rows, n, k),
+    )
+    with _device_guard(device):
+        _native.check(
+            _native.library().hst_matmul_blockscaled(
+                _DTYPES[out_dtype], a_pointer, *a_strides, a_scales.data_ptr(), *a_scales.stride(), b_pointer, *b_strides,
+                b_scales.data_ptr(), *sb_strides, ends, groups, y.data_ptr(), rows, n, k, ws_pointer, ws_bytes,
+                _stream(device),
+            )
+        )  # fmt: skip
+    del workspace  # stream-ordered reuse by the caching allocator is safe on this stream
+    return y
+
+
+def _product_fake(
+    a: torch.Tensor,
+    a_scales: torch.Tensor,
+    b: torch.Tensor,
+    b_scales: torch.Tensor,
+    group_ends: torch.Tensor | None,
+    out_dtype: torch.dtype,
+) -> torch.Tensor:
+    _check_product(a, a_scales, b, b_scales, group_ends, out_dtype)
+    return a.new_empty((a.shape[0], b.shape[-2]), dtype=out_dtype)
+
+
+_product = _operator(
+    "matmul_blockscaled(Tensor a, Tensor a_scales, Tensor b, Tensor b_scales, Tensor? group_ends, ScalarType out_dtype) -> Tensor",
+    _product_kernel,
+    _product_fake,
+)
 
 
 def matmul_blockscaled(
@@ -113,47 +208,4 @@ def matmul_blockscaled(
     ``b_scales [ceil(N / 128), ceil(K / 128)]`` FP32 with any strides; ``y [T, N]`` is ``out_dtype`` (FP16 or
     BF16). With ``group_ends [E]``, ``b`` is ``[E, N, K]``, ``b_scales [E, ...]``, and each row of ``a`` meets
     its expert's weight; rows past the last end are zero."""
-    _refuse_gradient("matmul_blockscaled", a, a_scales, b, b_scales)
-    if a.ndim != 2 or b.ndim != (2 if group_ends is None else 3):
-        raise ValueError("matmul_blockscaled expects a [T, K] and b [N, K], or b [E, N, K] with group_ends [E]")
-    if a.shape[1] != b.shape[-1]:
-        raise ValueError(f"incompatible shapes: a {tuple(a.shape)} and b {tuple(b.shape)}")
-    if not a.is_cuda or not b.is_cuda or b.get_device() != a.get_device():
-        raise ValueError("a and b must be on the same CUDA device")
-    if a.dtype != torch.float8_e4m3fn or b.dtype != torch.float8_e4m3fn:
-        raise ValueError("a and b must have dtype torch.float8_e4m3fn")
-    if out_dtype not in _DTYPES:
-        raise ValueError(f"out_dtype must be torch.float16 or torch.bfloat16, got {out_dtype}")
-    (rows, k), n, device = a.shape, b.shape[-2], a.device
-    index = a.get_device()
-    groups = 1
-    lead: tuple[int, ...] = ()
-    ends = None
-    if group_ends is not None:
-        groups = b.shape[0]
-        lead = (groups,)
-        if not 1 <= groups <= MAX_GROUPS:
-            raise ValueError(f"matmul_blockscaled serves 1 to {MAX_GROUPS} experts, got {groups}")
-        _check_ends(group_ends, groups, index)
-        ends = group_ends.data_ptr()
-    _check_scales("a_scales", a_scales, (rows, _blocks(k)), index)
-    _check_scales("b_scales", b_scales, (*lead, _blocks(n), _blocks(k)), index)
-    y = a.new_empty((rows, n), dtype=out_dtype)
-    a_pointer, a_strides, b_pointer = a.data_ptr(), a.stride(), b.data_ptr()
-    b_strides = b.stride() if lead else (0, *b.stride())
-    sb_strides = b_scales.stride() if lead else (0, *b_scales.stride())
-    workspace, ws_pointer, ws_bytes = _workspace(
-        "hst_matmul_blockscaled",
-        device,
-        (a_pointer & 15, *a_strides, b_pointer & 15, *b_strides, groups, rows, n, k),
-    )
-    with _device_guard(device):
-        _native.check(
-            _native.library().hst_matmul_blockscaled(
-                _DTYPES[out_dtype], a_pointer, *a_strides, a_scales.data_ptr(), *a_scales.stride(), b_pointer, *b_strides,
-                b_scales.data_ptr(), *sb_strides, ends, groups, y.data_ptr(), rows, n, k, ws_pointer, ws_bytes,
-                _stream(device),
-            )
-        )  # fmt: skip
-    del workspace  # stream-ordered reuse by the caching allocator is safe on this stream
-    return y
+    return _product(a, a_scales, b, b_scales, group_ends, out_dtype)

@@ -17,6 +17,10 @@ stream.) Rows past the last end belong to no expert: their outputs and input gra
 they enter no weight gradient. An expert without rows gets a zero weight gradient. Each end is taken
 clamped to ``[previous end, T]``.
 
+The products are ``torch.library`` operators (``heliostune_b200::grouped_matmul`` and
+``::grouped_weight_grad``), so that what traces a program (``torch.jit.trace``, ``make_fx``,
+``torch.compile``) records them. ``torch.func``'s transforms are refused.
+
 The heliostune reference has no counterpart (its products have one weight).
 """
 
@@ -24,6 +28,8 @@ from __future__ import annotations
 
 import ctypes
 import functools
+from collections.abc import Callable
+from typing import Any
 
 import torch
 from torch.autograd import forward_ad
@@ -36,6 +42,61 @@ from heliostune_b200.kernel import _device_guard, _stream
 MAX_GROUPS = 1024
 
 _DTYPES = {torch.float16: _native.HST_F16, torch.bfloat16: _native.HST_BF16}
+
+_LIBRARY = torch.library.Library("heliostune_b200", "DEF")
+#: What a thread adds to every call's dispatch keys by default, and in inference mode.
+_PLAIN_THREAD = (
+    torch._C.DispatchKeySet(torch._C.DispatchKey.BackendSelect).add(torch._C.DispatchKey.ADInplaceOrView).raw_repr(),
+    torch._C.DispatchKeySet(torch._C.DispatchKey.BackendSelect).raw_repr(),
+)
+_thread_keys = torch._C._dispatch_tls_local_include_set
+_PLAIN_TENSORS = (torch.Tensor, torch.nn.Parameter)
+
+
+def _operator(schema: str, kernel: Callable[..., Any], fake: Callable[..., Any]) -> Callable[..., Any]:
+    """The operator of ``schema``: ``kernel`` checks its arguments and launches, ``fake`` checks them and gives
+    the outputs' layout. Without it a tracer would see the outputs' allocation alone, and what it makes of a
+    program would return uninitialised memory."""
+    name = schema.split("(")[0]
+    _LIBRARY.define(schema)
+    # On every device: the kernels refuse those that are not CUDA, as they refuse other types.
+    _LIBRARY.impl(name, kernel, "CompositeExplicitAutograd")
+    torch.library.register_fake(f"heliostune_b200::{name}", fake, lib=_LIBRARY)
+    operator = getattr(torch.ops.heliostune_b200, name).default
+
+    def call(*args: Any) -> Any:
+        # The way through the dispatcher costs 3 us. Where it would lead straight to the kernel -- no tracer, mode or
+        # transform is on in this thread, and the operands are plain tensors as they stand in memory -- the
+        # kernel is called at once.
+        if torch.compiler.is_compiling():
+            return operator(*args)
+        if _thread_keys().raw_repr() not in _PLAIN_THREAD:
+            _refuse_transforms(name)
+            return operator(*args)
+        for arg in args:
+            if type(arg) in _PLAIN_TENSORS:
+                if arg.is_neg():
+                    return operator(*args)
+            elif arg is not None and type(arg) is not torch.dtype:
+                return operator(*args)
+        return kernel(*args)
+
+    return call
+
+
+def _refuse_transforms(what: str) -> None:
+    """Refuses torch.func's transforms: at their levels the operators have no derivatives."""
+    if torch._C._are_functorch_transforms_active():
+        raise ValueError(f"{what} is not available under torch.func's transforms")
+
+
+def _refuse_gradient(what: str, *tensors: torch.Tensor) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise ValueError(f"{what} has no gradient; detach its inputs or run it under torch.no_grad()")
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(what, *tensors)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -83,7 +144,21 @@ def _check_operands(what: str, x: torch.Tensor, other: torch.Tensor, names: tupl
         raise ValueError(f"{what} serves torch.float16 or torch.bfloat16, the same for {names[0]} and {names[1]}")
 
 
-def _forward(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tensor) -> torch.Tensor:
+def _check_matmul(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tensor) -> None:
+    if x.ndim != 2 or weight.ndim != 3:
+        raise ValueError("grouped_matmul expects x [T, K] and weight [E, K, N]")
+    if x.shape[1] != weight.shape[1]:
+        raise ValueError(f"incompatible shapes: x {tuple(x.shape)} and weight {tuple(weight.shape)}")
+    _check_operands("grouped_matmul", x, weight, ("x", "weight"))
+    if not 1 <= weight.shape[0] <= MAX_GROUPS:
+        raise ValueError(f"grouped_matmul serves 1 to {MAX_GROUPS} experts, got {weight.shape[0]}")
+    _check_ends(group_ends, weight.shape[0], x.get_device())
+
+
+def _matmul_kernel(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tensor) -> torch.Tensor:
+    # A recorded program calls the operator itself, which has no gradient.
+    _refuse_gradient("grouped_matmul", x, weight)
+    _check_matmul(x, weight, group_ends)
     groups, k, n = weight.shape
     rows, device = x.shape[0], x.device
     y = x.new_empty((rows, n))
@@ -102,7 +177,24 @@ def _forward(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tensor) ->
     return y
 
 
-def _weight_grad(left: torch.Tensor, right: torch.Tensor, group_ends: torch.Tensor) -> torch.Tensor:
+def _matmul_fake(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tensor) -> torch.Tensor:
+    _check_matmul(x, weight, group_ends)
+    return x.new_empty((x.shape[0], weight.shape[2]))
+
+
+def _check_weight_grad(x: torch.Tensor, dy: torch.Tensor, group_ends: torch.Tensor) -> None:
+    if x.ndim != 2 or dy.ndim != 2 or x.shape[0] != dy.shape[0]:
+        raise ValueError(f"grouped_weight_grad expects x [T, K] and dy [T, N], got {tuple(x.shape)} and {tuple(dy.shape)}")
+    _check_operands("grouped_weight_grad", x, dy, ("x", "dy"))
+    groups = int(group_ends.shape[0]) if group_ends.ndim == 1 else 0
+    if not 1 <= groups <= MAX_GROUPS:
+        raise ValueError(f"grouped_weight_grad serves 1 to {MAX_GROUPS} experts, got {groups}")
+    _check_ends(group_ends, groups, x.get_device())
+
+
+def _weight_grad_kernel(left: torch.Tensor, right: torch.Tensor, group_ends: torch.Tensor) -> torch.Tensor:
+    _refuse_gradient("grouped_weight_grad", left, right)
+    _check_weight_grad(left, right, group_ends)
     groups = group_ends.shape[0]
     (rows, lcols), rcols, device = left.shape, right.shape[1], left.device
     out = left.new_empty((groups, lcols, rcols))
@@ -123,32 +215,34 @@ def _weight_grad(left: torch.Tensor, right: torch.Tensor, group_ends: torch.Tens
     return out
 
 
+def _weight_grad_fake(left: torch.Tensor, right: torch.Tensor, group_ends: torch.Tensor) -> torch.Tensor:
+    _check_weight_grad(left, right, group_ends)
+    return left.new_empty((group_ends.shape[0], left.shape[1], right.shape[1]))
+
+
+_matmul = _operator("grouped_matmul(Tensor x, Tensor weight, Tensor group_ends) -> Tensor", _matmul_kernel, _matmul_fake)
+_weight_grad = _operator(
+    "grouped_weight_grad(Tensor x, Tensor dy, Tensor group_ends) -> Tensor", _weight_grad_kernel, _weight_grad_fake
+)
+
+
 def grouped_weight_grad(x: torch.Tensor, dy: torch.Tensor, group_ends: torch.Tensor) -> torch.Tensor:
     """``out[e] = x[rows of e].T @ dy[rows of e]``, ``[E, K, N]``: the weight gradient of
     :func:`grouped_matmul`, with FP32 sums over the rows and one rounding. ``x [T, K]`` and ``dy [T, N]``
     are FP16 or BF16 with any strides (copied once where their rows are not 16-byte aligned)."""
-    _refuse_tangents("grouped_weight_grad", x, dy)
-    if x.ndim != 2 or dy.ndim != 2 or x.shape[0] != dy.shape[0]:
-        raise ValueError(f"grouped_weight_grad expects x [T, K] and dy [T, N], got {tuple(x.shape)} and {tuple(dy.shape)}")
-    _check_operands("grouped_weight_grad", x, dy, ("x", "dy"))
-    groups = int(group_ends.shape[0]) if group_ends.ndim == 1 else 0
-    if not 1 <= groups <= MAX_GROUPS:
-        raise ValueError(f"grouped_weight_grad serves 1 to {MAX_GROUPS} experts, got {groups}")
-    _check_ends(group_ends, groups, x.get_device())
-    if torch.is_grad_enabled() and (x.requires_grad or dy.requires_grad):
-        raise ValueError("grouped_weight_grad has no gradient; detach its inputs")
     return _weight_grad(x, dy, group_ends)
 
 
 class _GroupedMatmul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, group_ends):  # type: ignore[no-untyped-def]
+        y = _matmul(x, weight, group_ends)
         # Each gradient reads the other operand: what is frozen keeps nothing alive.
         need_x, need_weight, _ = ctx.needs_input_grad
         ctx.save_for_backward(x if need_weight else None, weight if need_x else None, group_ends)
         # [E, N, K] storage: its gradient gets the same layout, so that it adds up in place.
         ctx.weight_by_n = weight.stride(1) == 1 and weight.stride(2) != 1
-        return _forward(x, weight, group_ends)
+        return y
 
     @staticmethod
     @once_differentiable
@@ -156,7 +250,7 @@ class _GroupedMatmul(torch.autograd.Function):
         x, weight, group_ends = ctx.saved_tensors
         dx = dweight = None
         if ctx.needs_input_grad[0]:
-            dx = _forward(dy, weight.transpose(1, 2), group_ends)
+            dx = _matmul(dy, weight.transpose(1, 2), group_ends)
         if ctx.needs_input_grad[1]:
             if ctx.weight_by_n:
                 dweight = _weight_grad(dy, x, group_ends).transpose(1, 2)
@@ -170,15 +264,9 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tens
     its last two dimensions contiguous), both FP16 or both BF16, ``y [T, N]`` of their type; 1 to
     :data:`MAX_GROUPS` experts. Any strides are served; operands whose rows are not 16-byte aligned
     are copied once. Differentiable in ``x`` and ``weight`` (once, in reverse mode)."""
-    _refuse_tangents("grouped_matmul", x, weight)
-    if x.ndim != 2 or weight.ndim != 3:
-        raise ValueError("grouped_matmul expects x [T, K] and weight [E, K, N]")
-    if x.shape[1] != weight.shape[1]:
-        raise ValueError(f"incompatible shapes: x {tuple(x.shape)} and weight {tuple(weight.shape)}")
-    _check_operands("grouped_matmul", x, weight, ("x", "weight"))
-    if not 1 <= weight.shape[0] <= MAX_GROUPS:
-        raise ValueError(f"grouped_matmul serves 1 to {MAX_GROUPS} experts, got {weight.shape[0]}")
-    _check_ends(group_ends, weight.shape[0], x.get_device())
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        if not torch.compiler.is_compiling():
+            _refuse_transforms("grouped_matmul")
+        _refuse_tangents("grouped_matmul", x, weight)
         return _GroupedMatmul.apply(x, weight, group_ends)
-    return _forward(x, weight, group_ends)
+    return _matmul(x, weight, group_ends)

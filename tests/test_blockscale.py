@@ -13,7 +13,9 @@ from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from heliostune_b200 import _native, blockscale, grouped
 from tests.test_grouped import _bounds, _ends
@@ -165,6 +167,59 @@ def _refused_calls() -> None:
         assert quantize(**kwargs) == _native.HST_ERR_INVALID, kwargs
         assert message in lib.hst_last_error(), kwargs
     assert quantize(rows=0) == _native.HST_OK
+
+
+# ------------------------------------------------------------------------------------------
+# Tracing
+# ------------------------------------------------------------------------------------------
+
+
+def _served(x: torch.Tensor, w: torch.Tensor, ends: torch.Tensor) -> torch.Tensor:
+    return blockscale.matmul_blockscaled(*blockscale.quantize_rows(x), *blockscale.quantize_tiles(w), ends, out_dtype=torch.float16)
+
+
+def test_tracing_records_the_operators() -> None:
+    """On fake CUDA tensors: the operators are recorded, and their outputs' layouts are the kernels'."""
+    with FakeTensorMode():
+        x = torch.empty((9, 130), device="cuda", dtype=torch.float16)
+        w = torch.empty((2, 200, 130), device="cuda", dtype=torch.float16)
+        ends = torch.empty(2, device="cuda", dtype=torch.int32)
+        traced = make_fx(_served)(x, w, ends)
+        called = [node.target for node in traced.graph.nodes if node.op == "call_function"]
+        ops = torch.ops.heliostune_b200
+        assert [t for t in called if t in (ops.quantize_rows.default, ops.quantize_tiles.default, ops.matmul_blockscaled.default)] == [
+            ops.quantize_rows.default, ops.quantize_tiles.default, ops.matmul_blockscaled.default,
+        ]  # fmt: skip
+        assert not any("empty" in str(t) for t in called)
+        q, s = blockscale.quantize_rows(x)
+        assert q.shape == (9, 130) and q.stride() == (144, 1) and s.shape == (9, 2) and s.stride() == (1, 9)
+        q, s = blockscale.quantize_tiles(w)
+        assert q.shape == (2, 200, 130) and q.stride() == (28800, 144, 1) and s.shape == (2, 2, 2) and s.is_contiguous()
+        assert _served(x, w, ends).shape == (9, 200)
+
+
+def test_transforms_are_refused() -> None:
+    x = torch.zeros((4, 128), dtype=torch.float16)
+    for quantize in (blockscale.quantize_rows, blockscale.quantize_tiles):
+        for transformed in (lambda q=quantize: torch.func.jvp(q, (x,), (x,)), lambda q=quantize: torch.vmap(q)(x[None])):
+            with pytest.raises(ValueError, match="torch.func's transforms"):
+                transformed()
+
+
+@gpu
+def test_traced_programs_compute_what_they_recorded() -> None:
+    g = torch.Generator(device="cuda").manual_seed(31)
+    x, other = (torch.randn((90, 264), generator=g, device="cuda").half() for _ in range(2))
+    w = torch.randn((3, 136, 264), generator=g, device="cuda").half()
+    ends = _ends([19, 19, 83])
+    expected = _served(other, w, ends)
+    for program in (
+        torch.jit.trace(_served, (x, w, ends)),
+        make_fx(_served)(x, w, ends),
+        make_fx(_served, tracing_mode="fake")(x, w, ends),
+        torch.compile(_served, fullgraph=True, backend="aot_eager"),
+    ):
+        assert torch.equal(program(other, w, ends), expected)
 
 
 # ------------------------------------------------------------------------------------------

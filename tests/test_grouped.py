@@ -14,7 +14,9 @@ from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from heliostune_b200 import _native, grouped
 
@@ -167,6 +169,104 @@ def _refused_calls() -> None:
     assert lib.hst_grouped_weight_grad(0, 17, 8, 1, 16, 8, 1, 16, 2, 16, 4, 8, 8, None, 0, None) == _native.HST_ERR_INVALID
     assert b"left must be aligned" in lib.hst_last_error()
     assert lib.hst_grouped_weight_grad(3, 16, 8, 1, 16, 8, 1, 16, 2, 16, 4, 8, 8, None, 0, None) == _native.HST_ERR_INVALID
+
+
+# ------------------------------------------------------------------------------------------
+# Tracing and transforms
+# ------------------------------------------------------------------------------------------
+
+
+def test_tracing_records_the_operators() -> None:
+    """On fake CUDA tensors: what is recorded are the operators, not the allocation of their outputs."""
+    with FakeTensorMode():
+        x = torch.empty((9, 32), device="cuda", dtype=torch.float16)
+        w = torch.empty((2, 32, 16), device="cuda", dtype=torch.float16)
+        dy = torch.empty((9, 16), device="cuda", dtype=torch.float16)
+        ends = torch.empty(2, device="cuda", dtype=torch.int32)
+
+        def step(x, w, dy, ends):  # type: ignore[no-untyped-def]
+            return grouped.grouped_matmul(x, w, ends), grouped.grouped_weight_grad(x, dy, ends)
+
+        traced = make_fx(step)(x, w, dy, ends)
+        called = [node.target for node in traced.graph.nodes if node.op == "call_function"]
+        ops = torch.ops.heliostune_b200
+        assert called == [ops.grouped_matmul.default, ops.grouped_weight_grad.default]
+        y, dw = step(x, w, dy, ends)
+        assert y.shape == (9, 16) and dw.shape == (2, 32, 16) and y.dtype == dw.dtype == torch.float16
+        with pytest.raises(ValueError, match="incompatible shapes"):
+            grouped.grouped_matmul(x[:, :8], w, ends)
+
+
+def test_transforms_are_refused() -> None:
+    x = torch.zeros((4, 16), dtype=torch.float16)
+    w = torch.zeros((2, 16, 8), dtype=torch.float16)
+    ends = torch.zeros(2, dtype=torch.int32)
+    one = torch.ones_like(x)
+
+    def product(x: torch.Tensor) -> torch.Tensor:
+        return grouped.grouped_matmul(x, w, ends)
+
+    for transformed in (
+        lambda: torch.func.jvp(product, (x,), (one,)),
+        lambda: torch.func.grad(lambda x: product(x).sum())(x),
+        lambda: torch.vmap(product)(x[None]),
+        lambda: torch.func.grad(lambda x: torch.vmap(product)(x[None]).sum())(x),
+        lambda: torch.func.jvp(lambda x: grouped.grouped_weight_grad(x, x, ends), (x,), (one,)),
+    ):
+        with pytest.raises(ValueError, match="torch.func's transforms"):
+            transformed()
+
+
+@gpu
+def test_traced_programs_compute_what_they_recorded() -> None:
+    x, w, dy = _operands(90, 3, 96, 56, torch.float16, "nk", seed=32)
+    ends = _ends([19, 19, 83])
+
+    def step(x, w, dy, ends):  # type: ignore[no-untyped-def]
+        return grouped.grouped_matmul(x, w, ends), grouped.grouped_weight_grad(x, dy, ends)
+
+    others = _operands(90, 3, 96, 56, torch.float16, "nk", seed=33)
+    expected = step(*others, _ends([40, 41, 90]))
+    for program in (
+        torch.jit.trace(step, (x, w, dy, ends)),
+        make_fx(step)(x, w, dy, ends),
+        make_fx(step, tracing_mode="fake")(x, w, dy, ends),
+        torch.compile(step, fullgraph=True, backend="aot_eager"),
+    ):
+        for got, want in zip(program(*others, _ends([40, 41, 90])), expected, strict=True):
+            assert torch.equal(got, want) and got.stride() == want.stride()
+    # A recorded operator has no gradient of its own; what the public call does with one stays as it is.
+    with pytest.raises(ValueError, match="no gradient"):
+        make_fx(step)(x, w, dy, ends)(x.clone().requires_grad_(), w, dy, ends)
+
+
+@gpu
+def test_views_that_stand_for_the_negative_of_their_memory() -> None:
+    """The imaginary part of a conjugate is a view with the negative bit set: its values are not those in memory."""
+    x, w, _ = _operands(60, 2, 64, 48, torch.float16, "kn", seed=35)
+    ends = _ends([23, 60])
+    x = torch.view_as_complex(x.view(60, 32, 2)).conj().imag
+    dy = torch.view_as_complex(torch.randn((60, 48, 2), device="cuda").half()).conj().imag
+    w = w[:, :32]
+    assert x.is_neg() and dy.is_neg()
+    assert torch.equal(grouped.grouped_matmul(x, w, ends), grouped.grouped_matmul(x.resolve_neg(), w, ends))
+    expected = grouped.grouped_weight_grad(x.resolve_neg(), dy.resolve_neg(), ends)
+    assert torch.equal(grouped.grouped_weight_grad(x, dy, ends), expected)
+    leaf = w.detach().clone().requires_grad_()
+    grouped.grouped_matmul(x, leaf, ends).backward(dy)
+    assert torch.equal(leaf.grad, expected)
+
+
+@gpu
+def test_a_compiled_step_has_the_eager_gradients() -> None:
+    x, w, dy = _operands(90, 3, 96, 56, torch.bfloat16, "kn", seed=34)
+    ends = _ends([19, 19, 83])
+    x.requires_grad_()
+    w = w.detach().requires_grad_()
+    eager = torch.autograd.grad(grouped.grouped_matmul(x, w, ends), (x, w), dy)
+    compiled = torch.compile(grouped.grouped_matmul, backend="aot_eager")
+    for got, want in zip(torch.autograd.grad(compiled(x, w, ends), (x, w), dy), eager, strict=True):
+        assert torch.equal(got, want)
 
 
 # ------------------------------------------------------------------------------------------
