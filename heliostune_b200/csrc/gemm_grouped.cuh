@@ -26,7 +26,7 @@
 //     register: on the R side the scales of 256 rows are 128 a thread and block, and their broadcast
 //     loads from shared memory, beside the UMMAs' operands, took three times the UMMAs' time. Bound now
 //     by the way of a block through the two buffers (UMMAs 512 cycles, hand-over, 128 columns a thread
-//     read and added, hand-back): 8192 x 14336 x 4096 in 470 us, 350 without the reading and adding.
+//     read and added, hand-back): 8192 x 14336 x 4096 in 479 us, 350 without the reading and adding.
 //   * kScaledFew is for few rows a group: as kForward, weights on the L side and at most 64 rows on
 //     the R side, in eight TMEM buffers. A block then costs 64 to 128 UMMA cycles instead of 512 and
 //     keeps all lanes busy, and the weights stream at the rate of HBM.
@@ -579,6 +579,23 @@ __device__ __forceinline__ void fma_pair(float& a0, float& a1, uint32_t p0, uint
       : "r"(p0), "r"(p1), "f"(s));
 }
 
+// The scale a * b of a block's sums, which are up to 2^25, may leave FP32's normal range where what it scales does
+// not (BF16's ends reach it: 2^100 x 2^60 with sums of zero, or 2^-109 x 2^-20). The sums then take one factor
+// at a time: the smaller first where the product is too large, the larger first where it is too small, so that
+// no step leaves the range before the result does.
+__device__ __forceinline__ bool is_normal(float v) {
+  return (__float_as_uint(v) << 1) - 0x01000000u < 0xfe000000u;  // neither zero, subnormal, infinite nor NaN
+}
+__device__ __forceinline__ void split_scale(float a, float b, float& before, float& scale) {
+  scale = a * b;
+  before = 1.f;
+  if (is_normal(scale) || a == 0.f || b == 0.f) return;
+  const bool a_first = (fabsf(a) < fabsf(b)) != (fabsf(scale) < 1.f);
+  before = a_first ? a : b;
+  scale = a_first ? b : a;
+}
+__device__ __forceinline__ uint32_t scaled_bits(uint32_t v, float s) { return __float_as_uint(__uint_as_float(v) * s); }
+
 template <typename T>
 __device__ __forceinline__ T from_f32(float v);
 template <>
@@ -1073,7 +1090,8 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
         for (int j = 0; j < 128; ++j) acc[j] = 0.f;
         bool ready = true;
         for (int kb = s.kb0; kb < s.kb1; ++kb) {
-          const float now = next_a * next_b;
+          float now = next_a * next_b;
+          const bool split = !__all_sync(0xffffffffu, is_normal(now));
           if (kb + 1 < s.kb1) {
             sa += args.rs_k;
             sb += args.ts_k;
@@ -1082,6 +1100,25 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
           }
           ready = wait_buf();
           if (!ready) break;
+          // Rare: the block's sums take the first factor in TMEM, so that the loop below stays as it is (with a copy of the
+          // loop for this, 8192 x 14336 x 4096 took 487 to 502 us; 470 without any of it, 479 so).
+          if (live && split) {
+            float before;
+            const int64_t back = kb + 1 < s.kb1 ? 1 : 0;
+            split_scale(*(sa - back * args.rs_k), *(sb - back * args.ts_k), before, now);
+#pragma unroll 1
+            for (int c = 0; c < 128; c += 16) {
+              const uint32_t taddr = lane_base + static_cast<uint32_t>(buf * kBufCols + half * 128 + c);
+              uint32_t v[16];
+              tmem_ld_32x32b_x16(taddr, v);
+              tmem_ld_wait();
+              tmem_ld_fence_regs(v);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) v[j] = scaled_bits(v[j], before);
+              tmem_st_32x32b_x16(taddr, v);
+            }
+            tmem_st_wait();
+          }
           if (live) {
             const uint32_t taddr = lane_base + static_cast<uint32_t>(buf * kBufCols + half * 128);
 #pragma unroll
@@ -1143,7 +1180,12 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
         float next_a = *sa, next_a32 = second ? *sa32 : 0.f, next_b = *sb;
         bool ready = true;
         for (int kb = s.kb0; kb < s.kb1; ++kb) {
-          const float now = next_a * next_b, now32 = next_a32 * next_b;
+          float now = next_a * next_b, now32 = next_a32 * next_b, before = 1.f, before32 = 1.f;
+          const bool split = !__all_sync(0xffffffffu, is_normal(now) && (!second || is_normal(now32)));
+          if (split) {
+            split_scale(next_a, next_b, before, now);
+            split_scale(next_a32, next_b, before32, now32);
+          }
           if (kb + 1 < s.kb1) {
             sa += args.rs_k;
             sb += args.ts_k;
@@ -1164,6 +1206,13 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
           tmem_ld_fence_regs(v[0]);
           tmem_ld_fence_regs(v[1]);
           release_buf();
+          if (split) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              v[0][j] = scaled_bits(v[0][j], __shfl_sync(0xffffffffu, before, j));
+              v[1][j] = scaled_bits(v[1][j], __shfl_sync(0xffffffffu, before32, j));
+            }
+          }
 #pragma unroll
           for (int j = 0; j < 32; ++j) acc[j] = fmaf(__uint_as_float(v[0][j]), __shfl_sync(0xffffffffu, now, j), acc[j]);
           if (second) {

@@ -220,7 +220,8 @@ int hst_grouped_weight_grad(int32_t dtype, const void* left, int64_t l_row, int6
 /* y[t, j] = sum over blocks c of 128 values of k: a_scales[t, c] * b_scales[g, j / 128, c] *
  * sum over the block of a[t, i] * b[g, j, i]. a [rows, k] and b [groups, n, k] E4M3, FP32 scales
  * with the strides given (in values), y [rows, n] of out_dtype. The block sums and their scaled sum
- * are FP32. For a plain product pass one group and a null `ends`. */
+ * are FP32; a product of scales outside FP32's normal range is not formed (the sum takes them one by
+ * one). For a plain product pass one group and a null `ends`. */
 int hst_matmul_blockscaled_workspace(const void* a, int64_t a_row, int64_t a_col, const void* b,
                                      int64_t b_group, int64_t b_row, int64_t b_col, int32_t groups,
                                      int64_t rows, int64_t n, int64_t k, int device, size_t* bytes);

@@ -355,6 +355,39 @@ def test_nan_and_infinity_stay_in_their_rows_and_columns(rows: int) -> None:
 
 
 @gpu
+@pytest.mark.parametrize("rows", (40, 400))
+@pytest.mark.parametrize("size", (130, -142))
+def test_scales_whose_product_leaves_the_range_of_fp32(rows: int, size: int) -> None:
+    """Scales of about 2^(size / 2) each: their product is no normal FP32 value, what they scale is. Where it is too
+    large, the last block, of zeros in ``a``, has the largest scales there are. One row's scales are zero."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    n, k = 200, 384
+
+    def values(*shape: int) -> torch.Tensor:
+        if size > 0:  # multiples of E4M3's least value: block sums of a few 2^-18
+            v = torch.randint(-1, 2, shape, generator=g, device="cuda") * 2.0**-9
+        else:
+            v = (torch.randn(shape, generator=g, device="cuda") * 200).clamp(-448, 448)
+        return v.to(torch.float8_e4m3fn)
+
+    def scales(*shape: int) -> torch.Tensor:
+        return (1 + torch.rand(shape, generator=g, device="cuda")) * 2.0 ** (size / 2)
+
+    a, b, sa, sb = values(rows, k), values(n, k), scales(rows, 3), scales(2, 3)
+    if size > 0:
+        a[:, 256:] = 0
+        sa[:, 2] = sb[:, 2] = torch.finfo(torch.float32).max
+    sa[7] = 0
+    y = blockscale.matmul_blockscaled(a, sa, b, sb)
+    assert bool(torch.isfinite(y).all()) and bool((y[7] == 0).all())
+    da, db = _dequantize(a, sa, False), _dequantize(b, sb, True)
+    exact, magnitude = da @ db.T, da.abs() @ db.abs().T
+    # As above, with one more rounding of each block's sum, and half a subnormal step of BF16 (2^-133).
+    bound = 2.0**-8 * exact.abs() + (1 + 2.0**-8) * (128 + 3 + 3) * 2.0**-23 * magnitude + 2.0**-134
+    assert bool(((y.double() - exact).abs() <= bound).all())
+
+
+@gpu
 def test_groups_keep_to_their_rows_next_to_nan() -> None:
     ends = [37, 120, 250]
     a, sa, b, sb = _operands(260, 136, 264, seed=3, groups=3)
