@@ -209,14 +209,15 @@ struct GradTiles {
   }
 };
 
-// How the line is shared: by whole tiles or by K blocks, and among how many pairs. `all`: there is
-// work for every pair already (the whole tiles of kWeightGrad).
+// How the line is shared: by whole tiles or by K blocks, and among how many pairs (the first ones; the
+// others have what precedes the line alone: cut into a share for every pair, the one tile left over of 75 cost
+// 4096 rows of 1280 x 3840 137 us, and 68 in shares of at least min_blocks).
 struct GroupShares {
   int shares;
   bool whole;
-  __host__ __device__ GroupShares(const GroupedArgs& a, int tiles, int total, int deepest, bool all) {
-    const int by_tiles = all ? a.pairs : at_least_one(a.pairs, tiles);
-    const int by_blocks = all ? a.pairs : at_least_one(a.pairs, total / a.min_blocks);
+  __host__ __device__ GroupShares(const GroupedArgs& a, int tiles, int total, int deepest) {
+    const int by_tiles = at_least_one(a.pairs, tiles);
+    const int by_blocks = at_least_one(a.pairs, total / a.min_blocks);
     const int64_t idle = static_cast<int64_t>(ceil_div(tiles, by_tiles)) * deepest - total / by_blocks;
     whole = a.whole != 0 || idle <= a.idle_limit;
     shares = whole ? by_tiles : by_blocks;
@@ -287,7 +288,7 @@ __device__ inline void build_group_rows(const GroupedArgs& a, const GroupTable& 
       t.tile_base(a.groups) = tiles;
       total = tiles * a.k_blocks;
     }
-    const GroupShares plan(a, tiles, total, deepest, kGrad && GradTiles(a).each > 0);
+    const GroupShares plan(a, tiles, total, deepest);
     const int shares = plan.shares;
     t.whole() = plan.whole;
     t.shares() = shares;
@@ -393,7 +394,7 @@ struct GroupWalk {
   __device__ GroupWalk(const GroupedArgs& a, const GroupTable& t, int pair)
       : GroupWalk(a, t, line_begin(a, t, pair), line_begin(a, t, pair + 1), min(pair, t.shares() - 1)) {
     if constexpr (MODE == GroupMode::kWeightGrad) {
-      if (pair < t.shares()) ahead = t.used() * GradTiles(a).each;
+      ahead = t.used() * GradTiles(a).each;
       if (t.whole()) {  // shares of whole tiles
         const int per = t.per_column(), more = t.tiles() - per * t.shares();
         lo = 0;

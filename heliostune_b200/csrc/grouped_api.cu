@@ -190,7 +190,7 @@ int launch_grouped(const GroupedProblem& p, const GroupedMaps& maps, GroupedArgs
   args.whole = whole_tiles<MODE>(p);
   if (args.ends == nullptr && MODE != GroupMode::kWeightGrad && args.whole == 0) {  // one group: its tiles are known
     const int tiles = group_row_tiles<MODE>(args, args.rows) * ceil_div(args.cols, 256);
-    args.whole = GroupShares(args, tiles, tiles * args.k_blocks, args.k_blocks, false).whole;
+    args.whole = GroupShares(args, tiles, tiles * args.k_blocks, args.k_blocks).whole;
   }
   args.vec = 32;
   while (args.vec > 2 && (p.cols * 2 % args.vec != 0 || reinterpret_cast<uintptr_t>(args.out) % args.vec != 0)) args.vec /= 2;

@@ -376,6 +376,40 @@ def test_weight_gradients_of_many_tiles(k: int, n: int, ends: list[int]) -> None
     _check_weight_grad(grouped.grouped_weight_grad(x, dy, _ends(ends)), x, dy, ends)
 
 
+def _pairs() -> int:
+    count = ctypes.c_int(0)
+    _native.check(_native.library().hst_device_sm_count(torch.cuda.current_device(), ctypes.byref(count)))
+    return count.value // 2
+
+
+def _cut_weight_grad(x: torch.Tensor, dy: torch.Tensor, ends: list[int]) -> tuple[torch.Tensor, int]:
+    """The weight gradient over the C ABI, and into how many FP32 pieces its cut tiles were written: those of
+    the workspace (one of 128 x 256 values for each CTA of a pair, contiguous operands) that hold anything."""
+    lib, (rows, k), n, groups = _native.library(), x.shape, dy.shape[1], len(ends)
+    size = ctypes.c_size_t(0)
+    operands = x.data_ptr(), k, 1, dy.data_ptr(), n, 1
+    _native.check(lib.hst_grouped_weight_grad_workspace(*operands, groups, rows, k, n, x.get_device(), ctypes.byref(size)))
+    workspace = torch.full((size.value // 4,), -1, device="cuda", dtype=torch.int32)
+    out, group_ends = torch.empty((groups, k, n), device="cuda", dtype=x.dtype), _ends(ends)
+    _native.check(
+        lib.hst_grouped_weight_grad(
+            grouped._DTYPES[x.dtype], *operands, group_ends.data_ptr(), groups, out.data_ptr(), rows, k, n,
+            workspace.data_ptr(), size.value, torch.cuda.current_stream().cuda_stream,
+        )
+    )  # fmt: skip
+    return out, int((workspace.view(-1, 2 * 128 * 256) != -1).any(dim=1).sum())
+
+
+@gpu
+def test_a_tile_left_over_by_the_pairs_is_cut_into_shares_worth_a_join() -> None:
+    """A tile more than there are pairs, 64 K blocks deep: the one left over is cut into shares of four blocks, the
+    least a share has, and not into one for each pair."""
+    x, _, dy = _operands(4096, 1, 256 * (_pairs() + 1), 256, torch.bfloat16, "kn", seed=41)
+    dw, pieces = _cut_weight_grad(x, dy, [4096])
+    _check_weight_grad(dw, x, dy, [4096])
+    assert pieces == 16
+
+
 @gpu
 def test_many_groups() -> None:
     groups = grouped.MAX_GROUPS
