@@ -74,6 +74,17 @@ Stack make_stack(const void* ptr, int64_t elem, int64_t groups, int64_t rows, in
   return s;
 }
 
+// Whether the copies a product needs can be counted in 64 bits and made by one grid; no GPU holds more. (Extents of
+// broadcast operands are not bound by the memory behind them.)
+constexpr int64_t kMaxCopyBytes = int64_t(1) << 44;
+int check_copies(const char* what, const Stack& a, const Stack& b) {
+  for (const Stack* s : {&a, &b}) {
+    if (!s->readable() && s->groups > kMaxCopyBytes / (s->rows * s->packed_row() * s->elem))
+      return fail(HST_ERR_UNSUPPORTED, "%s: an operand to be copied is too large", what);
+  }
+  return HST_OK;
+}
+
 size_t pack_bytes(const Stack& s) { return s.readable() ? 0 : s.packed_bytes(); }
 
 // Copies a stack that is not readable to `dst`, the weights of empty groups left out where `ends` tells
@@ -325,11 +336,13 @@ int hst_grouped_matmul_workspace(const void* x, int64_t x_row, int64_t x_col, co
   HST_TRY(check_groups("the grouped matmul", rows, groups, bytes));
   HST_TRY(check_extents("the grouped matmul", n, k));
   if (rows == 0 || n == 0 || k == 0) return HST_OK;
+  bool kn = false;
+  const Stack xs = make_stack(x, 2, 1, rows, k, 0, x_row, x_col);
+  const Stack ws = stored_weights(w, groups, k, n, w_group, w_k, w_n, &kn);
+  HST_TRY(check_copies("the grouped matmul", xs, ws));
   int sms = 0;
   HST_TRY(device_sms(device, &sms));
-  bool kn = false;
-  return total_bytes(piece_bytes<GroupMode::kForward>(forward_problem(rows, groups, n, k), sms),
-                     make_stack(x, 2, 1, rows, k, 0, x_row, x_col), stored_weights(w, groups, k, n, w_group, w_k, w_n, &kn), bytes);
+  return total_bytes(piece_bytes<GroupMode::kForward>(forward_problem(rows, groups, n, k), sms), xs, ws, bytes);
 }
 
 int hst_grouped_matmul(int32_t dtype, const void* x, int64_t x_row, int64_t x_col, const void* w, int64_t w_group,
@@ -347,12 +360,13 @@ int hst_grouped_matmul(int32_t dtype, const void* x, int64_t x_row, int64_t x_co
   HST_TRY(check_aligned("w", w, 2));
   HST_TRY(check_aligned("ends", ends, 4));
   HST_TRY(check_aligned("y", y, 2));
-  DeviceState* dev = nullptr;
-  HST_TRY(device_state(&dev));
-  const GroupedProblem p = forward_problem(rows, groups, n, k);
   bool kn = false;
   Stack xs = make_stack(x, 2, 1, rows, k, 0, x_row, x_col);
   Stack ws = stored_weights(w, groups, k, n, w_group, w_k, w_n, &kn);
+  HST_TRY(check_copies("the grouped matmul", xs, ws));
+  DeviceState* dev = nullptr;
+  HST_TRY(device_state(&dev));
+  const GroupedProblem p = forward_problem(rows, groups, n, k);
   HST_TRY(place_operands(piece_bytes<GroupMode::kForward>(p, dev->sm_count), &xs, nullptr, &ws, ends, rows, workspace,
                          workspace_bytes, s));
   GroupedMaps maps = {};
@@ -380,11 +394,11 @@ int hst_grouped_weight_grad_workspace(const void* left, int64_t l_row, int64_t l
   HST_TRY(check_groups("the grouped weight gradient", rows, groups, bytes));
   HST_TRY(check_extents("the grouped weight gradient", lcols, rcols));
   if (rows == 0 || lcols == 0 || rcols == 0) return HST_OK;
+  const Stack ls = make_stack(left, 2, 1, rows, lcols, 0, l_row, l_col), rs = make_stack(right, 2, 1, rows, rcols, 0, r_row, r_col);
+  HST_TRY(check_copies("the grouped weight gradient", ls, rs));
   int sms = 0;
   HST_TRY(device_sms(device, &sms));
-  return total_bytes(piece_bytes<GroupMode::kWeightGrad>(grad_problem(rows, groups, lcols, rcols), sms),
-                     make_stack(left, 2, 1, rows, lcols, 0, l_row, l_col), make_stack(right, 2, 1, rows, rcols, 0, r_row, r_col),
-                     bytes);
+  return total_bytes(piece_bytes<GroupMode::kWeightGrad>(grad_problem(rows, groups, lcols, rcols), sms), ls, rs, bytes);
 }
 
 int hst_grouped_weight_grad(int32_t dtype, const void* left, int64_t l_row, int64_t l_col, const void* right, int64_t r_row,
@@ -402,10 +416,11 @@ int hst_grouped_weight_grad(int32_t dtype, const void* left, int64_t l_row, int6
   HST_TRY(check_aligned("right", right, 2));
   HST_TRY(check_aligned("ends", ends, 4));
   HST_TRY(check_aligned("out", out, 2));
+  Stack ls = make_stack(left, 2, 1, rows, lcols, 0, l_row, l_col), rs = make_stack(right, 2, 1, rows, rcols, 0, r_row, r_col);
+  HST_TRY(check_copies("the grouped weight gradient", ls, rs));
   DeviceState* dev = nullptr;
   HST_TRY(device_state(&dev));
   const GroupedProblem p = grad_problem(rows, groups, lcols, rcols);
-  Stack ls = make_stack(left, 2, 1, rows, lcols, 0, l_row, l_col), rs = make_stack(right, 2, 1, rows, rcols, 0, r_row, r_col);
   HST_TRY(place_operands(piece_bytes<GroupMode::kWeightGrad>(p, dev->sm_count), &ls, nullptr, &rs, nullptr, rows, workspace,
                          workspace_bytes, s));
   GroupedMaps maps = {};
@@ -426,10 +441,11 @@ int hst_matmul_blockscaled_workspace(const void* a, int64_t a_row, int64_t a_col
   HST_TRY(check_groups("the block-scaled matmul", rows, groups, bytes));
   HST_TRY(check_extents("the block-scaled matmul", n, k));
   if (rows == 0 || n == 0 || k == 0) return HST_OK;
+  const Stack as = make_stack(a, 1, 1, rows, k, 0, a_row, a_col), bs = make_stack(b, 1, groups, n, k, b_group, b_row, b_col);
+  HST_TRY(check_copies("the block-scaled matmul", as, bs));
   int sms = 0;
   HST_TRY(device_sms(device, &sms));
-  return total_bytes(scaled_piece_bytes(scaled_problem(rows, groups, n, k), sms), make_stack(a, 1, 1, rows, k, 0, a_row, a_col),
-                     make_stack(b, 1, groups, n, k, b_group, b_row, b_col), bytes);
+  return total_bytes(scaled_piece_bytes(scaled_problem(rows, groups, n, k), sms), as, bs, bytes);
 }
 
 int hst_matmul_blockscaled(int32_t out_dtype, const void* a, int64_t a_row, int64_t a_col, const float* a_scales,
@@ -450,10 +466,11 @@ int hst_matmul_blockscaled(int32_t out_dtype, const void* a, int64_t a_row, int6
   HST_TRY(check_aligned("b_scales", b_scales, 4));
   HST_TRY(check_aligned("ends", ends, 4));
   HST_TRY(check_aligned("y", y, 2));
+  Stack as = make_stack(a, 1, 1, rows, k, 0, a_row, a_col), bs = make_stack(b, 1, groups, n, k, b_group, b_row, b_col);
+  HST_TRY(check_copies("the block-scaled matmul", as, bs));
   DeviceState* dev = nullptr;
   HST_TRY(device_state(&dev));
   const GroupedProblem p = scaled_problem(rows, groups, n, k);
-  Stack as = make_stack(a, 1, 1, rows, k, 0, a_row, a_col), bs = make_stack(b, 1, groups, n, k, b_group, b_row, b_col);
   HST_TRY(place_operands(scaled_piece_bytes(p, dev->sm_count), &as, nullptr, &bs, ends, rows, workspace, workspace_bytes, s));
   const CUtensorMapDataType type = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   GroupedMaps maps = {};

@@ -171,6 +171,30 @@ def _refused_calls() -> None:
     assert lib.hst_grouped_weight_grad(3, 16, 8, 1, 16, 8, 1, 16, 2, 16, 4, 8, 8, None, 0, None) == _native.HST_ERR_INVALID
 
 
+def test_broadcast_operands_too_large_to_copy_are_refused_before_any_cuda_work() -> None:
+    """1024 weights of 7 * 2^27 rows and columns that share one row: the bytes of their copy, 49 * 2^65, are 0 in 64 bits."""
+    with ThreadPoolExecutor(1) as thread:
+        thread.submit(_refused_copies).result()
+
+
+def _refused_copies() -> None:
+    _native.build_library()
+    lib = _native.library()
+    size = ctypes.c_size_t(0)
+    k = n = 7 * 2**27
+    calls = (
+        lambda: lib.hst_grouped_matmul_workspace(16, k, 1, 16, 0, 0, 1, 1024, 1, n, k, 0, ctypes.byref(size)),
+        lambda: lib.hst_grouped_matmul(0, 16, k, 1, 16, 0, 0, 1, 16, 1024, 16, 1, n, k, None, 0, None),
+        lambda: lib.hst_grouped_weight_grad_workspace(16, 0, 1, 16, 0, 1, 1, n, k, 8, 0, ctypes.byref(size)),
+        lambda: lib.hst_grouped_weight_grad(0, 16, 0, 1, 16, 8, 1, 16, 1, 16, n, k, 8, None, 0, None),
+        lambda: lib.hst_matmul_blockscaled_workspace(16, k, 1, 16, 0, 0, 1, 1024, 1, n, k, 0, ctypes.byref(size)),
+        lambda: lib.hst_matmul_blockscaled(0, 16, k, 1, 16, 1, 1, 16, 0, 0, 1, 16, 1, 1, 1, 16, 1024, 16, 1, n, k, None, 0, None),
+    )
+    for call in calls:
+        assert call() == _native.HST_ERR_UNSUPPORTED
+        assert b"too large" in lib.hst_last_error()
+
+
 # ------------------------------------------------------------------------------------------
 # Tracing and transforms
 # ------------------------------------------------------------------------------------------
