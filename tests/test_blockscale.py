@@ -9,6 +9,7 @@ output by ``eps / 2``.
 
 from __future__ import annotations
 
+import ctypes
 from concurrent.futures import ThreadPoolExecutor
 
 import pytest
@@ -18,7 +19,7 @@ from torch.autograd import forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 
 from heliostune_b200 import _native, blockscale, grouped
-from tests.test_grouped import _bounds, _ends
+from tests.test_grouped import _bounds, _ends, _pairs, _pieces, _rounding_excess
 
 gpu = pytest.mark.gpu
 DTYPES = (torch.float16, torch.bfloat16)
@@ -334,6 +335,82 @@ def test_grouped(rows: int, ends: list[int], n: int, k: int) -> None:
         _assert_product(y[start:end], da[start:end], db[e])
         last = end
     assert bool((y[last:] == 0).all())
+
+
+def _cut_product(a, sa, b, sb, ends: list[int] | None, out_dtype: torch.dtype) -> tuple[torch.Tensor, int]:  # type: ignore[no-untyped-def]
+    """The product over the C ABI, and into how many FP32 pieces its cut tiles were written."""
+    lib, (rows, k), n, groups = _native.library(), a.shape, b.shape[-2], 1 if ends is None else len(ends)
+    lead = (0,) if ends is None else ()
+    operands = b.data_ptr(), *lead, *b.stride()
+    size = ctypes.c_size_t(0)
+    _native.check(lib.hst_matmul_blockscaled_workspace(a.data_ptr(), *a.stride(), *operands, groups, rows, n, k, 0, ctypes.byref(size)))
+    workspace = torch.full((size.value // 4,), -1, device="cuda", dtype=torch.int32)
+    y, group_ends = torch.empty((rows, n), device="cuda", dtype=out_dtype), None if ends is None else _ends(ends)
+    _native.check(
+        lib.hst_matmul_blockscaled(
+            grouped._DTYPES[out_dtype], a.data_ptr(), *a.stride(), sa.data_ptr(), *sa.stride(), *operands, sb.data_ptr(), *lead,
+            *sb.stride(), None if ends is None else group_ends.data_ptr(), groups, y.data_ptr(), rows, n, k,
+            workspace.data_ptr(), size.value, torch.cuda.current_stream().cuda_stream,
+        )
+    )  # fmt: skip
+    width = min(64, -(-rows // 32) * 32) if rows <= 64 * groups else 256
+    return y, _pieces(workspace, width)
+
+
+@gpu
+@pytest.mark.parametrize("rows", (20, 40, 300))  # widths of 32 and 64 with few rows, and the wide form
+@pytest.mark.parametrize("blocks,cut", ((40, True), (5, False)))
+def test_more_tiles_than_pairs(rows: int, blocks: int, cut: bool) -> None:
+    """Six tiles more than there are pairs, cut where they are deep; shallow ones stay whole, two for some pairs."""
+    cols = (_pairs() + 6) // (2 if rows == 300 else 1)
+    a, sa, b, sb = _operands(rows, 256 * cols - 16, 128 * blocks - 16, seed=rows + blocks)
+    y, pieces = _cut_product(a, sa, b, sb, None, torch.float16)
+    assert pieces >= 2 if cut else pieces == 0
+    _assert_product(y, _dequantize(a, sa, False), _dequantize(b, sb, True))
+    assert torch.equal(y, blockscale.matmul_blockscaled(a, sa, b, sb, out_dtype=torch.float16))
+
+
+@gpu
+@pytest.mark.parametrize("n,k", ((136, 264), (1032, 4368)))
+@pytest.mark.parametrize(
+    "rows,ends",
+    (
+        (340, [0, 200, 200, 200, 330, 331, 331, 331]),  # few rows on average: tiles of 64, 64, 64 and 32 rows of one group
+        (500, [1, 66, 130, 386, 500, 500, 500, 500]),  # 1, 65, 64, 256 and 114 rows
+        (2000, [1, 65, 130, 386, 643, 963, 1284, 2000]),  # wide: 1, 64, 65, 256, 257, 320, 321 and 716 rows
+    ),
+)
+def test_groups_of_many_rows_in_both_forms(rows: int, ends: list[int], n: int, k: int) -> None:
+    a, sa, b, sb = _operands(rows, n, k, seed=rows + n, groups=len(ends))
+    y = blockscale.matmul_blockscaled(a, sa, b, sb, _ends(ends))
+    da, db = _dequantize(a, sa, False), _dequantize(b, sb, True)
+    for e, (start, end) in enumerate(_bounds(ends, rows)):
+        _assert_product(y[start:end], da[start:end], db[e])
+    assert bool((y[ends[-1] :] == 0).all())
+
+
+@gpu
+def test_hundreds_of_groups() -> None:
+    groups = 300
+    counts = torch.randint(0, 4, (groups,), generator=torch.Generator().manual_seed(7))
+    counts[123] = 200
+    ends = torch.cumsum(counts, 0).tolist()
+    a, sa, b, sb = _operands(ends[-1] + 3, 136, 264, seed=8, groups=groups)
+    y = blockscale.matmul_blockscaled(a, sa, b, sb, _ends(ends))
+    da, db = _dequantize(a, sa, False), _dequantize(b, sb, True)
+    for e, (start, end) in enumerate(_bounds(ends, a.shape[0])):
+        _assert_product(y[start:end], da[start:end], db[e])
+    assert bool((y[ends[-1] :] == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("rows", (3, 300))
+def test_pieces_are_joined_in_32_bits(rows: int) -> None:
+    """As for the 16-bit products: the error of cut tiles is that of one rounding."""
+    a, sa, b, sb = _operands(rows, 520, 5120, seed=rows)
+    y, pieces = _cut_product(a, sa, b, sb, None, torch.float16)
+    assert pieces >= 2
+    assert _rounding_excess(y, _dequantize(a, sa, False) @ _dequantize(b, sb, True).T) <= 1.05
 
 
 @gpu

@@ -421,7 +421,90 @@ def _cut_weight_grad(x: torch.Tensor, dy: torch.Tensor, ends: list[int]) -> tupl
             workspace.data_ptr(), size.value, torch.cuda.current_stream().cuda_stream,
         )
     )  # fmt: skip
-    return out, int((workspace.view(-1, 2 * 128 * 256) != -1).any(dim=1).sum())
+    return out, _pieces(workspace, 256)
+
+
+def _pieces(workspace: torch.Tensor, width: int) -> int:
+    """Pieces of a workspace, filled with ones before the call, that hold anything: 128 x width values for each of
+    the two CTAs of a pair."""
+    return int((workspace.view(-1, 2 * 128 * width) != -1).any(dim=1).sum())
+
+
+def _cut_forward(x: torch.Tensor, w: torch.Tensor, ends: list[int]) -> tuple[torch.Tensor, int]:
+    """The same for the forward product (no operand of which needs a copy)."""
+    lib, (rows, k), (groups, _, n) = _native.library(), x.shape, w.shape
+    size = ctypes.c_size_t(0)
+    operands = x.data_ptr(), *x.stride(), w.data_ptr(), *w.stride()
+    _native.check(lib.hst_grouped_matmul_workspace(*operands, groups, rows, n, k, x.get_device(), ctypes.byref(size)))
+    workspace = torch.full((size.value // 4,), -1, device="cuda", dtype=torch.int32)
+    y, group_ends = torch.empty((rows, n), device="cuda", dtype=x.dtype), _ends(ends)
+    _native.check(
+        lib.hst_grouped_matmul(
+            grouped._DTYPES[x.dtype], *operands, group_ends.data_ptr(), groups, y.data_ptr(), rows, n, k,
+            workspace.data_ptr(), size.value, torch.cuda.current_stream().cuda_stream,
+        )
+    )  # fmt: skip
+    return y, _pieces(workspace, min(256, -(-rows // 32) * 32))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ("kn", "nk"))
+@pytest.mark.parametrize(
+    "rows,ends,tiles",  # tiles of 224 and 256 rows, of 160 twice, of 32 twice
+    ((456, [200, 200, 456], 2), (300, [0, 300], 2), (20, [3, 3, 20], 2)),
+)
+def test_more_tiles_than_pairs_are_cut(dtype: torch.dtype, layout: str, rows: int, ends: list[int], tiles: int) -> None:
+    """Six tiles more than there are pairs, 66 K blocks deep: a pair takes a whole tile and parts of others."""
+    cols = (_pairs() + 6) // tiles
+    x, w, _ = _operands(rows, len(ends), 4168, 256 * cols - 8, dtype, layout, seed=rows)
+    y, pieces = _cut_forward(x, w, ends)
+    assert tiles * cols > _pairs() and pieces >= 2
+    _check_forward(y, x, w, ends)
+    assert torch.equal(y, grouped.grouped_matmul(x, w, _ends(ends)))
+
+
+@gpu
+@pytest.mark.parametrize("ends", ([300, 300, 4900], [4096], [700, 3600, 3601]))
+def test_weight_gradients_cut_what_whole_tiles_leave(ends: list[int]) -> None:
+    """Each pair takes whole tiles of every group first; the line of what remains is cut (over 40 K blocks deep)."""
+    pairs = _pairs()
+    k, n = 256 * (pairs + 16) // 9 // 256 * 256 + 8, 2056  # 11 x 9 tiles of a group with 74 pairs: one for each pair, 25 over
+    assert pairs < -(-k // 256) * 9 < 2 * pairs
+    x, _, dy = _operands(5000, 1, k, n, torch.bfloat16, "kn", seed=43)
+    dw, pieces = _cut_weight_grad(x, dy, ends)
+    assert pieces >= 2
+    _check_weight_grad(dw, x, dy, ends)
+    assert torch.equal(dw, grouped.grouped_weight_grad(x, dy, _ends(ends)))
+
+
+def _rounding_excess(out: torch.Tensor, exact: torch.Tensor) -> float:
+    """The RMS error of ``out`` over that of the exact values rounded once."""
+    once = exact.to(out.dtype).double() - exact
+    return ((out.double() - exact).square().mean() / once.square().mean()).sqrt().item()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_pieces_are_joined_in_32_bits(dtype: torch.dtype) -> None:
+    """The error of cut tiles is that of one rounding. FP32 sums of up to 6200 products, 16 at a time, are off by at most
+    388 * 2^-23 = 2^-14.4 of the sum's size; one rounding of FP16 by 2^-11 / sqrt(3) or so (2^-12.3 on the average of
+    the mantissas): the two together are at most 3% more, and less in BF16. Pieces rounded to 16 bits have as much error
+    as the result's rounding, 41% more."""
+    ends = [33, 33, 70]
+    x, w, _ = _operands(70, 3, 4168, 520, dtype, "kn", seed=44)
+    y, pieces = _cut_forward(x, w, ends)
+    exact = torch.cat([x[s:e].double() @ w[i].double() for i, (s, e) in enumerate(_bounds(ends, 70))])
+    assert pieces >= 2 and _rounding_excess(y, exact) <= 1.05
+    ends = [0, 3100, 6200]
+    x, _, dy = _operands(6200, 1, 264, 136, dtype, "kn", seed=45)
+    dw, pieces = _cut_weight_grad(x, dy, ends)
+    exact = torch.stack([x[s:e].double().T @ dy[s:e].double() for s, e in _bounds(ends, 6200)])
+    assert pieces >= 2 and _rounding_excess(dw, exact) <= 1.05
+    # The test tells the two apart: the same sums from pieces of 256 rows rounded to 16 bits.
+    parts = [(x[s : s + 256].double().T @ dy[s : s + 256].double()).to(dtype) for s in range(0, 3100, 256)]
+    rough = torch.stack(parts).double().sum(0).to(dtype)
+    assert _rounding_excess(rough, x[:3100].double().T @ dy[:3100].double()) > 1.2
 
 
 @gpu
