@@ -310,9 +310,15 @@ GroupedProblem forward_problem(int64_t rows, int groups, int64_t n, int64_t k) {
 GroupedProblem grad_problem(int64_t rows, int groups, int64_t lcols, int64_t rcols) {
   return GroupedProblem{rows, groups, rcols, lcols, 0, 256};
 }
-// Up to 64 rows a group on average the rows go on the R side (kScaledFew; K = 4096, N = 12800: 64 rows 25.4 us
-// there and 28.9 on the L side, 96 rows 35.0 and 30.9).
-bool scaled_few(int64_t rows, int groups) { return rows <= int64_t(64) * groups; }
+// Few rows go on the R side (kScaledFew): up to 64 (K = 4096, N = 12800: 64 rows 25.4 us there and 28.9 on the L
+// side, 96 rows 35.0 and 30.9), or up to 8 a group on average. How they are spread is known to the GPU alone, and
+// a group of many costs 64 rows a tile there, each reading its weight. 4096 x 4096, us there / on the L side:
+//   rows a group, groups   even      in a quarter of the groups   in one
+//   8 x 32                 135/143   55/57                        31/34
+//   8 x 128                418/498   156/152                      82/37
+//   16 x 32                141/143   62/57                        49/33
+//   64 x 32                160/156   139/64                       137/53
+bool scaled_few(int64_t rows, int groups) { return rows <= std::max<int64_t>(64, int64_t(8) * groups); }
 GroupedProblem scaled_problem(int64_t rows, int groups, int64_t n, int64_t k) {
   return GroupedProblem{rows, groups, n, 0, cdiv(k, 128), scaled_few(rows, groups) ? width_cap(rows, 64) : 256};
 }

@@ -353,7 +353,7 @@ def _cut_product(a, sa, b, sb, ends: list[int] | None, out_dtype: torch.dtype) -
             workspace.data_ptr(), size.value, torch.cuda.current_stream().cuda_stream,
         )
     )  # fmt: skip
-    width = min(64, -(-rows // 32) * 32) if rows <= 64 * groups else 256
+    width = min(64, -(-rows // 32) * 32) if rows <= max(64, 8 * groups) else 256
     return y, _pieces(workspace, width)
 
 
@@ -375,18 +375,43 @@ def test_more_tiles_than_pairs(rows: int, blocks: int, cut: bool) -> None:
 @pytest.mark.parametrize(
     "rows,ends",
     (
-        (340, [0, 200, 200, 200, 330, 331, 331, 331]),  # few rows on average: tiles of 64, 64, 64 and 32 rows of one group
+        (340, [0, 200, 200, 200, 330, 331, 331, 331]),
         (500, [1, 66, 130, 386, 500, 500, 500, 500]),  # 1, 65, 64, 256 and 114 rows
-        (2000, [1, 65, 130, 386, 643, 963, 1284, 2000]),  # wide: 1, 64, 65, 256, 257, 320, 321 and 716 rows
+        (2000, [1, 65, 130, 386, 643, 963, 1284, 2000]),  # 1, 64, 65, 256, 257, 320, 321 and 716 rows
     ),
 )
-def test_groups_of_many_rows_in_both_forms(rows: int, ends: list[int], n: int, k: int) -> None:
+def test_groups_of_many_rows(rows: int, ends: list[int], n: int, k: int) -> None:
     a, sa, b, sb = _operands(rows, n, k, seed=rows + n, groups=len(ends))
     y = blockscale.matmul_blockscaled(a, sa, b, sb, _ends(ends))
     da, db = _dequantize(a, sa, False), _dequantize(b, sb, True)
     for e, (start, end) in enumerate(_bounds(ends, rows)):
         _assert_product(y[start:end], da[start:end], db[e])
     assert bool((y[ends[-1] :] == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize("n,k", ((136, 264), (1032, 4368)))
+def test_groups_of_many_rows_among_few(n: int, k: int) -> None:
+    """270 rows over 40 groups, so in the few-rows form: groups of 200 (tiles of 64, 64, 64 and 32), 65 and 1 rows."""
+    ends = [1] * 5 + [201] * 20 + [266] * 10 + [267] * 5
+    a, sa, b, sb = _operands(270, n, k, seed=n, groups=40)
+    y = blockscale.matmul_blockscaled(a, sa, b, sb, _ends(ends))
+    da, db = _dequantize(a, sa, False), _dequantize(b, sb, True)
+    for e, (start, end) in enumerate(_bounds(ends, 270)):
+        _assert_product(y[start:end], da[start:end], db[e])
+    assert bool((y[267:] == 0).all())
+
+
+@gpu
+@pytest.mark.parametrize(
+    "rows,groups,width", ((64, 1, 64), (65, 1, 256), (64, 8, 64), (65, 8, 256), (256, 32, 64), (257, 32, 256), (2000, 32, 256))
+)
+def test_the_form_goes_by_the_rows_of_all_groups(rows: int, groups: int, width: int) -> None:
+    """2000 rows over 32 groups may be 2000 of one: 64 rows a tile would read its weight 32 times."""
+    size = ctypes.c_size_t(0)
+    n, k = 25600, 6400  # deep, and tiles enough for every pair
+    status = _native.library().hst_matmul_blockscaled_workspace(16, k, 1, 16, n * k, k, 1, groups, rows, n, k, 0, ctypes.byref(size))
+    assert status == _native.HST_OK and size.value == _pairs() * 4 * 128 * width * 4
 
 
 @gpu
