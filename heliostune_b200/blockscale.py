@@ -33,16 +33,27 @@ def _blocks(extent: int) -> int:
     return -(-extent // BLOCK)
 
 
-def _outputs(what: str, x: torch.Tensor, tiles: bool) -> tuple[torch.Tensor, torch.Tensor]:
-    """Checks ``x`` and allocates its values and scales."""
-    if tiles and x.ndim not in (2, 3):
-        raise ValueError("quantize_tiles expects weight [N, K] or [E, N, K]")
-    if not tiles and x.ndim != 2:
-        raise ValueError("quantize_rows expects x [T, K]")
+def _check_quantize(what: str, x: torch.Tensor) -> None:
+    _refuse_gradient(what, x)
     if not x.is_cuda:
         raise ValueError(f"{what} expects a CUDA tensor")
     if x.dtype not in _DTYPES:
         raise ValueError(f"{what} serves torch.float16 or torch.bfloat16, got {x.dtype}")
+
+
+def _check_rows(x: torch.Tensor) -> None:
+    if x.ndim != 2:
+        raise ValueError("quantize_rows expects x [T, K]")
+    _check_quantize("quantize_rows", x)
+
+
+def _check_tiles(weight: torch.Tensor) -> None:
+    if weight.ndim not in (2, 3):
+        raise ValueError("quantize_tiles expects weight [N, K] or [E, N, K]")
+    _check_quantize("quantize_tiles", weight)
+
+
+def _outputs(x: torch.Tensor, tiles: bool) -> tuple[torch.Tensor, torch.Tensor]:
     *batch, rows, cols = x.shape
     # Rows of q start on 16 bytes, so that the products read them in place.
     width = -(-cols // 16) * 16
@@ -55,9 +66,8 @@ def _outputs(what: str, x: torch.Tensor, tiles: bool) -> tuple[torch.Tensor, tor
     return q, x.new_empty_strided((rows, _blocks(cols)), (1, rows), dtype=torch.float32)
 
 
-def _quantize(what: str, x: torch.Tensor, tiles: bool) -> tuple[torch.Tensor, torch.Tensor]:
-    _refuse_gradient(what, x)
-    q, scales = _outputs(what, x, tiles)
+def _quantize(x: torch.Tensor, tiles: bool) -> tuple[torch.Tensor, torch.Tensor]:
+    q, scales = _outputs(x, tiles)
     *batch, rows, cols = x.shape
     device = x.device
     width = -(-cols // 16) * 16
@@ -75,15 +85,14 @@ def _quantize(what: str, x: torch.Tensor, tiles: bool) -> tuple[torch.Tensor, to
     return q, scales
 
 
-_quantize_rows = _operator(
-    "quantize_rows(Tensor x) -> (Tensor, Tensor)",
-    lambda x: _quantize("quantize_rows", x, False),
-    lambda x: _outputs("quantize_rows", x, False),
+_quantize_rows, _ = _operator(
+    "quantize_rows(Tensor x) -> (Tensor, Tensor)", _check_rows, lambda x: _quantize(x, False), lambda x: _outputs(x, False)
 )
-_quantize_tiles = _operator(
+_quantize_tiles, _ = _operator(
     "quantize_tiles(Tensor weight) -> (Tensor, Tensor)",
-    lambda weight: _quantize("quantize_tiles", weight, True),
-    lambda weight: _outputs("quantize_tiles", weight, True),
+    _check_tiles,
+    lambda weight: _quantize(weight, True),
+    lambda weight: _outputs(weight, True),
 )
 
 
@@ -118,6 +127,7 @@ def _check_product(
     group_ends: torch.Tensor | None,
     out_dtype: torch.dtype,
 ) -> None:
+    _refuse_gradient("matmul_blockscaled", a, a_scales, b, b_scales)
     if a.ndim != 2 or b.ndim != (2 if group_ends is None else 3):
         raise ValueError("matmul_blockscaled expects a [T, K] and b [N, K], or b [E, N, K] with group_ends [E]")
     if a.shape[1] != b.shape[-1]:
@@ -140,7 +150,7 @@ def _check_product(
     _check_scales("b_scales", b_scales, (*lead, _blocks(n), _blocks(k)), index)
 
 
-def _product_kernel(
+def _launch_product(
     a: torch.Tensor,
     a_scales: torch.Tensor,
     b: torch.Tensor,
@@ -148,8 +158,6 @@ def _product_kernel(
     group_ends: torch.Tensor | None,
     out_dtype: torch.dtype,
 ) -> torch.Tensor:
-    _refuse_gradient("matmul_blockscaled", a, a_scales, b, b_scales)
-    _check_product(a, a_scales, b, b_scales, group_ends, out_dtype)
     (rows, k), n, device = a.shape, b.shape[-2], a.device
     y = a.new_empty((rows, n), dtype=out_dtype)
     a_pointer, a_strides, b_pointer, b_strides, sb_strides = a.data_ptr(), a.stride(), b.data_ptr(), b.stride(), b_scales.stride()
@@ -174,7 +182,7 @@ def _product_kernel(
     return y
 
 
-def _product_fake(
+def _empty_product(
     a: torch.Tensor,
     a_scales: torch.Tensor,
     b: torch.Tensor,
@@ -182,14 +190,14 @@ def _product_fake(
     group_ends: torch.Tensor | None,
     out_dtype: torch.dtype,
 ) -> torch.Tensor:
-    _check_product(a, a_scales, b, b_scales, group_ends, out_dtype)
     return a.new_empty((a.shape[0], b.shape[-2]), dtype=out_dtype)
 
 
-_product = _operator(
+_product, _ = _operator(
     "matmul_blockscaled(Tensor a, Tensor a_scales, Tensor b, Tensor b_scales, Tensor? group_ends, ScalarType out_dtype) -> Tensor",
-    _product_kernel,
-    _product_fake,
+    _check_product,
+    _launch_product,
+    _empty_product,
 )
 
 

@@ -53,11 +53,22 @@ _thread_keys = torch._C._dispatch_tls_local_include_set
 _PLAIN_TENSORS = (torch.Tensor, torch.nn.Parameter)
 
 
-def _operator(schema: str, kernel: Callable[..., Any], fake: Callable[..., Any]) -> Callable[..., Any]:
-    """The operator of ``schema``: ``kernel`` checks its arguments and launches, ``fake`` checks them and gives
-    the outputs' layout. Without it a tracer would see the outputs' allocation alone, and what it makes of a
-    program would return uninitialised memory."""
+def _operator(
+    schema: str, check: Callable[..., None], launch: Callable[..., Any], empty: Callable[..., Any]
+) -> tuple[Callable[..., Any], Callable[..., Any]]:
+    """The operator of ``schema``: ``check`` refuses arguments, ``launch`` runs the kernel, ``empty`` gives the outputs'
+    layout. Without it a tracer would see the outputs' allocation alone, and what it makes of a program would
+    return uninitialised memory. Returns the function to call and the operator behind it."""
     name = schema.split("(")[0]
+
+    def kernel(*args: Any) -> Any:
+        check(*args)
+        return launch(*args)
+
+    def fake(*args: Any) -> Any:
+        check(*args)
+        return empty(*args)
+
     _LIBRARY.define(schema)
     # On every device: the kernels refuse those that are not CUDA, as they refuse other types.
     _LIBRARY.impl(name, kernel, "CompositeExplicitAutograd")
@@ -65,29 +76,33 @@ def _operator(schema: str, kernel: Callable[..., Any], fake: Callable[..., Any])
     operator = getattr(torch.ops.heliostune_b200, name).default
 
     def call(*args: Any) -> Any:
-        # The way through the dispatcher costs 3 us. Where it would lead straight to the kernel -- no tracer, mode or
-        # transform is on in this thread, and the operands are plain tensors as they stand in memory -- the
-        # kernel is called at once.
-        if torch.compiler.is_compiling():
-            return operator(*args)
-        if _thread_keys().raw_repr() not in _PLAIN_THREAD:
-            _refuse_transforms(name)
-            return operator(*args)
-        for arg in args:
-            if type(arg) in _PLAIN_TENSORS:
-                if arg.is_neg():
-                    return operator(*args)
-            elif arg is not None and type(arg) is not torch.dtype:
-                return operator(*args)
-        return kernel(*args)
+        return kernel(*args) if _plain(args) else operator(*args)
 
-    return call
+    return call, operator
 
 
-def _refuse_transforms(what: str) -> None:
+def _plain(args: tuple[Any, ...]) -> bool:
+    """Whether the dispatcher would lead a call of these arguments straight to the kernel: no tracer, mode or transform
+    is on in this thread, and the operands are plain tensors as they stand in memory. The kernel is then called
+    at once, which saves 3 us; torch.func's transforms are refused."""
+    if torch.compiler.is_compiling():
+        return False
+    if _thread_keys().raw_repr() not in _PLAIN_THREAD:
+        _refuse_transforms()
+        return False
+    for arg in args:
+        if type(arg) in _PLAIN_TENSORS:
+            if arg.is_neg():
+                return False
+        elif arg is not None and type(arg) is not torch.dtype:
+            return False
+    return True
+
+
+def _refuse_transforms() -> None:
     """Refuses torch.func's transforms: at their levels the operators have no derivatives."""
     if torch._C._are_functorch_transforms_active():
-        raise ValueError(f"{what} is not available under torch.func's transforms")
+        raise ValueError("the grouped, quantising and block-scaled operators are not available under torch.func's transforms")
 
 
 def _refuse_gradient(what: str, *tensors: torch.Tensor) -> None:
@@ -145,6 +160,8 @@ def _check_operands(what: str, x: torch.Tensor, other: torch.Tensor, names: tupl
 
 
 def _check_matmul(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tensor) -> None:
+    # A recorded program calls the operator itself, which has no gradient.
+    _refuse_gradient("grouped_matmul", x, weight)
     if x.ndim != 2 or weight.ndim != 3:
         raise ValueError("grouped_matmul expects x [T, K] and weight [E, K, N]")
     if x.shape[1] != weight.shape[1]:
@@ -155,10 +172,7 @@ def _check_matmul(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tenso
     _check_ends(group_ends, weight.shape[0], x.get_device())
 
 
-def _matmul_kernel(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tensor) -> torch.Tensor:
-    # A recorded program calls the operator itself, which has no gradient.
-    _refuse_gradient("grouped_matmul", x, weight)
-    _check_matmul(x, weight, group_ends)
+def _launch_matmul(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tensor) -> torch.Tensor:
     groups, k, n = weight.shape
     rows, device = x.shape[0], x.device
     y = x.new_empty((rows, n))
@@ -177,12 +191,12 @@ def _matmul_kernel(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tens
     return y
 
 
-def _matmul_fake(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tensor) -> torch.Tensor:
-    _check_matmul(x, weight, group_ends)
+def _empty_matmul(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tensor) -> torch.Tensor:
     return x.new_empty((x.shape[0], weight.shape[2]))
 
 
 def _check_weight_grad(x: torch.Tensor, dy: torch.Tensor, group_ends: torch.Tensor) -> None:
+    _refuse_gradient("grouped_weight_grad", x, dy)
     if x.ndim != 2 or dy.ndim != 2 or x.shape[0] != dy.shape[0]:
         raise ValueError(f"grouped_weight_grad expects x [T, K] and dy [T, N], got {tuple(x.shape)} and {tuple(dy.shape)}")
     _check_operands("grouped_weight_grad", x, dy, ("x", "dy"))
@@ -192,9 +206,7 @@ def _check_weight_grad(x: torch.Tensor, dy: torch.Tensor, group_ends: torch.Tens
     _check_ends(group_ends, groups, x.get_device())
 
 
-def _weight_grad_kernel(left: torch.Tensor, right: torch.Tensor, group_ends: torch.Tensor) -> torch.Tensor:
-    _refuse_gradient("grouped_weight_grad", left, right)
-    _check_weight_grad(left, right, group_ends)
+def _launch_weight_grad(left: torch.Tensor, right: torch.Tensor, group_ends: torch.Tensor) -> torch.Tensor:
     groups = group_ends.shape[0]
     (rows, lcols), rcols, device = left.shape, right.shape[1], left.device
     out = left.new_empty((groups, lcols, rcols))
@@ -215,14 +227,18 @@ def _weight_grad_kernel(left: torch.Tensor, right: torch.Tensor, group_ends: tor
     return out
 
 
-def _weight_grad_fake(left: torch.Tensor, right: torch.Tensor, group_ends: torch.Tensor) -> torch.Tensor:
-    _check_weight_grad(left, right, group_ends)
+def _empty_weight_grad(left: torch.Tensor, right: torch.Tensor, group_ends: torch.Tensor) -> torch.Tensor:
     return left.new_empty((group_ends.shape[0], left.shape[1], right.shape[1]))
 
 
-_matmul = _operator("grouped_matmul(Tensor x, Tensor weight, Tensor group_ends) -> Tensor", _matmul_kernel, _matmul_fake)
-_weight_grad = _operator(
-    "grouped_weight_grad(Tensor x, Tensor dy, Tensor group_ends) -> Tensor", _weight_grad_kernel, _weight_grad_fake
+_matmul, _matmul_operator = _operator(
+    "grouped_matmul(Tensor x, Tensor weight, Tensor group_ends) -> Tensor", _check_matmul, _launch_matmul, _empty_matmul
+)
+_weight_grad, _weight_grad_operator = _operator(
+    "grouped_weight_grad(Tensor x, Tensor dy, Tensor group_ends) -> Tensor",
+    _check_weight_grad,
+    _launch_weight_grad,
+    _empty_weight_grad,
 )
 
 
@@ -248,14 +264,19 @@ class _GroupedMatmul(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):  # type: ignore[no-untyped-def]
         x, weight, group_ends = ctx.saved_tensors
+        _refuse_tangents("grouped_matmul's gradient", dy)
+        # Launched unchecked: the forward call took the saved tensors, and autograd gives dy the output's shape, type
+        # and device.
+        plain = _plain((dy, x, weight, group_ends))
+        matmul, weight_grad = (_launch_matmul, _launch_weight_grad) if plain else (_matmul_operator, _weight_grad_operator)
         dx = dweight = None
         if ctx.needs_input_grad[0]:
-            dx = _matmul(dy, weight.transpose(1, 2), group_ends)
+            dx = matmul(dy, weight.transpose(1, 2), group_ends)
         if ctx.needs_input_grad[1]:
             if ctx.weight_by_n:
-                dweight = _weight_grad(dy, x, group_ends).transpose(1, 2)
+                dweight = weight_grad(dy, x, group_ends).transpose(1, 2)
             else:
-                dweight = _weight_grad(x, dy, group_ends)
+                dweight = weight_grad(x, dy, group_ends)
         return dx, dweight, None
 
 
@@ -266,7 +287,7 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tens
     are copied once. Differentiable in ``x`` and ``weight`` (once, in reverse mode)."""
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         if not torch.compiler.is_compiling():
-            _refuse_transforms("grouped_matmul")
+            _refuse_transforms()
         _refuse_tangents("grouped_matmul", x, weight)
         return _GroupedMatmul.apply(x, weight, group_ends)
     return _matmul(x, weight, group_ends)

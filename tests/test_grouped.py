@@ -130,6 +130,9 @@ def test_a_forward_gradient_is_refused_on_the_gpu_and_its_primal_taken() -> None
         assert torch.equal(grouped.grouped_matmul(forward_ad.unpack_dual(forward_ad.make_dual(x, x)).primal, w, ends), expected)
         with pytest.raises(ValueError, match="forward-mode"):
             grouped.grouped_weight_grad(forward_ad.make_dual(x, x), dy, ends)
+        leaf = x.clone().requires_grad_()
+        with pytest.raises(ValueError, match="forward-mode"):
+            torch.autograd.grad(grouped.grouped_matmul(leaf, w, ends), (leaf,), forward_ad.make_dual(dy, dy))
 
 
 def test_the_library_refuses_bad_calls_before_any_cuda_work() -> None:
@@ -590,6 +593,19 @@ def test_empty_extents() -> None:
     assert bool((grouped.grouped_matmul(x[:, :0], w[:, :0], ends) == 0).all())
     assert bool((grouped.grouped_weight_grad(x[:0], dy[:0], ends) == 0).all())
     assert grouped.grouped_weight_grad(x[:, :0], dy, ends).shape == (2, 0, 24)
+
+
+@gpu
+@pytest.mark.parametrize("rows,k,n", ((0, 16, 24), (4, 0, 24), (4, 16, 0)))
+def test_gradients_of_empty_extents(rows: int, k: int, n: int) -> None:
+    x, w, dy = _operands(rows, 2, k, n, torch.float16, "kn", seed=46)
+    x.requires_grad_()
+    w.requires_grad_()
+    y = grouped.grouped_matmul(x, w, _ends([2, 4]))
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    assert y.shape == (rows, n) and dx.shape == x.shape and dw.shape == w.shape
+    for t in (y, dx, dw):
+        assert bool((t == 0).all())
 
 
 @gpu
