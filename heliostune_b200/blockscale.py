@@ -85,10 +85,10 @@ def _quantize(x: torch.Tensor, tiles: bool) -> tuple[torch.Tensor, torch.Tensor]
     return q, scales
 
 
-_quantize_rows, _ = _operator(
+_quantize_rows, *_ = _operator(
     "quantize_rows(Tensor x) -> (Tensor, Tensor)", _check_rows, lambda x: _quantize(x, False), lambda x: _outputs(x, False)
 )
-_quantize_tiles, _ = _operator(
+_quantize_tiles, *_ = _operator(
     "quantize_tiles(Tensor weight) -> (Tensor, Tensor)",
     _check_tiles,
     lambda weight: _quantize(weight, True),
@@ -193,7 +193,7 @@ def _empty_product(
     return a.new_empty((a.shape[0], b.shape[-2]), dtype=out_dtype)
 
 
-_product, _ = _operator(
+_product, *_ = _operator(
     "matmul_blockscaled(Tensor a, Tensor a_scales, Tensor b, Tensor b_scales, Tensor? group_ends, ScalarType out_dtype) -> Tensor",
     _check_product,
     _launch_product,

@@ -55,10 +55,11 @@ _PLAIN_TENSORS = (torch.Tensor, torch.nn.Parameter)
 
 def _operator(
     schema: str, check: Callable[..., None], launch: Callable[..., Any], empty: Callable[..., Any]
-) -> tuple[Callable[..., Any], Callable[..., Any]]:
+) -> tuple[Callable[..., Any], Callable[..., Any], Callable[..., Any]]:
     """The operator of ``schema``: ``check`` refuses arguments, ``launch`` runs the kernel, ``empty`` gives the outputs'
     layout. Without it a tracer would see the outputs' allocation alone, and what it makes of a program would
-    return uninitialised memory. Returns the function to call and the operator behind it."""
+    return uninitialised memory. Returns the function to call and what
+    it calls, the kernel or the operator (:func:`_plain`)."""
     name = schema.split("(")[0]
 
     def kernel(*args: Any) -> Any:
@@ -78,7 +79,7 @@ def _operator(
     def call(*args: Any) -> Any:
         return kernel(*args) if _plain(args) else operator(*args)
 
-    return call, operator
+    return call, kernel, operator
 
 
 def _plain(args: tuple[Any, ...]) -> bool:
@@ -231,10 +232,10 @@ def _empty_weight_grad(left: torch.Tensor, right: torch.Tensor, group_ends: torc
     return left.new_empty((group_ends.shape[0], left.shape[1], right.shape[1]))
 
 
-_matmul, _matmul_operator = _operator(
+_matmul, _matmul_kernel, _matmul_operator = _operator(
     "grouped_matmul(Tensor x, Tensor weight, Tensor group_ends) -> Tensor", _check_matmul, _launch_matmul, _empty_matmul
 )
-_weight_grad, _weight_grad_operator = _operator(
+_weight_grad, _weight_grad_kernel, _weight_grad_operator = _operator(
     "grouped_weight_grad(Tensor x, Tensor dy, Tensor group_ends) -> Tensor",
     _check_weight_grad,
     _launch_weight_grad,
@@ -264,11 +265,9 @@ class _GroupedMatmul(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):  # type: ignore[no-untyped-def]
         x, weight, group_ends = ctx.saved_tensors
-        _refuse_tangents("grouped_matmul's gradient", dy)
-        # Launched unchecked: the forward call took the saved tensors, and autograd gives dy the output's shape, type
-        # and device.
+        # The saved tensors are checked again: a hook may have packed and unpacked them.
         plain = _plain((dy, x, weight, group_ends))
-        matmul, weight_grad = (_launch_matmul, _launch_weight_grad) if plain else (_matmul_operator, _weight_grad_operator)
+        matmul, weight_grad = (_matmul_kernel, _weight_grad_kernel) if plain else (_matmul_operator, _weight_grad_operator)
         dx = dweight = None
         if ctx.needs_input_grad[0]:
             dx = matmul(dy, weight.transpose(1, 2), group_ends)

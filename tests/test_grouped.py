@@ -674,6 +674,18 @@ def test_a_frozen_operand_keeps_the_other_out_of_the_graph() -> None:
 
 
 @gpu
+@pytest.mark.parametrize("moved", (lambda t: t.cpu(), lambda t: t.float()))
+def test_what_a_saved_tensors_hook_gives_back_is_checked(moved) -> None:  # type: ignore[no-untyped-def]
+    x, w, dy = _operands(9, 2, 32, 16, torch.float16, "kn", seed=47)
+    for frozen_x in (False, True):
+        leaf_x, leaf_w = x.clone().requires_grad_(not frozen_x), w.clone().requires_grad_(frozen_x)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, moved):
+            y = grouped.grouped_matmul(leaf_x, leaf_w, _ends([4, 9]))
+        with pytest.raises(ValueError):
+            y.backward(dy)
+
+
+@gpu
 def test_bad_arguments_are_rejected() -> None:
     x, w, dy = _operands(9, 2, 32, 16, torch.float16, "kn", seed=13)
     ends = _ends([4, 9])
