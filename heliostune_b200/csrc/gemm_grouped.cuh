@@ -26,7 +26,7 @@
 //     register: on the R side the scales of 256 rows are 128 a thread and block, and their broadcast
 //     loads from shared memory, beside the UMMAs' operands, took three times the UMMAs' time. Bound now
 //     by the way of a block through the two buffers (UMMAs 512 cycles, hand-over, 128 columns a thread
-//     read and added, hand-back): 8192 x 14336 x 4096 in 479 us, 350 without the reading and adding.
+//     read and added, hand-back): 8192 x 14336 x 4096 in 481 us, 350 without the reading and adding.
 //   * kScaledFew is for few rows a group: as kForward, weights on the L side and at most 64 rows on
 //     the R side, in eight TMEM buffers. A block then costs 64 to 128 UMMA cycles instead of 512 and
 //     keeps all lanes busy, and the weights stream at the rate of HBM.
@@ -1091,8 +1091,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
         for (int j = 0; j < 128; ++j) acc[j] = 0.f;
         bool ready = true;
         for (int kb = s.kb0; kb < s.kb1; ++kb) {
-          float now = next_a * next_b;
-          const bool split = !__all_sync(0xffffffffu, is_normal(now));
+          const float a = next_a, b = next_b;
           if (kb + 1 < s.kb1) {
             sa += args.rs_k;
             sb += args.ts_k;
@@ -1101,12 +1100,14 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
           }
           ready = wait_buf();
           if (!ready) break;
+          float now = a * b;
+          const bool split = !__all_sync(0xffffffffu, is_normal(now));
           // Rare: the block's sums take the first factor in TMEM, so that the loop below stays as it is (with a copy of the
-          // loop for this, 8192 x 14336 x 4096 took 487 to 502 us; 470 without any of it, 479 so).
+          // loop for this, 8192 x 14336 x 4096 took 487 to 502 us). The vote itself costs 481 against 470 us there, and
+          // 42.7 against 41.3 for 257 x 12800 x 4096.
           if (live && split) {
             float before;
-            const int64_t back = kb + 1 < s.kb1 ? 1 : 0;
-            split_scale(*(sa - back * args.rs_k), *(sb - back * args.ts_k), before, now);
+            split_scale(a, b, before, now);
 #pragma unroll 1
             for (int c = 0; c < 128; c += 16) {
               const uint32_t taddr = lane_base + static_cast<uint32_t>(buf * kBufCols + half * 128 + c);
@@ -1181,12 +1182,7 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
         float next_a = *sa, next_a32 = second ? *sa32 : 0.f, next_b = *sb;
         bool ready = true;
         for (int kb = s.kb0; kb < s.kb1; ++kb) {
-          float now = next_a * next_b, now32 = next_a32 * next_b, before = 1.f, before32 = 1.f;
-          const bool split = !__all_sync(0xffffffffu, is_normal(now) && (!second || is_normal(now32)));
-          if (split) {
-            split_scale(next_a, next_b, before, now);
-            split_scale(next_a32, next_b, before32, now32);
-          }
+          const float a = next_a, a32 = next_a32, b = next_b;
           if (kb + 1 < s.kb1) {
             sa += args.rs_k;
             sb += args.ts_k;
@@ -1203,17 +1199,33 @@ __global__ void __launch_bounds__(group_threads(MODE), 1)
           uint32_t v[2][32];
           tmem_ld_32x32b_x32(taddr, v[0]);
           if (second) tmem_ld_32x32b_x32(taddr + 32, v[1]);
+          float now = a * b, now32 = a32 * b;
+          const bool split = !__all_sync(0xffffffffu, is_normal(now) & is_normal(second ? now32 : 1.f));
           tmem_ld_wait();
+          // Rare: as in the wide form, and loaded again. The vote costs 23.8 against 23.3 us for 1 x 18944 x 3584, 43.4
+          // against 41.9 for 128 rows over 32 groups of 2816 x 2048 (24.5 and 46.2 where it comes before the loads).
+          if (split) {
+            float before, before32;
+            split_scale(a, b, before, now);
+            split_scale(a32, b, before32, now32);
+#pragma unroll 1
+            for (int c = 0; c < s.width; c += 16) {
+              uint32_t w[16];
+              tmem_ld_32x32b_x16(taddr + c, w);
+              tmem_ld_wait();
+              tmem_ld_fence_regs(w);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) w[j] = scaled_bits(w[j], __shfl_sync(0xffffffffu, c < 32 ? before : before32, (c & 31) + j));
+              tmem_st_32x32b_x16(taddr + c, w);
+            }
+            tmem_st_wait();
+            tmem_ld_32x32b_x32(taddr, v[0]);
+            if (second) tmem_ld_32x32b_x32(taddr + 32, v[1]);
+            tmem_ld_wait();
+          }
           tmem_ld_fence_regs(v[0]);
           tmem_ld_fence_regs(v[1]);
           release_buf();
-          if (split) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              v[0][j] = scaled_bits(v[0][j], __shfl_sync(0xffffffffu, before, j));
-              v[1][j] = scaled_bits(v[1][j], __shfl_sync(0xffffffffu, before32, j));
-            }
-          }
 #pragma unroll
           for (int j = 0; j < 32; ++j) acc[j] = fmaf(__uint_as_float(v[0][j]), __shfl_sync(0xffffffffu, now, j), acc[j]);
           if (second) {

@@ -457,7 +457,7 @@ def test_nan_and_infinity_stay_in_their_rows_and_columns(rows: int) -> None:
 
 
 @gpu
-@pytest.mark.parametrize("rows", (40, 400))
+@pytest.mark.parametrize("rows", (20, 40, 400))
 @pytest.mark.parametrize("size", (130, -142))
 def test_scales_whose_product_leaves_the_range_of_fp32(rows: int, size: int) -> None:
     """Scales of about 2^(size / 2) each: their product is no normal FP32 value, what they scale is. Where it is too
