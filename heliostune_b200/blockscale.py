@@ -106,7 +106,8 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 def quantize_tiles(weight: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """``(q, scales)`` of ``weight [N, K]`` or ``[E, N, K]`` (FP16 or BF16, any strides): ``q`` of its shape
     in ``torch.float8_e4m3fn`` and FP32 ``scales [..., ceil(N / 128), ceil(K / 128)]``, one for each
-    128 x 128 tile."""
+    128 x 128 tile. Contiguous rows are read at the rate of HBM, those of a transposed view a value at a time
+    (18944 x 3584: 37 us and 531)."""
     return _quantize_tiles(weight)
 
 

@@ -246,7 +246,8 @@ _weight_grad, _weight_grad_kernel, _weight_grad_operator = _operator(
 def grouped_weight_grad(x: torch.Tensor, dy: torch.Tensor, group_ends: torch.Tensor) -> torch.Tensor:
     """``out[e] = x[rows of e].T @ dy[rows of e]``, ``[E, K, N]``: the weight gradient of
     :func:`grouped_matmul`, with FP32 sums over the rows and one rounding. ``x [T, K]`` and ``dy [T, N]``
-    are FP16 or BF16 with any strides (copied once where their rows are not 16-byte aligned)."""
+    are FP16 or BF16 with any strides (copied in every call where their rows are
+    not 16-byte aligned)."""
     return _weight_grad(x, dy, group_ends)
 
 
@@ -283,7 +284,8 @@ def grouped_matmul(x: torch.Tensor, weight: torch.Tensor, group_ends: torch.Tens
     """``y[t] = x[t] @ weight[e(t)]`` with FP32 accumulation: ``x [T, K]``, ``weight [E, K, N]`` (either of
     its last two dimensions contiguous), both FP16 or both BF16, ``y [T, N]`` of their type; 1 to
     :data:`MAX_GROUPS` experts. Any strides are served; operands whose rows are not 16-byte aligned
-    are copied once. Differentiable in ``x`` and ``weight`` (once, in reverse mode)."""
+    are copied in every call, the weights of experts that have rows (4096 rows over 32 experts, N 1408, FP16: K 2048
+    53 us, 2047 with rows along N 59, along K 130). Differentiable in ``x`` and ``weight`` (once, in reverse mode)."""
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         if not torch.compiler.is_compiling():
             _refuse_transforms()
